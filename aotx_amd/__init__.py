@@ -34,6 +34,9 @@ AOTX_LAYER_KIND_ATTENTION_NO_QK_NORM = 1
 AOTX_LAYER_KIND_FFN_EXPERTS = 2
 AOTX_ROPE_PAIRS_SPLIT = 0
 AOTX_ROPE_PAIRS_ADJACENT = 1
+AOTX_ROPE_AXES_MAX = 4
+AOTX_ROPE_AXES_RUNS = 0
+AOTX_ROPE_AXES_TURN = 1
 AOTX_MODEL_ABSENT = (1 << 64) - 1
 AOTX_MODEL_ROWS_ALL = 0
 AOTX_MODEL_ROWS_LAST = 1
@@ -189,6 +192,12 @@ class ModelBinding(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * AOTX_DESC_BUFFER), ("slot", u32), ("needed", u32)]
 
 
+class RopeHow(ctypes.Structure):
+    """include/aotx_hybrid.h aotx_rope_how."""
+    _fields_ = [("theta", f32), ("eps", f32), ("rope_dim", u32), ("pairs", u32), ("axes", u32),
+                ("order", u32), ("span", u32 * AOTX_ROPE_AXES_MAX)]
+
+
 PROTOTYPES = {
     "aotx_mem_weights_set": (i32, [u64, u64]),
     "aotx_mem_weights_base": (u64, []),
@@ -250,6 +259,16 @@ PROTOTYPES = {
     "aotx_synth_f16": (i32, [vp, u64, f32, u64, vp]),
     "aotx_synth_f16_host": (i32, [vp, u64, f32, u64, u32]),
     "aotx_version": (ctypes.c_char_p, []),
+    # the operators of hybrid models' layers (include/aotx_hybrid.h)
+    "aotx_delta_conv": (i32, [vp, u32, vp, vp, vp, vp, vp, u32, u32, u32, u32, vp, u32, vp, vp]),
+    "aotx_delta_step": (i32, [vp, u32, vp, vp, u32, vp, vp, vp, vp, u32, u32, u32, u32, f32, vp,
+                              u32, vp, vp]),
+    "aotx_delta_work": (u64, [u32, u32, u32, u32]),
+    "aotx_delta_chunk": (i32, [vp, u32, vp, vp, u32, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32,
+                               f32, vp, u32, vp, u64, vp, vp]),
+    "aotx_norm_gate": (i32, [vp, vp, u32, vp, u32, u32, u32, f32, vp, vp]),
+    "aotx_rope_axes": (i32, [vp, u32, vp, vp, ctypes.POINTER(RopeHow), vp, vp, u32, u32, u32,
+                             u32, vp, vp, vp, vp]),
     # GGUF model files (include/aotx_modelfile.h)
     "aotx_modelfile_open": (i32, [ctypes.c_char_p, ctypes.POINTER(vp)]),
     "aotx_modelfile_close": (None, [vp]),
