@@ -6,19 +6,8 @@
  *   S <- exp(g) S;  u = beta (v - S^T k');  S <- S + k' u^T;  out = S^T q'.
  * Columns of S never meet, so a head's columns are shared out over workgroups freely.
  */
-#include "delta_dev.h"
+#include "delta_chunk.h"
 #include "../../include/aotx_hybrid.h"
-
-struct aotx_delta_args {
-    const unsigned short *qkv;
-    const float *a, *b, *decay, *dt;
-    float *state;
-    unsigned short *out;
-    unsigned int stride, ab_stride;
-    unsigned int key_heads, heads, group;
-    float eps;
-    aotx_seqs seqs;
-};
 
 /* ---------------------------------------------------------------------------------------
  * Row by row. A workgroup holds CS columns of one head's S in registers, four columns and
@@ -38,7 +27,9 @@ __global__ __launch_bounds__(256) void aotx_delta_rows_kernel(aotx_delta_args p)
     const unsigned int unit = blockIdx.x / SLICES, slice = blockIdx.x % SLICES;
     const unsigned int i = unit / p.heads, h = unit % p.heads;
     const unsigned int lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const aotx_seq_view seq = aotx_seq_of(p.seqs, i);
+    unsigned int first, last;
+    aotx_seq_rows(p.seqs, &first, &last);
+    const aotx_seq_view seq = aotx_seq_of(p.seqs, i, first, last);
     if (seq.start >= seq.end) return;
     const unsigned int c4 = (threadIdx.x % LC) * 4u, rg = threadIdx.x / LC;
     const unsigned int col = slice * CS + c4;
@@ -209,10 +200,29 @@ extern "C" int aotx_delta_step(const void *qkv, unsigned int stride, const float
     return 0;
 }
 
+/* Chunks of a call at most: every sequence ends with a part of one. */
+static unsigned int aotx_delta_chunks_max(unsigned int tokens, unsigned int seqs)
+{
+    return tokens / AOTX_DELTA_CHUNK + seqs;
+}
+
 extern "C" unsigned long long aotx_delta_work(unsigned int tokens, unsigned int seqs,
                                               unsigned int heads, unsigned int head_dim)
 {
-    return 256ull;
+    /* T, P and factors for every head, K^T for as many key heads */
+    return (unsigned long long)aotx_delta_chunks_max(tokens, seqs) * heads
+        * (sizeof(aotx_delta_chunk_work) + (unsigned long long)head_dim * AOTX_DELTA_CHUNK * 2u);
+}
+
+template <int D>
+static void aotx_delta_chunked(const aotx_delta_args &p, hipStream_t s)
+{
+    constexpr unsigned int NT = 1u, slices = D / (16u * NT);
+    hipLaunchKernelGGL((aotx_delta_within<D>), dim3(p.chunks * p.heads), dim3(256), 0, s, p);
+    AOTX_LAUNCH_CHECK();
+    const unsigned int units = (p.seqs.seqs * p.heads + 7u) / 8u * 8u;
+    hipLaunchKernelGGL((aotx_delta_across<D, NT>), dim3(units * slices), dim3(256), 0, s, p);
+    AOTX_LAUNCH_CHECK();
 }
 
 extern "C" int aotx_delta_chunk(const void *qkv, unsigned int stride, const float *a,
@@ -233,7 +243,10 @@ extern "C" int aotx_delta_chunk(const void *qkv, unsigned int stride, const floa
     if (tokens == 0u || seqs == 0u) return 0;
     if ((p.seqs.faults = aotx_faults(stream)) == nullptr) return 1;
     p.seqs.offset = offset;
-    if (head_dim == 128u) aotx_delta_rows<128>(p, aotx_stream(stream));
-    else aotx_delta_rows<64>(p, aotx_stream(stream));
+    p.chunks = aotx_delta_chunks_max(tokens, seqs);
+    p.work = (aotx_delta_chunk_work *)work;
+    p.kt = (aotx_h8 *)(p.work + (unsigned long long)p.chunks * heads);
+    if (head_dim == 128u) aotx_delta_chunked<128>(p, aotx_stream(stream));
+    else aotx_delta_chunked<64>(p, aotx_stream(stream));
     return 0;
 }

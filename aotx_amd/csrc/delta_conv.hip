@@ -37,14 +37,11 @@ __global__ __launch_bounds__(256) void aotx_delta_conv_kernel(aotx_conv_args p)
         if (p.bias != nullptr) bias = *(const aotx_f4 *)(p.bias + c);
     }
     /* the first sequence with rows from t0 on: those that end at or before t0 come first */
-    unsigned int i = t0;
-    if (p.seqs.offset != nullptr) {
-        unsigned int b = 0u, e = 0u;
-        if (lane < p.seqs.seqs) aotx_seq_rows(p.seqs, lane, &b, &e);
-        i = (unsigned int)__popcll(__ballot(lane < p.seqs.seqs && e <= t0));
-    }
+    unsigned int b, e;
+    aotx_seq_rows(p.seqs, &b, &e);
+    unsigned int i = (unsigned int)__popcll(__ballot(lane < p.seqs.seqs && e <= t0));
     for (; i < p.seqs.seqs; ++i) {
-        const aotx_seq_view seq = aotx_seq_of(p.seqs, i);
+        const aotx_seq_view seq = aotx_seq_of(p.seqs, i, b, e);
         if (seq.start >= stop) break;
         /* The run that holds a sequence's first row takes its first W - 1 rows, so that no
          * other run needs the slot's rows, which that run replaces. */

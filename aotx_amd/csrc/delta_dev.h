@@ -28,31 +28,43 @@ struct aotx_seq_view {
     bool refused;               /* no slot, or a slot that an earlier sequence has */
 };
 
-/* Rows of sequence i, in bounds whatever the offsets hold. */
-static __device__ __forceinline__ void aotx_seq_rows(const aotx_seqs &s, unsigned int i,
-                                                     unsigned int *start, unsigned int *end)
+/* Rows of sequence `lane`, for the first `seqs` lanes of a wave (all 64 call this): in bounds,
+ * and none before an earlier sequence's last, whatever the offsets hold. */
+static __device__ __forceinline__ void aotx_seq_rows(const aotx_seqs &s, unsigned int *start,
+                                                     unsigned int *end)
 {
+    const unsigned int lane = threadIdx.x & 63u;
+    unsigned int b = 0u, e = 0u;
     if (s.offset == nullptr) {
-        *start = i;
-        *end = i + 1u;
-        return;
+        if (lane < s.seqs) {
+            b = lane;
+            e = lane + 1u;
+        }
+    } else {
+        if (lane < s.seqs) {
+            b = s.offset[lane];
+            e = s.offset[lane + 1u];
+            b = b < s.tokens ? b : s.tokens;
+            e = e < s.tokens ? e : s.tokens;
+        }
+        for (unsigned int off = 1u; off < s.seqs; off <<= 1) {
+            const unsigned int o = (unsigned int)__shfl_up((int)b, off, 64);
+            if (lane >= off && o > b) b = o;
+        }
+        if (e < b) e = b;
     }
-    const unsigned int b = s.offset[i], e = s.offset[i + 1u];
-    *start = b < s.tokens ? b : s.tokens;
-    const unsigned int c = e < s.tokens ? e : s.tokens;
-    *end = c > *start ? c : *start;
+    *start = b;
+    *end = e;
 }
 
 /* Sequence i (wave-uniform), read by all 64 lanes of a wave: lane j looks at sequence j, which
- * tells whether an earlier one with rows has the same slot (at most 64 sequences a call). */
-static __device__ __forceinline__ aotx_seq_view aotx_seq_of(const aotx_seqs &s, unsigned int i)
+ * tells whether an earlier one with rows has the same slot (at most 64 sequences a call). b and
+ * e are the lanes' rows from aotx_seq_rows. */
+static __device__ __forceinline__ aotx_seq_view aotx_seq_of(const aotx_seqs &s, unsigned int i,
+                                                            unsigned int b, unsigned int e)
 {
     const unsigned int lane = threadIdx.x & 63u;
-    unsigned int b = 0u, e = 0u, a = 0xFFFFFFFFu;
-    if (lane < s.seqs) {
-        aotx_seq_rows(s, lane, &b, &e);
-        a = s.agent[lane];
-    }
+    const unsigned int a = lane < s.seqs ? s.agent[lane] : 0xFFFFFFFFu;
     aotx_seq_view v;
     v.start = (unsigned int)__builtin_amdgcn_readlane((int)b, (int)i);
     v.end = (unsigned int)__builtin_amdgcn_readlane((int)e, (int)i);

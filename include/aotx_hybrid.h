@@ -20,8 +20,8 @@
  * offset[i] .. offset[i + 1] - 1, its state is that of slot agent[i], and pos[i] is the cache
  * position of its first row. A sequence at position 0 starts from zeros, whatever its slot
  * held. A sequence without rows leaves its slot as it was. Rows before offset[0] and from
- * offset[seqs] on are neither read nor written; offsets past `tokens` are taken as `tokens`. A
- * sequence that names no slot of the caller's (agent[i] >= slots), or a slot that an earlier
+ * offset[seqs] on are neither read nor written; an offset past `tokens` is taken as `tokens`, and
+ * one below an earlier one as that one. A sequence that names no slot of the caller's (agent[i] >= slots), or a slot that an earlier
  * sequence with rows names too, gets rows of zeros, changes no state, and adds 1 to
  * aotx_model_faulted(). At most AOTX_SLOTS sequences and slots.
  *

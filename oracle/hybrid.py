@@ -11,12 +11,9 @@ def silu(x):
 
 
 def spans_of(offset, tokens):
-    """(start, end) of every sequence, in bounds."""
-    got = []
-    for b, e in zip(offset[:-1], offset[1:]):
-        b = min(int(b), tokens)
-        got.append((b, max(b, min(int(e), tokens))))
-    return got
+    """(start, end) of every sequence: in bounds, none before an earlier one's last row."""
+    at = np.maximum.accumulate([min(int(o), tokens) for o in offset])
+    return list(zip(at[:-1].tolist(), at[1:].tolist()))
 
 
 def walk(offset, agent, slots, tokens):
