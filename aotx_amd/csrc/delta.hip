@@ -155,7 +155,7 @@ static int aotx_delta_fill(aotx_delta_args *p, const void *qkv, unsigned int str
         return 1;
     if (head_dim != 64u && head_dim != 128u) return 1;
     if (heads == 0u || heads > 256u || key_heads == 0u || heads % key_heads != 0u) return 1;
-    if (stride % 8u != 0u || stride < (2u * key_heads + heads) * head_dim) return 1;
+    if (stride % 8u != 0u || stride < (2u * key_heads + heads) * head_dim || stride > (1u << 22)) return 1;
     if (ab_stride < heads || !(eps > 0.0f)) return 1;
     if (seqs > AOTX_SLOTS || slots == 0u || slots > AOTX_SLOTS || tokens > (1u << 20)) return 1;
     if (!aotx_aligned16(qkv) || !aotx_aligned16(state) || !aotx_aligned16(out)) return 1;
@@ -221,7 +221,7 @@ static void aotx_delta_chunked(const aotx_delta_args &p, hipStream_t s)
     hipLaunchKernelGGL((aotx_delta_within<D>), dim3(p.chunks * p.heads), dim3(256), 0, s, p);
     AOTX_LAUNCH_CHECK();
     const unsigned int units = (p.seqs.seqs * p.heads + 7u) / 8u * 8u;
-    hipLaunchKernelGGL((aotx_delta_across<D, NT>), dim3(units * slices), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((aotx_delta_across<D, NT>), dim3(units * slices), dim3(512), 0, s, p);
     AOTX_LAUNCH_CHECK();
 }
 

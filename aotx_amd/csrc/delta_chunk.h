@@ -10,14 +10,13 @@
  * aotx_delta_across, walks a sequence's chunks with a slice of columns of S in registers.
  *
  * Numbers. K, Q and V are fp16 and enter the matrix cores as they are; S, U, X = V - K S, T and
- * P enter as two fp16 parts (high and rest, 22 bits), so that their products are as good as
- * fp32 ones at three times the work of plain fp16 instead of sixteen times for fp32 matrix
- * instructions. The parts have fp16's range: T and P are at most 1 (the rule only ever takes
- * away from what a unit key finds), K is scaled to a length of 1 to 2 by a power of two where
- * its scale goes into U, and S, X and U are scaled by a power of two for every column that
- * follows from the column's largest entries a chunk before: |S| grows by at most the sum of 64
- * values' lengths in a chunk, so 2^7 of headroom is enough, and 15 - 7 bits above 1 leave the rest
- * part's smallest step, 2^-24, below 2^-31 of the largest entry.
+ * P enter as two fp16 parts (high and rest, 21 bits), so that their products are nearly as good
+ * as fp32 ones at two or three times the work of plain fp16 instead of sixteen times for fp32
+ * matrix instructions. The parts have fp16's range: T and P are at most 1 (the rule only ever
+ * takes away from what a unit key finds), K is scaled to a length of 1 to 2 by a power of two
+ * where its scale goes into U, and S, X and U carry a power of two for every column, set anew
+ * every four chunks from the column's largest entries: a state's column grows by at most the
+ * sum of the 256 values' sizes in that time.
  *
  * A row whose K, a or b is no number is taken out (its K, g and beta are zeros) and remembered:
  * from that row on, out and the state are NaN; the same for one column from a bad value in V on.
@@ -41,9 +40,11 @@ struct aotx_delta_chunk_work {
     float of_k[64];         /* exp(G) r_k */
     float of_q[64];         /* exp(G) r_q */
     float of_u[64];         /* exp(G_last - G) r_k 2^e; K^T of that row is over 2^e */
+    unsigned char vmax[128];/* of every column of V the exponent field of its largest size */
     float fade;             /* exp(G_last) */
     unsigned int bad;       /* first row that is taken out, 64 for none */
-    unsigned int pad[62];
+    unsigned int badv;      /* V has a value that is no number */
+    unsigned int pad[29];
 };
 
 struct aotx_delta_args {
@@ -72,6 +73,19 @@ static __device__ __forceinline__ void aotx_split(float x, _Float16 *hi, _Float1
     *lo = (_Float16)(x - (float)*hi);
 }
 
+/* Four of them, rounded toward zero: the rest makes up for the high part's rounding, and ends
+ * 2^-21 below x at most. */
+typedef _Float16 aotx_h2 __attribute__((ext_vector_type(2)));
+static __device__ __forceinline__ void aotx_split4(aotx_f4 x, aotx_h4 *hi, aotx_h4 *lo)
+{
+    const aotx_h2 a = __builtin_bit_cast(aotx_h2, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));
+    const aotx_h2 b = __builtin_bit_cast(aotx_h2, __builtin_amdgcn_cvt_pkrtz(x[2], x[3]));
+    const aotx_h2 c = __builtin_bit_cast(aotx_h2, __builtin_amdgcn_cvt_pkrtz(x[0] - (float)a[0], x[1] - (float)a[1]));
+    const aotx_h2 d = __builtin_bit_cast(aotx_h2, __builtin_amdgcn_cvt_pkrtz(x[2] - (float)b[0], x[3] - (float)b[1]));
+    *hi = aotx_h4{a[0], a[1], b[0], b[1]};
+    *lo = aotx_h4{c[0], c[1], d[0], d[1]};
+}
+
 static __device__ __forceinline__ aotx_f4 aotx_mma(aotx_h8 a, aotx_h8 b, aotx_f4 c)
 {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -98,21 +112,46 @@ static __device__ __forceinline__ unsigned int aotx_delta_place(unsigned int j)
     return (j & ~31u) + ((j >> 2) & 3u) * 8u + ((j >> 4) & 1u) * 4u + (j & 3u);
 }
 
+/* Rows r0 .. r0 + n - 1 of a call's qkv: what is read past them is zeros. */
+struct aotx_rows_view {
+    __amdgpu_buffer_rsrc_t rs;
+};
+static __device__ __forceinline__ aotx_rows_view aotx_rows_of(const aotx_delta_args &p, unsigned int r0, unsigned int n)
+{
+    aotx_rows_view v;
+    v.rs = __builtin_amdgcn_make_buffer_rsrc((void *)(p.qkv + (unsigned long long)r0 * p.stride), (short)0,
+                                             (int)(n * p.stride * 2u), 0x00020000);
+    return v;
+}
+static __device__ __forceinline__ aotx_h8 aotx_rows_16(const aotx_rows_view &v, unsigned int at)
+{
+    return __builtin_bit_cast(aotx_h8, __builtin_amdgcn_raw_buffer_load_b128(v.rs, (int)at, 0, 0));
+}
+static __device__ __forceinline__ unsigned short aotx_rows_2(const aotx_rows_view &v, unsigned int at)
+{
+    return __builtin_amdgcn_raw_buffer_load_b16(v.rs, (int)at, 0, 0);
+}
+
 /* ---------------------------------------------------------------------------------------
  * T, P, K^T and the row factors of one chunk and head; a workgroup of four waves, wave w has
- * rows 16 w .. 16 w + 15.
+ * rows 16 w .. 16 w + 15. The products are taken transposed (K_j Q_i^T), so that a lane holds
+ * one row i and four columns j along its registers, as the operands above need them.
  * ------------------------------------------------------------------------------------- */
 template <int D>
 __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
 {
     constexpr int KS = D / 32;
-    __shared__ aotx_h8 kfrag[4][KS][64];
+    __shared__ union {
+        aotx_h8 kfrag[4][KS][64];                           /* rows of K, as operands */
+        __align__(16) unsigned short tp[2][64][72];         /* T, to be read by rows */
+    } lds;
     __shared__ __align__(16) float M[64][68];
     __shared__ __align__(16) float Dm[4][16][20];
-    __shared__ __align__(16) unsigned short tp[2][64][72];
-    __shared__ float ghi[64], glo[64], beta[64], rk[64], rq[64], ks[64];
-    __shared__ unsigned int badk[4], badg;
-    const unsigned int lane = threadIdx.x & 63u, w = threadIdx.x >> 6, m = lane & 15u, g = lane >> 4;
+    __shared__ __align__(16) float ghi[64], glo[64], beta[64], rk[64], rq[64], ks[64], near_end[64];
+    __shared__ __align__(16) unsigned int vm[4][64];
+    __shared__ unsigned int badk[4], badv[4], badg;
+    const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4;
+    const unsigned int w = (unsigned int)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const unsigned int c = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
 
     unsigned int b, e, mine, before;
@@ -124,75 +163,108 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
     if (seq.refused) return;
     const unsigned int r0 = seq.start + (c - (unsigned int)__builtin_amdgcn_readlane((int)before, (int)i)) * 64u;
     const unsigned int n = seq.end - r0 < 64u ? seq.end - r0 : 64u;
+    aotx_delta_chunk_work *to = p.work + (unsigned long long)c * p.heads + h;
 
-    /* rows of K and Q, 8 columns 32 s + 8 g .. of row 16 w + m */
+    /* rows of K and Q, columns 32 s + 8 g .. of row 16 w + m; rows past the chunk read as zeros */
     const unsigned int kh = h / p.group;
     const unsigned int row = 16u * w + m;
+    const aotx_rows_view rows = aotx_rows_of(p, r0, n);
+    const unsigned int at_q = row * p.stride * 2u + (kh * D + 8u * g) * 2u, at_k = at_q + p.key_heads * D * 2u;
     aotx_h8 kf[KS], qf[KS];
-    float kk = 0.0f, qq = 0.0f;
-    {
-        const unsigned short *q = p.qkv + (unsigned long long)(r0 + (row < n ? row : n - 1u)) * p.stride + kh * D + 8u * g;
-        const unsigned short *k = q + (unsigned long long)p.key_heads * D;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            kf[s] = aotx_h8_of(*(const aotx_u16x8 *)(k + 32 * s));
-            qf[s] = aotx_h8_of(*(const aotx_u16x8 *)(q + 32 * s));
-        }
-    }
-    /* gates, a row a lane (every wave for itself; wave 0 keeps them) */
-    const unsigned int gr = r0 + (lane < n ? lane : n - 1u);
-    float gate = aotx_delta_gate(p.a[(unsigned long long)gr * p.ab_stride + h], p.dt[h], p.decay[h]);
-    float rate = 1.0f / (1.0f + expf(-p.b[(unsigned long long)gr * p.ab_stride + h]));
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int v = 0; v < 8; ++v) {
-            kk += (float)kf[s][v] * (float)kf[s][v];
-            qq += (float)qf[s][v] * (float)qf[s][v];
-        }
-    kk += __shfl_xor(kk, 16, 64);
-    kk += __shfl_xor(kk, 32, 64);
-    qq += __shfl_xor(qq, 16, 64);
-    qq += __shfl_xor(qq, 32, 64);
-    const bool out_of = row >= n, bad = !out_of && !(kk < __builtin_inff());
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-        if (out_of || bad) kf[s] = aotx_h8{0, 0, 0, 0, 0, 0, 0, 0};
-        if (out_of) qf[s] = aotx_h8{0, 0, 0, 0, 0, 0, 0, 0};
-        kfrag[w][s][lane] = kf[s];
+        kf[s] = aotx_rows_16(rows, at_k + 64u * s);
+        qf[s] = aotx_rows_16(rows, at_q + 64u * s);
     }
-    const unsigned long long badrows = __ballot(bad) & 0xFFFFull;
-    if (lane == 0u) badk[w] = badrows != 0ull ? 16u * w + (unsigned int)__builtin_ctzll(badrows) : 64u;
-    if (g == 0u) {
-        if (out_of || bad) kk = 0.0f;
-        if (out_of) qq = 0.0f;
-        const float len = sqrtf(kk + p.eps);
-        int ex;
-        (void)frexpf(len, &ex);
-        rk[row] = 1.0f / len;
-        ks[row] = ldexpf(1.0f, -ex);
-        rq[row] = 1.0f / sqrtf(qq + p.eps) * (D == 128 ? 0.08838834764831845f : 0.125f);
-    }
-    {
+    /* V: eight columns of every 256 / (D / 8)-th row a thread */
+    constexpr unsigned int VR = 256 / (D / 8);
+    aotx_u16x8 vv[64 / VR];
+#pragma unroll
+    for (unsigned int r = 0; r < 64u / VR; ++r)
+        vv[r] = __builtin_bit_cast(aotx_u16x8, aotx_rows_16(rows, (r * VR + threadIdx.x / (D / 8)) * p.stride * 2u
+                                   + (2u * p.key_heads * D + h * D + threadIdx.x % (D / 8) * 8u) * 2u));
+    /* gates, a row a lane; sums of g in 64 bits, kept as two floats, so that differences of far
+     * sums stay exact */
+    if (w == 0u) {
+        const unsigned int gr = r0 + (lane < n ? lane : n - 1u);
+        float gate = aotx_delta_gate(p.a[(unsigned long long)gr * p.ab_stride + h], p.dt[h], p.decay[h]);
+        float rate = 1.0f / (1.0f + expf(-p.b[(unsigned long long)gr * p.ab_stride + h]));
         const bool badgate = lane < n && (gate != gate || rate != rate);
         const unsigned long long badgates = __ballot(badgate);
         if (lane >= n || badgate) gate = rate = 0.0f;
-        /* sums of g in 64 bits, kept as two floats: differences of far sums stay exact */
         double sum = (double)gate;
         for (unsigned int off = 1u; off < 64u; off <<= 1) {
             const double o = __shfl_up(sum, off, 64);
             if (lane >= off) sum += o;
         }
-        if (w == 0u) {
-            ghi[lane] = (float)sum;
-            glo[lane] = (float)(sum - (double)(float)sum);
-            beta[lane] = rate;
-            if (lane == 0u) badg = badgates != 0ull ? (unsigned int)__builtin_ctzll(badgates) : 64u;
+        ghi[lane] = (float)sum;
+        glo[lane] = (float)(sum - (double)(float)sum);
+        near_end[lane] = expf((float)(__shfl(sum, (int)(lane | 15u), 64) - sum));
+        beta[lane] = rate;
+        if (lane == 0u) badg = badgates != 0ull ? (unsigned int)__builtin_ctzll(badgates) : 64u;
+    }
+    float kk = 0.0f, qq = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int v = 0; v < 8; v += 2) {
+            const aotx_h2 k2 = {kf[s][v], kf[s][v + 1]}, q2 = {qf[s][v], qf[s][v + 1]};
+            kk = __builtin_amdgcn_fdot2(k2, k2, kk, false);
+            qq = __builtin_amdgcn_fdot2(q2, q2, qq, false);
         }
+    kk += __shfl_xor(kk, 16, 64);
+    kk += __shfl_xor(kk, 32, 64);
+    qq += __shfl_xor(qq, 16, 64);
+    qq += __shfl_xor(qq, 32, 64);
+    const bool bad = !(kk < __builtin_inff());
+    if (bad) kk = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        if (bad) kf[s] = aotx_h8{0, 0, 0, 0, 0, 0, 0, 0};
+        lds.kfrag[w][s][lane] = kf[s];
+    }
+    const unsigned long long badrows = __ballot(bad) & 0xFFFFull;
+    if (lane == 0u) badk[w] = badrows != 0ull ? 16u * w + (unsigned int)__builtin_ctzll(badrows) : 64u;
+    const float len = sqrtf(kk + p.eps), inv = 1.0f / len;
+    const float qinv = 1.0f / sqrtf(qq + p.eps) * (D == 128 ? 0.08838834764831845f : 0.125f);
+    if (g == 0u) {
+        int ex;
+        (void)frexpf(len, &ex);
+        rk[row] = inv;
+        ks[row] = ldexpf(1.0f, -ex);
+        rq[row] = qinv;
+    }
+    /* the largest size of V's columns: sizes of fp16 are in the order of their bits. What is no
+     * number is left out, and told of. */
+    {
+        aotx_u16x8 top = vv[0] & (unsigned short)0x7FFF;
+#pragma unroll
+        for (unsigned int r = 1; r < 64u / VR; ++r) top = __builtin_elementwise_max(top, vv[r] & (unsigned short)0x7FFF);
+        const bool none = __builtin_reduce_max(top) >= 0x7C00;
+        if (none) {
+            top = aotx_u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (unsigned int r = 0; r < 64u / VR; ++r)
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const unsigned short v = vv[r][x] & 0x7FFF;
+                    if (v < 0x7C00 && v > top[x]) top[x] = v;
+                }
+        }
+        const unsigned long long told = __ballot(none);
+        if (lane == 0u) badv[w] = told != 0ull ? 1u : 0u;
+        typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (unsigned int off = D / 8; off < 64u; off <<= 1) {
+            u4 o = __builtin_bit_cast(u4, top);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[x] = (unsigned int)__shfl_xor((int)o[x], off, 64);
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(aotx_u16x8, o));
+        }
+        if (lane < D / 8) *(aotx_u16x8 *)((unsigned short *)vm[w] + lane * 8u) = top;
     }
     __syncthreads();
 
-    aotx_delta_chunk_work *to = p.work + (unsigned long long)c * p.heads + h;
     if (w == 0u) {
         const float last = (ghi[63] - ghi[lane]) + (glo[63] - glo[lane]), all = expf(ghi[lane]);
         to->of_k[lane] = all * rk[lane];
@@ -204,47 +276,62 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
             to->fade = expf(ghi[63]);
             to->bad = first;
         }
+    } else if (w == 1u) {
+        if (lane < D / 2) {             /* two columns a lane */
+            typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+            u2 v = __builtin_bit_cast(u2, vm[0][lane]);
+#pragma unroll
+            for (int x = 1; x < 4; ++x) v = __builtin_elementwise_max(v, __builtin_bit_cast(u2, vm[x][lane]));
+            *(unsigned short *)&to->vmax[2u * lane] = (unsigned short)((v[0] >> 10) | ((v[1] >> 10) << 8));
+        }
+        if (lane == 0u) to->badv = badv[0] | badv[1] | badv[2] | badv[3];
     }
 
-    /* K K^T and Q K^T of this wave's rows, and M and P from them */
-    const unsigned int i0 = 16u * w + 4u * g;
-    const aotx_f4 gi = *(const aotx_f4 *)&ghi[i0], gl = *(const aotx_f4 *)&glo[i0], bi = *(const aotx_f4 *)&beta[i0],
-                  rki = *(const aotx_f4 *)&rk[i0], rqi = *(const aotx_f4 *)&rq[i0];
+    /* P and M of row 16 w + m. Between blocks, exp(G_i - G_j) is the product of two factors by
+     * way of the last row of j's block: both are at most 1, and one exponential a row serves
+     * four columns. */
+    const float gi = ghi[row], gil = glo[row], bi = beta[row] * inv;
+    aotx_f4 pt[4];
 #pragma unroll
     for (unsigned int jt = 0; jt < 4u; ++jt) {
-        const unsigned int j = 16u * jt + m, at = aotx_delta_place(j);
-        if (jt > w) {
-            if (jt == (w | 1u))
-#pragma unroll
-                for (int r = 0; r < 4; ++r) tp[0][i0 + r][at] = tp[1][i0 + r][at] = 0;
-            continue;
-        }
+        pt[jt] = aotx_f4{0, 0, 0, 0};
+        if (jt > w) continue;
         aotx_f4 kks = {0, 0, 0, 0}, qks = {0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            const aotx_h8 kj = kfrag[jt][s][lane];
-            kks = aotx_mma(kf[s], kj, kks);
-            qks = aotx_mma(qf[s], kj, qks);
+            const aotx_h8 kj = lds.kfrag[jt][s][lane];
+            kks = aotx_mma(kj, kf[s], kks);
+            qks = aotx_mma(kj, qf[s], qks);
         }
-        const float gj = ghi[j], gjl = glo[j], rkj = rk[j];
+        const unsigned int j0 = 16u * jt + 4u * g;
+        const aotx_f4 rkj = *(const aotx_f4 *)&rk[j0];
+        aotx_f4 fade;
+        if (jt == w) {
+            const aotx_f4 gj = *(const aotx_f4 *)&ghi[j0], gjl = *(const aotx_f4 *)&glo[j0];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const unsigned int ii = i0 + r;
-            const float fade = expf((gi[r] - gj) + (gl[r] - gjl)) * rkj;
-            M[ii][j] = ii > j ? bi[r] * rki[r] * kks[r] * fade : 0.0f;
-            _Float16 hi, lo;
-            aotx_split(ii >= j ? rqi[r] * qks[r] * fade : 0.0f, &hi, &lo);
-            tp[0][ii][at] = __builtin_bit_cast(unsigned short, hi);
-            tp[1][ii][at] = __builtin_bit_cast(unsigned short, lo);
+            for (int r = 0; r < 4; ++r) {
+                fade[r] = expf((gi - gj[r]) + (gil - gjl[r])) * rkj[r];
+                kks[r] = row > j0 + r ? kks[r] : 0.0f;
+                qks[r] = row >= j0 + r ? qks[r] : 0.0f;
+                fade[r] = row >= j0 + r ? fade[r] : 0.0f;
+            }
+        } else {
+            const float from = expf((gi - ghi[16u * jt + 15u]) + (gil - glo[16u * jt + 15u]));
+            fade = *(const aotx_f4 *)&near_end[j0] * rkj * from;
         }
+        *(aotx_f4 *)&M[row][j0] = kks * fade * bi;
+        pt[jt] = qks * fade * qinv;
     }
-    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (unsigned int s = 0; s < 2u; ++s) {
         if (s > w / 2u) continue;
-        to->p_hi[w][s][lane] = *(const aotx_h8 *)&tp[0][row][32u * s + 8u * g];
-        to->p_lo[w][s][lane] = *(const aotx_h8 *)&tp[1][row][32u * s + 8u * g];
+        aotx_h4 hi[2], lo[2];
+        aotx_split4(pt[2u * s], &hi[0], &lo[0]);
+        aotx_split4(pt[2u * s + 1u], &hi[1], &lo[1]);
+        to->p_hi[w][s][lane] = __builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        to->p_lo[w][s][lane] = __builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3, 4, 5, 6, 7);
     }
+    __builtin_amdgcn_wave_barrier();
 
     /* inverse of the diagonal block by substitution, a column a lane */
     {
@@ -259,6 +346,31 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
         if (g == 0u)
 #pragma unroll
             for (int r = 0; r < 16; ++r) Dm[w][r][m] = x[r];
+    }
+    /* K^T for the state's update: rows of the identity pick its columns, which come out with
+     * the rows of K along a lane's registers, the order that operand needs */
+    if (h % p.group == 0u) {
+        const unsigned int s = w & 1u;
+        aotx_h8 *kt = p.kt + ((unsigned long long)c * p.key_heads + kh) * (D / 16) * 2 * 64;
+        const aotx_f4 sc0 = *(const aotx_f4 *)&ks[32u * s + 4u * g], sc1 = *(const aotx_f4 *)&ks[32u * s + 16u + 4u * g];
+#pragma unroll
+        for (unsigned int v = 0; v < D / 32u; ++v) {
+            const unsigned int t = (w >> 1) * (D / 32u) + v, st = t >> 1;
+            aotx_h8 pick;
+#pragma unroll
+            for (unsigned int x = 0; x < 8u; ++x)
+                pick[x] = g == (m >> 2) && x == 4u * (t & 1u) + (m & 3u) ? (_Float16)1.0f : (_Float16)0.0f;
+            const aotx_f4 z = {0, 0, 0, 0};
+            const aotx_f4 k0 = aotx_mma(lds.kfrag[2u * s][st][lane], pick, z) * sc0;
+            const aotx_f4 k1 = aotx_mma(lds.kfrag[2u * s + 1u][st][lane], pick, z) * sc1;
+            aotx_h8 o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                o[r] = (_Float16)k0[r];
+                o[4 + r] = (_Float16)k1[r];
+            }
+            kt[(t * 2u + s) * 64u + lane] = o;
+        }
     }
     __syncthreads();
 
@@ -285,116 +397,73 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
         tc[off] = t;
     }
     {
-        const unsigned int j = 16u * w + m, at = aotx_delta_place(j);
-        const float bj = beta[j];
+        const unsigned int at = aotx_delta_place(row);
+        const float bj = beta[row];
 #pragma unroll
         for (unsigned int off = 0; off < 4u; ++off) {
             const unsigned int bt = w + off;
             if (bt > 3u) break;
+            aotx_h4 hi, lo;
+            aotx_split4(tc[off] * bj, &hi, &lo);
+            const aotx_u16x4 hb = __builtin_bit_cast(aotx_u16x4, hi), lb = __builtin_bit_cast(aotx_u16x4, lo);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                _Float16 hi, lo;
-                aotx_split(tc[off][r] * bj, &hi, &lo);
-                tp[0][16u * bt + 4u * g + r][at] = __builtin_bit_cast(unsigned short, hi);
-                tp[1][16u * bt + 4u * g + r][at] = __builtin_bit_cast(unsigned short, lo);
+                lds.tp[0][16u * bt + 4u * g + r][at] = hb[r];
+                lds.tp[1][16u * bt + 4u * g + r][at] = lb[r];
             }
         }
         if (w & 1u)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                tp[0][16u * (w - 1u) + 4u * g + r][at] = tp[1][16u * (w - 1u) + 4u * g + r][at] = 0;
-    }
-    /* K^T for the state's update: rows of the identity pick its columns, which come out with
-     * the rows of K along a lane's registers, the order that operand needs */
-    if (h % p.group == 0u) {
-        const unsigned int s = w & 1u;
-        aotx_h8 *kt = p.kt + ((unsigned long long)c * p.key_heads + kh) * (D / 16) * 2 * 64;
-#pragma unroll
-        for (unsigned int v = 0; v < D / 32u; ++v) {
-            const unsigned int t = (w >> 1) * (D / 32u) + v, st = t >> 1;
-            aotx_h8 pick;
-#pragma unroll
-            for (unsigned int x = 0; x < 8u; ++x)
-                pick[x] = g == (m >> 2) && x == 4u * (t & 1u) + (m & 3u) ? (_Float16)1.0f : (_Float16)0.0f;
-            aotx_h8 o;
-#pragma unroll
-            for (unsigned int half = 0; half < 2u; ++half) {
-                const aotx_f4 acc = aotx_mma(kfrag[2u * s + half][st][lane], pick, aotx_f4{0, 0, 0, 0});
-                const aotx_f4 sc = *(const aotx_f4 *)&ks[32u * s + 16u * half + 4u * g];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[4 * half + r] = (_Float16)(acc[r] * sc[r]);
-            }
-            kt[(t * 2u + s) * 64u + lane] = o;
-        }
+                lds.tp[0][16u * (w - 1u) + 4u * g + r][at] = lds.tp[1][16u * (w - 1u) + 4u * g + r][at] = 0;
     }
     __syncthreads();
 #pragma unroll
     for (unsigned int s = 0; s < 2u; ++s) {
         if (s > w / 2u) continue;
-        to->t_hi[w][s][lane] = *(const aotx_h8 *)&tp[0][row][32u * s + 8u * g];
-        to->t_lo[w][s][lane] = *(const aotx_h8 *)&tp[1][row][32u * s + 8u * g];
+        to->t_hi[w][s][lane] = *(const aotx_h8 *)&lds.tp[0][row][32u * s + 8u * g];
+        to->t_lo[w][s][lane] = *(const aotx_h8 *)&lds.tp[1][row][32u * s + 8u * g];
     }
 }
 
 /* ---------------------------------------------------------------------------------------
- * The walk over a sequence's chunks. A workgroup has 16 NT columns of one head's S: wave w the
- * rows of S that one step of K S takes (D / 4 of them, in accumulators), and rows 16 w ..
- * 16 w + 15 of the chunk. S, X and U pass between the waves through LDS as operands, a barrier
- * each; everything else a chunk needs is loaded into registers while the one before is worked on.
+ * The walk over a sequence's chunks. A workgroup has 16 NT columns of one head's S. Waves 0 to
+ * 3 carry the state: wave w has the rows of S that one step of K S takes (D / 4 of them, in
+ * accumulators), and rows 16 w .. 16 w + 15 of the chunk. Waves 4 to 7 make the output of the
+ * same rows from what the others lay out. S, X and U pass through LDS as operands, a barrier
+ * each; everything else a chunk needs is loaded into registers two chunks ahead, each register
+ * as soon as it has been used.
  * Row x of tile t of S is key 32 (t / 2) + 8 (x / 4) + 4 (t % 2) + x % 4, so that two tiles'
  * accumulators hold keys 8 g .. 8 g + 7 of a step, as 16 bytes of a row of K do.
  * ------------------------------------------------------------------------------------- */
-template <int D, int NT>
-struct aotx_delta_tile {
-    static constexpr int KS = D / 32, TW = D / 64;
-    aotx_h8 k[KS], q[KS], th[2], tl[2], ph[2], pl[2], kt[TW][2];
-    unsigned short v[4][NT];
-    aotx_f4 of_k, of_q, of_u;
-    float fade;
-    unsigned int bad;
-};
+#define AOTX_DELTA_PERIOD 4u        /* chunks for which a column's scale holds */
 
 template <int D, int NT>
-static __device__ __forceinline__ void aotx_delta_load(aotx_delta_tile<D, NT> &x, const aotx_delta_args &p,
-                                                       unsigned int c, unsigned int r0, unsigned int n, unsigned int h,
-                                                       unsigned int col, unsigned int w, unsigned int m, unsigned int g)
+struct aotx_delta_lds {
+    aotx_h8 s[D / 32][2][NT][64];           /* step of keys, part, tile of columns */
+    aotx_h8 x[2][2][NT][64];                /* step of rows, part, tile of columns */
+    aotx_h8 u[2][2][NT][64], v[2][2][NT][64];   /* U, and U with the state update's factors */
+    int size[4][16 * NT];                   /* exponents of the state's columns, by wave */
+    unsigned int bad[4][16 * NT];           /* first bad rows of V's columns, by wave */
+};
+
+/* What both kinds of waves know. */
+struct aotx_delta_walk {
+    aotx_seq_view seq;
+    unsigned int c0, chunks, h, col, w, m, g, lane;
+};
+
+/* The chunk that is loaded `ahead` of c: the last one again past the end, so that every pass
+ * has the same loads in flight. */
+static __device__ __forceinline__ unsigned int aotx_delta_ahead(const aotx_delta_walk &k, unsigned int c)
 {
-    constexpr int KS = D / 32, TW = D / 64;
-    const unsigned int lane = 16u * g + m, kh = h / p.group;
-    const unsigned int row = 16u * w + m;
-    const unsigned short *q = p.qkv + (unsigned long long)(r0 + (row < n ? row : n - 1u)) * p.stride + kh * D + 8u * g;
-    const unsigned short *k = q + (unsigned long long)p.key_heads * D;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        x.k[s] = aotx_h8_of(*(const aotx_u16x8 *)(k + 32 * s));
-        x.q[s] = aotx_h8_of(*(const aotx_u16x8 *)(q + 32 * s));
-    }
-    const aotx_delta_chunk_work *from = p.work + (unsigned long long)c * p.heads + h;
-#pragma unroll
-    for (unsigned int s = 0; s < 2u; ++s) {
-        if (s > w / 2u) continue;
-        x.th[s] = from->t_hi[w][s][lane];
-        x.tl[s] = from->t_lo[w][s][lane];
-        x.ph[s] = from->p_hi[w][s][lane];
-        x.pl[s] = from->p_lo[w][s][lane];
-    }
-    const aotx_h8 *kt = p.kt + ((unsigned long long)c * p.key_heads + kh) * (D / 16) * 2 * 64;
-#pragma unroll
-    for (int t = 0; t < TW; ++t)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) x.kt[t][s] = kt[((w * TW + t) * 2 + s) * 64u + lane];
-    const unsigned int i0 = 16u * w + 4u * g;
-    const unsigned short *v = p.qkv + 2ull * p.key_heads * D + (unsigned long long)h * D + col;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-            x.v[r][t] = v[(unsigned long long)(r0 + (i0 + r < n ? i0 + r : n - 1u)) * p.stride + t];
-    x.of_k = *(const aotx_f4 *)&from->of_k[i0];
-    x.of_q = *(const aotx_f4 *)&from->of_q[i0];
-    x.of_u = *(const aotx_f4 *)&from->of_u[i0];
-    x.fade = from->fade;
-    x.bad = from->bad;
+    return c + 2u < k.chunks ? c + 2u : k.chunks - 1u;
+}
+
+static __device__ __forceinline__ unsigned int aotx_delta_left(const aotx_delta_walk &k, unsigned int c)
+{
+    const unsigned int n = k.seq.end - k.seq.start - c * 64u;
+    return n < 64u ? n : 64u;
 }
 
 /* exponent of |x|: |x| < 2^(e + 1) */
@@ -403,43 +472,91 @@ static __device__ __forceinline__ int aotx_exponent(float x)
     return (int)((__float_as_uint(x) >> 23) & 0xFFu) - 127;
 }
 
-template <int D, int NT>
-__global__ __launch_bounds__(256) void aotx_delta_across(aotx_delta_args p)
+/* Scales of a period: the exponents that the four waves left, as a shift of at most 100. */
+template <int NT>
+static __device__ __forceinline__ int aotx_delta_shift(const int (*size)[16 * NT], unsigned int at)
 {
-    constexpr int KS = D / 32, TW = D / 64, SLICES = D / (16 * NT);
-    __shared__ aotx_h8 Sx[KS][2][NT][64];           /* step of keys, part, tile of columns */
-    __shared__ aotx_h8 Xx[2][2][NT][64];            /* step of rows, part, tile of columns */
-    __shared__ aotx_h8 Ux[2][2][NT][64], Vx[2][2][NT][64];
-    __shared__ int post[2][4][16 * NT];             /* exponents, first bad rows; by wave */
-    const unsigned int lane = threadIdx.x & 63u, w = threadIdx.x >> 6, m = lane & 15u, g = lane >> 4;
-    /* the slices of a head go to one XCD (workgroup b runs on XCD b % 8), whose L2 then holds
-     * what they share */
-    const unsigned int units = p.seqs.seqs * p.heads;
-    const unsigned int unit = blockIdx.x / (8u * SLICES) * 8u + blockIdx.x % 8u;
-    const unsigned int slice = blockIdx.x / 8u % SLICES;
-    if (unit >= units) return;
-    const unsigned int i = unit / p.heads, h = unit % p.heads;
-    unsigned int b, e, mine, before;
-    aotx_seq_rows(p.seqs, &b, &e);
-    aotx_delta_chunks(b, e, &mine, &before);
-    const aotx_seq_view seq = aotx_seq_of(p.seqs, i, b, e);
-    const unsigned int c0 = (unsigned int)__builtin_amdgcn_readlane((int)before, (int)i);
-    if (seq.start >= seq.end) return;
-    const unsigned int col = slice * 16u * NT + m * NT;     /* this lane's NT columns */
-    const unsigned long long width = (unsigned long long)p.heads * D;
-    unsigned short *out = p.out + (unsigned long long)h * D + col;
-    if (seq.refused) {
-        if (threadIdx.x == 0u && slice == 0u && h == 0u) atomicAdd(p.seqs.faults, 1u);
-        for (unsigned int t = seq.start + threadIdx.x / 16u; t < seq.end; t += 16u)
+    int ex = size[0][at];
 #pragma unroll
-            for (int u = 0; u < NT; ++u) out[t * width + u] = 0;
-        return;
-    }
-    const unsigned int chunks = (seq.end - seq.start + 63u) / 64u;
-    const unsigned int i0 = 16u * w + 4u * g;
+    for (int v = 1; v < 4; ++v) ex = size[v][at] > ex ? size[v][at] : ex;
+    ex = 14 - ex;
+    return ex > 100 ? 100 : ex < -100 ? -100 : ex;
+}
 
-    aotx_f4 S[TW][NT];
-    float *sp = p.state + ((unsigned long long)seq.slot * p.heads + h) * D * D + col;
+template <int NT>
+static __device__ __forceinline__ unsigned int aotx_delta_first(const unsigned int (*bad)[16 * NT], unsigned int at)
+{
+    unsigned int first = bad[0][at];
+#pragma unroll
+    for (int v = 1; v < 4; ++v) first = bad[v][at] < first ? bad[v][at] : first;
+    return first;
+}
+
+/* ---- waves 0 to 3 ---- */
+template <int D, int NT>
+struct aotx_delta_state_tile {
+    aotx_h8 k[D / 32], th[2], tl[2], kt[D / 64][2];
+    unsigned short v[4][NT];
+    aotx_f4 of_k, of_u;
+    float fade;
+    unsigned int bad, badv;
+};
+
+template <int D, int NT>
+static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p, const aotx_delta_walk k,
+                                                        aotx_delta_lds<D, NT> &lds)
+{
+    constexpr int KS = D / 32, TW = D / 64;
+    typedef aotx_delta_state_tile<D, NT> tile_t;
+    const unsigned int w = k.w, g = k.g, lane = k.lane, i0 = 16u * w + 4u * g, kh = k.h / p.group;
+    const unsigned int at_k = (16u * w + k.m) * p.stride * 2u + (p.key_heads * D + kh * D + 8u * g) * 2u;
+    const unsigned int at_v = i0 * p.stride * 2u + (2u * p.key_heads * D + k.h * D + k.col) * 2u;
+    auto from = [&](unsigned int c) { return p.work + (unsigned long long)(k.c0 + c) * p.heads + k.h; };
+    auto load_k = [&](tile_t &x, unsigned int c) {
+        const aotx_rows_view rows = aotx_rows_of(p, k.seq.start + c * 64u, aotx_delta_left(k, c));
+#pragma unroll
+        for (int s = 0; s < KS; ++s) x.k[s] = aotx_rows_16(rows, at_k + 64u * s);
+    };
+    auto load_t = [&](tile_t &x, unsigned int c) {
+        const aotx_delta_chunk_work *f = from(c);
+#pragma unroll
+        for (unsigned int s = 0; s < 2u; ++s) {
+            x.th[s] = f->t_hi[w][s][lane];
+            x.tl[s] = f->t_lo[w][s][lane];
+        }
+    };
+    auto load_kt = [&](tile_t &x, unsigned int c) {
+        const aotx_h8 *kt = p.kt + (((unsigned long long)(k.c0 + c) * p.key_heads + kh) * (D / 16) + w * TW) * 2 * 64;
+#pragma unroll
+        for (int t = 0; t < TW; ++t)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) x.kt[t][s] = kt[(t * 2 + s) * 64 + lane];
+    };
+    auto load_rest = [&](tile_t &x, unsigned int c) {
+        const aotx_rows_view rows = aotx_rows_of(p, k.seq.start + c * 64u, aotx_delta_left(k, c));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int u = 0; u < NT; ++u) x.v[r][u] = aotx_rows_2(rows, at_v + r * p.stride * 2u + 2u * u);
+        const aotx_delta_chunk_work *f = from(c);
+        x.of_k = *(const aotx_f4 *)&f->of_k[i0];
+        x.of_u = *(const aotx_f4 *)&f->of_u[i0];
+        x.fade = f->fade;
+        x.bad = f->bad;
+        x.badv = f->badv;
+    };
+    unsigned char top[AOTX_DELTA_PERIOD][NT];       /* V's exponents in the coming period */
+    auto load_top = [&](unsigned int c) {
+#pragma unroll
+        for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q)
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+                top[q][u] = from(c + q < k.chunks ? c + q : k.chunks - 1u)->vmax[k.col + u];
+    };
+
+    aotx_f4 S[TW][NT];                              /* times 2^shift */
+    int shift[NT];
+    float *sp = p.state + ((unsigned long long)k.seq.slot * p.heads + k.h) * D * D + k.col;
 #pragma unroll
     for (int t = 0; t < TW; ++t)
 #pragma unroll
@@ -447,203 +564,152 @@ __global__ __launch_bounds__(256) void aotx_delta_across(aotx_delta_args p)
             const unsigned int tile = w * TW + t;
             const unsigned int key = 32u * (tile >> 1) + 8u * g + 4u * (tile & 1u) + r;
 #pragma unroll
-            for (int u = 0; u < NT; ++u) S[t][u][r] = seq.fresh ? 0.0f : sp[key * D + u];
-        }
-
-    aotx_delta_tile<D, NT> now, next;
-    aotx_delta_load<D, NT>(now, p, c0, seq.start, seq.end - seq.start < 64u ? seq.end - seq.start : 64u, h, col, w, m, g);
-
-    /* This wave's share of the next chunk's column scales and bad rows, into `post`. */
-    auto tell = [&](const aotx_delta_tile<D, NT> &x, unsigned int n, const aotx_f4 (&s)[TW][NT], const int (&floor)[NT],
-                    int (&own)[NT]) {
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            float ms = 0.0f, mv = 0.0f;
-            unsigned int first = 64u;
-#pragma unroll
-            for (int t = 0; t < TW; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) ms = fmaxf(ms, fabsf(s[t][u][r]));
-#pragma unroll
-            for (int r = 3; r >= 0; --r) {
-                const float v = fabsf(aotx_h2f(x.v[r][u]));
-                if (v < __builtin_inff()) mv = fmaxf(mv, v);
-                else if (i0 + r < n) first = i0 + r;
-            }
-            ms = fmaxf(ms, __shfl_xor(ms, 16, 64));
-            ms = fmaxf(ms, __shfl_xor(ms, 32, 64));
-            mv = fmaxf(mv, __shfl_xor(mv, 16, 64));
-            mv = fmaxf(mv, __shfl_xor(mv, 32, 64));
-            unsigned int o = (unsigned int)__shfl_xor((int)first, 16, 64);
-            first = o < first ? o : first;
-            o = (unsigned int)__shfl_xor((int)first, 32, 64);
-            first = o < first ? o : first;
-            own[u] = aotx_exponent(mv) + 8;
-            int ex = aotx_exponent(ms) + 5;
-            ex = ex > own[u] ? ex : own[u];
-            ex = ex > floor[u] ? ex : floor[u];
-            if (g == 0u) {
-                post[0][w][m * NT + u] = ex;
-                post[1][w][m * NT + u] = (int)first;
+            for (int u = 0; u < NT; ++u) {
+                S[t][u][r] = k.seq.fresh ? 0.0f : sp[key * D + u];
+                shift[u] = 0;
             }
         }
-    };
-    float up[NT], down[NT];             /* this chunk's column scales, a power of two and its inverse */
-    unsigned int badv[NT];
-    auto heard = [&]() {
+    tile_t A, B;
+    load_top(0u);
+    load_k(A, 0u);
+    load_rest(A, 0u);
+    load_t(A, 0u);
+    load_kt(A, 0u);
+    const unsigned int c1 = k.chunks > 1u ? 1u : 0u;
+    load_k(B, c1);
+    load_rest(B, c1);
+    load_t(B, c1);
+    load_kt(B, c1);
+
+    auto pass = [&](tile_t &x, unsigned int c) {
+        const unsigned int n = aotx_delta_left(k, c), far = aotx_delta_ahead(k, c);
+        if (c % AOTX_DELTA_PERIOD == 0u) {
+            /* |U| and |S| of a column stay below sqrt(d) max|S| + (64 periods + 1) max|V| */
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            int ex = post[0][0][m * NT + u];
-            unsigned int first = (unsigned int)post[1][0][m * NT + u];
+            for (int u = 0; u < NT; ++u) {
+                float ms = 0.0f;
 #pragma unroll
-            for (int v = 1; v < 4; ++v) {
-                const int o = post[0][v][m * NT + u];
-                ex = o > ex ? o : ex;
-                const unsigned int f = (unsigned int)post[1][v][m * NT + u];
-                first = f < first ? f : first;
+                for (int t = 0; t < TW; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) ms = fmaxf(ms, fabsf(S[t][u][r]));
+                ms = fmaxf(ms, __shfl_xor(ms, 16, 64));
+                ms = fmaxf(ms, __shfl_xor(ms, 32, 64));
+                int ex = aotx_exponent(ms) - shift[u] + 5, ev = 0;
+#pragma unroll
+                for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q) ev = top[q][u] > ev ? top[q][u] : ev;
+                ev += 10 - 15;
+                ex = ex > ev ? ex : ev;
+                if (g == 0u) lds.size[w][k.m * NT + u] = ex;
             }
-            ex = 14 - ex;
-            ex = ex > 100 ? 100 : ex < -100 ? -100 : ex;
-            up[u] = __uint_as_float((unsigned int)(ex + 127) << 23);
-            down[u] = __uint_as_float((unsigned int)(127 - ex) << 23);
-            badv[u] = first;
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                const int to = aotx_delta_shift<NT>(lds.size, k.m * NT + u);
+#pragma unroll
+                for (int t = 0; t < TW; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[t][u][r] = ldexpf(S[t][u][r], to - shift[u]);
+                shift[u] = to;
+            }
+            load_top(c + AOTX_DELTA_PERIOD);
         }
-    };
-    int vex[NT], none[NT];
+        unsigned int lim[NT];
 #pragma unroll
-    for (int u = 0; u < NT; ++u) none[u] = -1000;
-    tell(now, seq.end - seq.start < 64u ? seq.end - seq.start : 64u, S, none, vex);
-    __syncthreads();
-    heard();
-
-    for (unsigned int c = 0; c < chunks; ++c) {
-        const unsigned int r0 = seq.start + c * 64u;
-        const unsigned int n = seq.end - r0 < 64u ? seq.end - r0 : 64u;
-        const bool more = c + 1u < chunks;
-        const unsigned int n1 = !more ? 0u : seq.end - r0 - 64u < 64u ? seq.end - r0 - 64u : 64u;
-        if (more) aotx_delta_load<D, NT>(next, p, c0 + c + 1u, r0 + 64u, n1, h, col, w, m, g);
-
-        /* S as an operand */
+        for (int u = 0; u < NT; ++u) lim[u] = x.bad;
+        if (x.badv != 0u) {
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
+            for (int u = 0; u < NT; ++u) {
+                unsigned int first = 64u;
+#pragma unroll
+                for (int r = 3; r >= 0; --r)
+                    if ((x.v[r][u] & 0x7FFFu) >= 0x7C00u) first = i0 + r;
+                unsigned int o = (unsigned int)__shfl_xor((int)first, 16, 64);
+                first = o < first ? o : first;
+                o = (unsigned int)__shfl_xor((int)first, 32, 64);
+                first = o < first ? o : first;
+                if (g == 0u) lds.bad[w][k.m * NT + u] = first;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                const unsigned int first = aotx_delta_first<NT>(lds.bad, k.m * NT + u);
+                lim[u] = first < lim[u] ? first : lim[u];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
 #pragma unroll
             for (int t = 0; t < TW; ++t) {
                 aotx_h4 hi, lo;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    _Float16 a, z;
-                    aotx_split(S[t][u][r] * up[u], &a, &z);
-                    hi[r] = a;
-                    lo[r] = z;
-                }
+                aotx_split4(S[t][u], &hi, &lo);
                 const unsigned int tile = w * TW + t;
-                *((aotx_h4 *)&Sx[tile >> 1][0][u][lane] + (tile & 1u)) = hi;
-                *((aotx_h4 *)&Sx[tile >> 1][1][u][lane] + (tile & 1u)) = lo;
+                *((aotx_h4 *)&lds.s[tile >> 1][0][u][lane] + (tile & 1u)) = hi;
+                *((aotx_h4 *)&lds.s[tile >> 1][1][u][lane] + (tile & 1u)) = lo;
             }
-        }
         __syncthreads();
-        aotx_f4 x[NT], o[NT];
-        unsigned int lim[NT];
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            aotx_f4 ks = {0, 0, 0, 0}, kl = {0, 0, 0, 0}, qs = {0, 0, 0, 0}, ql = {0, 0, 0, 0};
+            aotx_f4 a = {0, 0, 0, 0}, l = {0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                const aotx_h8 hi = Sx[s][0][u][lane], lo = Sx[s][1][u][lane];
-                ks = aotx_mma(now.k[s], hi, ks);
-                kl = aotx_mma(now.k[s], lo, kl);
-                qs = aotx_mma(now.q[s], hi, qs);
-                ql = aotx_mma(now.q[s], lo, ql);
+                a = aotx_mma(x.k[s], lds.s[s][0][u][lane], a);
+                l = aotx_mma(x.k[s], lds.s[s][1][u][lane], l);
             }
-            lim[u] = badv[u] < now.bad ? badv[u] : now.bad;
             const unsigned int upto = lim[u] < n ? lim[u] : n;
+            aotx_f4 y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                y[r] = ldexpf(aotx_h2f(x.v[r][u]), shift[u]) - x.of_k[r] * (a[r] + l[r]);
+                if (i0 + r >= upto) y[r] = 0.0f;
+            }
             aotx_h4 hi, lo;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                x[u][r] = i0 + r < upto ? aotx_h2f(now.v[r][u]) * up[u] - now.of_k[r] * (ks[r] + kl[r]) : 0.0f;
-                o[u][r] = now.of_q[r] * (qs[r] + ql[r]);
-                _Float16 a, z;
-                aotx_split(x[u][r], &a, &z);
-                hi[r] = a;
-                lo[r] = z;
-            }
-            *((aotx_h4 *)&Xx[w >> 1][0][u][lane] + (w & 1u)) = hi;
-            *((aotx_h4 *)&Xx[w >> 1][1][u][lane] + (w & 1u)) = lo;
+            aotx_split4(y, &hi, &lo);
+            *((aotx_h4 *)&lds.x[w >> 1][0][u][lane] + (w & 1u)) = hi;
+            *((aotx_h4 *)&lds.x[w >> 1][1][u][lane] + (w & 1u)) = lo;
         }
+        load_k(x, far);
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            aotx_f4 t = {0, 0, 0, 0}, tl = {0, 0, 0, 0};
+            aotx_f4 a = {0, 0, 0, 0}, l = {0, 0, 0, 0};
 #pragma unroll
             for (unsigned int s = 0; s < 2u; ++s) {
                 if (s > w / 2u) continue;
-                const aotx_h8 hi = Xx[s][0][u][lane], lo = Xx[s][1][u][lane];
-                t = aotx_mma(now.th[s], hi, t);
-                tl = aotx_mma(now.th[s], lo, tl);
-                tl = aotx_mma(now.tl[s], hi, tl);
+                const aotx_h8 hi = lds.x[s][0][u][lane], lo = lds.x[s][1][u][lane];
+                a = aotx_mma(x.th[s], hi, a);
+                l = aotx_mma(x.th[s], lo, l);
+                l = aotx_mma(x.tl[s], hi, l);
             }
-            aotx_h4 hi, lo, vhi, vlo;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float y = t[r] + tl[r];
-                _Float16 a, z;
-                aotx_split(y, &a, &z);
-                hi[r] = a;
-                lo[r] = z;
-                aotx_split(y * now.of_u[r], &a, &z);
-                vhi[r] = a;
-                vlo[r] = z;
-            }
-            *((aotx_h4 *)&Ux[w >> 1][0][u][lane] + (w & 1u)) = hi;
-            *((aotx_h4 *)&Ux[w >> 1][1][u][lane] + (w & 1u)) = lo;
-            *((aotx_h4 *)&Vx[w >> 1][0][u][lane] + (w & 1u)) = vhi;
-            *((aotx_h4 *)&Vx[w >> 1][1][u][lane] + (w & 1u)) = vlo;
+            a += l;
+            aotx_h4 hi, lo;
+            aotx_split4(a * x.of_u, &hi, &lo);
+            *((aotx_h4 *)&lds.v[w >> 1][0][u][lane] + (w & 1u)) = hi;
+            *((aotx_h4 *)&lds.v[w >> 1][1][u][lane] + (w & 1u)) = lo;
+            aotx_split4(a, &hi, &lo);
+            *((aotx_h4 *)&lds.u[w >> 1][0][u][lane] + (w & 1u)) = hi;
+            *((aotx_h4 *)&lds.u[w >> 1][1][u][lane] + (w & 1u)) = lo;
         }
-        if (more) {
-            int was[NT];
-#pragma unroll
-            for (int u = 0; u < NT; ++u) was[u] = vex[u];
-            tell(next, n1, S, was, vex);
-        }
+        load_t(x, far);
         __syncthreads();
-        float down_now[NT];
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            aotx_f4 lo_part = {0, 0, 0, 0};
-#pragma unroll
-            for (unsigned int s = 0; s < 2u; ++s) {
-                if (s > w / 2u) continue;
-                const aotx_h8 hi = Ux[s][0][u][lane], lo = Ux[s][1][u][lane];
-                o[u] = aotx_mma(now.ph[s], hi, o[u]);
-                lo_part = aotx_mma(now.ph[s], lo, lo_part);
-                lo_part = aotx_mma(now.pl[s], hi, lo_part);
-            }
-            down_now[u] = down[u];
-            const float fade = now.fade * up[u];
+        for (int u = 0; u < NT; ++u)
 #pragma unroll
             for (int t = 0; t < TW; ++t) {
-                aotx_f4 acc = S[t][u] * fade, low = {0, 0, 0, 0};
+                aotx_f4 a = S[t][u] * x.fade, l = {0, 0, 0, 0};
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    acc = aotx_mma(now.kt[t][s], Vx[s][0][u][lane], acc);
-                    low = aotx_mma(now.kt[t][s], Vx[s][1][u][lane], low);
+                    a = aotx_mma(x.kt[t][s], lds.v[s][0][u][lane], a);
+                    l = aotx_mma(x.kt[t][s], lds.v[s][1][u][lane], l);
                 }
-                S[t][u] = (acc + low) * down[u];
+                S[t][u] = a + l;
                 if (lim[u] < n) S[t][u] = aotx_f4{1, 1, 1, 1} * __builtin_nanf("");
             }
-            o[u] = (o[u] + lo_part) * down_now[u];
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (i0 + r >= n) continue;
-#pragma unroll
-            for (int u = 0; u < NT; ++u)
-                out[(r0 + i0 + r) * width + u] = i0 + r >= lim[u] ? 0x7E00u : aotx_f2h(o[u][r]);
-        }
-        if (more) {
-            heard();
-            now = next;
-        }
+        load_rest(x, far);
+        load_kt(x, far);
+    };
+    for (unsigned int c = 0; c < k.chunks; c += 2u) {
+        pass(A, c);
+        if (c + 1u < k.chunks) pass(B, c + 1u);
     }
 #pragma unroll
     for (int t = 0; t < TW; ++t)
@@ -652,8 +718,150 @@ __global__ __launch_bounds__(256) void aotx_delta_across(aotx_delta_args p)
             const unsigned int tile = w * TW + t;
             const unsigned int key = 32u * (tile >> 1) + 8u * g + 4u * (tile & 1u) + r;
 #pragma unroll
-            for (int u = 0; u < NT; ++u) sp[key * D + u] = S[t][u][r];
+            for (int u = 0; u < NT; ++u) sp[key * D + u] = ldexpf(S[t][u][r], -shift[u]);
         }
+}
+
+/* ---- waves 4 to 7: out = diag(exp(G) r_q) Q S + P U ---- */
+template <int D, int NT>
+struct aotx_delta_out_tile {
+    aotx_h8 q[D / 32], ph[2], pl[2];
+    aotx_f4 of_q;
+    unsigned int bad, badv;
+};
+
+template <int D, int NT>
+static __device__ __forceinline__ void aotx_delta_answer(const aotx_delta_args &p, const aotx_delta_walk k,
+                                                         aotx_delta_lds<D, NT> &lds)
+{
+    constexpr int KS = D / 32;
+    typedef aotx_delta_out_tile<D, NT> tile_t;
+    const unsigned int w = k.w, g = k.g, lane = k.lane, i0 = 16u * w + 4u * g, kh = k.h / p.group;
+    const unsigned int at_q = (16u * w + k.m) * p.stride * 2u + (kh * D + 8u * g) * 2u;
+    const unsigned int width = p.heads * D * 2u;        /* bytes of a row of out */
+    const unsigned int at_out = i0 * width + (k.h * D + k.col) * 2u;
+    auto load_q = [&](tile_t &x, unsigned int c) {
+        const aotx_rows_view rows = aotx_rows_of(p, k.seq.start + c * 64u, aotx_delta_left(k, c));
+#pragma unroll
+        for (int s = 0; s < KS; ++s) x.q[s] = aotx_rows_16(rows, at_q + 64u * s);
+    };
+    auto load_p = [&](tile_t &x, unsigned int c) {
+        const aotx_delta_chunk_work *f = p.work + (unsigned long long)(k.c0 + c) * p.heads + k.h;
+#pragma unroll
+        for (unsigned int s = 0; s < 2u; ++s) {
+            x.ph[s] = f->p_hi[w][s][lane];
+            x.pl[s] = f->p_lo[w][s][lane];
+        }
+        x.of_q = *(const aotx_f4 *)&f->of_q[i0];
+        x.bad = f->bad;
+        x.badv = f->badv;
+    };
+    tile_t A, B;
+    load_q(A, 0u);
+    load_p(A, 0u);
+    const unsigned int c1 = k.chunks > 1u ? 1u : 0u;
+    load_q(B, c1);
+    load_p(B, c1);
+    int shift[NT];
+    auto pass = [&](tile_t &x, unsigned int c) {
+        const unsigned int n = aotx_delta_left(k, c), far = aotx_delta_ahead(k, c);
+        if (c % AOTX_DELTA_PERIOD == 0u) {
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < NT; ++u) shift[u] = aotx_delta_shift<NT>(lds.size, k.m * NT + u);
+        }
+        unsigned int lim[NT];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) lim[u] = x.bad;
+        if (x.badv != 0u) {
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                const unsigned int first = aotx_delta_first<NT>(lds.bad, k.m * NT + u);
+                lim[u] = first < lim[u] ? first : lim[u];
+            }
+        }
+        __syncthreads();
+        aotx_f4 o[NT];
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            aotx_f4 a = {0, 0, 0, 0}, l = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                a = aotx_mma(x.q[s], lds.s[s][0][u][lane], a);
+                l = aotx_mma(x.q[s], lds.s[s][1][u][lane], l);
+            }
+            o[u] = x.of_q * (a + l);
+        }
+        load_q(x, far);
+        __syncthreads();
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            aotx_f4 l = {0, 0, 0, 0};
+#pragma unroll
+            for (unsigned int s = 0; s < 2u; ++s) {
+                if (s > w / 2u) continue;
+                const aotx_h8 hi = lds.u[s][0][u][lane], lo = lds.u[s][1][u][lane];
+                o[u] = aotx_mma(x.ph[s], hi, o[u]);
+                l = aotx_mma(x.ph[s], lo, l);
+                l = aotx_mma(x.pl[s], hi, l);
+            }
+            o[u] += l;
+        }
+        load_p(x, far);
+        /* rows past the chunk are past the view's end: the store drops them */
+        const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
+            (char *)p.out + (unsigned long long)(k.seq.start + c * 64u) * width, (short)0, (int)(n * width), 0x00020000);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                const unsigned short v = i0 + r >= lim[u] ? 0x7E00u : aotx_f2h(ldexpf(o[u][r], -shift[u]));
+                __builtin_amdgcn_raw_buffer_store_b16(v, to, (int)(at_out + r * width + 2u * u), 0, 0);
+            }
+    };
+    for (unsigned int c = 0; c < k.chunks; c += 2u) {
+        pass(A, c);
+        if (c + 1u < k.chunks) pass(B, c + 1u);
+    }
+}
+
+template <int D, int NT>
+__global__ __launch_bounds__(512) void aotx_delta_across(aotx_delta_args p)
+{
+    constexpr unsigned int SLICES = D / (16 * NT);
+    __shared__ aotx_delta_lds<D, NT> lds;
+    aotx_delta_walk k;
+    k.lane = threadIdx.x & 63u;
+    k.m = k.lane & 15u;
+    k.g = k.lane >> 4;
+    const unsigned int wave = (unsigned int)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    k.w = wave & 3u;
+    /* the slices of a head go to one XCD (workgroup b runs on XCD b % 8), whose L2 then holds
+     * what they share */
+    const unsigned int unit = blockIdx.x / (8u * SLICES) * 8u + blockIdx.x % 8u;
+    const unsigned int slice = blockIdx.x / 8u % SLICES;
+    if (unit >= p.seqs.seqs * p.heads) return;
+    const unsigned int i = unit / p.heads;
+    k.h = unit % p.heads;
+    unsigned int b, e, mine, before;
+    aotx_seq_rows(p.seqs, &b, &e);
+    aotx_delta_chunks(b, e, &mine, &before);
+    k.seq = aotx_seq_of(p.seqs, i, b, e);
+    k.c0 = (unsigned int)__builtin_amdgcn_readlane((int)before, (int)i);
+    if (k.seq.start >= k.seq.end) return;
+    k.chunks = (k.seq.end - k.seq.start + 63u) / 64u;
+    k.col = slice * 16u * NT + k.m * NT;                /* this lane's NT columns */
+    if (k.seq.refused) {
+        if (threadIdx.x == 0u && slice == 0u && k.h == 0u) atomicAdd(p.seqs.faults, 1u);
+        for (unsigned int t = k.seq.start + threadIdx.x / 16u; t < k.seq.end; t += 32u)
+#pragma unroll
+            for (int u = 0; u < NT; ++u) p.out[((unsigned long long)t * p.heads + k.h) * D + k.col + u] = 0;
+        return;
+    }
+    if (wave < 4u) aotx_delta_carry<D, NT>(p, k, lds);
+    else aotx_delta_answer<D, NT>(p, k, lds);
 }
 
 #endif

@@ -225,7 +225,10 @@ def test_chunk_offsets_out_of_order_stay_in_bounds(torch, lib, offset):
 def test_chunk_inf_and_nan_reach_no_earlier_row(torch, lib, what, bad, at):
     """Row `at` of the first sequence gets a value that is no number. Rows before it, the second
     sequence, heads of other keys (or, from v, a and b, all other heads), and columns beside a bad
-    value are what they are without it, bit for bit; a bad q reaches its row alone."""
+    value are what they are without it, bit for bit; a bad q reaches its row alone. In the column of
+    a bad v the rows before it are right, but not always to the bit: a column's numbers are split
+    into two parts at a scale that goes by the sizes of its values in four chunks, the replaced one
+    among them, so they may round elsewhere, by 2^-21 a product, which the sums' own bound holds."""
     heads, d = 4, 128
     clean = Delta(torch, 15, [130, 20], 2, heads, d).up().call(lib)
     base, S0 = clean.got()
@@ -250,7 +253,13 @@ def test_chunk_inf_and_nan_reach_no_earlier_row(torch, lib, what, bad, at):
     else:
         hit[at:130, 1] = True
         hit_state[slot, 1] = True
-    assert np.array_equal(out[~hit], base[~hit])
+    near = np.zeros(out.shape, dtype=bool)
+    if what == "v":
+        near[:at, 1, 9] = True
+        want, _, _, top = clean.want()
+        far = 4 * np.sqrt(d * 130) * 2.0 ** -24 * top
+        assert (np.abs(out[near] - want[near]) <= 2.0 ** -11 * np.abs(want[near]) + 2.0 ** -25 + far).all()
+    assert np.array_equal(out[~hit & ~near], base[~hit & ~near])
     assert np.array_equal(S[~hit_state], S0[~hit_state])
     if what not in ("a", "b") or np.isnan(bad):
         assert not np.isfinite(out[hit]).any()
