@@ -209,9 +209,9 @@ static unsigned int aotx_delta_chunks_max(unsigned int tokens, unsigned int seqs
 extern "C" unsigned long long aotx_delta_work(unsigned int tokens, unsigned int seqs,
                                               unsigned int heads, unsigned int head_dim)
 {
-    /* T, P and factors for every head, K^T for as many key heads */
+    /* T, P and factors for every head; K, Q and K^T for as many key heads */
     return (unsigned long long)aotx_delta_chunks_max(tokens, seqs) * heads
-        * (sizeof(aotx_delta_chunk_work) + (unsigned long long)head_dim * AOTX_DELTA_CHUNK * 2u);
+        * (sizeof(aotx_delta_chunk_work) + (unsigned long long)head_dim * AOTX_DELTA_CHUNK * 6u);
 }
 
 template <int D>
@@ -245,7 +245,7 @@ extern "C" int aotx_delta_chunk(const void *qkv, unsigned int stride, const floa
     p.seqs.offset = offset;
     p.chunks = aotx_delta_chunks_max(tokens, seqs);
     p.work = (aotx_delta_chunk_work *)work;
-    p.kt = (aotx_h8 *)(p.work + (unsigned long long)p.chunks * heads);
+    p.rows = (aotx_h8 *)(p.work + (unsigned long long)p.chunks * heads);
     if (head_dim == 128u) aotx_delta_chunked<128>(p, aotx_stream(stream));
     else aotx_delta_chunked<64>(p, aotx_stream(stream));
     return 0;

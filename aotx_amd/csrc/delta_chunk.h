@@ -58,9 +58,18 @@ struct aotx_delta_args {
     aotx_seqs seqs;
     /* chunks */
     aotx_delta_chunk_work *work;    /* [chunks][heads] */
-    aotx_h8 *kt;                    /* [chunks][key_heads][d / 16][2][64]: K^T, scaled rows */
+    aotx_h8 *rows;                  /* [chunks][key_heads] of K, Q and K^T (aotx_delta_rows_of) */
     unsigned int chunks;            /* at most: rows / 64 + sequences */
 };
+
+/* K, Q and K^T (rows scaled) of a chunk and key head as operands: [4 row tiles][d / 32 steps][64]
+ * twice, [d / 16 tiles of keys][2 steps][64]. Rows of the call's tensor lie a power of two apart
+ * as a rule, so that one head's are in one channel of the L2; these are not. */
+static __device__ __forceinline__ aotx_h8 *aotx_delta_rows_of(const aotx_delta_args &p, unsigned int c, unsigned int kh,
+                                                              unsigned int d, unsigned int which)
+{
+    return p.rows + (((unsigned long long)c * p.key_heads + kh) * 3u + which) * (8u * d);
+}
 
 static __device__ __forceinline__ aotx_h8 aotx_h8_of(aotx_u16x8 v) { return __builtin_bit_cast(aotx_h8, v); }
 
@@ -223,6 +232,14 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
         if (bad) kf[s] = aotx_h8{0, 0, 0, 0, 0, 0, 0, 0};
         lds.kfrag[w][s][lane] = kf[s];
     }
+    if (h % p.group == 0u) {
+        aotx_h8 *k = aotx_delta_rows_of(p, c, kh, D, 0u) + w * KS * 64u, *q = aotx_delta_rows_of(p, c, kh, D, 1u) + w * KS * 64u;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            *(aotx_h8 *)((char *)(k + s * 64) + lane * 16u) = kf[s];
+            *(aotx_h8 *)((char *)(q + s * 64) + lane * 16u) = qf[s];
+        }
+    }
     const unsigned long long badrows = __ballot(bad) & 0xFFFFull;
     if (lane == 0u) badk[w] = badrows != 0ull ? 16u * w + (unsigned int)__builtin_ctzll(badrows) : 64u;
     const float len = sqrtf(kk + p.eps), inv = 1.0f / len;
@@ -351,7 +368,7 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
      * the rows of K along a lane's registers, the order that operand needs */
     if (h % p.group == 0u) {
         const unsigned int s = w & 1u;
-        aotx_h8 *kt = p.kt + ((unsigned long long)c * p.key_heads + kh) * (D / 16) * 2 * 64;
+        aotx_h8 *kt = aotx_delta_rows_of(p, c, kh, D, 2u);
         const aotx_f4 sc0 = *(const aotx_f4 *)&ks[32u * s + 4u * g], sc1 = *(const aotx_f4 *)&ks[32u * s + 16u + 4u * g];
 #pragma unroll
         for (unsigned int v = 0; v < D / 32u; ++v) {
@@ -447,6 +464,16 @@ struct aotx_delta_lds {
     unsigned int bad[4][16 * NT];           /* first bad rows of V's columns, by wave */
 };
 
+/* 16 bytes a lane of what starts at `from` (the same for the wave). */
+static __device__ __forceinline__ aotx_h8 aotx_lane_16(const void *from, unsigned int lane16)
+{
+    return *(const aotx_h8 *)((const char *)from + lane16);
+}
+static __device__ __forceinline__ aotx_f4 aotx_lane_f4(const void *from, unsigned int at)
+{
+    return *(const aotx_f4 *)((const char *)from + at);
+}
+
 /* What both kinds of waves know. */
 struct aotx_delta_walk {
     aotx_seq_view seq;
@@ -509,28 +536,27 @@ static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p
     constexpr int KS = D / 32, TW = D / 64;
     typedef aotx_delta_state_tile<D, NT> tile_t;
     const unsigned int w = k.w, g = k.g, lane = k.lane, i0 = 16u * w + 4u * g, kh = k.h / p.group;
-    const unsigned int at_k = (16u * w + k.m) * p.stride * 2u + (p.key_heads * D + kh * D + 8u * g) * 2u;
     const unsigned int at_v = i0 * p.stride * 2u + (2u * p.key_heads * D + k.h * D + k.col) * 2u;
     auto from = [&](unsigned int c) { return p.work + (unsigned long long)(k.c0 + c) * p.heads + k.h; };
     auto load_k = [&](tile_t &x, unsigned int c) {
-        const aotx_rows_view rows = aotx_rows_of(p, k.seq.start + c * 64u, aotx_delta_left(k, c));
+        const aotx_h8 *f = aotx_delta_rows_of(p, k.c0 + c, kh, D, 0u) + w * KS * 64u;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) x.k[s] = aotx_rows_16(rows, at_k + 64u * s);
+        for (int s = 0; s < KS; ++s) x.k[s] = aotx_lane_16(f + s * 64, lane * 16u);
     };
     auto load_t = [&](tile_t &x, unsigned int c) {
         const aotx_delta_chunk_work *f = from(c);
 #pragma unroll
         for (unsigned int s = 0; s < 2u; ++s) {
-            x.th[s] = f->t_hi[w][s][lane];
-            x.tl[s] = f->t_lo[w][s][lane];
+            x.th[s] = aotx_lane_16(f->t_hi[w][s], lane * 16u);
+            x.tl[s] = aotx_lane_16(f->t_lo[w][s], lane * 16u);
         }
     };
     auto load_kt = [&](tile_t &x, unsigned int c) {
-        const aotx_h8 *kt = p.kt + (((unsigned long long)(k.c0 + c) * p.key_heads + kh) * (D / 16) + w * TW) * 2 * 64;
+        const aotx_h8 *kt = aotx_delta_rows_of(p, k.c0 + c, kh, D, 2u) + w * TW * 2u * 64u;
 #pragma unroll
         for (int t = 0; t < TW; ++t)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) x.kt[t][s] = kt[(t * 2 + s) * 64 + lane];
+            for (int s = 0; s < 2; ++s) x.kt[t][s] = aotx_lane_16(kt + (t * 2 + s) * 64, lane * 16u);
     };
     auto load_rest = [&](tile_t &x, unsigned int c) {
         const aotx_rows_view rows = aotx_rows_of(p, k.seq.start + c * 64u, aotx_delta_left(k, c));
@@ -539,8 +565,8 @@ static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p
 #pragma unroll
             for (int u = 0; u < NT; ++u) x.v[r][u] = aotx_rows_2(rows, at_v + r * p.stride * 2u + 2u * u);
         const aotx_delta_chunk_work *f = from(c);
-        x.of_k = *(const aotx_f4 *)&f->of_k[i0];
-        x.of_u = *(const aotx_f4 *)&f->of_u[i0];
+        x.of_k = aotx_lane_f4(f->of_k, i0 * 4u);
+        x.of_u = aotx_lane_f4(f->of_u, i0 * 4u);
         x.fade = f->fade;
         x.bad = f->bad;
         x.badv = f->badv;
@@ -569,50 +595,52 @@ static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p
                 shift[u] = 0;
             }
         }
+    /* in the order in which the passes load, so that the waits for them count alike */
     tile_t A, B;
     load_top(0u);
     load_k(A, 0u);
-    load_rest(A, 0u);
     load_t(A, 0u);
+    load_rest(A, 0u);
     load_kt(A, 0u);
     const unsigned int c1 = k.chunks > 1u ? 1u : 0u;
     load_k(B, c1);
-    load_rest(B, c1);
     load_t(B, c1);
+    load_rest(B, c1);
     load_kt(B, c1);
 
+    auto scale = [&](unsigned int c) {
+        /* in the period |S| and |U| of a column stay below sqrt(d) max|S| + 257 max|V|, which the
+         * exponents plus 5 and plus 10 are bounds of */
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            float ms = 0.0f;
+#pragma unroll
+            for (int t = 0; t < TW; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) ms = fmaxf(ms, fabsf(S[t][u][r]));
+            ms = fmaxf(ms, __shfl_xor(ms, 16, 64));
+            ms = fmaxf(ms, __shfl_xor(ms, 32, 64));
+            int ex = aotx_exponent(ms) - shift[u] + 5, ev = 0;
+#pragma unroll
+            for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q) ev = top[q][u] > ev ? top[q][u] : ev;
+            ev += 10 - 15;
+            ex = ex > ev ? ex : ev;
+            if (g == 0u) lds.size[w][k.m * NT + u] = ex;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            const int to = aotx_delta_shift<NT>(lds.size, k.m * NT + u);
+#pragma unroll
+            for (int t = 0; t < TW; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[t][u][r] = ldexpf(S[t][u][r], to - shift[u]);
+            shift[u] = to;
+        }
+        load_top(c + AOTX_DELTA_PERIOD);
+    };
     auto pass = [&](tile_t &x, unsigned int c) {
         const unsigned int n = aotx_delta_left(k, c), far = aotx_delta_ahead(k, c);
-        if (c % AOTX_DELTA_PERIOD == 0u) {
-            /* |U| and |S| of a column stay below sqrt(d) max|S| + (64 periods + 1) max|V| */
-#pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                float ms = 0.0f;
-#pragma unroll
-                for (int t = 0; t < TW; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) ms = fmaxf(ms, fabsf(S[t][u][r]));
-                ms = fmaxf(ms, __shfl_xor(ms, 16, 64));
-                ms = fmaxf(ms, __shfl_xor(ms, 32, 64));
-                int ex = aotx_exponent(ms) - shift[u] + 5, ev = 0;
-#pragma unroll
-                for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q) ev = top[q][u] > ev ? top[q][u] : ev;
-                ev += 10 - 15;
-                ex = ex > ev ? ex : ev;
-                if (g == 0u) lds.size[w][k.m * NT + u] = ex;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                const int to = aotx_delta_shift<NT>(lds.size, k.m * NT + u);
-#pragma unroll
-                for (int t = 0; t < TW; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) S[t][u][r] = ldexpf(S[t][u][r], to - shift[u]);
-                shift[u] = to;
-            }
-            load_top(c + AOTX_DELTA_PERIOD);
-        }
         unsigned int lim[NT];
 #pragma unroll
         for (int u = 0; u < NT; ++u) lim[u] = x.bad;
@@ -707,9 +735,17 @@ static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p
         load_rest(x, far);
         load_kt(x, far);
     };
-    for (unsigned int c = 0; c < k.chunks; c += 2u) {
+    /* a period a turn: no branch but the ways out, and the loads in flight are always the same */
+    for (unsigned int c = 0;;) {
+        scale(c);
         pass(A, c);
-        if (c + 1u < k.chunks) pass(B, c + 1u);
+        if (++c >= k.chunks) break;
+        pass(B, c);
+        if (++c >= k.chunks) break;
+        pass(A, c);
+        if (++c >= k.chunks) break;
+        pass(B, c);
+        if (++c >= k.chunks) break;
     }
 #pragma unroll
     for (int t = 0; t < TW; ++t)
@@ -737,22 +773,21 @@ static __device__ __forceinline__ void aotx_delta_answer(const aotx_delta_args &
     constexpr int KS = D / 32;
     typedef aotx_delta_out_tile<D, NT> tile_t;
     const unsigned int w = k.w, g = k.g, lane = k.lane, i0 = 16u * w + 4u * g, kh = k.h / p.group;
-    const unsigned int at_q = (16u * w + k.m) * p.stride * 2u + (kh * D + 8u * g) * 2u;
     const unsigned int width = p.heads * D * 2u;        /* bytes of a row of out */
     const unsigned int at_out = i0 * width + (k.h * D + k.col) * 2u;
     auto load_q = [&](tile_t &x, unsigned int c) {
-        const aotx_rows_view rows = aotx_rows_of(p, k.seq.start + c * 64u, aotx_delta_left(k, c));
+        const aotx_h8 *f = aotx_delta_rows_of(p, k.c0 + c, kh, D, 1u) + w * KS * 64u;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) x.q[s] = aotx_rows_16(rows, at_q + 64u * s);
+        for (int s = 0; s < KS; ++s) x.q[s] = aotx_lane_16(f + s * 64, lane * 16u);
     };
     auto load_p = [&](tile_t &x, unsigned int c) {
         const aotx_delta_chunk_work *f = p.work + (unsigned long long)(k.c0 + c) * p.heads + k.h;
 #pragma unroll
         for (unsigned int s = 0; s < 2u; ++s) {
-            x.ph[s] = f->p_hi[w][s][lane];
-            x.pl[s] = f->p_lo[w][s][lane];
+            x.ph[s] = aotx_lane_16(f->p_hi[w][s], lane * 16u);
+            x.pl[s] = aotx_lane_16(f->p_lo[w][s], lane * 16u);
         }
-        x.of_q = *(const aotx_f4 *)&f->of_q[i0];
+        x.of_q = aotx_lane_f4(f->of_q, i0 * 4u);
         x.bad = f->bad;
         x.badv = f->badv;
     };
@@ -763,13 +798,25 @@ static __device__ __forceinline__ void aotx_delta_answer(const aotx_delta_args &
     load_q(B, c1);
     load_p(B, c1);
     int shift[NT];
-    auto pass = [&](tile_t &x, unsigned int c) {
-        const unsigned int n = aotx_delta_left(k, c), far = aotx_delta_ahead(k, c);
-        if (c % AOTX_DELTA_PERIOD == 0u) {
-            __syncthreads();
+    /* what is left of the chunk before: its rows are stored while the next one's U is made */
+    aotx_f4 o[NT];
+    unsigned int o_lim[NT], o_c = 0u;
+    int o_shift[NT];
+    auto store = [&]() {
+        /* rows past the chunk are past the view's end: the store drops them */
+        const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
+            (char *)p.out + (unsigned long long)(k.seq.start + o_c * 64u) * width, (short)0,
+            (int)(aotx_delta_left(k, o_c) * width), 0x00020000);
 #pragma unroll
-            for (int u = 0; u < NT; ++u) shift[u] = aotx_delta_shift<NT>(lds.size, k.m * NT + u);
-        }
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                const unsigned short v = i0 + r >= o_lim[u] ? 0x7E00u : aotx_f2h(ldexpf(o[u][r], -o_shift[u]));
+                __builtin_amdgcn_raw_buffer_store_b16(v, to, (int)(at_out + r * width + 2u * u), 0, 0);
+            }
+    };
+    auto pass = [&](tile_t &x, unsigned int c) {
+        const unsigned int far = aotx_delta_ahead(k, c);
         unsigned int lim[NT];
 #pragma unroll
         for (int u = 0; u < NT; ++u) lim[u] = x.bad;
@@ -782,49 +829,53 @@ static __device__ __forceinline__ void aotx_delta_answer(const aotx_delta_args &
             }
         }
         __syncthreads();
-        aotx_f4 o[NT];
+        aotx_f4 a[NT], l[NT];
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            aotx_f4 a = {0, 0, 0, 0}, l = {0, 0, 0, 0};
+            a[u] = l[u] = aotx_f4{0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                a = aotx_mma(x.q[s], lds.s[s][0][u][lane], a);
-                l = aotx_mma(x.q[s], lds.s[s][1][u][lane], l);
+                a[u] = aotx_mma(x.q[s], lds.s[s][0][u][lane], a[u]);
+                l[u] = aotx_mma(x.q[s], lds.s[s][1][u][lane], l[u]);
             }
-            o[u] = x.of_q * (a + l);
         }
         load_q(x, far);
         __syncthreads();
+        if (c != 0u) store();
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            aotx_f4 l = {0, 0, 0, 0};
+            o[u] = x.of_q * (a[u] + l[u]);
+            aotx_f4 lo_part = {0, 0, 0, 0};
 #pragma unroll
             for (unsigned int s = 0; s < 2u; ++s) {
                 if (s > w / 2u) continue;
                 const aotx_h8 hi = lds.u[s][0][u][lane], lo = lds.u[s][1][u][lane];
                 o[u] = aotx_mma(x.ph[s], hi, o[u]);
-                l = aotx_mma(x.ph[s], lo, l);
-                l = aotx_mma(x.pl[s], hi, l);
+                lo_part = aotx_mma(x.ph[s], lo, lo_part);
+                lo_part = aotx_mma(x.pl[s], hi, lo_part);
             }
-            o[u] += l;
+            o[u] += lo_part;
+            o_lim[u] = lim[u];
+            o_shift[u] = shift[u];
         }
+        o_c = c;
         load_p(x, far);
-        /* rows past the chunk are past the view's end: the store drops them */
-        const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
-            (char *)p.out + (unsigned long long)(k.seq.start + c * 64u) * width, (short)0, (int)(n * width), 0x00020000);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                const unsigned short v = i0 + r >= lim[u] ? 0x7E00u : aotx_f2h(ldexpf(o[u][r], -shift[u]));
-                __builtin_amdgcn_raw_buffer_store_b16(v, to, (int)(at_out + r * width + 2u * u), 0, 0);
-            }
     };
-    for (unsigned int c = 0; c < k.chunks; c += 2u) {
+    for (unsigned int c = 0;;) {
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < NT; ++u) shift[u] = aotx_delta_shift<NT>(lds.size, k.m * NT + u);
         pass(A, c);
-        if (c + 1u < k.chunks) pass(B, c + 1u);
+        if (++c >= k.chunks) break;
+        pass(B, c);
+        if (++c >= k.chunks) break;
+        pass(A, c);
+        if (++c >= k.chunks) break;
+        pass(B, c);
+        if (++c >= k.chunks) break;
     }
+    store();
 }
 
 template <int D, int NT>
