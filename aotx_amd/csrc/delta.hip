@@ -209,9 +209,9 @@ static unsigned int aotx_delta_chunks_max(unsigned int tokens, unsigned int seqs
 extern "C" unsigned long long aotx_delta_work(unsigned int tokens, unsigned int seqs,
                                               unsigned int heads, unsigned int head_dim)
 {
-    /* T, P and factors for every head; K, Q and K^T for as many key heads */
+    /* T, P and factors for every head, K and Q for as many key heads */
     return (unsigned long long)aotx_delta_chunks_max(tokens, seqs) * heads
-        * (sizeof(aotx_delta_chunk_work) + (unsigned long long)head_dim * AOTX_DELTA_CHUNK * 6u);
+        * (sizeof(aotx_delta_chunk_work) + (unsigned long long)head_dim * AOTX_DELTA_CHUNK * 4u);
 }
 
 template <int D>
@@ -221,7 +221,7 @@ static void aotx_delta_chunked(const aotx_delta_args &p, hipStream_t s)
     hipLaunchKernelGGL((aotx_delta_within<D>), dim3(p.chunks * p.heads), dim3(256), 0, s, p);
     AOTX_LAUNCH_CHECK();
     const unsigned int units = (p.seqs.seqs * p.heads + 7u) / 8u * 8u;
-    hipLaunchKernelGGL((aotx_delta_across<D, NT>), dim3(units * slices), dim3(512), 0, s, p);
+    hipLaunchKernelGGL((aotx_delta_across<D, NT>), dim3(units * slices), dim3(256), 0, s, p);
     AOTX_LAUNCH_CHECK();
 }
 

@@ -9,12 +9,14 @@
  * T and P need no state: aotx_delta_within makes them for every chunk at once. What is left,
  * aotx_delta_across, walks a sequence's chunks with a slice of columns of S in registers.
  *
- * Numbers. K, Q and V are fp16 and enter the matrix cores as they are; S, U, X = V - K S, T and
- * P enter as two fp16 parts (high and rest, 21 bits), so that their products are nearly as good
- * as fp32 ones at two or three times the work of plain fp16 instead of sixteen times for fp32
- * matrix instructions. The parts have fp16's range: T and P are at most 1 (the rule only ever
- * takes away from what a unit key finds), K is scaled to a length of 1 to 2 by a power of two
- * where its scale goes into U, and S, X and U carry a power of two for every column, set anew
+ * Numbers. K, Q and V are fp16 and enter the matrix cores as they are; S, U, X = V - K S and T
+ * enter as two fp16 parts (high and rest, 21 bits), so that the state's products are nearly as
+ * good as fp32 ones at two or three times the work of plain fp16 instead of sixteen times for
+ * fp32 matrix instructions. P, which only the output sees, is rounded to fp16 once, by 2^-11 as
+ * the output itself is. The parts have fp16's range: T and P are at most 1 (the rule only ever
+ * takes away from what a unit key finds), rows of K are brought to lengths of 1/2 to 1 by a power
+ * of two 2^e (entries below 2^-14 lose bits, 2^-24 of the length at most), whose scale goes
+ * into the factors of X and U, and S, X and U carry a power of two for every column, set anew
  * every four chunks from the column's largest entries: a state's column grows by at most the
  * sum of the 256 values' sizes in that time.
  *
@@ -26,6 +28,8 @@
 
 #include "delta_dev.h"
 
+#include <stddef.h>
+
 typedef _Float16 aotx_h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 aotx_h8 __attribute__((ext_vector_type(8)));
 
@@ -36,15 +40,14 @@ typedef _Float16 aotx_h8 __attribute__((ext_vector_type(8)));
  * 16 w + m, columns 32 s + 16 (e / 4) + 4 g + e % 4 for e < 8, which is the order in which a
  * wave's accumulators of two row tiles make the other operand. */
 struct aotx_delta_chunk_work {
-    aotx_h8 p_hi[4][2][64], p_lo[4][2][64], t_hi[4][2][64], t_lo[4][2][64];
-    float of_k[64];         /* exp(G) r_k */
+    aotx_h8 p[4][2][64], t_hi[4][2][64], t_lo[4][2][64];
+    float of_k[64];         /* exp(G) r_k 2^e; the rows of K are over 2^e */
     float of_q[64];         /* exp(G) r_q */
-    float of_u[64];         /* exp(G_last - G) r_k 2^e; K^T of that row is over 2^e */
+    float of_u[64];         /* exp(G_last - G) r_k 2^e */
     unsigned char vmax[128];/* of every column of V the exponent field of its largest size */
     float fade;             /* exp(G_last) */
-    unsigned int bad;       /* first row that is taken out, 64 for none */
-    unsigned int badv;      /* V has a value that is no number */
-    unsigned int pad[29];
+    unsigned int odd;       /* first row that is taken out, 64 for none; + 256 if V has a value that is no number */
+    unsigned int pad[30];
 };
 
 struct aotx_delta_args {
@@ -58,17 +61,17 @@ struct aotx_delta_args {
     aotx_seqs seqs;
     /* chunks */
     aotx_delta_chunk_work *work;    /* [chunks][heads] */
-    aotx_h8 *rows;                  /* [chunks][key_heads] of K, Q and K^T (aotx_delta_rows_of) */
+    aotx_h8 *rows;                  /* [chunks][key_heads] of K and Q (aotx_delta_rows_of) */
     unsigned int chunks;            /* at most: rows / 64 + sequences */
 };
 
-/* K, Q and K^T (rows scaled) of a chunk and key head as operands: [4 row tiles][d / 32 steps][64]
- * twice, [d / 16 tiles of keys][2 steps][64]. Rows of the call's tensor lie a power of two apart
- * as a rule, so that one head's are in one channel of the L2; these are not. */
+/* K (rows over 2^e) and Q of a chunk and key head as operands, [4 row tiles][d / 32 steps][64]
+ * each. Rows of the call's tensor lie a power of two apart as a rule, so that one head's are in
+ * one channel of the L2; these are not. */
 static __device__ __forceinline__ aotx_h8 *aotx_delta_rows_of(const aotx_delta_args &p, unsigned int c, unsigned int kh,
-                                                              unsigned int d, unsigned int which)
+                                                              unsigned int d)
 {
-    return p.rows + (((unsigned long long)c * p.key_heads + kh) * 3u + which) * (8u * d);
+    return p.rows + ((unsigned long long)c * p.key_heads + kh) * (16u * d);
 }
 
 static __device__ __forceinline__ aotx_h8 aotx_h8_of(aotx_u16x8 v) { return __builtin_bit_cast(aotx_h8, v); }
@@ -89,8 +92,8 @@ static __device__ __forceinline__ void aotx_split4(aotx_f4 x, aotx_h4 *hi, aotx_
 {
     const aotx_h2 a = __builtin_bit_cast(aotx_h2, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));
     const aotx_h2 b = __builtin_bit_cast(aotx_h2, __builtin_amdgcn_cvt_pkrtz(x[2], x[3]));
-    const aotx_h2 c = __builtin_bit_cast(aotx_h2, __builtin_amdgcn_cvt_pkrtz(x[0] - (float)a[0], x[1] - (float)a[1]));
-    const aotx_h2 d = __builtin_bit_cast(aotx_h2, __builtin_amdgcn_cvt_pkrtz(x[2] - (float)b[0], x[3] - (float)b[1]));
+    const aotx_h2 c = __builtin_bit_cast(aotx_h2, __builtin_amdgcn_cvt_pkrtz(fmaf((float)a[0], -1.0f, x[0]), fmaf((float)a[1], -1.0f, x[1])));
+    const aotx_h2 d = __builtin_bit_cast(aotx_h2, __builtin_amdgcn_cvt_pkrtz(fmaf((float)b[0], -1.0f, x[2]), fmaf((float)b[1], -1.0f, x[3])));
     *hi = aotx_h4{a[0], a[1], b[0], b[1]};
     *lo = aotx_h4{c[0], c[1], d[0], d[1]};
 }
@@ -232,24 +235,27 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
         if (bad) kf[s] = aotx_h8{0, 0, 0, 0, 0, 0, 0, 0};
         lds.kfrag[w][s][lane] = kf[s];
     }
-    if (h % p.group == 0u) {
-        aotx_h8 *k = aotx_delta_rows_of(p, c, kh, D, 0u) + w * KS * 64u, *q = aotx_delta_rows_of(p, c, kh, D, 1u) + w * KS * 64u;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            *(aotx_h8 *)((char *)(k + s * 64) + lane * 16u) = kf[s];
-            *(aotx_h8 *)((char *)(q + s * 64) + lane * 16u) = qf[s];
-        }
-    }
     const unsigned long long badrows = __ballot(bad) & 0xFFFFull;
     if (lane == 0u) badk[w] = badrows != 0ull ? 16u * w + (unsigned int)__builtin_ctzll(badrows) : 64u;
     const float len = sqrtf(kk + p.eps), inv = 1.0f / len;
     const float qinv = 1.0f / sqrtf(qq + p.eps) * (D == 128 ? 0.08838834764831845f : 0.125f);
+    int ex;
+    (void)frexpf(len, &ex);
     if (g == 0u) {
-        int ex;
-        (void)frexpf(len, &ex);
         rk[row] = inv;
-        ks[row] = ldexpf(1.0f, -ex);
+        ks[row] = ldexpf(inv, ex);
         rq[row] = qinv;
+    }
+    if (h % p.group == 0u) {
+        aotx_h8 *k = aotx_delta_rows_of(p, c, kh, D) + w * KS * 64u, *q = k + 8u * D;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            aotx_h8 o;
+#pragma unroll
+            for (int v = 0; v < 8; ++v) o[v] = (_Float16)ldexpf((float)kf[s][v], -ex);
+            *(aotx_h8 *)((char *)(k + s * 64) + lane * 16u) = o;
+            *(aotx_h8 *)((char *)(q + s * 64) + lane * 16u) = qf[s];
+        }
     }
     /* the largest size of V's columns: sizes of fp16 are in the order of their bits. What is no
      * number is left out, and told of. */
@@ -284,14 +290,14 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
 
     if (w == 0u) {
         const float last = (ghi[63] - ghi[lane]) + (glo[63] - glo[lane]), all = expf(ghi[lane]);
-        to->of_k[lane] = all * rk[lane];
+        to->of_k[lane] = all * ks[lane];
         to->of_q[lane] = all * rq[lane];
-        to->of_u[lane] = expf(last) * rk[lane] / ks[lane];
+        to->of_u[lane] = expf(last) * ks[lane];
         if (lane == 0u) {
             unsigned int first = badg;
             for (int v = 0; v < 4; ++v) first = badk[v] < first ? badk[v] : first;
             to->fade = expf(ghi[63]);
-            to->bad = first;
+            to->odd = first | (badv[0] | badv[1] | badv[2] | badv[3]) << 8;
         }
     } else if (w == 1u) {
         if (lane < D / 2) {             /* two columns a lane */
@@ -301,7 +307,6 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
             for (int x = 1; x < 4; ++x) v = __builtin_elementwise_max(v, __builtin_bit_cast(u2, vm[x][lane]));
             *(unsigned short *)&to->vmax[2u * lane] = (unsigned short)((v[0] >> 10) | ((v[1] >> 10) << 8));
         }
-        if (lane == 0u) to->badv = badv[0] | badv[1] | badv[2] | badv[3];
     }
 
     /* P and M of row 16 w + m. Between blocks, exp(G_i - G_j) is the product of two factors by
@@ -342,11 +347,13 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
 #pragma unroll
     for (unsigned int s = 0; s < 2u; ++s) {
         if (s > w / 2u) continue;
-        aotx_h4 hi[2], lo[2];
-        aotx_split4(pt[2u * s], &hi[0], &lo[0]);
-        aotx_split4(pt[2u * s + 1u], &hi[1], &lo[1]);
-        to->p_hi[w][s][lane] = __builtin_shufflevector(hi[0], hi[1], 0, 1, 2, 3, 4, 5, 6, 7);
-        to->p_lo[w][s][lane] = __builtin_shufflevector(lo[0], lo[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        aotx_h8 o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            o[r] = (_Float16)pt[2u * s][r];
+            o[4 + r] = (_Float16)pt[2u * s + 1u][r];
+        }
+        *(aotx_h8 *)((char *)to->p[w][s] + lane * 16u) = o;
     }
     __builtin_amdgcn_wave_barrier();
 
@@ -363,31 +370,6 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
         if (g == 0u)
 #pragma unroll
             for (int r = 0; r < 16; ++r) Dm[w][r][m] = x[r];
-    }
-    /* K^T for the state's update: rows of the identity pick its columns, which come out with
-     * the rows of K along a lane's registers, the order that operand needs */
-    if (h % p.group == 0u) {
-        const unsigned int s = w & 1u;
-        aotx_h8 *kt = aotx_delta_rows_of(p, c, kh, D, 2u);
-        const aotx_f4 sc0 = *(const aotx_f4 *)&ks[32u * s + 4u * g], sc1 = *(const aotx_f4 *)&ks[32u * s + 16u + 4u * g];
-#pragma unroll
-        for (unsigned int v = 0; v < D / 32u; ++v) {
-            const unsigned int t = (w >> 1) * (D / 32u) + v, st = t >> 1;
-            aotx_h8 pick;
-#pragma unroll
-            for (unsigned int x = 0; x < 8u; ++x)
-                pick[x] = g == (m >> 2) && x == 4u * (t & 1u) + (m & 3u) ? (_Float16)1.0f : (_Float16)0.0f;
-            const aotx_f4 z = {0, 0, 0, 0};
-            const aotx_f4 k0 = aotx_mma(lds.kfrag[2u * s][st][lane], pick, z) * sc0;
-            const aotx_f4 k1 = aotx_mma(lds.kfrag[2u * s + 1u][st][lane], pick, z) * sc1;
-            aotx_h8 o;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                o[r] = (_Float16)k0[r];
-                o[4 + r] = (_Float16)k1[r];
-            }
-            kt[(t * 2u + s) * 64u + lane] = o;
-        }
     }
     __syncthreads();
 
@@ -444,12 +426,13 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
 }
 
 /* ---------------------------------------------------------------------------------------
- * The walk over a sequence's chunks. A workgroup has 16 NT columns of one head's S. Waves 0 to
- * 3 carry the state: wave w has the rows of S that one step of K S takes (D / 4 of them, in
- * accumulators), and rows 16 w .. 16 w + 15 of the chunk. Waves 4 to 7 make the output of the
- * same rows from what the others lay out. S, X and U pass through LDS as operands, a barrier
- * each; everything else a chunk needs is loaded into registers two chunks ahead, each register
- * as soon as it has been used.
+ * The walk over a sequence's chunks. A workgroup of four waves has 16 NT columns of one head's
+ * S: wave w the rows of S that one step of K S takes (D / 4 of them, in accumulators), and rows
+ * 16 w .. 16 w + 15 of the chunk. S, X and U pass between the waves through LDS as operands, a
+ * barrier each; everything else a chunk needs is loaded into registers two chunks ahead, each
+ * register as soon as it has been used. A chunk's output is made where the state's chain waits:
+ * Q S while X is on its way, P U behind the state's update, its rounding and stores while the
+ * next chunk's S is read.
  * Row x of tile t of S is key 32 (t / 2) + 8 (x / 4) + 4 (t % 2) + x % 4, so that two tiles'
  * accumulators hold keys 8 g .. 8 g + 7 of a step, as 16 bytes of a row of K do.
  * ------------------------------------------------------------------------------------- */
@@ -460,31 +443,25 @@ struct aotx_delta_lds {
     aotx_h8 s[D / 32][2][NT][64];           /* step of keys, part, tile of columns */
     aotx_h8 x[2][2][NT][64];                /* step of rows, part, tile of columns */
     aotx_h8 u[2][2][NT][64], v[2][2][NT][64];   /* U, and U with the state update's factors */
+    __align__(16) unsigned short k[64][D + 8];  /* the chunk's rows of K, to be read by columns */
     int size[4][16 * NT];                   /* exponents of the state's columns, by wave */
     unsigned int bad[4][16 * NT];           /* first bad rows of V's columns, by wave */
 };
 
-/* 16 bytes a lane of what starts at `from` (the same for the wave). */
-static __device__ __forceinline__ aotx_h8 aotx_lane_16(const void *from, unsigned int lane16)
-{
-    return *(const aotx_h8 *)((const char *)from + lane16);
-}
-static __device__ __forceinline__ aotx_f4 aotx_lane_f4(const void *from, unsigned int at)
-{
-    return *(const aotx_f4 *)((const char *)from + at);
-}
-
-/* What both kinds of waves know. */
 struct aotx_delta_walk {
     aotx_seq_view seq;
     unsigned int c0, chunks, h, col, w, m, g, lane;
 };
 
-/* The chunk that is loaded `ahead` of c: the last one again past the end, so that every pass
- * has the same loads in flight. */
-static __device__ __forceinline__ unsigned int aotx_delta_ahead(const aotx_delta_walk &k, unsigned int c)
+/* 16 bytes a lane of a part of the workspace: the part's start is the wave's, and no lane has an
+ * address of its own to compute. */
+static __device__ __forceinline__ __amdgpu_buffer_rsrc_t aotx_part(const char *from, unsigned int bytes)
 {
-    return c + 2u < k.chunks ? c + 2u : k.chunks - 1u;
+    return __builtin_amdgcn_make_buffer_rsrc((void *)from, (short)0, (int)bytes, 0x00020000);
+}
+static __device__ __forceinline__ aotx_h8 aotx_lane_16(__amdgpu_buffer_rsrc_t from, unsigned int at, unsigned int step)
+{
+    return __builtin_bit_cast(aotx_h8, __builtin_amdgcn_raw_buffer_load_b128(from, (int)at, (int)step, 0));
 }
 
 static __device__ __forceinline__ unsigned int aotx_delta_left(const aotx_delta_walk &k, unsigned int c)
@@ -499,77 +476,76 @@ static __device__ __forceinline__ int aotx_exponent(float x)
     return (int)((__float_as_uint(x) >> 23) & 0xFFu) - 127;
 }
 
-/* Scales of a period: the exponents that the four waves left, as a shift of at most 100. */
-template <int NT>
-static __device__ __forceinline__ int aotx_delta_shift(const int (*size)[16 * NT], unsigned int at)
-{
-    int ex = size[0][at];
-#pragma unroll
-    for (int v = 1; v < 4; ++v) ex = size[v][at] > ex ? size[v][at] : ex;
-    ex = 14 - ex;
-    return ex > 100 ? 100 : ex < -100 ? -100 : ex;
-}
-
-template <int NT>
-static __device__ __forceinline__ unsigned int aotx_delta_first(const unsigned int (*bad)[16 * NT], unsigned int at)
-{
-    unsigned int first = bad[0][at];
-#pragma unroll
-    for (int v = 1; v < 4; ++v) first = bad[v][at] < first ? bad[v][at] : first;
-    return first;
-}
-
-/* ---- waves 0 to 3 ---- */
-template <int D, int NT>
-struct aotx_delta_state_tile {
-    aotx_h8 k[D / 32], th[2], tl[2], kt[D / 64][2];
+template <int D, int NT, int NS>
+struct aotx_delta_tile {
+    aotx_h8 k[D / 32], q[D / 32], th[NS], tl[NS], p[NS];
     unsigned short v[4][NT];
-    aotx_f4 of_k, of_u;
+    aotx_f4 of_k, of_u, of_q;
     float fade;
-    unsigned int bad, badv;
+    unsigned int odd;
 };
 
-template <int D, int NT>
-static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p, const aotx_delta_walk k,
-                                                        aotx_delta_lds<D, NT> &lds)
+/* NS: steps of 32 columns that the wave's rows of T and P have, 1 for waves 0 and 1, else 2. */
+template <int D, int NT, int NS>
+static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &p, const aotx_delta_walk k,
+                                                         aotx_delta_lds<D, NT> &lds)
 {
     constexpr int KS = D / 32, TW = D / 64;
-    typedef aotx_delta_state_tile<D, NT> tile_t;
-    const unsigned int w = k.w, g = k.g, lane = k.lane, i0 = 16u * w + 4u * g, kh = k.h / p.group;
+    typedef aotx_delta_tile<D, NT, NS> tile_t;
+    const unsigned int w = k.w, g = k.g, lane = k.lane, i0 = 16u * w + 4u * g, kh = k.h / p.group, l16 = lane * 16u;
+    const unsigned int width = p.heads * D * 2u;        /* bytes of a row of out */
+    const unsigned int at_out = i0 * width + (k.h * D + k.col) * 2u;
+    /* a wave's places within a chunk's parts, in bytes */
+    typedef aotx_delta_chunk_work work_t;
+    const unsigned int at_k = w * KS * 1024u + l16, at_p = w * 2048u + l16;
+    const unsigned int at_of = (unsigned int)offsetof(work_t, of_k) + i0 * 4u;
     const unsigned int at_v = i0 * p.stride * 2u + (2u * p.key_heads * D + k.h * D + k.col) * 2u;
-    auto from = [&](unsigned int c) { return p.work + (unsigned long long)(k.c0 + c) * p.heads + k.h; };
-    auto load_k = [&](tile_t &x, unsigned int c) {
-        const aotx_h8 *f = aotx_delta_rows_of(p, k.c0 + c, kh, D, 0u) + w * KS * 64u;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) x.k[s] = aotx_lane_16(f + s * 64, lane * 16u);
+    /* the chunk that is loaded: it stays the last one past the end, so that every pass has the
+     * same loads in flight */
+    unsigned int ahead = 0u;
+    const char *work = (const char *)(p.work + (unsigned long long)k.c0 * p.heads + k.h);
+    const char *rows = (const char *)aotx_delta_rows_of(p, k.c0, kh, D);
+    const unsigned long long work_step = sizeof(work_t) * (unsigned long long)p.heads;
+    const unsigned long long rows_step = 256ull * D * p.key_heads;
+    auto advance = [&]() {
+        const bool more = ahead + 1u < k.chunks;
+        ahead += more ? 1u : 0u;
+        work += more ? work_step : 0ull;
+        rows += more ? rows_step : 0ull;
     };
-    auto load_t = [&](tile_t &x, unsigned int c) {
-        const aotx_delta_chunk_work *f = from(c);
+    auto load_k = [&](tile_t &x) {
+        const __amdgpu_buffer_rsrc_t f = aotx_part(rows, 256u * D);
 #pragma unroll
-        for (unsigned int s = 0; s < 2u; ++s) {
-            x.th[s] = aotx_lane_16(f->t_hi[w][s], lane * 16u);
-            x.tl[s] = aotx_lane_16(f->t_lo[w][s], lane * 16u);
+        for (int s = 0; s < KS; ++s) x.k[s] = aotx_lane_16(f, at_k, s * 1024u);
+    };
+    auto load_q = [&](tile_t &x) {
+        const __amdgpu_buffer_rsrc_t f = aotx_part(rows, 256u * D);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) x.q[s] = aotx_lane_16(f, at_k, 128u * D + s * 1024u);
+    };
+    auto load_t = [&](tile_t &x) {
+        const __amdgpu_buffer_rsrc_t f = aotx_part(work, sizeof(work_t));
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            x.th[s] = aotx_lane_16(f, at_p, (unsigned int)offsetof(work_t, t_hi) + s * 1024u);
+            x.tl[s] = aotx_lane_16(f, at_p, (unsigned int)offsetof(work_t, t_lo) + s * 1024u);
         }
     };
-    auto load_kt = [&](tile_t &x, unsigned int c) {
-        const aotx_h8 *kt = aotx_delta_rows_of(p, k.c0 + c, kh, D, 2u) + w * TW * 2u * 64u;
+    auto load_rest = [&](tile_t &x) {
+        const __amdgpu_buffer_rsrc_t f = aotx_part(work, sizeof(work_t));
 #pragma unroll
-        for (int t = 0; t < TW; ++t)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) x.kt[t][s] = aotx_lane_16(kt + (t * 2 + s) * 64, lane * 16u);
-    };
-    auto load_rest = [&](tile_t &x, unsigned int c) {
-        const aotx_rows_view rows = aotx_rows_of(p, k.seq.start + c * 64u, aotx_delta_left(k, c));
+        for (int s = 0; s < NS; ++s) x.p[s] = aotx_lane_16(f, at_p, s * 1024u);
+        const aotx_rows_view v = aotx_rows_of(p, k.seq.start + ahead * 64u, aotx_delta_left(k, ahead));
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int u = 0; u < NT; ++u) x.v[r][u] = aotx_rows_2(rows, at_v + r * p.stride * 2u + 2u * u);
-        const aotx_delta_chunk_work *f = from(c);
-        x.of_k = aotx_lane_f4(f->of_k, i0 * 4u);
-        x.of_u = aotx_lane_f4(f->of_u, i0 * 4u);
-        x.fade = f->fade;
-        x.bad = f->bad;
-        x.badv = f->badv;
+            for (int u = 0; u < NT; ++u) x.v[r][u] = aotx_rows_2(v, at_v + r * p.stride * 2u + 2u * u);
+        x.of_k = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 0u));
+        x.of_q = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 256u));
+        x.of_u = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 512u));
+        x.fade = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(f, 0, (int)offsetof(work_t, fade), 0));
+        x.odd = __builtin_amdgcn_raw_buffer_load_b32(f, 0, (int)offsetof(work_t, odd), 0);
+        advance();
     };
     unsigned char top[AOTX_DELTA_PERIOD][NT];       /* V's exponents in the coming period */
     auto load_top = [&](unsigned int c) {
@@ -577,7 +553,8 @@ static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p
         for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q)
 #pragma unroll
             for (int u = 0; u < NT; ++u)
-                top[q][u] = from(c + q < k.chunks ? c + q : k.chunks - 1u)->vmax[k.col + u];
+                top[q][u] = p.work[(unsigned long long)(k.c0 + (c + q < k.chunks ? c + q : k.chunks - 1u)) * p.heads
+                                   + k.h].vmax[k.col + u];
     };
 
     aotx_f4 S[TW][NT];                              /* times 2^shift */
@@ -598,16 +575,30 @@ static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p
     /* in the order in which the passes load, so that the waits for them count alike */
     tile_t A, B;
     load_top(0u);
-    load_k(A, 0u);
-    load_t(A, 0u);
-    load_rest(A, 0u);
-    load_kt(A, 0u);
-    const unsigned int c1 = k.chunks > 1u ? 1u : 0u;
-    load_k(B, c1);
-    load_t(B, c1);
-    load_rest(B, c1);
-    load_kt(B, c1);
+    load_k(A);
+    load_q(A);
+    load_t(A);
+    load_rest(A);
+    load_k(B);
+    load_q(B);
+    load_t(B);
+    load_rest(B);
 
+    /* the chunk before: its output, still to be stored */
+    aotx_f4 o[NT];
+    int o_shift[NT];
+    auto store = [&](unsigned int c) {
+        /* rows past the chunk are past the view's end: the store drops them */
+        const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
+            (char *)p.out + (unsigned long long)(k.seq.start + c * 64u) * width, (short)0,
+            (int)(aotx_delta_left(k, c) * width), 0x00020000);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                __builtin_amdgcn_raw_buffer_store_b16(aotx_f2h(ldexpf(o[u][r], -o_shift[u])), to, (int)(at_out + r * width + 2u * u), 0, 0);
+            }
+    };
     auto scale = [&](unsigned int c) {
         /* in the period |S| and |U| of a column stay below sqrt(d) max|S| + 257 max|V|, which the
          * exponents plus 5 and plus 10 are bounds of */
@@ -630,39 +621,47 @@ static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            const int to = aotx_delta_shift<NT>(lds.size, k.m * NT + u);
+            int ex = lds.size[0][k.m * NT + u];
+#pragma unroll
+            for (int v = 1; v < 4; ++v) ex = lds.size[v][k.m * NT + u] > ex ? lds.size[v][k.m * NT + u] : ex;
+            ex = 14 - ex;
+            ex = ex > 100 ? 100 : ex < -100 ? -100 : ex;
 #pragma unroll
             for (int t = 0; t < TW; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[t][u][r] = ldexpf(S[t][u][r], to - shift[u]);
-            shift[u] = to;
+                for (int r = 0; r < 4; ++r) S[t][u][r] = ldexpf(S[t][u][r], ex - shift[u]);
+            shift[u] = ex;
         }
         load_top(c + AOTX_DELTA_PERIOD);
     };
     auto pass = [&](tile_t &x, unsigned int c) {
-        const unsigned int n = aotx_delta_left(k, c), far = aotx_delta_ahead(k, c);
+        /* rows that are taken out, or past the chunk, have zeros in K, Q and V: their X, U and T
+         * are zeros by themselves. Only a chunk with values that are no numbers asks more. */
+        const unsigned int odd = (unsigned int)__builtin_amdgcn_readfirstlane((int)x.odd);
         unsigned int lim[NT];
 #pragma unroll
-        for (int u = 0; u < NT; ++u) lim[u] = x.bad;
-        if (x.badv != 0u) {
+        for (int u = 0; u < NT; ++u) lim[u] = odd & 0xFFu;
+        if (odd != 64u) {
 #pragma unroll
             for (int u = 0; u < NT; ++u) {
                 unsigned int first = 64u;
 #pragma unroll
                 for (int r = 3; r >= 0; --r)
                     if ((x.v[r][u] & 0x7FFFu) >= 0x7C00u) first = i0 + r;
-                unsigned int o = (unsigned int)__shfl_xor((int)first, 16, 64);
-                first = o < first ? o : first;
-                o = (unsigned int)__shfl_xor((int)first, 32, 64);
-                first = o < first ? o : first;
+                unsigned int f = (unsigned int)__shfl_xor((int)first, 16, 64);
+                first = f < first ? f : first;
+                f = (unsigned int)__shfl_xor((int)first, 32, 64);
+                first = f < first ? f : first;
                 if (g == 0u) lds.bad[w][k.m * NT + u] = first;
             }
             __syncthreads();
 #pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                const unsigned int first = aotx_delta_first<NT>(lds.bad, k.m * NT + u);
-                lim[u] = first < lim[u] ? first : lim[u];
-            }
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const unsigned int f = lds.bad[v][k.m * NT + u];
+                    lim[u] = f < lim[u] ? f : lim[u];
+                }
         }
 #pragma unroll
         for (int u = 0; u < NT; ++u)
@@ -675,40 +674,69 @@ static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p
                 *((aotx_h4 *)&lds.s[tile >> 1][1][u][lane] + (tile & 1u)) = lo;
             }
         __syncthreads();
+        aotx_h8 sh[NT][KS], sl[NT][KS];
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            aotx_f4 a = {0, 0, 0, 0}, l = {0, 0, 0, 0};
+        for (int u = 0; u < NT; ++u)
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                a = aotx_mma(x.k[s], lds.s[s][0][u][lane], a);
-                l = aotx_mma(x.k[s], lds.s[s][1][u][lane], l);
+                sh[u][s] = lds.s[s][0][u][lane];
+                sl[u][s] = lds.s[s][1][u][lane];
             }
-            const unsigned int upto = lim[u] < n ? lim[u] : n;
+        if (c != 0u) store(c - 1u);
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            aotx_f4 a = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                a = aotx_mma(x.k[s], sl[u][s], a);
+                a = aotx_mma(x.k[s], sh[u][s], a);
+            }
+            const float up = ldexpf(1.0f, shift[u]);
             aotx_f4 y;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                y[r] = ldexpf(aotx_h2f(x.v[r][u]), shift[u]) - x.of_k[r] * (a[r] + l[r]);
-                if (i0 + r >= upto) y[r] = 0.0f;
+            for (int r = 0; r < 4; ++r) y[r] = fmaf(aotx_h2f(x.v[r][u]), up, -(x.of_k[r] * a[r]));
+            if (odd != 64u) {
+                asm volatile("");               /* a branch that is not taken, no selects */
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (i0 + r >= lim[u]) y[r] = 0.0f;
             }
             aotx_h4 hi, lo;
             aotx_split4(y, &hi, &lo);
             *((aotx_h4 *)&lds.x[w >> 1][0][u][lane] + (w & 1u)) = hi;
             *((aotx_h4 *)&lds.x[w >> 1][1][u][lane] + (w & 1u)) = lo;
         }
-        load_k(x, far);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) *(aotx_h8 *)&lds.k[16u * w + k.m][32 * s + 8u * g] = x.k[s];
         __syncthreads();
+        load_k(x);
+        aotx_h8 xh[NT][NS], xl[NT][NS];
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                xh[u][s] = lds.x[s][0][u][lane];
+                xl[u][s] = lds.x[s][1][u][lane];
+            }
+        aotx_f4 qs[NT];
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            aotx_f4 a = {0, 0, 0, 0}, l = {0, 0, 0, 0};
+            qs[u] = aotx_f4{0, 0, 0, 0};
 #pragma unroll
-            for (unsigned int s = 0; s < 2u; ++s) {
-                if (s > w / 2u) continue;
-                const aotx_h8 hi = lds.x[s][0][u][lane], lo = lds.x[s][1][u][lane];
-                a = aotx_mma(x.th[s], hi, a);
-                l = aotx_mma(x.th[s], lo, l);
-                l = aotx_mma(x.tl[s], hi, l);
+            for (int s = 0; s < KS; ++s) {
+                qs[u] = aotx_mma(x.q[s], sl[u][s], qs[u]);
+                qs[u] = aotx_mma(x.q[s], sh[u][s], qs[u]);
             }
-            a += l;
+        }
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            aotx_f4 a = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                a = aotx_mma(x.th[s], xl[u][s], a);
+                a = aotx_mma(x.tl[s], xh[u][s], a);
+                a = aotx_mma(x.th[s], xh[u][s], a);
+            }
             aotx_h4 hi, lo;
             aotx_split4(a * x.of_u, &hi, &lo);
             *((aotx_h4 *)&lds.v[w >> 1][0][u][lane] + (w & 1u)) = hi;
@@ -717,23 +745,64 @@ static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p
             *((aotx_h4 *)&lds.u[w >> 1][0][u][lane] + (w & 1u)) = hi;
             *((aotx_h4 *)&lds.u[w >> 1][1][u][lane] + (w & 1u)) = lo;
         }
-        load_t(x, far);
         __syncthreads();
+        /* K by columns: lane (m, g) addresses row m / 4 of four, keys 8 (m % 4) .. + 3 of the
+         * tile's 16, and gets key m of it for all four rows */
+        aotx_h8 kt[TW][2];
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
+        for (int t = 0; t < TW; ++t)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                typedef short s4 __attribute__((ext_vector_type(4)));
+                const unsigned int tile = w * TW + t;
+                unsigned short *at = &lds.k[32 * s + 4u * g + (k.m >> 2)][32u * (tile >> 1) + 4u * (tile & 1u) + 8u * (k.m & 3u)];
+                const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at);
+                const s4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(at + 16 * (D + 8)));
+                kt[t][s] = __builtin_bit_cast(aotx_h8, __builtin_shufflevector(a, z, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+        load_q(x);
+        load_t(x);
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+            aotx_h8 vh[2], vl[2], uh[NS], ul[NS];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                vh[s] = lds.v[s][0][u][lane];
+                vl[s] = lds.v[s][1][u][lane];
+            }
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                uh[s] = lds.u[s][0][u][lane];
+                ul[s] = lds.u[s][1][u][lane];
+            }
 #pragma unroll
             for (int t = 0; t < TW; ++t) {
-                aotx_f4 a = S[t][u] * x.fade, l = {0, 0, 0, 0};
+                S[t][u] *= x.fade;
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    a = aotx_mma(x.kt[t][s], lds.v[s][0][u][lane], a);
-                    l = aotx_mma(x.kt[t][s], lds.v[s][1][u][lane], l);
+                    S[t][u] = aotx_mma(kt[t][s], vl[s], S[t][u]);
+                    S[t][u] = aotx_mma(kt[t][s], vh[s], S[t][u]);
                 }
-                S[t][u] = a + l;
-                if (lim[u] < n) S[t][u] = aotx_f4{1, 1, 1, 1} * __builtin_nanf("");
             }
-        load_rest(x, far);
-        load_kt(x, far);
+            o[u] = x.of_q * qs[u];
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                o[u] = aotx_mma(x.p[s], ul[s], o[u]);
+                o[u] = aotx_mma(x.p[s], uh[s], o[u]);
+            }
+            o_shift[u] = shift[u];
+            if (odd != 64u) {
+                asm volatile("");
+                const float nan = __builtin_nanf("");
+#pragma unroll
+                for (int t = 0; t < TW; ++t)
+                    if (lim[u] < 64u) S[t][u] = aotx_f4{nan, nan, nan, nan};
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (i0 + r >= lim[u]) o[u][r] = nan;
+            }
+        }
+        load_rest(x);
     };
     /* a period a turn: no branch but the ways out, and the loads in flight are always the same */
     for (unsigned int c = 0;;) {
@@ -747,6 +816,7 @@ static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p
         pass(B, c);
         if (++c >= k.chunks) break;
     }
+    store(k.chunks - 1u);
 #pragma unroll
     for (int t = 0; t < TW; ++t)
 #pragma unroll
@@ -758,128 +828,8 @@ static __device__ __forceinline__ void aotx_delta_carry(const aotx_delta_args &p
         }
 }
 
-/* ---- waves 4 to 7: out = diag(exp(G) r_q) Q S + P U ---- */
 template <int D, int NT>
-struct aotx_delta_out_tile {
-    aotx_h8 q[D / 32], ph[2], pl[2];
-    aotx_f4 of_q;
-    unsigned int bad, badv;
-};
-
-template <int D, int NT>
-static __device__ __forceinline__ void aotx_delta_answer(const aotx_delta_args &p, const aotx_delta_walk k,
-                                                         aotx_delta_lds<D, NT> &lds)
-{
-    constexpr int KS = D / 32;
-    typedef aotx_delta_out_tile<D, NT> tile_t;
-    const unsigned int w = k.w, g = k.g, lane = k.lane, i0 = 16u * w + 4u * g, kh = k.h / p.group;
-    const unsigned int width = p.heads * D * 2u;        /* bytes of a row of out */
-    const unsigned int at_out = i0 * width + (k.h * D + k.col) * 2u;
-    auto load_q = [&](tile_t &x, unsigned int c) {
-        const aotx_h8 *f = aotx_delta_rows_of(p, k.c0 + c, kh, D, 1u) + w * KS * 64u;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) x.q[s] = aotx_lane_16(f + s * 64, lane * 16u);
-    };
-    auto load_p = [&](tile_t &x, unsigned int c) {
-        const aotx_delta_chunk_work *f = p.work + (unsigned long long)(k.c0 + c) * p.heads + k.h;
-#pragma unroll
-        for (unsigned int s = 0; s < 2u; ++s) {
-            x.ph[s] = aotx_lane_16(f->p_hi[w][s], lane * 16u);
-            x.pl[s] = aotx_lane_16(f->p_lo[w][s], lane * 16u);
-        }
-        x.of_q = aotx_lane_f4(f->of_q, i0 * 4u);
-        x.bad = f->bad;
-        x.badv = f->badv;
-    };
-    tile_t A, B;
-    load_q(A, 0u);
-    load_p(A, 0u);
-    const unsigned int c1 = k.chunks > 1u ? 1u : 0u;
-    load_q(B, c1);
-    load_p(B, c1);
-    int shift[NT];
-    /* what is left of the chunk before: its rows are stored while the next one's U is made */
-    aotx_f4 o[NT];
-    unsigned int o_lim[NT], o_c = 0u;
-    int o_shift[NT];
-    auto store = [&]() {
-        /* rows past the chunk are past the view's end: the store drops them */
-        const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
-            (char *)p.out + (unsigned long long)(k.seq.start + o_c * 64u) * width, (short)0,
-            (int)(aotx_delta_left(k, o_c) * width), 0x00020000);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                const unsigned short v = i0 + r >= o_lim[u] ? 0x7E00u : aotx_f2h(ldexpf(o[u][r], -o_shift[u]));
-                __builtin_amdgcn_raw_buffer_store_b16(v, to, (int)(at_out + r * width + 2u * u), 0, 0);
-            }
-    };
-    auto pass = [&](tile_t &x, unsigned int c) {
-        const unsigned int far = aotx_delta_ahead(k, c);
-        unsigned int lim[NT];
-#pragma unroll
-        for (int u = 0; u < NT; ++u) lim[u] = x.bad;
-        if (x.badv != 0u) {
-            __syncthreads();
-#pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                const unsigned int first = aotx_delta_first<NT>(lds.bad, k.m * NT + u);
-                lim[u] = first < lim[u] ? first : lim[u];
-            }
-        }
-        __syncthreads();
-        aotx_f4 a[NT], l[NT];
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            a[u] = l[u] = aotx_f4{0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                a[u] = aotx_mma(x.q[s], lds.s[s][0][u][lane], a[u]);
-                l[u] = aotx_mma(x.q[s], lds.s[s][1][u][lane], l[u]);
-            }
-        }
-        load_q(x, far);
-        __syncthreads();
-        if (c != 0u) store();
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            o[u] = x.of_q * (a[u] + l[u]);
-            aotx_f4 lo_part = {0, 0, 0, 0};
-#pragma unroll
-            for (unsigned int s = 0; s < 2u; ++s) {
-                if (s > w / 2u) continue;
-                const aotx_h8 hi = lds.u[s][0][u][lane], lo = lds.u[s][1][u][lane];
-                o[u] = aotx_mma(x.ph[s], hi, o[u]);
-                lo_part = aotx_mma(x.ph[s], lo, lo_part);
-                lo_part = aotx_mma(x.pl[s], hi, lo_part);
-            }
-            o[u] += lo_part;
-            o_lim[u] = lim[u];
-            o_shift[u] = shift[u];
-        }
-        o_c = c;
-        load_p(x, far);
-    };
-    for (unsigned int c = 0;;) {
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < NT; ++u) shift[u] = aotx_delta_shift<NT>(lds.size, k.m * NT + u);
-        pass(A, c);
-        if (++c >= k.chunks) break;
-        pass(B, c);
-        if (++c >= k.chunks) break;
-        pass(A, c);
-        if (++c >= k.chunks) break;
-        pass(B, c);
-        if (++c >= k.chunks) break;
-    }
-    store();
-}
-
-template <int D, int NT>
-__global__ __launch_bounds__(512) void aotx_delta_across(aotx_delta_args p)
+__global__ __launch_bounds__(256, 2) void aotx_delta_across(aotx_delta_args p)
 {
     constexpr unsigned int SLICES = D / (16 * NT);
     __shared__ aotx_delta_lds<D, NT> lds;
@@ -887,8 +837,7 @@ __global__ __launch_bounds__(512) void aotx_delta_across(aotx_delta_args p)
     k.lane = threadIdx.x & 63u;
     k.m = k.lane & 15u;
     k.g = k.lane >> 4;
-    const unsigned int wave = (unsigned int)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    k.w = wave & 3u;
+    k.w = (unsigned int)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     /* the slices of a head go to one XCD (workgroup b runs on XCD b % 8), whose L2 then holds
      * what they share */
     const unsigned int unit = blockIdx.x / (8u * SLICES) * 8u + blockIdx.x % 8u;
@@ -906,13 +855,14 @@ __global__ __launch_bounds__(512) void aotx_delta_across(aotx_delta_args p)
     k.col = slice * 16u * NT + k.m * NT;                /* this lane's NT columns */
     if (k.seq.refused) {
         if (threadIdx.x == 0u && slice == 0u && k.h == 0u) atomicAdd(p.seqs.faults, 1u);
-        for (unsigned int t = k.seq.start + threadIdx.x / 16u; t < k.seq.end; t += 32u)
+        for (unsigned int t = k.seq.start + threadIdx.x / 16u; t < k.seq.end; t += 16u)
 #pragma unroll
             for (int u = 0; u < NT; ++u) p.out[((unsigned long long)t * p.heads + k.h) * D + k.col + u] = 0;
         return;
     }
-    if (wave < 4u) aotx_delta_carry<D, NT>(p, k, lds);
-    else aotx_delta_answer<D, NT>(p, k, lds);
+    /* (scalar: the barriers of both ways count together) */
+    if (k.w < 2u) aotx_delta_follow<D, NT, 1>(p, k, lds);
+    else aotx_delta_follow<D, NT, 2>(p, k, lds);
 }
 
 #endif

@@ -65,10 +65,11 @@ def rows(qkv, key_heads, heads, d, eps):
 
 def delta(qkv, a, b, decay, dt, offset, pos, agent, key_heads, heads, d, eps, state, out):
     """out [rows][heads][d] and state [slots][heads][d][d] are changed in place. Returns (faults,
-    the largest magnitude that a state entry or a value had)."""
+    the largest magnitude that a state entry or a value had, and for every output the sum of the
+    sizes of the terms (q' . k'_j) exp(G - G_j) u_j of the rows j of its own 64, itself among them)."""
     q, k, v = rows(qkv, key_heads, heads, d, eps)
     g, beta = gates(a, b, decay, dt)
-    faults, top = 0, 0.0
+    faults, top, near = 0, 0.0, np.zeros(out.shape)
     for i, lo, hi, slot in walk(offset, agent, len(state), len(qkv)):
         if slot is None:
             out[lo:hi], faults = 0, faults + 1
@@ -76,14 +77,20 @@ def delta(qkv, a, b, decay, dt, offset, pos, agent, key_heads, heads, d, eps, st
         S = np.zeros_like(state[slot]) if pos[i] == 0 else state[slot].copy()
         top = max(top, np.abs(S).max())
         for t in range(lo, hi):
+            if (t - lo) % 64 == 0:
+                us, fade, first = [], np.zeros((0, heads)), t
             S = S * np.exp(g[t])[:, None, None]
             u = beta[t][:, None] * (v[t] - np.einsum("hkv,hk->hv", S, k[t]))
             S = S + k[t][:, :, None] * u[:, None, :]
             out[t] = np.einsum("hkv,hk->hv", S, q[t])
+            us.append(np.abs(u))
+            fade = np.concatenate([fade * np.exp(g[t]), np.ones((1, heads))])
+            size = np.abs(np.einsum("hk,nhk->nh", q[t], k[first:t + 1])) * fade
+            near[t] = np.einsum("nh,nhv->hv", size, np.array(us))
             top = max(top, np.abs(S).max())
         top = max(top, np.abs(v[lo:hi]).max())
         state[slot] = S
-    return faults, top
+    return faults, top, near
 
 
 def delta_chunked(qkv, a, b, decay, dt, key_heads, heads, d, eps, S, chunk=64):

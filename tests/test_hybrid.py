@@ -29,7 +29,7 @@ def test_oracle_chunks_equal_tokens(rows):
     want, W = H.delta_chunked(x, a, b, decay, dt, 2, 4, 16, 1e-6, S[0])
     out = np.zeros((rows, 4, 16))
     state = S.copy()
-    faults, top = H.delta(x, a, b, decay, dt, [0, rows], [5], [0], 2, 4, 16, 1e-6, state, out)
+    faults, top, _ = H.delta(x, a, b, decay, dt, [0, rows], [5], [0], 2, 4, 16, 1e-6, state, out)
     assert faults == 0
     assert np.abs(out - want).max() < 1e-12 * top
     assert np.abs(state[0] - W).max() < 1e-12 * top

@@ -6,8 +6,10 @@ Tolerances. A result rounded to fp16 is within 2^-11 of its value or 2^-25 of a 
 fp32 sum of n terms of size m is off by about sqrt(n) 2^-24 m (roundings add like a random walk),
 and T updates of a state add their errors the same way, so a state entry is held to
 4 sqrt(d T) 2^-24 of the largest entry or value, four times what is expected; operands that are
-taken as two fp16 parts are good to 2^-22, less than the sums' own errors. A delta output is S^T q'
-with |q'| <= 1 / sqrt(d), so the sum of |q'| is at most 1 and the state's error bounds its own."""
+taken as two fp16 parts are good to 2^-21, less than the sums' own errors. A delta output is S^T q'
+with |q'| <= 1 / sqrt(d), so the sum of |q'| is at most 1 and the state's error bounds its own; the
+factors (q' . k'_j) exp(G - G_j) of the rows of an output's own chunk are rounded to fp16 on the way,
+which adds 2^-11 of the sum of those terms' sizes at most."""
 import ctypes
 
 import numpy as np
@@ -67,9 +69,10 @@ class Delta:
     def want(self):
         state = self.state.astype(np.float64)
         out = np.full((self.tokens, self.heads, self.d), 7.0)
-        faults, top = H.delta(self.x, self.a[:, :self.heads], self.b[:, :self.heads], self.decay.astype(np.float64),
+        faults, top, near = H.delta(self.x, self.a[:, :self.heads], self.b[:, :self.heads], self.decay.astype(np.float64),
                               self.dt.astype(np.float64), self.offset, self.pos, self.agent, self.key_heads, self.heads,
                               self.d, EPS, state, out)
+        self.round = 2.0 ** -11 * (np.abs(out) + near) + 2.0 ** -25      # of out and of its factors
         return out, state, faults, top
 
     def up(self):
@@ -106,7 +109,7 @@ class Delta:
         out, S = self.got()
         far = 4 * np.sqrt(self.d * max(1, max(self.lens))) * 2.0 ** -24 * top
         assert np.abs(S - state).max() <= far, (np.abs(S - state).max(), far)
-        off = np.abs(out - want) - (2.0 ** -11 * np.abs(want) + 2.0 ** -25 + far)
+        off = np.abs(out - want) - (self.round + far)
         assert off.max() <= 0, (off.max(), far)
         assert lib.aotx_model_faulted() == faults
         # slots that no sequence with rows names, bit for bit
@@ -197,7 +200,7 @@ def test_chunk_equals_steps(torch, lib):
     _, _, _, top = c.want()
     far = 8 * np.sqrt(128 * 70) * 2.0 ** -24 * top       # both sides' errors
     assert np.abs(S - S1).max() <= far
-    assert (np.abs(out - whole) - (2.0 ** -10 * np.abs(out) + 2.0 ** -24 + far)).max() <= 0
+    assert (np.abs(out - whole) - (2 * c.round + far)).max() <= 0
 
 
 def test_chunk_slots_missing_and_named_twice(torch, lib):
@@ -216,7 +219,7 @@ def test_chunk_offsets_out_of_order_stay_in_bounds(torch, lib, offset):
     c.up().call(lib)
     out, S = c.got()
     far = 4 * np.sqrt(128 * 120) * 2.0 ** -24 * top + 1e-6
-    assert np.abs(S - state).max() <= far and np.abs(out - want).max() <= far + 2.0 ** -11 * np.abs(want).max()
+    assert np.abs(S - state).max() <= far and (np.abs(out - want) <= far + c.round).all()
 
 
 @pytest.mark.parametrize("what,bad", [("v", np.inf), ("v", np.nan), ("k", np.nan), ("k", -np.inf), ("q", np.nan),
@@ -258,7 +261,7 @@ def test_chunk_inf_and_nan_reach_no_earlier_row(torch, lib, what, bad, at):
         near[:at, 1, 9] = True
         want, _, _, top = clean.want()
         far = 4 * np.sqrt(d * 130) * 2.0 ** -24 * top
-        assert (np.abs(out[near] - want[near]) <= 2.0 ** -11 * np.abs(want[near]) + 2.0 ** -25 + far).all()
+        assert (np.abs(out[near] - want[near]) <= clean.round[near] + far).all()
     assert np.array_equal(out[~hit & ~near], base[~hit & ~near])
     assert np.array_equal(S[~hit_state], S0[~hit_state])
     if what not in ("a", "b") or np.isnan(bad):
@@ -268,7 +271,7 @@ def test_chunk_inf_and_nan_reach_no_earlier_row(torch, lib, what, bad, at):
         want, state, _, top = c.want()
         far = 4 * np.sqrt(d * 130) * 2.0 ** -24 * top
         assert np.abs(S - state).max() <= far
-        assert (np.abs(out - want) - (2.0 ** -11 * np.abs(want) + 2.0 ** -25 + far)).max() <= 0
+        assert (np.abs(out - want) - (c.round + far)).max() <= 0
 
 
 # ---- convolution -----------------------------------------------------------------------------
