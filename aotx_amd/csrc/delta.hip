@@ -27,9 +27,7 @@ __global__ __launch_bounds__(256) void aotx_delta_rows_kernel(aotx_delta_args p)
     const unsigned int unit = blockIdx.x / SLICES, slice = blockIdx.x % SLICES;
     const unsigned int i = unit / p.heads, h = unit % p.heads;
     const unsigned int lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    unsigned int first, last;
-    aotx_seq_rows(p.seqs, &first, &last);
-    const aotx_seq_view seq = aotx_seq_of(p.seqs, i, first, last);
+    const aotx_seq_view seq = aotx_seq_of(p.seqs, i, aotx_seqs_read(p.seqs));
     if (seq.start >= seq.end) return;
     const unsigned int c4 = (threadIdx.x % LC) * 4u, rg = threadIdx.x / LC;
     const unsigned int col = slice * CS + c4;

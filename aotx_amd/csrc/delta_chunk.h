@@ -103,14 +103,14 @@ static __device__ __forceinline__ aotx_f4 aotx_mma(aotx_h8 a, aotx_h8 b, aotx_f4
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-/* Chunks of sequence `lane` and of the sequences before it, from the lanes' rows. */
-static __device__ __forceinline__ void aotx_delta_chunks(unsigned int b, unsigned int e, unsigned int *mine,
+/* Chunks of sequence `lane` and of the sequences before it. */
+static __device__ __forceinline__ void aotx_delta_chunks(const aotx_seq_lanes &l, unsigned int seqs, unsigned int *mine,
                                                          unsigned int *before)
 {
     const unsigned int lane = threadIdx.x & 63u;
-    const unsigned int n = (e - b + AOTX_DELTA_CHUNK - 1u) / AOTX_DELTA_CHUNK;
+    const unsigned int n = (l.end - l.start + AOTX_DELTA_CHUNK - 1u) / AOTX_DELTA_CHUNK;
     unsigned int sum = n;
-    for (unsigned int off = 1u; off < 64u; off <<= 1) {
+    for (unsigned int off = 1u; off < seqs; off <<= 1) {
         const unsigned int o = (unsigned int)__shfl_up((int)sum, off, 64);
         if (lane >= off) sum += o;
     }
@@ -166,17 +166,24 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
     const unsigned int w = (unsigned int)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const unsigned int c = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
 
-    unsigned int b, e, mine, before;
-    aotx_seq_rows(p.seqs, &b, &e);
-    aotx_delta_chunks(b, e, &mine, &before);
+    unsigned int mine, before;
+    const aotx_seq_lanes seqs = aotx_seqs_read(p.seqs);
+    aotx_delta_chunks(seqs, p.seqs.seqs, &mine, &before);
     const unsigned int i = (unsigned int)__popcll(__ballot(lane < p.seqs.seqs && before + mine <= c));
     if (i >= p.seqs.seqs) return;
-    const aotx_seq_view seq = aotx_seq_of(p.seqs, i, b, e);
+    const aotx_seq_view seq = aotx_seq_of(p.seqs, i, seqs);
     if (seq.refused) return;
     const unsigned int r0 = seq.start + (c - (unsigned int)__builtin_amdgcn_readlane((int)before, (int)i)) * 64u;
     const unsigned int n = seq.end - r0 < 64u ? seq.end - r0 : 64u;
     aotx_delta_chunk_work *to = p.work + (unsigned long long)c * p.heads + h;
 
+    /* what the gates need comes first: its way is the longest */
+    float ga = 0.0f, gb = 0.0f;
+    if (w == 0u) {
+        const unsigned long long gr = (unsigned long long)(r0 + (lane < n ? lane : n - 1u)) * p.ab_stride + h;
+        ga = p.a[gr];
+        gb = p.b[gr];
+    }
     /* rows of K and Q, columns 32 s + 8 g .. of row 16 w + m; rows past the chunk read as zeros */
     const unsigned int kh = h / p.group;
     const unsigned int row = 16u * w + m;
@@ -198,17 +205,12 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
     /* gates, a row a lane; sums of g in 64 bits, kept as two floats, so that differences of far
      * sums stay exact */
     if (w == 0u) {
-        const unsigned int gr = r0 + (lane < n ? lane : n - 1u);
-        float gate = aotx_delta_gate(p.a[(unsigned long long)gr * p.ab_stride + h], p.dt[h], p.decay[h]);
-        float rate = 1.0f / (1.0f + expf(-p.b[(unsigned long long)gr * p.ab_stride + h]));
+        float gate = aotx_delta_gate(ga, p.dt[h], p.decay[h]);
+        float rate = 1.0f / (1.0f + expf(-gb));
         const bool badgate = lane < n && (gate != gate || rate != rate);
         const unsigned long long badgates = __ballot(badgate);
         if (lane >= n || badgate) gate = rate = 0.0f;
-        double sum = (double)gate;
-        for (unsigned int off = 1u; off < 64u; off <<= 1) {
-            const double o = __shfl_up(sum, off, 64);
-            if (lane >= off) sum += o;
-        }
+        const double sum = aotx_wave_scan((double)gate);
         ghi[lane] = (float)sum;
         glo[lane] = (float)(sum - (double)(float)sum);
         near_end[lane] = expf((float)(__shfl(sum, (int)(lane | 15u), 64) - sum));
@@ -357,16 +359,21 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
     }
     __builtin_amdgcn_wave_barrier();
 
-    /* inverse of the diagonal block by substitution, a column a lane */
+    /* inverse of the diagonal block by substitution, a column a lane; every value found is taken
+     * from all rows below at once, which do not wait for one another */
     {
         float x[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            float v = m == (unsigned int)r ? 1.0f : 0.0f;
+        for (int r = 0; r < 16; ++r) x[r] = m == (unsigned int)r ? 1.0f : 0.0f;
+        aotx_f4 row4[16][4];
 #pragma unroll
-            for (int q = 0; q < r; ++q) v -= M[16u * w + r][16u * w + q] * x[q];
-            x[r] = v;
-        }
+        for (int r = 1; r < 16; ++r)
+#pragma unroll
+            for (int q = 0; 4 * q < r; ++q) row4[r][q] = *(const aotx_f4 *)&M[16u * w + r][16u * w + 4 * q];
+#pragma unroll
+        for (int q = 0; q < 15; ++q)
+#pragma unroll
+            for (int r = q + 1; r < 16; ++r) x[r] -= row4[r][q / 4][q % 4] * x[q];
         if (g == 0u)
 #pragma unroll
             for (int r = 0; r < 16; ++r) Dm[w][r][m] = x[r];
@@ -845,10 +852,10 @@ __global__ __launch_bounds__(256, 2) void aotx_delta_across(aotx_delta_args p)
     if (unit >= p.seqs.seqs * p.heads) return;
     const unsigned int i = unit / p.heads;
     k.h = unit % p.heads;
-    unsigned int b, e, mine, before;
-    aotx_seq_rows(p.seqs, &b, &e);
-    aotx_delta_chunks(b, e, &mine, &before);
-    k.seq = aotx_seq_of(p.seqs, i, b, e);
+    unsigned int mine, before;
+    const aotx_seq_lanes seqs = aotx_seqs_read(p.seqs);
+    aotx_delta_chunks(seqs, p.seqs.seqs, &mine, &before);
+    k.seq = aotx_seq_of(p.seqs, i, seqs);
     k.c0 = (unsigned int)__builtin_amdgcn_readlane((int)before, (int)i);
     if (k.seq.start >= k.seq.end) return;
     k.chunks = (k.seq.end - k.seq.start + 63u) / 64u;

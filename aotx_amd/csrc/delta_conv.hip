@@ -37,11 +37,10 @@ __global__ __launch_bounds__(256) void aotx_delta_conv_kernel(aotx_conv_args p)
         if (p.bias != nullptr) bias = *(const aotx_f4 *)(p.bias + c);
     }
     /* the first sequence with rows from t0 on: those that end at or before t0 come first */
-    unsigned int b, e;
-    aotx_seq_rows(p.seqs, &b, &e);
-    unsigned int i = (unsigned int)__popcll(__ballot(lane < p.seqs.seqs && e <= t0));
+    const aotx_seq_lanes seqs = aotx_seqs_read(p.seqs);
+    unsigned int i = (unsigned int)__popcll(__ballot(lane < p.seqs.seqs && seqs.end <= t0));
     for (; i < p.seqs.seqs; ++i) {
-        const aotx_seq_view seq = aotx_seq_of(p.seqs, i, b, e);
+        const aotx_seq_view seq = aotx_seq_of(p.seqs, i, seqs);
         if (seq.start >= stop) break;
         /* The run that holds a sequence's first row takes its first W - 1 rows, so that no
          * other run needs the slot's rows, which that run replaces. */

@@ -28,50 +28,46 @@ struct aotx_seq_view {
     bool refused;               /* no slot, or a slot that an earlier sequence has */
 };
 
-/* Rows of sequence `lane`, for the first `seqs` lanes of a wave (all 64 call this): in bounds,
- * and none before an earlier sequence's last, whatever the offsets hold. */
-static __device__ __forceinline__ void aotx_seq_rows(const aotx_seqs &s, unsigned int *start,
-                                                     unsigned int *end)
+/* The call's sequences as a wave holds them, sequence j in lane j (at most 64 a call). */
+struct aotx_seq_lanes {
+    unsigned int start, end;    /* rows: in bounds, none before an earlier sequence's last, whatever the offsets hold */
+    unsigned int slot, pos;
+};
+
+static __device__ __forceinline__ aotx_seq_lanes aotx_seqs_read(const aotx_seqs &s)
 {
     const unsigned int lane = threadIdx.x & 63u;
-    unsigned int b = 0u, e = 0u;
-    if (s.offset == nullptr) {
-        if (lane < s.seqs) {
-            b = lane;
-            e = lane + 1u;
-        }
-    } else {
-        if (lane < s.seqs) {
-            b = s.offset[lane];
-            e = s.offset[lane + 1u];
-            b = b < s.tokens ? b : s.tokens;
-            e = e < s.tokens ? e : s.tokens;
-        }
-        for (unsigned int off = 1u; off < s.seqs; off <<= 1) {
-            const unsigned int o = (unsigned int)__shfl_up((int)b, off, 64);
-            if (lane >= off && o > b) b = o;
-        }
-        if (e < b) e = b;
+    aotx_seq_lanes v = {0u, 0u, 0xFFFFFFFFu, 0u};
+    if (lane < s.seqs) {
+        v.start = s.offset != nullptr ? s.offset[lane] : lane;
+        v.end = s.offset != nullptr ? s.offset[lane + 1u] : lane + 1u;
+        v.slot = s.agent[lane];
+        v.pos = s.pos[lane];
     }
-    *start = b;
-    *end = e;
+    if (s.offset != nullptr) {
+        v.start = v.start < s.tokens ? v.start : s.tokens;
+        v.end = v.end < s.tokens ? v.end : s.tokens;
+        if (lane >= s.seqs) v.start = v.end = 0u;
+        for (unsigned int off = 1u; off < s.seqs; off <<= 1) {
+            const unsigned int o = (unsigned int)__shfl_up((int)v.start, off, 64);
+            if (lane >= off && o > v.start) v.start = o;
+        }
+        if (v.end < v.start) v.end = v.start;
+    }
+    return v;
 }
 
-/* Sequence i (wave-uniform), read by all 64 lanes of a wave: lane j looks at sequence j, which
- * tells whether an earlier one with rows has the same slot (at most 64 sequences a call). b and
- * e are the lanes' rows from aotx_seq_rows. */
-static __device__ __forceinline__ aotx_seq_view aotx_seq_of(const aotx_seqs &s, unsigned int i,
-                                                            unsigned int b, unsigned int e)
+/* Sequence i (wave-uniform): a ballot tells whether an earlier one with rows has the same slot. */
+static __device__ __forceinline__ aotx_seq_view aotx_seq_of(const aotx_seqs &s, unsigned int i, const aotx_seq_lanes &l)
 {
     const unsigned int lane = threadIdx.x & 63u;
-    const unsigned int a = lane < s.seqs ? s.agent[lane] : 0xFFFFFFFFu;
     aotx_seq_view v;
-    v.start = (unsigned int)__builtin_amdgcn_readlane((int)b, (int)i);
-    v.end = (unsigned int)__builtin_amdgcn_readlane((int)e, (int)i);
-    v.slot = (unsigned int)__builtin_amdgcn_readlane((int)a, (int)i);
-    const unsigned long long same = __ballot(lane < i && b < e && a == v.slot);
+    v.start = (unsigned int)__builtin_amdgcn_readlane((int)l.start, (int)i);
+    v.end = (unsigned int)__builtin_amdgcn_readlane((int)l.end, (int)i);
+    v.slot = (unsigned int)__builtin_amdgcn_readlane((int)l.slot, (int)i);
+    const unsigned long long same = __ballot(lane < i && l.start < l.end && l.slot == v.slot);
     v.refused = v.slot >= s.slots || same != 0ull;
-    v.fresh = s.pos[i] == 0u;
+    v.fresh = (unsigned int)__builtin_amdgcn_readlane((int)l.pos, (int)i) == 0u;
     return v;
 }
 
@@ -79,6 +75,26 @@ static __device__ __forceinline__ aotx_seq_view aotx_seq_of(const aotx_seqs &s, 
 static __device__ __forceinline__ float aotx_wave_sum(float v)
 {
     for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+
+/* Running sum of 64 lanes' values, in 64 bits. */
+template <int CTRL, int ROWS>
+static __device__ __forceinline__ double aotx_dpp_add(double v)
+{
+    const long long b = __builtin_bit_cast(long long, v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xF, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xF, false);
+    return v + __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned int)lo);
+}
+static __device__ __forceinline__ double aotx_wave_scan(double v)
+{
+    v = aotx_dpp_add<0x111, 0xF>(v);        /* lanes 1, 2, 4 and 8 before, within rows of 16 */
+    v = aotx_dpp_add<0x112, 0xF>(v);
+    v = aotx_dpp_add<0x114, 0xF>(v);
+    v = aotx_dpp_add<0x118, 0xF>(v);
+    v = aotx_dpp_add<0x142, 0xA>(v);        /* the last lane of row 0 to row 1, of row 2 to row 3 */
+    v = aotx_dpp_add<0x143, 0xC>(v);        /* lane 31 to rows 2 and 3 */
     return v;
 }
 
