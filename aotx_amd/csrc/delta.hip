@@ -154,7 +154,7 @@ static int aotx_delta_fill(aotx_delta_args *p, const void *qkv, unsigned int str
     if (head_dim != 64u && head_dim != 128u) return 1;
     if (heads == 0u || heads > 256u || key_heads == 0u || heads % key_heads != 0u) return 1;
     if (stride % 8u != 0u || stride < (2u * key_heads + heads) * head_dim || stride > (1u << 22)) return 1;
-    if (ab_stride < heads || !(eps > 0.0f)) return 1;
+    if (ab_stride < heads || !(eps >= 1e-30f)) return 1;
     if (seqs > AOTX_SLOTS || slots == 0u || slots > AOTX_SLOTS || tokens > (1u << 20)) return 1;
     if (!aotx_aligned16(qkv) || !aotx_aligned16(state) || !aotx_aligned16(out)) return 1;
     p->qkv = (const unsigned short *)qkv;

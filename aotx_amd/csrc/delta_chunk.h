@@ -150,18 +150,133 @@ static __device__ __forceinline__ unsigned short aotx_rows_2(const aotx_rows_vie
  * one row i and four columns j along its registers, as the operands above need them.
  * ------------------------------------------------------------------------------------- */
 template <int D>
+struct aotx_delta_within_lds {
+    union {
+        aotx_h8 kfrag[4][D / 32][64];                       /* rows of K, as operands */
+        __align__(16) unsigned short tp[2][64][72];         /* T, to be read by rows */
+    };
+    __align__(16) float diag[4][16][20];                    /* M's diagonal blocks, then their inverses */
+    __align__(16) unsigned short below[2][48][56];          /* M's blocks below them, rows 16 .. 63, two parts */
+    __align__(16) float ghi[64], glo[64], near_end[64], beta[64], rk[64], rq[64], ks[64];
+    __align__(16) unsigned int vm[4][64];
+    unsigned int badk[4], badv[4], badg;
+};
+
+/* P and M of row 16 W + m. Between blocks, exp(G_i - G_j) is the product of two factors by way of
+ * the last row of j's block: both are at most 1, and one exponential a row serves four columns. */
+template <int D, int W>
+static __device__ __forceinline__ void aotx_delta_pairs(aotx_delta_within_lds<D> &lds, aotx_delta_chunk_work *to,
+                                                        const aotx_h8 (&kf)[D / 32], const aotx_h8 (&qf)[D / 32], float inv,
+                                                        float qinv)
+{
+    constexpr int KS = D / 32;
+    const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4, row = 16u * W + m;
+    const float gi = lds.ghi[row], gil = lds.glo[row], bi = lds.beta[row] * inv;
+    aotx_f4 pt[4];
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt) pt[jt] = aotx_f4{0, 0, 0, 0};
+#pragma unroll
+    for (int jt = 0; jt <= W; ++jt) {
+        aotx_f4 kks = {0, 0, 0, 0}, qks = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const aotx_h8 kj = lds.kfrag[jt][s][lane];
+            kks = aotx_mma(kj, kf[s], kks);
+            qks = aotx_mma(kj, qf[s], qks);
+        }
+        const unsigned int j0 = 16u * jt + 4u * g;
+        const aotx_f4 rkj = *(const aotx_f4 *)&lds.rk[j0];
+        if (jt == W) {
+            const aotx_f4 gj = *(const aotx_f4 *)&lds.ghi[j0], gjl = *(const aotx_f4 *)&lds.glo[j0];
+            aotx_f4 fade;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                /* above the diagonal the exponential is of a positive number, and of no use */
+                fade[r] = expf((gi - gj[r]) + (gil - gjl[r])) * rkj[r];
+                fade[r] = row >= j0 + r ? fade[r] : 0.0f;
+                kks[r] = row > j0 + r ? kks[r] : 0.0f;
+                qks[r] = row >= j0 + r ? qks[r] : 0.0f;
+            }
+            *(aotx_f4 *)&lds.diag[W][m][4u * g] = kks * fade * bi;
+            pt[jt] = qks * fade * qinv;
+        } else {
+            const float from = expf((gi - lds.ghi[16 * jt + 15]) + (gil - lds.glo[16 * jt + 15]));
+            const aotx_f4 fade = *(const aotx_f4 *)&lds.near_end[j0] * rkj * from;
+            aotx_h4 hi, lo;
+            aotx_split4(kks * fade * bi, &hi, &lo);
+            *(aotx_h4 *)&lds.below[0][row - 16u][j0] = hi;
+            *(aotx_h4 *)&lds.below[1][row - 16u][j0] = lo;
+            pt[jt] = qks * fade * qinv;
+        }
+    }
+#pragma unroll
+    for (int s = 0; s <= W / 2; ++s) {
+        aotx_h8 o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            o[r] = (_Float16)pt[2 * s][r];
+            o[4 + r] = (_Float16)pt[2 * s + 1][r];
+        }
+        *(aotx_h8 *)((char *)to->p[W][s] + lane * 16u) = o;
+    }
+}
+
+/* a b c: both in two parts, 16 x 16 blocks; b in accumulator order */
+static __device__ __forceinline__ aotx_f4 aotx_mma_parts(aotx_h4 ahi, aotx_h4 alo, aotx_h4 bhi, aotx_h4 blo, aotx_f4 c)
+{
+    c = __builtin_amdgcn_mfma_f32_16x16x16f16(ahi, blo, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x16f16(alo, bhi, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(ahi, bhi, c, 0, 0, 0);
+}
+
+/* Column W of blocks of T, downwards: T_b = -D_b (sum of M_bq T_q), then times beta. A block in
+ * accumulator order is the right operand of the next product as it stands. */
+template <int D, int W>
+static __device__ __forceinline__ void aotx_delta_column(aotx_delta_within_lds<D> &lds)
+{
+    const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4;
+    const unsigned int row = 16u * W + m, at = aotx_delta_place(row);
+    const float bj = lds.beta[row];
+    aotx_f4 tc[4];
+    aotx_h4 hi[4], lo[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) tc[0][r] = lds.diag[W][4u * g + r][m];
+    aotx_split4(tc[0], &hi[0], &lo[0]);
+#pragma unroll
+    for (int off = 1; off < 4 - W; ++off) {
+        const int bt = W + off;
+        aotx_f4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int q = 0; q < off; ++q)
+            acc = aotx_mma_parts(*(const aotx_h4 *)&lds.below[0][16 * (bt - 1) + m][16 * (W + q) + 4u * g],
+                                 *(const aotx_h4 *)&lds.below[1][16 * (bt - 1) + m][16 * (W + q) + 4u * g], hi[q], lo[q], acc);
+        aotx_h4 dhi, dlo, yhi, ylo;
+        aotx_split4(*(const aotx_f4 *)&lds.diag[bt][m][4u * g], &dhi, &dlo);
+        aotx_split4(-acc, &yhi, &ylo);
+        tc[off] = aotx_mma_parts(dhi, dlo, yhi, ylo, aotx_f4{0, 0, 0, 0});
+        aotx_split4(tc[off], &hi[off], &lo[off]);
+    }
+#pragma unroll
+    for (int off = 0; off < 4 - W; ++off) {
+        aotx_h4 th, tl;
+        aotx_split4(tc[off] * bj, &th, &tl);
+        const aotx_u16x4 hb = __builtin_bit_cast(aotx_u16x4, th), lb = __builtin_bit_cast(aotx_u16x4, tl);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            lds.tp[0][16u * (W + off) + 4u * g + r][at] = hb[r];
+            lds.tp[1][16u * (W + off) + 4u * g + r][at] = lb[r];
+        }
+    }
+    if (W & 1)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) lds.tp[0][16u * (W & 2) + 4u * g + r][at] = lds.tp[1][16u * (W & 2) + 4u * g + r][at] = 0;
+}
+
+template <int D>
 __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
 {
     constexpr int KS = D / 32;
-    __shared__ union {
-        aotx_h8 kfrag[4][KS][64];                           /* rows of K, as operands */
-        __align__(16) unsigned short tp[2][64][72];         /* T, to be read by rows */
-    } lds;
-    __shared__ __align__(16) float M[64][68];
-    __shared__ __align__(16) float Dm[4][16][20];
-    __shared__ __align__(16) float ghi[64], glo[64], beta[64], rk[64], rq[64], ks[64], near_end[64];
-    __shared__ __align__(16) unsigned int vm[4][64];
-    __shared__ unsigned int badk[4], badv[4], badg;
+    __shared__ aotx_delta_within_lds<D> lds;
     const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4;
     const unsigned int w = (unsigned int)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const unsigned int c = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
@@ -211,11 +326,11 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
         const unsigned long long badgates = __ballot(badgate);
         if (lane >= n || badgate) gate = rate = 0.0f;
         const double sum = aotx_wave_scan((double)gate);
-        ghi[lane] = (float)sum;
-        glo[lane] = (float)(sum - (double)(float)sum);
-        near_end[lane] = expf((float)(__shfl(sum, (int)(lane | 15u), 64) - sum));
-        beta[lane] = rate;
-        if (lane == 0u) badg = badgates != 0ull ? (unsigned int)__builtin_ctzll(badgates) : 64u;
+        lds.ghi[lane] = (float)sum;
+        lds.glo[lane] = (float)(sum - (double)(float)sum);
+        lds.near_end[lane] = expf((float)(__shfl(sum, (int)(lane | 15u), 64) - sum));
+        lds.beta[lane] = rate;
+        if (lane == 0u) lds.badg = badgates != 0ull ? (unsigned int)__builtin_ctzll(badgates) : 64u;
     }
     float kk = 0.0f, qq = 0.0f;
 #pragma unroll
@@ -238,24 +353,24 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
         lds.kfrag[w][s][lane] = kf[s];
     }
     const unsigned long long badrows = __ballot(bad) & 0xFFFFull;
-    if (lane == 0u) badk[w] = badrows != 0ull ? 16u * w + (unsigned int)__builtin_ctzll(badrows) : 64u;
-    const float len = sqrtf(kk + p.eps), inv = 1.0f / len;
-    const float qinv = 1.0f / sqrtf(qq + p.eps) * (D == 128 ? 0.08838834764831845f : 0.125f);
-    int ex;
-    (void)frexpf(len, &ex);
+    if (lane == 0u) lds.badk[w] = badrows != 0ull ? 16u * w + (unsigned int)__builtin_ctzll(badrows) : 64u;
+    const float inv = __builtin_amdgcn_rsqf(kk + p.eps);
+    const float qinv = __builtin_amdgcn_rsqf(qq + p.eps) * (D == 128 ? 0.08838834764831845f : 0.125f);
+    /* 2^ex: the row's length over it is 1/2 to 1 */
+    const int ex = __builtin_amdgcn_frexp_expf(__builtin_amdgcn_sqrtf(kk + p.eps));
     if (g == 0u) {
-        rk[row] = inv;
-        ks[row] = ldexpf(inv, ex);
-        rq[row] = qinv;
+        lds.rk[row] = inv;
+        lds.ks[row] = ldexpf(inv, ex);
+        lds.rq[row] = qinv;
     }
     if (h % p.group == 0u) {
         aotx_h8 *k = aotx_delta_rows_of(p, c, kh, D) + w * KS * 64u, *q = k + 8u * D;
+        /* over 2^ex in two steps, each a number of fp16; ex below -28 is of rows of zeros */
+        const int one = ex > 14 ? 14 : ex < -14 ? -14 : ex, two = ex - one < -14 ? -14 : ex - one;
+        const _Float16 a = (_Float16)ldexpf(1.0f, -one), z = (_Float16)ldexpf(1.0f, -two);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            aotx_h8 o;
-#pragma unroll
-            for (int v = 0; v < 8; ++v) o[v] = (_Float16)ldexpf((float)kf[s][v], -ex);
-            *(aotx_h8 *)((char *)(k + s * 64) + lane * 16u) = o;
+            *(aotx_h8 *)((char *)(k + s * 64) + lane * 16u) = kf[s] * a * z;
             *(aotx_h8 *)((char *)(q + s * 64) + lane * 16u) = qf[s];
         }
     }
@@ -277,7 +392,7 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
                 }
         }
         const unsigned long long told = __ballot(none);
-        if (lane == 0u) badv[w] = told != 0ull ? 1u : 0u;
+        if (lane == 0u) lds.badv[w] = told != 0ull ? 1u : 0u;
         typedef unsigned int u4 __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (unsigned int off = D / 8; off < 64u; off <<= 1) {
@@ -286,77 +401,35 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
             for (int x = 0; x < 4; ++x) o[x] = (unsigned int)__shfl_xor((int)o[x], off, 64);
             top = __builtin_elementwise_max(top, __builtin_bit_cast(aotx_u16x8, o));
         }
-        if (lane < D / 8) *(aotx_u16x8 *)((unsigned short *)vm[w] + lane * 8u) = top;
+        if (lane < D / 8) *(aotx_u16x8 *)((unsigned short *)lds.vm[w] + lane * 8u) = top;
     }
     __syncthreads();
 
     if (w == 0u) {
-        const float last = (ghi[63] - ghi[lane]) + (glo[63] - glo[lane]), all = expf(ghi[lane]);
-        to->of_k[lane] = all * ks[lane];
-        to->of_q[lane] = all * rq[lane];
-        to->of_u[lane] = expf(last) * ks[lane];
+        const float last = (lds.ghi[63] - lds.ghi[lane]) + (lds.glo[63] - lds.glo[lane]), all = expf(lds.ghi[lane]);
+        to->of_k[lane] = all * lds.ks[lane];
+        to->of_q[lane] = all * lds.rq[lane];
+        to->of_u[lane] = expf(last) * lds.ks[lane];
         if (lane == 0u) {
-            unsigned int first = badg;
-            for (int v = 0; v < 4; ++v) first = badk[v] < first ? badk[v] : first;
-            to->fade = expf(ghi[63]);
-            to->odd = first | (badv[0] | badv[1] | badv[2] | badv[3]) << 8;
+            unsigned int first = lds.badg;
+            for (int v = 0; v < 4; ++v) first = lds.badk[v] < first ? lds.badk[v] : first;
+            to->fade = expf(lds.ghi[63]);
+            to->odd = first | (lds.badv[0] | lds.badv[1] | lds.badv[2] | lds.badv[3]) << 8;
         }
     } else if (w == 1u) {
         if (lane < D / 2) {             /* two columns a lane */
             typedef unsigned short u2 __attribute__((ext_vector_type(2)));
-            u2 v = __builtin_bit_cast(u2, vm[0][lane]);
+            u2 v = __builtin_bit_cast(u2, lds.vm[0][lane]);
 #pragma unroll
-            for (int x = 1; x < 4; ++x) v = __builtin_elementwise_max(v, __builtin_bit_cast(u2, vm[x][lane]));
+            for (int x = 1; x < 4; ++x) v = __builtin_elementwise_max(v, __builtin_bit_cast(u2, lds.vm[x][lane]));
             *(unsigned short *)&to->vmax[2u * lane] = (unsigned short)((v[0] >> 10) | ((v[1] >> 10) << 8));
         }
     }
 
-    /* P and M of row 16 w + m. Between blocks, exp(G_i - G_j) is the product of two factors by
-     * way of the last row of j's block: both are at most 1, and one exponential a row serves
-     * four columns. */
-    const float gi = ghi[row], gil = glo[row], bi = beta[row] * inv;
-    aotx_f4 pt[4];
-#pragma unroll
-    for (unsigned int jt = 0; jt < 4u; ++jt) {
-        pt[jt] = aotx_f4{0, 0, 0, 0};
-        if (jt > w) continue;
-        aotx_f4 kks = {0, 0, 0, 0}, qks = {0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const aotx_h8 kj = lds.kfrag[jt][s][lane];
-            kks = aotx_mma(kj, kf[s], kks);
-            qks = aotx_mma(kj, qf[s], qks);
-        }
-        const unsigned int j0 = 16u * jt + 4u * g;
-        const aotx_f4 rkj = *(const aotx_f4 *)&rk[j0];
-        aotx_f4 fade;
-        if (jt == w) {
-            const aotx_f4 gj = *(const aotx_f4 *)&ghi[j0], gjl = *(const aotx_f4 *)&glo[j0];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                fade[r] = expf((gi - gj[r]) + (gil - gjl[r])) * rkj[r];
-                kks[r] = row > j0 + r ? kks[r] : 0.0f;
-                qks[r] = row >= j0 + r ? qks[r] : 0.0f;
-                fade[r] = row >= j0 + r ? fade[r] : 0.0f;
-            }
-        } else {
-            const float from = expf((gi - ghi[16u * jt + 15u]) + (gil - glo[16u * jt + 15u]));
-            fade = *(const aotx_f4 *)&near_end[j0] * rkj * from;
-        }
-        *(aotx_f4 *)&M[row][j0] = kks * fade * bi;
-        pt[jt] = qks * fade * qinv;
-    }
-#pragma unroll
-    for (unsigned int s = 0; s < 2u; ++s) {
-        if (s > w / 2u) continue;
-        aotx_h8 o;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            o[r] = (_Float16)pt[2u * s][r];
-            o[4 + r] = (_Float16)pt[2u * s + 1u][r];
-        }
-        *(aotx_h8 *)((char *)to->p[w][s] + lane * 16u) = o;
-    }
+    if (w == 0u) aotx_delta_pairs<D, 0>(lds, to, kf, qf, inv, qinv);
+    else if (w == 1u) aotx_delta_pairs<D, 1>(lds, to, kf, qf, inv, qinv);
+    else if (w == 2u) aotx_delta_pairs<D, 2>(lds, to, kf, qf, inv, qinv);
+    else aotx_delta_pairs<D, 3>(lds, to, kf, qf, inv, qinv);
     __builtin_amdgcn_wave_barrier();
 
     /* inverse of the diagonal block by substitution, a column a lane; every value found is taken
@@ -369,60 +442,21 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
 #pragma unroll
         for (int r = 1; r < 16; ++r)
 #pragma unroll
-            for (int q = 0; 4 * q < r; ++q) row4[r][q] = *(const aotx_f4 *)&M[16u * w + r][16u * w + 4 * q];
+            for (int q = 0; 4 * q < r; ++q) row4[r][q] = *(const aotx_f4 *)&lds.diag[w][r][4 * q];
 #pragma unroll
         for (int q = 0; q < 15; ++q)
 #pragma unroll
             for (int r = q + 1; r < 16; ++r) x[r] -= row4[r][q / 4][q % 4] * x[q];
         if (g == 0u)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) Dm[w][r][m] = x[r];
+            for (int r = 0; r < 16; ++r) lds.diag[w][r][m] = x[r];
     }
     __syncthreads();
 
-    /* Column w of blocks of the inverse, downwards: T_b = -D_b (sum of M_bq T_q). A block in
-     * accumulator order is the right operand of the next product as it stands. */
-    aotx_f4 tc[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) tc[0][r] = Dm[w][4u * g + r][m];
-#pragma unroll
-    for (unsigned int off = 1; off < 4u; ++off) {
-        const unsigned int bt = w + off;
-        if (bt > 3u) break;
-        aotx_f4 acc = {0, 0, 0, 0};
-#pragma unroll
-        for (unsigned int q = 0; q < off; ++q) {
-            const aotx_f4 a = *(const aotx_f4 *)&M[16u * bt + m][16u * (w + q) + 4u * g];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], tc[q][r], acc, 0, 0, 0);
-        }
-        const aotx_f4 a = *(const aotx_f4 *)&Dm[bt][m][4u * g];
-        aotx_f4 t = {0, 0, 0, 0};
-#pragma unroll
-        for (int r = 0; r < 4; ++r) t = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], -acc[r], t, 0, 0, 0);
-        tc[off] = t;
-    }
-    {
-        const unsigned int at = aotx_delta_place(row);
-        const float bj = beta[row];
-#pragma unroll
-        for (unsigned int off = 0; off < 4u; ++off) {
-            const unsigned int bt = w + off;
-            if (bt > 3u) break;
-            aotx_h4 hi, lo;
-            aotx_split4(tc[off] * bj, &hi, &lo);
-            const aotx_u16x4 hb = __builtin_bit_cast(aotx_u16x4, hi), lb = __builtin_bit_cast(aotx_u16x4, lo);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                lds.tp[0][16u * bt + 4u * g + r][at] = hb[r];
-                lds.tp[1][16u * bt + 4u * g + r][at] = lb[r];
-            }
-        }
-        if (w & 1u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                lds.tp[0][16u * (w - 1u) + 4u * g + r][at] = lds.tp[1][16u * (w - 1u) + 4u * g + r][at] = 0;
-    }
+    if (w == 0u) aotx_delta_column<D, 0>(lds);
+    else if (w == 1u) aotx_delta_column<D, 1>(lds);
+    else if (w == 2u) aotx_delta_column<D, 2>(lds);
+    else aotx_delta_column<D, 3>(lds);
     __syncthreads();
 #pragma unroll
     for (unsigned int s = 0; s < 2u; ++s) {

@@ -63,7 +63,7 @@ int aotx_delta_conv(const float *x, unsigned int stride, const float *w, const f
  * t at a + t * ab_stride, [heads] values. decay, dt fp32 [heads]; decay at most 0 (g above 0
  * is taken as 0). state fp32 [slots][heads][head_dim][head_dim]. out fp16
  * [tokens][heads][head_dim]. head_dim 64 or 128, key_heads divides heads, at most 256 heads,
- * eps > 0; stride a multiple of 8 up to 2^22; qkv, state and out 16-byte aligned. All arithmetic on the
+ * eps at least 1e-30; stride a multiple of 8 up to 2^22; qkv, state and out 16-byte aligned. All arithmetic on the
  * state is fp32 or as near (the products of aotx_delta_chunk take their operands as two fp16
  * parts each). A value of Inf or NaN reaches the rows from its own on and no earlier ones.
  *

@@ -110,7 +110,7 @@ def _rope(**change):
     dict(agent=None), dict(state=None), dict(out=None), dict(qkv=A4), dict(state=A4), dict(out=A4),
     dict(head_dim=96), dict(head_dim=0), dict(heads=3, key_heads=2), dict(heads=0), dict(key_heads=0),
     dict(heads=512, stride=1 << 20), dict(stride=511), dict(stride=504), dict(stride=516), dict(ab_stride=1),
-    dict(eps=0.0), dict(eps=float("nan")), dict(slots=0), dict(slots=65)])
+    dict(eps=0.0), dict(eps=1e-31), dict(eps=float("nan")), dict(slots=0), dict(slots=65), dict(stride=(1 << 22) + 8)])
 def test_delta_refusals(lib, change):
     assert lib.aotx_delta_step(*{**STEP, **change}.values()) == 1
     assert lib.aotx_delta_chunk(*{**CHUNK, **change}.values()) == 1
