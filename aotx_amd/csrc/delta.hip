@@ -216,7 +216,7 @@ template <int D>
 static void aotx_delta_chunked(const aotx_delta_args &p, hipStream_t s)
 {
     constexpr unsigned int NT = 1u, slices = D / (16u * NT);
-    hipLaunchKernelGGL((aotx_delta_within<D>), dim3(p.chunks * p.heads), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((aotx_delta_within<D>), dim3(p.chunks * p.heads), dim3(320), 0, s, p);
     AOTX_LAUNCH_CHECK();
     const unsigned int units = (p.seqs.seqs * p.heads + 7u) / 8u * 8u;
     hipLaunchKernelGGL((aotx_delta_across<D, NT>), dim3(units * slices), dim3(256), 0, s, p);

@@ -145,8 +145,8 @@ static __device__ __forceinline__ unsigned short aotx_rows_2(const aotx_rows_vie
 }
 
 /* ---------------------------------------------------------------------------------------
- * T, P, K^T and the row factors of one chunk and head; a workgroup of four waves, wave w has
- * rows 16 w .. 16 w + 15. The products are taken transposed (K_j Q_i^T), so that a lane holds
+ * T, P and the row factors of one chunk and head, and K and Q as operands; a workgroup of five
+ * waves, wave w < 4 has rows 16 w .. 16 w + 15, wave 4 the gates of all. The products are taken transposed (K_j Q_i^T), so that a lane holds
  * one row i and four columns j along its registers, as the operands above need them.
  * ------------------------------------------------------------------------------------- */
 template <int D>
@@ -159,7 +159,7 @@ struct aotx_delta_within_lds {
     __align__(16) unsigned short below[2][48][56];          /* M's blocks below them, rows 16 .. 63, two parts */
     __align__(16) float ghi[64], glo[64], near_end[64], beta[64], rk[64], rq[64], ks[64];
     __align__(16) unsigned int vm[4][64];
-    unsigned int badk[4], badv[4], badg;
+    unsigned int badk[4], badv[4];
 };
 
 /* P and M of row 16 W + m. Between blocks, exp(G_i - G_j) is the product of two factors by way of
@@ -172,7 +172,7 @@ static __device__ __forceinline__ void aotx_delta_pairs(aotx_delta_within_lds<D>
     constexpr int KS = D / 32;
     const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4, row = 16u * W + m;
     const float gi = lds.ghi[row], gil = lds.glo[row], bi = lds.beta[row] * inv;
-    aotx_f4 pt[4];
+    aotx_f4 pt[4], block;
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt) pt[jt] = aotx_f4{0, 0, 0, 0};
 #pragma unroll
@@ -197,7 +197,7 @@ static __device__ __forceinline__ void aotx_delta_pairs(aotx_delta_within_lds<D>
                 kks[r] = row > j0 + r ? kks[r] : 0.0f;
                 qks[r] = row >= j0 + r ? qks[r] : 0.0f;
             }
-            *(aotx_f4 *)&lds.diag[W][m][4u * g] = kks * fade * bi;
+            block = kks * fade * bi;
             pt[jt] = qks * fade * qinv;
         } else {
             const float from = expf((gi - lds.ghi[16 * jt + 15]) + (gil - lds.glo[16 * jt + 15]));
@@ -219,6 +219,25 @@ static __device__ __forceinline__ void aotx_delta_pairs(aotx_delta_within_lds<D>
         }
         *(aotx_h8 *)((char *)to->p[W][s] + lane * 16u) = o;
     }
+    /* inverse of 1 + the diagonal block by substitution, a column a lane; every value found is
+     * taken from all rows below at once, which do not wait for one another */
+    *(aotx_f4 *)&lds.diag[W][m][4u * g] = block;
+    __builtin_amdgcn_wave_barrier();
+    float x[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = m == (unsigned int)r ? 1.0f : 0.0f;
+    aotx_f4 row4[16][4];
+#pragma unroll
+    for (int r = 1; r < 16; ++r)
+#pragma unroll
+        for (int q = 0; 4 * q < r; ++q) row4[r][q] = *(const aotx_f4 *)&lds.diag[W][r][4 * q];
+#pragma unroll
+    for (int q = 0; q < 15; ++q)
+#pragma unroll
+        for (int r = q + 1; r < 16; ++r) x[r] -= row4[r][q / 4][q % 4] * x[q];
+    if (g == 0u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) lds.diag[W][r][m] = x[r];
 }
 
 /* a b c: both in two parts, 16 x 16 blocks; b in accumulator order */
@@ -272,8 +291,50 @@ static __device__ __forceinline__ void aotx_delta_column(aotx_delta_within_lds<D
         for (int r = 0; r < 4; ++r) lds.tp[0][16u * (W & 2) + 4u * g + r][at] = lds.tp[1][16u * (W & 2) + 4u * g + r][at] = 0;
 }
 
+/* The fifth wave: gates, a row a lane, and what follows from them. Sums of g are in 64 bits,
+ * kept as two floats, so that differences of far sums stay exact. */
 template <int D>
-__global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
+static __device__ __forceinline__ void aotx_delta_rates(const aotx_delta_args &p, aotx_delta_within_lds<D> &lds,
+                                                        aotx_delta_chunk_work *to, unsigned int r0, unsigned int n,
+                                                        unsigned int h)
+{
+    const unsigned int lane = threadIdx.x & 63u;
+    const unsigned long long at = (unsigned long long)(r0 + (lane < n ? lane : n - 1u)) * p.ab_stride + h;
+    const float a = p.a[at], b = p.b[at];
+    float gate = aotx_delta_gate(a, p.dt[h], p.decay[h]);
+    float rate = 1.0f / (1.0f + expf(-b));
+    const bool badgate = lane < n && (gate != gate || rate != rate);
+    const unsigned long long badgates = __ballot(badgate);
+    if (lane >= n || badgate) gate = rate = 0.0f;
+    const double sum = aotx_wave_scan((double)gate);
+    const float all = expf((float)sum), last = expf((float)(__shfl(sum, 63, 64) - sum));
+    lds.ghi[lane] = (float)sum;
+    lds.glo[lane] = (float)(sum - (double)(float)sum);
+    lds.near_end[lane] = expf((float)(__shfl(sum, (int)(lane | 15u), 64) - sum));
+    lds.beta[lane] = rate;
+    __syncthreads();
+    to->of_k[lane] = all * lds.ks[lane];
+    to->of_q[lane] = all * lds.rq[lane];
+    to->of_u[lane] = last * lds.ks[lane];
+    if (lane < D / 2) {                 /* two columns a lane */
+        typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+        u2 v = __builtin_bit_cast(u2, lds.vm[0][lane]);
+#pragma unroll
+        for (int x = 1; x < 4; ++x) v = __builtin_elementwise_max(v, __builtin_bit_cast(u2, lds.vm[x][lane]));
+        *(unsigned short *)&to->vmax[2u * lane] = (unsigned short)((v[0] >> 10) | ((v[1] >> 10) << 8));
+    }
+    if (lane == 63u) {
+        unsigned int first = badgates != 0ull ? (unsigned int)__builtin_ctzll(badgates) : 64u;
+        for (int v = 0; v < 4; ++v) first = lds.badk[v] < first ? lds.badk[v] : first;
+        to->fade = all;
+        to->odd = first | (lds.badv[0] | lds.badv[1] | lds.badv[2] | lds.badv[3]) << 8;
+    }
+    __syncthreads();
+    __syncthreads();
+}
+
+template <int D>
+__global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
 {
     constexpr int KS = D / 32;
     __shared__ aotx_delta_within_lds<D> lds;
@@ -292,12 +353,9 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
     const unsigned int n = seq.end - r0 < 64u ? seq.end - r0 : 64u;
     aotx_delta_chunk_work *to = p.work + (unsigned long long)c * p.heads + h;
 
-    /* what the gates need comes first: its way is the longest */
-    float ga = 0.0f, gb = 0.0f;
-    if (w == 0u) {
-        const unsigned long long gr = (unsigned long long)(r0 + (lane < n ? lane : n - 1u)) * p.ab_stride + h;
-        ga = p.a[gr];
-        gb = p.b[gr];
+    if (w == 4u) {
+        aotx_delta_rates<D>(p, lds, to, r0, n, h);
+        return;
     }
     /* rows of K and Q, columns 32 s + 8 g .. of row 16 w + m; rows past the chunk read as zeros */
     const unsigned int kh = h / p.group;
@@ -317,21 +375,6 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
     for (unsigned int r = 0; r < 64u / VR; ++r)
         vv[r] = __builtin_bit_cast(aotx_u16x8, aotx_rows_16(rows, (r * VR + threadIdx.x / (D / 8)) * p.stride * 2u
                                    + (2u * p.key_heads * D + h * D + threadIdx.x % (D / 8) * 8u) * 2u));
-    /* gates, a row a lane; sums of g in 64 bits, kept as two floats, so that differences of far
-     * sums stay exact */
-    if (w == 0u) {
-        float gate = aotx_delta_gate(ga, p.dt[h], p.decay[h]);
-        float rate = 1.0f / (1.0f + expf(-gb));
-        const bool badgate = lane < n && (gate != gate || rate != rate);
-        const unsigned long long badgates = __ballot(badgate);
-        if (lane >= n || badgate) gate = rate = 0.0f;
-        const double sum = aotx_wave_scan((double)gate);
-        lds.ghi[lane] = (float)sum;
-        lds.glo[lane] = (float)(sum - (double)(float)sum);
-        lds.near_end[lane] = expf((float)(__shfl(sum, (int)(lane | 15u), 64) - sum));
-        lds.beta[lane] = rate;
-        if (lane == 0u) lds.badg = badgates != 0ull ? (unsigned int)__builtin_ctzll(badgates) : 64u;
-    }
     float kk = 0.0f, qq = 0.0f;
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -404,53 +447,10 @@ __global__ __launch_bounds__(256) void aotx_delta_within(aotx_delta_args p)
         if (lane < D / 8) *(aotx_u16x8 *)((unsigned short *)lds.vm[w] + lane * 8u) = top;
     }
     __syncthreads();
-
-    if (w == 0u) {
-        const float last = (lds.ghi[63] - lds.ghi[lane]) + (lds.glo[63] - lds.glo[lane]), all = expf(lds.ghi[lane]);
-        to->of_k[lane] = all * lds.ks[lane];
-        to->of_q[lane] = all * lds.rq[lane];
-        to->of_u[lane] = expf(last) * lds.ks[lane];
-        if (lane == 0u) {
-            unsigned int first = lds.badg;
-            for (int v = 0; v < 4; ++v) first = lds.badk[v] < first ? lds.badk[v] : first;
-            to->fade = expf(lds.ghi[63]);
-            to->odd = first | (lds.badv[0] | lds.badv[1] | lds.badv[2] | lds.badv[3]) << 8;
-        }
-    } else if (w == 1u) {
-        if (lane < D / 2) {             /* two columns a lane */
-            typedef unsigned short u2 __attribute__((ext_vector_type(2)));
-            u2 v = __builtin_bit_cast(u2, lds.vm[0][lane]);
-#pragma unroll
-            for (int x = 1; x < 4; ++x) v = __builtin_elementwise_max(v, __builtin_bit_cast(u2, lds.vm[x][lane]));
-            *(unsigned short *)&to->vmax[2u * lane] = (unsigned short)((v[0] >> 10) | ((v[1] >> 10) << 8));
-        }
-    }
-
     if (w == 0u) aotx_delta_pairs<D, 0>(lds, to, kf, qf, inv, qinv);
     else if (w == 1u) aotx_delta_pairs<D, 1>(lds, to, kf, qf, inv, qinv);
     else if (w == 2u) aotx_delta_pairs<D, 2>(lds, to, kf, qf, inv, qinv);
     else aotx_delta_pairs<D, 3>(lds, to, kf, qf, inv, qinv);
-    __builtin_amdgcn_wave_barrier();
-
-    /* inverse of the diagonal block by substitution, a column a lane; every value found is taken
-     * from all rows below at once, which do not wait for one another */
-    {
-        float x[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = m == (unsigned int)r ? 1.0f : 0.0f;
-        aotx_f4 row4[16][4];
-#pragma unroll
-        for (int r = 1; r < 16; ++r)
-#pragma unroll
-            for (int q = 0; 4 * q < r; ++q) row4[r][q] = *(const aotx_f4 *)&lds.diag[w][r][4 * q];
-#pragma unroll
-        for (int q = 0; q < 15; ++q)
-#pragma unroll
-            for (int r = q + 1; r < 16; ++r) x[r] -= row4[r][q / 4][q % 4] * x[q];
-        if (g == 0u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) lds.diag[w][r][m] = x[r];
-    }
     __syncthreads();
 
     if (w == 0u) aotx_delta_column<D, 0>(lds);
