@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256) void aotx_delta_rows_kernel(aotx_delta_args p)
     const unsigned int i = unit / p.heads, h = unit % p.heads;
     const unsigned int lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const aotx_seq_view seq = aotx_seq_of(p.seqs, i, aotx_seqs_read(p.seqs));
-    if (seq.start >= seq.end) return;
+    if (seq.start >= seq.end || seq.end - seq.start > p.few) return;
     const unsigned int c4 = (threadIdx.x % LC) * 4u, rg = threadIdx.x / LC;
     const unsigned int col = slice * CS + c4;
     const unsigned long long width = (unsigned long long)p.heads * D;
@@ -181,6 +181,7 @@ static int aotx_delta_fill(aotx_delta_args *p, const void *qkv, unsigned int str
     p->seqs.seqs = seqs;
     p->seqs.tokens = tokens;
     p->seqs.slots = slots;
+    p->few = 0xFFFFFFFFu;
     return 0;
 }
 
@@ -203,8 +204,6 @@ extern "C" int aotx_delta_step(const void *qkv, unsigned int stride, const float
     return 0;
 }
 
-#define AOTX_DELTA_ROWS 4u
-
 /* Chunks of a call at most: every sequence ends with a part of one. */
 static unsigned int aotx_delta_chunks_max(unsigned int tokens, unsigned int seqs)
 {
@@ -222,11 +221,16 @@ extern "C" unsigned long long aotx_delta_work(unsigned int tokens, unsigned int 
 template <int D>
 static void aotx_delta_chunked(const aotx_delta_args &p, hipStream_t s)
 {
-    constexpr unsigned int NT = 1u, slices = D / (16u * NT);
     hipLaunchKernelGGL((aotx_delta_within<D>), dim3(p.chunks * p.heads), dim3(320), 0, s, p);
     AOTX_LAUNCH_CHECK();
     const unsigned int units = (p.seqs.seqs * p.heads + 7u) / 8u * 8u;
-    hipLaunchKernelGGL((aotx_delta_across<D, NT>), dim3(units * slices), dim3(256), 0, s, p);
+    /* Two chunks' loads in flight where few workgroups share a CU or sequences are long; else one,
+     * in so few registers that three workgroups do (32 heads of 128: 4 sequences of 2048 rows 231
+     * us with two and 251 with one, 64 of 16 rows 245 and 204, 8 of 512 rows 124 and 121). */
+    if (units * (D / 16) <= 512u || p.seqs.tokens >= 1024u * p.seqs.seqs)
+        hipLaunchKernelGGL((aotx_delta_across<D, 2>), dim3(units * (D / 16)), dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((aotx_delta_across<D, 1>), dim3(units * (D / 16)), dim3(256), 0, s, p);
     AOTX_LAUNCH_CHECK();
 }
 
@@ -251,9 +255,14 @@ extern "C" int aotx_delta_chunk(const void *qkv, unsigned int stride, const floa
     p.chunks = aotx_delta_chunks_max(tokens, seqs);
     p.work = (aotx_delta_chunk_work *)work;
     p.rows = (aotx_h8 *)(p.work + (unsigned long long)p.chunks * heads);
-    /* a few rows go one by one: no matrices to make first */
-    const bool by_rows = tokens <= AOTX_DELTA_ROWS;
-    if (head_dim == 128u) by_rows ? aotx_delta_rows<128>(p, aotx_stream(stream)) : aotx_delta_chunked<128>(p, aotx_stream(stream));
-    else by_rows ? aotx_delta_rows<64>(p, aotx_stream(stream)) : aotx_delta_chunked<64>(p, aotx_stream(stream));
+    /* Sequences of few rows go row by row: no matrices to make first, and a decode row beside a
+     * prompt costs what a step does. A row takes 1.7 us, a chunk 7 to 12 if the chip is idle beside
+     * (32 heads of 128: 4 rows 9.8 us and 11.4, 8 rows 16.9 and 11.4); a chip full of sequences is
+     * kept busy longer by chunks (64 sequences of 8 rows 136 us row by row and 202 in chunks, of 16
+     * rows 214 and 204). */
+    p.few = seqs * heads >= 1024u ? 12u : 4u;
+    hipStream_t s = aotx_stream(stream);
+    if (tokens <= p.few || seqs > 1u) head_dim == 128u ? aotx_delta_rows<128>(p, s) : aotx_delta_rows<64>(p, s);
+    if (tokens > p.few) head_dim == 128u ? aotx_delta_chunked<128>(p, s) : aotx_delta_chunked<64>(p, s);
     return 0;
 }

@@ -63,6 +63,7 @@ struct aotx_delta_args {
     aotx_delta_chunk_work *work;    /* [chunks][heads] */
     aotx_h8 *rows;                  /* [chunks][key_heads] of K and Q (aotx_delta_rows_of) */
     unsigned int chunks;            /* at most: rows / 64 + sequences */
+    unsigned int few;               /* sequences of up to this many rows go row by row */
 };
 
 /* K (rows over 2^e) and Q of a chunk and key head as operands, [4 row tiles][d / 32 steps][64]
@@ -104,13 +105,13 @@ static __device__ __forceinline__ aotx_f4 aotx_mma(aotx_h8 a, aotx_h8 b, aotx_f4
 }
 
 /* Chunks of sequence `lane` and of the sequences before it. */
-static __device__ __forceinline__ void aotx_delta_chunks(const aotx_seq_lanes &l, unsigned int seqs, unsigned int *mine,
-                                                         unsigned int *before)
+static __device__ __forceinline__ void aotx_delta_chunks(const aotx_delta_args &p, const aotx_seq_lanes &l,
+                                                         unsigned int *mine, unsigned int *before)
 {
-    const unsigned int lane = threadIdx.x & 63u;
-    const unsigned int n = (l.end - l.start + AOTX_DELTA_CHUNK - 1u) / AOTX_DELTA_CHUNK;
+    const unsigned int lane = threadIdx.x & 63u, rows = l.end - l.start;
+    const unsigned int n = rows > p.few ? (rows + AOTX_DELTA_CHUNK - 1u) / AOTX_DELTA_CHUNK : 0u;
     unsigned int sum = n;
-    for (unsigned int off = 1u; off < seqs; off <<= 1) {
+    for (unsigned int off = 1u; off < p.seqs.seqs; off <<= 1) {
         const unsigned int o = (unsigned int)__shfl_up((int)sum, off, 64);
         if (lane >= off) sum += o;
     }
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
 
     unsigned int mine, before;
     const aotx_seq_lanes seqs = aotx_seqs_read(p.seqs);
-    aotx_delta_chunks(seqs, p.seqs.seqs, &mine, &before);
+    aotx_delta_chunks(p, seqs, &mine, &before);
     const unsigned int i = (unsigned int)__popcll(__ballot(lane < p.seqs.seqs && before + mine <= c));
     if (i >= p.seqs.seqs) return;
     const aotx_seq_view seq = aotx_seq_of(p.seqs, i, seqs);
@@ -467,9 +468,9 @@ __global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
 }
 
 /* ---------------------------------------------------------------------------------------
- * The walk over a sequence's chunks. A workgroup of four waves has 16 NT columns of one head's
- * S: wave w the rows of S that one step of K S takes (D / 4 of them, in accumulators), and rows
- * 16 w .. 16 w + 15 of the chunk. S, X and U pass between the waves through LDS as operands, a
+ * The walk over a sequence's chunks. Four waves have 16 columns of one head's S: wave w the rows
+ * of S that one step of K S takes (D / 4 of them, in accumulators), and rows 16 w .. 16 w + 15 of
+ * the chunk. S, X and U pass between the waves through LDS as operands, a
  * barrier each; everything else a chunk needs is loaded into registers two chunks ahead, each
  * register as soon as it has been used. A chunk's output is made where the state's chain waits:
  * Q S while X is on its way, P U behind the state's update, its rounding and stores while the
@@ -479,14 +480,14 @@ __global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
  * ------------------------------------------------------------------------------------- */
 #define AOTX_DELTA_PERIOD 4u        /* chunks for which a column's scale holds */
 
-template <int D, int NT>
+template <int D>
 struct aotx_delta_lds {
-    aotx_h8 s[D / 32][2][NT][64];           /* step of keys, part, tile of columns */
-    aotx_h8 x[2][2][NT][64];                /* step of rows, part, tile of columns */
-    aotx_h8 u[2][2][NT][64], v[2][2][NT][64];   /* U, and U with the state update's factors */
+    aotx_h8 s[D / 32][2][64];               /* S by steps of keys, two parts */
+    aotx_h8 x[2][2][64];                    /* X by steps of rows */
+    aotx_h8 u[2][2][64], v[2][2][64];       /* U, and U with the state update's factors */
     __align__(16) unsigned short k[64][D + 8];  /* the chunk's rows of K, to be read by columns */
-    int size[4][16 * NT];                   /* exponents of the state's columns, by wave */
-    unsigned int bad[4][16 * NT];           /* first bad rows of V's columns, by wave */
+    int size[4][16];                        /* exponents of the state's columns, by wave */
+    unsigned int bad[4][16];                /* first bad rows of V's columns, by wave */
 };
 
 struct aotx_delta_walk {
@@ -517,22 +518,23 @@ static __device__ __forceinline__ int aotx_exponent(float x)
     return (int)((__float_as_uint(x) >> 23) & 0xFFu) - 127;
 }
 
-template <int D, int NT, int NS>
+template <int D, int NS>
 struct aotx_delta_tile {
     aotx_h8 k[D / 32], q[D / 32], th[NS], tl[NS], p[NS];
-    unsigned short v[4][NT];
+    unsigned short v[4];
     aotx_f4 of_k, of_u, of_q;
     float fade;
     unsigned int odd;
 };
 
-/* NS: steps of 32 columns that the wave's rows of T and P have, 1 for waves 0 and 1, else 2. */
-template <int D, int NT, int NS>
+/* NS: steps of 32 columns that the wave's rows of T and P have, 1 for waves 0 and 1, else 2.
+ * SETS: how many chunks ahead the loads run, one or two. */
+template <int D, int NS, int SETS>
 static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &p, const aotx_delta_walk k,
-                                                         aotx_delta_lds<D, NT> &lds)
+                                                         aotx_delta_lds<D> &lds)
 {
     constexpr int KS = D / 32, TW = D / 64;
-    typedef aotx_delta_tile<D, NT, NS> tile_t;
+    typedef aotx_delta_tile<D, NS> tile_t;
     const unsigned int w = k.w, g = k.g, lane = k.lane, i0 = 16u * w + 4u * g, kh = k.h / p.group, l16 = lane * 16u;
     const unsigned int width = p.heads * D * 2u;        /* bytes of a row of out */
     const unsigned int at_out = i0 * width + (k.h * D + k.col) * 2u;
@@ -541,31 +543,31 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
     const unsigned int at_k = w * KS * 1024u + l16, at_p = w * 2048u + l16;
     const unsigned int at_of = (unsigned int)offsetof(work_t, of_k) + i0 * 4u;
     const unsigned int at_v = i0 * p.stride * 2u + (2u * p.key_heads * D + k.h * D + k.col) * 2u;
-    /* the chunk that is loaded: it stays the last one past the end, so that every pass has the
-     * same loads in flight */
-    unsigned int ahead = 0u;
+    /* the chunk that is loaded, and 1 while there is one: past the end the loads go through views
+     * of no size, which read zeros and touch no memory, so that every pass has the same in flight */
+    unsigned int ahead = 0u, there = 1u;
     const char *work = (const char *)(p.work + (unsigned long long)k.c0 * p.heads + k.h);
     const char *rows = (const char *)aotx_delta_rows_of(p, k.c0, kh, D);
     const unsigned long long work_step = sizeof(work_t) * (unsigned long long)p.heads;
     const unsigned long long rows_step = 256ull * D * p.key_heads;
     auto advance = [&]() {
-        const bool more = ahead + 1u < k.chunks;
-        ahead += more ? 1u : 0u;
-        work += more ? work_step : 0ull;
-        rows += more ? rows_step : 0ull;
+        ++ahead;
+        there = ahead < k.chunks ? 1u : 0u;
+        work += work_step;
+        rows += rows_step;
     };
     auto load_k = [&](tile_t &x) {
-        const __amdgpu_buffer_rsrc_t f = aotx_part(rows, 256u * D);
+        const __amdgpu_buffer_rsrc_t f = aotx_part(rows, there * 256u * D);
 #pragma unroll
         for (int s = 0; s < KS; ++s) x.k[s] = aotx_lane_16(f, at_k, s * 1024u);
     };
     auto load_q = [&](tile_t &x) {
-        const __amdgpu_buffer_rsrc_t f = aotx_part(rows, 256u * D);
+        const __amdgpu_buffer_rsrc_t f = aotx_part(rows, there * 256u * D);
 #pragma unroll
         for (int s = 0; s < KS; ++s) x.q[s] = aotx_lane_16(f, at_k, 128u * D + s * 1024u);
     };
     auto load_t = [&](tile_t &x) {
-        const __amdgpu_buffer_rsrc_t f = aotx_part(work, sizeof(work_t));
+        const __amdgpu_buffer_rsrc_t f = aotx_part(work, there * (unsigned int)sizeof(work_t));
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             x.th[s] = aotx_lane_16(f, at_p, (unsigned int)offsetof(work_t, t_hi) + s * 1024u);
@@ -573,14 +575,13 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         }
     };
     auto load_rest = [&](tile_t &x) {
-        const __amdgpu_buffer_rsrc_t f = aotx_part(work, sizeof(work_t));
+        const __amdgpu_buffer_rsrc_t f = aotx_part(work, there * (unsigned int)sizeof(work_t));
 #pragma unroll
         for (int s = 0; s < NS; ++s) x.p[s] = aotx_lane_16(f, at_p, s * 1024u);
-        const aotx_rows_view v = aotx_rows_of(p, k.seq.start + ahead * 64u, aotx_delta_left(k, ahead));
+        const aotx_rows_view v = aotx_rows_of(p, k.seq.start + ahead * 64u, there * aotx_delta_left(k, ahead));
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int u = 0; u < NT; ++u) x.v[r][u] = aotx_rows_2(v, at_v + r * p.stride * 2u + 2u * u);
+            x.v[r] = aotx_rows_2(v, at_v + r * p.stride * 2u);
         x.of_k = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 0u));
         x.of_q = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 256u));
         x.of_u = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 512u));
@@ -588,18 +589,16 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         x.odd = __builtin_amdgcn_raw_buffer_load_b32(f, 0, (int)offsetof(work_t, odd), 0);
         advance();
     };
-    unsigned char top[AOTX_DELTA_PERIOD][NT];       /* V's exponents in the coming period */
+    unsigned char top[AOTX_DELTA_PERIOD];       /* V's exponents in the coming period */
     auto load_top = [&](unsigned int c) {
 #pragma unroll
         for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q)
-#pragma unroll
-            for (int u = 0; u < NT; ++u)
-                top[q][u] = p.work[(unsigned long long)(k.c0 + (c + q < k.chunks ? c + q : k.chunks - 1u)) * p.heads
-                                   + k.h].vmax[k.col + u];
+                top[q] = p.work[(unsigned long long)(k.c0 + (c + q < k.chunks ? c + q : k.chunks - 1u)) * p.heads
+                                   + k.h].vmax[k.col];
     };
 
-    aotx_f4 S[TW][NT];                              /* times 2^shift */
-    int shift[NT];
+    aotx_f4 S[TW];                              /* times 2^shift */
+    int shift = 0;
     float *sp = p.state + ((unsigned long long)k.seq.slot * p.heads + k.h) * D * D + k.col;
 #pragma unroll
     for (int t = 0; t < TW; ++t)
@@ -607,11 +606,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         for (int r = 0; r < 4; ++r) {
             const unsigned int tile = w * TW + t;
             const unsigned int key = 32u * (tile >> 1) + 8u * g + 4u * (tile & 1u) + r;
-#pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                S[t][u][r] = k.seq.fresh ? 0.0f : sp[key * D + u];
-                shift[u] = 0;
-            }
+            S[t][r] = k.seq.fresh ? 0.0f : sp[key * D];
         }
     /* in the order in which the passes load, so that the waits for them count alike */
     tile_t A, B;
@@ -620,14 +615,16 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
     load_q(A);
     load_t(A);
     load_rest(A);
-    load_k(B);
-    load_q(B);
-    load_t(B);
-    load_rest(B);
+    if constexpr (SETS == 2) {
+        load_k(B);
+        load_q(B);
+        load_t(B);
+        load_rest(B);
+    }
 
     /* the chunk before: its output, still to be stored */
-    aotx_f4 o[NT];
-    int o_shift[NT];
+    aotx_f4 o;
+    int o_shift;
     auto store = [&](unsigned int c) {
         /* rows past the chunk are past the view's end: the store drops them */
         const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(
@@ -635,157 +632,120 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             (int)(aotx_delta_left(k, c) * width), 0x00020000);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                __builtin_amdgcn_raw_buffer_store_b16(aotx_f2h(ldexpf(o[u][r], -o_shift[u])), to, (int)(at_out + r * width + 2u * u), 0, 0);
-            }
+            __builtin_amdgcn_raw_buffer_store_b16(aotx_f2h(ldexpf(o[r], -o_shift)), to, (int)(at_out + r * width), 0, 0);
     };
     auto scale = [&](unsigned int c) {
         /* in the period |S| and |U| of a column stay below sqrt(d) max|S| + 257 max|V|, which the
          * exponents plus 5 and plus 10 are bounds of */
+        float ms = 0.0f;
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            float ms = 0.0f;
+        for (int t = 0; t < TW; ++t)
 #pragma unroll
-            for (int t = 0; t < TW; ++t)
+            for (int r = 0; r < 4; ++r) ms = fmaxf(ms, fabsf(S[t][r]));
+        ms = fmaxf(ms, __shfl_xor(ms, 16, 64));
+        ms = fmaxf(ms, __shfl_xor(ms, 32, 64));
+        int ex = aotx_exponent(ms) - shift + 5, ev = 0;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) ms = fmaxf(ms, fabsf(S[t][u][r]));
-            ms = fmaxf(ms, __shfl_xor(ms, 16, 64));
-            ms = fmaxf(ms, __shfl_xor(ms, 32, 64));
-            int ex = aotx_exponent(ms) - shift[u] + 5, ev = 0;
-#pragma unroll
-            for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q) ev = top[q][u] > ev ? top[q][u] : ev;
-            ev += 10 - 15;
-            ex = ex > ev ? ex : ev;
-            if (g == 0u) lds.size[w][k.m * NT + u] = ex;
-        }
+        for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q) ev = top[q] > ev ? top[q] : ev;
+        ev += 10 - 15;
+        ex = ex > ev ? ex : ev;
+        if (g == 0u) lds.size[w][k.m] = ex;
         __syncthreads();
+        ex = lds.size[0][k.m];
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            int ex = lds.size[0][k.m * NT + u];
+        for (int v = 1; v < 4; ++v) ex = lds.size[v][k.m] > ex ? lds.size[v][k.m] : ex;
+        ex = 14 - ex;
+        ex = ex > 100 ? 100 : ex < -100 ? -100 : ex;
 #pragma unroll
-            for (int v = 1; v < 4; ++v) ex = lds.size[v][k.m * NT + u] > ex ? lds.size[v][k.m * NT + u] : ex;
-            ex = 14 - ex;
-            ex = ex > 100 ? 100 : ex < -100 ? -100 : ex;
+        for (int t = 0; t < TW; ++t)
 #pragma unroll
-            for (int t = 0; t < TW; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) S[t][u][r] = ldexpf(S[t][u][r], ex - shift[u]);
-            shift[u] = ex;
-        }
+            for (int r = 0; r < 4; ++r) S[t][r] = ldexpf(S[t][r], ex - shift);
+        shift = ex;
         load_top(c + AOTX_DELTA_PERIOD);
     };
     auto pass = [&](tile_t &x, unsigned int c) {
         /* rows that are taken out, or past the chunk, have zeros in K, Q and V: their X, U and T
          * are zeros by themselves. Only a chunk with values that are no numbers asks more. */
         const unsigned int odd = (unsigned int)__builtin_amdgcn_readfirstlane((int)x.odd);
-        unsigned int lim[NT];
-#pragma unroll
-        for (int u = 0; u < NT; ++u) lim[u] = odd & 0xFFu;
+        unsigned int lim = odd & 0xFFu;
         if (odd != 64u) {
+            unsigned int first = 64u;
 #pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                unsigned int first = 64u;
-#pragma unroll
-                for (int r = 3; r >= 0; --r)
-                    if ((x.v[r][u] & 0x7FFFu) >= 0x7C00u) first = i0 + r;
-                unsigned int f = (unsigned int)__shfl_xor((int)first, 16, 64);
-                first = f < first ? f : first;
-                f = (unsigned int)__shfl_xor((int)first, 32, 64);
-                first = f < first ? f : first;
-                if (g == 0u) lds.bad[w][k.m * NT + u] = first;
-            }
+            for (int r = 3; r >= 0; --r)
+                if ((x.v[r] & 0x7FFFu) >= 0x7C00u) first = i0 + r;
+            unsigned int f = (unsigned int)__shfl_xor((int)first, 16, 64);
+            first = f < first ? f : first;
+            f = (unsigned int)__shfl_xor((int)first, 32, 64);
+            first = f < first ? f : first;
+            if (g == 0u) lds.bad[w][k.m] = first;
             __syncthreads();
 #pragma unroll
-            for (int u = 0; u < NT; ++u)
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const unsigned int f = lds.bad[v][k.m * NT + u];
-                    lim[u] = f < lim[u] ? f : lim[u];
-                }
+            for (int v = 0; v < 4; ++v) lim = lds.bad[v][k.m] < lim ? lds.bad[v][k.m] : lim;
         }
+        aotx_h4 hi, lo;
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
-#pragma unroll
-            for (int t = 0; t < TW; ++t) {
-                aotx_h4 hi, lo;
-                aotx_split4(S[t][u], &hi, &lo);
-                const unsigned int tile = w * TW + t;
-                *((aotx_h4 *)&lds.s[tile >> 1][0][u][lane] + (tile & 1u)) = hi;
-                *((aotx_h4 *)&lds.s[tile >> 1][1][u][lane] + (tile & 1u)) = lo;
-            }
+        for (int t = 0; t < TW; ++t) {
+            aotx_split4(S[t], &hi, &lo);
+            const unsigned int tile = w * TW + t;
+            *((aotx_h4 *)&lds.s[tile >> 1][0][lane] + (tile & 1u)) = hi;
+            *((aotx_h4 *)&lds.s[tile >> 1][1][lane] + (tile & 1u)) = lo;
+        }
         __syncthreads();
-        aotx_h8 sh[NT][KS], sl[NT][KS];
+        aotx_h8 sh[KS], sl[KS];
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                sh[u][s] = lds.s[s][0][u][lane];
-                sl[u][s] = lds.s[s][1][u][lane];
-            }
-        if (c != 0u) store(c - 1u);
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            aotx_f4 a = {0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                a = aotx_mma(x.k[s], sl[u][s], a);
-                a = aotx_mma(x.k[s], sh[u][s], a);
-            }
-            const float up = ldexpf(1.0f, shift[u]);
-            aotx_f4 y;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) y[r] = fmaf(aotx_h2f(x.v[r][u]), up, -(x.of_k[r] * a[r]));
-            if (odd != 64u) {
-                asm volatile("");               /* a branch that is not taken, no selects */
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (i0 + r >= lim[u]) y[r] = 0.0f;
-            }
-            aotx_h4 hi, lo;
-            aotx_split4(y, &hi, &lo);
-            *((aotx_h4 *)&lds.x[w >> 1][0][u][lane] + (w & 1u)) = hi;
-            *((aotx_h4 *)&lds.x[w >> 1][1][u][lane] + (w & 1u)) = lo;
+        for (int s = 0; s < KS; ++s) {
+            sh[s] = lds.s[s][0][lane];
+            sl[s] = lds.s[s][1][lane];
         }
+        if (c != 0u) store(c - 1u);
+        aotx_f4 a = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            a = aotx_mma(x.k[s], sl[s], a);
+            a = aotx_mma(x.k[s], sh[s], a);
+        }
+        const float up = ldexpf(1.0f, shift);
+        aotx_f4 y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = fmaf(aotx_h2f(x.v[r]), up, -(x.of_k[r] * a[r]));
+        if (odd != 64u) {
+            asm volatile("");               /* a branch that is not taken, no selects */
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (i0 + r >= lim) y[r] = 0.0f;
+        }
+        aotx_split4(y, &hi, &lo);
+        *((aotx_h4 *)&lds.x[w >> 1][0][lane] + (w & 1u)) = hi;
+        *((aotx_h4 *)&lds.x[w >> 1][1][lane] + (w & 1u)) = lo;
 #pragma unroll
         for (int s = 0; s < KS; ++s) *(aotx_h8 *)&lds.k[16u * w + k.m][32 * s + 8u * g] = x.k[s];
         __syncthreads();
         load_k(x);
-        aotx_h8 xh[NT][NS], xl[NT][NS];
+        aotx_h8 xh[NS], xl[NS];
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                xh[u][s] = lds.x[s][0][u][lane];
-                xl[u][s] = lds.x[s][1][u][lane];
-            }
-        aotx_f4 qs[NT];
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            qs[u] = aotx_f4{0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                qs[u] = aotx_mma(x.q[s], sl[u][s], qs[u]);
-                qs[u] = aotx_mma(x.q[s], sh[u][s], qs[u]);
-            }
+        for (int s = 0; s < NS; ++s) {
+            xh[s] = lds.x[s][0][lane];
+            xl[s] = lds.x[s][1][lane];
         }
+        aotx_f4 qs = {0, 0, 0, 0};
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            aotx_f4 a = {0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                a = aotx_mma(x.th[s], xl[u][s], a);
-                a = aotx_mma(x.tl[s], xh[u][s], a);
-                a = aotx_mma(x.th[s], xh[u][s], a);
-            }
-            aotx_h4 hi, lo;
-            aotx_split4(a * x.of_u, &hi, &lo);
-            *((aotx_h4 *)&lds.v[w >> 1][0][u][lane] + (w & 1u)) = hi;
-            *((aotx_h4 *)&lds.v[w >> 1][1][u][lane] + (w & 1u)) = lo;
-            aotx_split4(a, &hi, &lo);
-            *((aotx_h4 *)&lds.u[w >> 1][0][u][lane] + (w & 1u)) = hi;
-            *((aotx_h4 *)&lds.u[w >> 1][1][u][lane] + (w & 1u)) = lo;
+        for (int s = 0; s < KS; ++s) {
+            qs = aotx_mma(x.q[s], sl[s], qs);
+            qs = aotx_mma(x.q[s], sh[s], qs);
         }
+        a = aotx_f4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            a = aotx_mma(x.th[s], xl[s], a);
+            a = aotx_mma(x.tl[s], xh[s], a);
+            a = aotx_mma(x.th[s], xh[s], a);
+        }
+        aotx_split4(a * x.of_u, &hi, &lo);
+        *((aotx_h4 *)&lds.v[w >> 1][0][lane] + (w & 1u)) = hi;
+        *((aotx_h4 *)&lds.v[w >> 1][1][lane] + (w & 1u)) = lo;
+        aotx_split4(a, &hi, &lo);
+        *((aotx_h4 *)&lds.u[w >> 1][0][lane] + (w & 1u)) = hi;
+        *((aotx_h4 *)&lds.u[w >> 1][1][lane] + (w & 1u)) = lo;
         __syncthreads();
         /* K by columns: lane (m, g) addresses row m / 4 of four, keys 8 (m % 4) .. + 3 of the
          * tile's 16, and gets key m of it for all four rows */
@@ -803,45 +763,42 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             }
         load_q(x);
         load_t(x);
+        aotx_h8 vh[2], vl[2], uh[NS], ul[NS];
 #pragma unroll
-        for (int u = 0; u < NT; ++u) {
-            aotx_h8 vh[2], vl[2], uh[NS], ul[NS];
+        for (int s = 0; s < 2; ++s) {
+            vh[s] = lds.v[s][0][lane];
+            vl[s] = lds.v[s][1][lane];
+        }
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            uh[s] = lds.u[s][0][lane];
+            ul[s] = lds.u[s][1][lane];
+        }
+#pragma unroll
+        for (int t = 0; t < TW; ++t) {
+            S[t] *= x.fade;
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                vh[s] = lds.v[s][0][u][lane];
-                vl[s] = lds.v[s][1][u][lane];
+                S[t] = aotx_mma(kt[t][s], vl[s], S[t]);
+                S[t] = aotx_mma(kt[t][s], vh[s], S[t]);
             }
+        }
+        o = x.of_q * qs;
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                uh[s] = lds.u[s][0][u][lane];
-                ul[s] = lds.u[s][1][u][lane];
-            }
+        for (int s = 0; s < NS; ++s) {
+            o = aotx_mma(x.p[s], ul[s], o);
+            o = aotx_mma(x.p[s], uh[s], o);
+        }
+        o_shift = shift;
+        if (odd != 64u) {
+            asm volatile("");
+            const float nan = __builtin_nanf("");
 #pragma unroll
-            for (int t = 0; t < TW; ++t) {
-                S[t][u] *= x.fade;
+            for (int t = 0; t < TW; ++t)
+                if (lim < 64u) S[t] = aotx_f4{nan, nan, nan, nan};
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    S[t][u] = aotx_mma(kt[t][s], vl[s], S[t][u]);
-                    S[t][u] = aotx_mma(kt[t][s], vh[s], S[t][u]);
-                }
-            }
-            o[u] = x.of_q * qs[u];
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                o[u] = aotx_mma(x.p[s], ul[s], o[u]);
-                o[u] = aotx_mma(x.p[s], uh[s], o[u]);
-            }
-            o_shift[u] = shift[u];
-            if (odd != 64u) {
-                asm volatile("");
-                const float nan = __builtin_nanf("");
-#pragma unroll
-                for (int t = 0; t < TW; ++t)
-                    if (lim[u] < 64u) S[t][u] = aotx_f4{nan, nan, nan, nan};
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (i0 + r >= lim[u]) o[u][r] = nan;
-            }
+            for (int r = 0; r < 4; ++r)
+                if (i0 + r >= lim) o[r] = nan;
         }
         load_rest(x);
     };
@@ -850,11 +807,11 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         scale(c);
         pass(A, c);
         if (++c >= k.chunks) break;
-        pass(B, c);
+        pass(SETS == 2 ? B : A, c);
         if (++c >= k.chunks) break;
         pass(A, c);
         if (++c >= k.chunks) break;
-        pass(B, c);
+        pass(SETS == 2 ? B : A, c);
         if (++c >= k.chunks) break;
     }
     store(k.chunks - 1u);
@@ -864,16 +821,15 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         for (int r = 0; r < 4; ++r) {
             const unsigned int tile = w * TW + t;
             const unsigned int key = 32u * (tile >> 1) + 8u * g + 4u * (tile & 1u) + r;
-#pragma unroll
-            for (int u = 0; u < NT; ++u) sp[key * D + u] = ldexpf(S[t][u][r], -shift[u]);
+            sp[key * D] = ldexpf(S[t][r], -shift);
         }
 }
 
-template <int D, int NT>
-__global__ __launch_bounds__(256, 2) void aotx_delta_across(aotx_delta_args p)
+template <int D, int SETS>
+__global__ __launch_bounds__(256, SETS == 2 ? 2 : 3) void aotx_delta_across(aotx_delta_args p)
 {
-    constexpr unsigned int SLICES = D / (16 * NT);
-    __shared__ aotx_delta_lds<D, NT> lds;
+    constexpr unsigned int SLICES = D / 16;
+    __shared__ aotx_delta_lds<D> lds;
     aotx_delta_walk k;
     k.lane = threadIdx.x & 63u;
     k.m = k.lane & 15u;
@@ -888,22 +844,21 @@ __global__ __launch_bounds__(256, 2) void aotx_delta_across(aotx_delta_args p)
     k.h = unit % p.heads;
     unsigned int mine, before;
     const aotx_seq_lanes seqs = aotx_seqs_read(p.seqs);
-    aotx_delta_chunks(seqs, p.seqs.seqs, &mine, &before);
+    aotx_delta_chunks(p, seqs, &mine, &before);
     k.seq = aotx_seq_of(p.seqs, i, seqs);
     k.c0 = (unsigned int)__builtin_amdgcn_readlane((int)before, (int)i);
-    if (k.seq.start >= k.seq.end) return;
+    if (k.seq.end - k.seq.start <= p.few) return;
     k.chunks = (k.seq.end - k.seq.start + 63u) / 64u;
-    k.col = slice * 16u * NT + k.m * NT;                /* this lane's NT columns */
+    k.col = slice * 16u + k.m;                          /* this lane's column */
     if (k.seq.refused) {
         if (threadIdx.x == 0u && slice == 0u && k.h == 0u) atomicAdd(p.seqs.faults, 1u);
-        for (unsigned int t = k.seq.start + threadIdx.x / 16u; t < k.seq.end; t += 16u)
-#pragma unroll
-            for (int u = 0; u < NT; ++u) p.out[((unsigned long long)t * p.heads + k.h) * D + k.col + u] = 0;
+        for (unsigned int t = k.seq.start + k.w * 4u + k.g; t < k.seq.end; t += 16u)
+            p.out[((unsigned long long)t * p.heads + k.h) * D + k.col] = 0;
         return;
     }
     /* (scalar: the barriers of both ways count together) */
-    if (k.w < 2u) aotx_delta_follow<D, NT, 1>(p, k, lds);
-    else aotx_delta_follow<D, NT, 2>(p, k, lds);
+    if (k.w < 2u) aotx_delta_follow<D, 1, SETS>(p, k, lds);
+    else aotx_delta_follow<D, 2, SETS>(p, k, lds);
 }
 
 #endif
