@@ -26,7 +26,8 @@
  * aotx_model_faulted(). At most AOTX_SLOTS sequences and slots.
  *
  * Two calls that use the same state, or the same workspace, have to follow one another (one
- * stream, or an event between streams).
+ * stream, or an event between streams). What a call writes overlaps nothing that it reads, but
+ * where a description says that it may.
  */
 #ifndef AOTX_HYBRID_H
 #define AOTX_HYBRID_H
@@ -63,9 +64,11 @@ int aotx_delta_conv(const float *x, unsigned int stride, const float *w, const f
  * t at a + t * ab_stride, [heads] values. decay, dt fp32 [heads]; decay at most 0 (g above 0
  * is taken as 0). state fp32 [slots][heads][head_dim][head_dim]. out fp16
  * [tokens][heads][head_dim]. head_dim 64 or 128, key_heads divides heads, at most 256 heads,
- * eps at least 1e-30; stride a multiple of 8 up to 2^22; qkv, state and out 16-byte aligned. All arithmetic on the
- * state is fp32 or as near (the products of aotx_delta_chunk take their operands as two fp16
- * parts each). A value of Inf or NaN reaches the rows from its own on and no earlier ones.
+ * eps at least 1e-30; stride a multiple of 8 up to 2^22; qkv, state and out 16-byte aligned. The
+ * state is fp32, and its arithmetic is that or as near: the products of aotx_delta_chunk take
+ * their operands as two fp16 parts, 2^-21 each; the weights with which an output takes the rows
+ * of its own 64 are rounded to fp16 once, as the output is. A value of Inf or NaN reaches the rows
+ * from its own on and no earlier ones.
  *
  * aotx_delta_step: one token of each of `tokens` slots (row i is sequence i). */
 int aotx_delta_step(const void *qkv, unsigned int stride, const float *a, const float *b,

@@ -150,6 +150,34 @@ def test_chunk_whole_calls(torch, lib, lens):
     Delta(torch, len(lens) + lens[0], lens, 1, 2, 128, slots=32, pad=8).up().call(lib).check(lib)
 
 
+@pytest.mark.parametrize("key_heads,heads,d", [(16, 32, 64), (32, 32, 128)])
+def test_chunk_few_rows_beside_many(torch, lib, key_heads, heads, d):
+    """Sequences of few rows go row by row, the others in chunks, in one call: lengths on both
+    sides of either limit, and so many heads and sequences that the higher one holds."""
+    lens = [1, 12, 13, 4, 5, 0, 200, 2, 11, 64] + [1, 3, 14] * 8
+    Delta(torch, heads + d, lens, key_heads, heads, d, lead=1, tail=2, slots=40, fresh=(1, 6, 9),
+          agent=list(range(33)) + [5]).up().call(lib).check(lib)
+
+
+@pytest.mark.parametrize("lens", [[3], [70, 1, 130]])
+def test_chunk_keeps_to_its_workspace(torch, lib, lens):
+    """What lies behind the workspace's stated size stays as it was, and what a workspace holds
+    from before makes no difference."""
+    outs = []
+    for fill in (0x00, 0x7F):
+        c = Delta(torch, 16, lens, 2, 4, 64).up()
+        need = lib.aotx_delta_work(sum(lens), len(lens), 4, 64)
+        work = torch.full((need + 4096,), fill, dtype=torch.uint8, device="cuda")
+        KEEP.append(work)
+        g = {k: p(v) for k, v in c.dev.items()}
+        assert lib.aotx_delta_chunk(g["x"], c.stride, g["a"], g["b"], c.ab_stride, g["decay"], g["dt"], g["offset"], g["pos"],
+                                    g["agent"], len(lens), c.tokens, 2, 4, 64, EPS, g["state"], 8, p(work), need, g["out"],
+                                    None) == 0
+        outs.append(c.got())
+        assert (work[need:] == fill).all()
+    assert np.array_equal(outs[0][0], outs[1][0]) and np.array_equal(outs[0][1], outs[1][1])
+
+
 def test_chunk_long(torch, lib):
     Delta(torch, 21, [6000], 1, 2, 64, slots=1, fresh=(0,)).up().call(lib).check(lib)
 
@@ -600,6 +628,38 @@ def test_linear_layer_in_a_graph(torch, lib):
         torch.cuda.synchronize()
         L.linear(x, 2, token, s)
         assert torch.equal(now()[0][:2], want["token"][0][:2])
+
+
+def test_rope_axes_in_a_graph(torch, lib):
+    """A captured turn, replayed with other places and rows in the same buffers: the frequencies
+    are the call's, everything else is read at the replay."""
+    rng = np.random.default_rng(90)
+    tokens, heads, kv, d = 9, 4, 2, 64
+    how = aotx_amd.RopeHow(theta=1e4, eps=EPS, rope_dim=32, pairs=1, axes=2, order=1, span=(ctypes.c_uint32 * 4)(8, 8))
+    x = torch.zeros(tokens, (heads + 2 * kv) * d, device="cuda")
+    place = torch.zeros(tokens, 2, dtype=torch.int32, device="cuda")
+    q, k, v = (torch.zeros(tokens, n, d, dtype=torch.float16, device="cuda") for n in (heads, kv, kv))
+
+    def call(s):
+        assert lib.aotx_rope_axes(p(x), x.shape[1], None, None, ctypes.byref(how), None, p(place), tokens, heads, kv, d, p(q),
+                                  p(k), p(v), s) == 0
+
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        call(ctypes.c_void_p(side.cuda_stream))
+    for turn in range(3):
+        x.copy_(torch.from_numpy(rng.normal(0, 1, tuple(x.shape)).astype(np.float32)))
+        place.copy_(torch.from_numpy(rng.integers(0, 9999, (tokens, 2)).astype(np.int32)))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (q, k, v)]
+        call(None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, (q, k, v))), turn
+        assert q.abs().sum() > 0
 
 
 def test_two_streams_of_their_own(torch, lib):
