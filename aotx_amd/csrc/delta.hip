@@ -226,11 +226,16 @@ static void aotx_delta_chunked(const aotx_delta_args &p, hipStream_t s)
     const unsigned int units = (p.seqs.seqs * p.heads + 7u) / 8u * 8u;
     /* Two chunks' loads in flight where few workgroups share a CU or sequences are long; else one,
      * in so few registers that three workgroups do (32 heads of 128: 4 sequences of 2048 rows 231
-     * us with two and 251 with one, 64 of 16 rows 245 and 204, 8 of 512 rows 124 and 121). */
-    if (units * (D / 16) <= 512u || p.seqs.tokens >= 1024u * p.seqs.seqs)
-        hipLaunchKernelGGL((aotx_delta_across<D, 2>), dim3(units * (D / 16)), dim3(256), 0, s, p);
+     * us with two and 251 with one, 64 of 16 rows 245 and 204, 8 of 512 rows 124 and 121). Lines
+     * are asked for early where the caches of the XCDs do not hold the workspace any more (8192
+     * rows 265 us with and 280 without, 2048 rows 74 and 68). */
+    const dim3 grid(units * (D / 16));
+    if (grid.x > 512u && p.seqs.tokens < 1024u * p.seqs.seqs)
+        hipLaunchKernelGGL((aotx_delta_across<D, 1>), grid, dim3(256), 0, s, p);
+    else if ((unsigned long long)p.chunks * p.heads * sizeof(aotx_delta_chunk_work) < (80ull << 20))
+        hipLaunchKernelGGL((aotx_delta_across<D, 2>), grid, dim3(256), 0, s, p);
     else
-        hipLaunchKernelGGL((aotx_delta_across<D, 1>), dim3(units * (D / 16)), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((aotx_delta_across<D, 3>), grid, dim3(256), 0, s, p);
     AOTX_LAUNCH_CHECK();
 }
 

@@ -525,11 +525,13 @@ struct aotx_delta_tile {
     aotx_f4 of_k, of_u, of_q;
     float fade;
     unsigned int odd;
+    unsigned int touched;
 };
 
 /* NS: steps of 32 columns that the wave's rows of T and P have, 1 for waves 0 and 1, else 2.
- * SETS: how many chunks ahead the loads run, one or two. */
-template <int D, int NS, int SETS>
+ * AHEAD: how many chunks ahead the loads run, one or two; with 3, two, and their lines are asked
+ * for before. */
+template <int D, int NS, int AHEAD>
 static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &p, const aotx_delta_walk k,
                                                          aotx_delta_lds<D> &lds)
 {
@@ -555,6 +557,38 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         there = ahead < k.chunks ? 1u : 0u;
         work += work_step;
         rows += rows_step;
+    };
+    /* What a chunk needs comes from memory once for the head's slices, which share an L2, and each
+     * would wait for the whole of it. So each asks for its share of the lines of a chunk some
+     * passes before any is loaded: a line a lane of waves 0 (K, Q and V) and 1 (P, T, factors).
+     * The last chunk, which may be a part of one, is left out. */
+    const char *line = rows + (k.col >> 4) * 4096u + lane * 128u;
+    unsigned long long line_step = rows_step;
+    unsigned int line_c = 2u;
+    if constexpr (NS == 1 && AHEAD == 3) {
+        constexpr unsigned int SLICES = D / 16, OF_WORK = 152u / SLICES;
+        bool some = lane < 32u;
+        if (w == 0u && lane >= 32u) {
+            const unsigned int l = (k.col >> 4) * 16u + (lane & 15u);
+            line = (const char *)(p.qkv + (unsigned long long)(k.seq.start + l / (D / 64)) * p.stride + 2u * p.key_heads * D
+                                  + k.h * D) + l % (D / 64) * 128u;
+            line_step = 128ull * p.stride;
+            some = lane < 48u;
+        } else if (w == 1u) {
+            const unsigned int l = (k.col >> 4) * OF_WORK + lane, part = l / 48u, block = l % 48u / 8u;
+            line = work + (part < 3u ? part * 8192u + (block < 2u ? 2u * block : block + 2u) * 1024u : 24576u) + l % 8u * 128u;
+            line_step = work_step;
+            some = lane < OF_WORK;
+        }
+        some = some && k.chunks > 3u;
+        if (!some) line_step = 0ull;            /* the lane asks for a chunk's first line again */
+        if (!some) line = work;
+        line += 2u * line_step;
+    }
+    auto touch = [&]() {
+        const unsigned int v = *(const unsigned int *)line;
+        if (++line_c < k.chunks - 1u) line += line_step;
+        return v;
     };
     auto load_k = [&](tile_t &x) {
         const __amdgpu_buffer_rsrc_t f = aotx_part(rows, there * 256u * D);
@@ -587,6 +621,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         x.of_u = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 512u));
         x.fade = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(f, 0, (int)offsetof(work_t, fade), 0));
         x.odd = __builtin_amdgcn_raw_buffer_load_b32(f, 0, (int)offsetof(work_t, odd), 0);
+        if constexpr (NS == 1 && AHEAD == 3) x.touched = touch();
         advance();
     };
     unsigned char top[AOTX_DELTA_PERIOD];       /* V's exponents in the coming period */
@@ -615,7 +650,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
     load_q(A);
     load_t(A);
     load_rest(A);
-    if constexpr (SETS == 2) {
+    if constexpr (AHEAD > 1) {
         load_k(B);
         load_q(B);
         load_t(B);
@@ -667,6 +702,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         /* rows that are taken out, or past the chunk, have zeros in K, Q and V: their X, U and T
          * are zeros by themselves. Only a chunk with values that are no numbers asks more. */
         const unsigned int odd = (unsigned int)__builtin_amdgcn_readfirstlane((int)x.odd);
+        if constexpr (NS == 1 && AHEAD == 3) asm volatile("" ::"v"(x.touched));
         unsigned int lim = odd & 0xFFu;
         if (odd != 64u) {
             unsigned int first = 64u;
@@ -807,11 +843,11 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         scale(c);
         pass(A, c);
         if (++c >= k.chunks) break;
-        pass(SETS == 2 ? B : A, c);
+        pass(AHEAD > 1 ? B : A, c);
         if (++c >= k.chunks) break;
         pass(A, c);
         if (++c >= k.chunks) break;
-        pass(SETS == 2 ? B : A, c);
+        pass(AHEAD > 1 ? B : A, c);
         if (++c >= k.chunks) break;
     }
     store(k.chunks - 1u);
@@ -825,8 +861,8 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         }
 }
 
-template <int D, int SETS>
-__global__ __launch_bounds__(256, SETS == 2 ? 2 : 3) void aotx_delta_across(aotx_delta_args p)
+template <int D, int AHEAD>
+__global__ __launch_bounds__(256, AHEAD > 1 ? 2 : 3) void aotx_delta_across(aotx_delta_args p)
 {
     constexpr unsigned int SLICES = D / 16;
     __shared__ aotx_delta_lds<D> lds;
@@ -857,8 +893,8 @@ __global__ __launch_bounds__(256, SETS == 2 ? 2 : 3) void aotx_delta_across(aotx
         return;
     }
     /* (scalar: the barriers of both ways count together) */
-    if (k.w < 2u) aotx_delta_follow<D, 1, SETS>(p, k, lds);
-    else aotx_delta_follow<D, 2, SETS>(p, k, lds);
+    if (k.w < 2u) aotx_delta_follow<D, 1, AHEAD>(p, k, lds);
+    else aotx_delta_follow<D, 2, AHEAD>(p, k, lds);
 }
 
 #endif
