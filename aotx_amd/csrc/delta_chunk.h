@@ -104,6 +104,13 @@ static __device__ __forceinline__ aotx_f4 aotx_mma(aotx_h8 a, aotx_h8 b, aotx_f4
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+/* Workgroup b runs on XCD b % 8. Heads are dealt out so that those of one key head, one after
+ * another, come to the same XCD, in both kernels: its L2 then fetches the rows of K and Q once. */
+static __device__ __forceinline__ unsigned int aotx_delta_head(const aotx_delta_args &p, unsigned int x)
+{
+    return p.heads % 8u == 0u ? x % 8u * (p.heads / 8u) + x / 8u : x;
+}
+
 /* Chunks of sequence `lane` and of the sequences before it. */
 static __device__ __forceinline__ void aotx_delta_chunks(const aotx_delta_args &p, const aotx_seq_lanes &l,
                                                          unsigned int *mine, unsigned int *before)
@@ -341,7 +348,7 @@ __global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
     __shared__ aotx_delta_within_lds<D> lds;
     const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4;
     const unsigned int w = (unsigned int)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const unsigned int c = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
+    const unsigned int c = blockIdx.x / p.heads, h = aotx_delta_head(p, blockIdx.x % p.heads);
 
     unsigned int mine, before;
     const aotx_seq_lanes seqs = aotx_seqs_read(p.seqs);
@@ -871,13 +878,12 @@ __global__ __launch_bounds__(256, AHEAD > 1 ? 2 : 3) void aotx_delta_across(aotx
     k.m = k.lane & 15u;
     k.g = k.lane >> 4;
     k.w = (unsigned int)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    /* the slices of a head go to one XCD (workgroup b runs on XCD b % 8), whose L2 then holds
-     * what they share */
+    /* the slices of a head go to one XCD, too, whose L2 then holds what they share */
     const unsigned int unit = blockIdx.x / (8u * SLICES) * 8u + blockIdx.x % 8u;
     const unsigned int slice = blockIdx.x / 8u % SLICES;
     if (unit >= p.seqs.seqs * p.heads) return;
     const unsigned int i = unit / p.heads;
-    k.h = unit % p.heads;
+    k.h = aotx_delta_head(p, unit % p.heads);
     unsigned int mine, before;
     const aotx_seq_lanes seqs = aotx_seqs_read(p.seqs);
     aotx_delta_chunks(p, seqs, &mine, &before);
