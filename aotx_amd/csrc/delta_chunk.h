@@ -132,6 +132,139 @@ static __device__ __forceinline__ unsigned int aotx_delta_place(unsigned int j)
     return (j & ~31u) + ((j >> 2) & 3u) * 8u + ((j >> 4) & 1u) * 4u + (j & 3u);
 }
 
+/* ---------------------------------------------------------------------------------------
+ * Row by row. A workgroup holds CS columns of one head's S in registers, four columns and
+ * every RG-th row a thread; S^T k' and S^T q' come from one walk over them, since
+ *   out = exp(g) S^T q' + (k' . q') u,
+ * so a token costs one reduction over the rows: lanes of a wave first, then the four waves
+ * through LDS with one barrier. The next token's rows are normed by wave 0 before it.
+ * ------------------------------------------------------------------------------------- */
+template <int D, int CS>
+struct aotx_delta_rows_lds {
+    __align__(16) float kq[2][2][D];
+    float gate[2][4];                            /* exp(g), beta, k' . q' */
+    __align__(16) float part[2][4][2][CS];
+};
+
+template <int D, int CS>
+static __device__ __forceinline__ void aotx_delta_by_rows(const aotx_delta_args &p, aotx_delta_rows_lds<D, CS> &lds,
+                                                          unsigned int block)
+{
+    constexpr int LC = CS / 4, RG = 256 / LC, NR = D / RG;
+    constexpr int SLICES = D / CS;
+    const unsigned int unit = block / SLICES, slice = block % SLICES;
+    const unsigned int i = unit / p.heads, h = unit % p.heads;
+    const unsigned int lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const aotx_seq_view seq = aotx_seq_of(p.seqs, i, aotx_seqs_read(p.seqs));
+    if (seq.start >= seq.end || seq.end - seq.start > p.few) return;
+    if (threadIdx.x >= 256u) {                   /* a wave that the launch has over */
+        if (!seq.refused)
+            for (unsigned int t = seq.start; t <= seq.end; ++t) __syncthreads();
+        return;
+    }
+    const unsigned int c4 = (threadIdx.x % LC) * 4u, rg = threadIdx.x / LC;
+    const unsigned int col = slice * CS + c4;
+    const unsigned long long width = (unsigned long long)p.heads * D;
+    unsigned short *out = p.out + (unsigned long long)h * D + col;
+    if (seq.refused) {
+        if (threadIdx.x == 0u && slice == 0u && h == 0u) atomicAdd(p.seqs.faults, 1u);
+        for (unsigned int t = seq.start + rg; t < seq.end; t += RG)
+            *(aotx_u16x4 *)(out + t * width) = aotx_u16x4{0, 0, 0, 0};
+        return;
+    }
+    float *sp = p.state + ((unsigned long long)seq.slot * p.heads + h) * D * D + col;
+    aotx_f4 S[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+        S[n] = seq.fresh ? aotx_f4{0, 0, 0, 0} : __builtin_nontemporal_load((const aotx_f4 *)(sp + (n * RG + rg) * D));
+
+    const unsigned short *q = p.qkv + (unsigned long long)(h / p.group) * D;
+    const unsigned short *k = q + (unsigned long long)p.key_heads * D;
+    const unsigned short *v = p.qkv + 2ull * p.key_heads * D + (unsigned long long)h * D + col;
+    const float decay = p.decay[h], dt = p.dt[h];
+    auto stage = [&](unsigned int t, unsigned int at) {
+        if (wave != 0u) return;
+        const unsigned long long row = (unsigned long long)t * p.stride;
+        float kv[D / 64], qv[D / 64], kk = 0.0f, qq = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n) {
+            kv[n] = aotx_h2f(k[row + n * 64 + lane]);
+            qv[n] = aotx_h2f(q[row + n * 64 + lane]);
+            kk += kv[n] * kv[n];
+            qq += qv[n] * qv[n];
+            dot += kv[n] * qv[n];
+        }
+        const float g = aotx_delta_gate(p.a[(unsigned long long)t * p.ab_stride + h], dt, decay);
+        const float beta = 1.0f / (1.0f + expf(-p.b[(unsigned long long)t * p.ab_stride + h]));
+        kk = aotx_wave_sum(kk);
+        qq = aotx_wave_sum(qq);
+        dot = aotx_wave_sum(dot);
+        const float rk = 1.0f / sqrtf(kk + p.eps);
+        const float rq = 1.0f / sqrtf(qq + p.eps) * (D == 128 ? 0.08838834764831845f : 0.125f);
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n) {
+            lds.kq[at][0][n * 64 + lane] = kv[n] * rk;
+            lds.kq[at][1][n * 64 + lane] = qv[n] * rq;
+        }
+        if (lane == 0u) {
+            lds.gate[at][0] = expf(g);
+            lds.gate[at][1] = beta;
+            lds.gate[at][2] = dot * rk * rq;
+        }
+    };
+    stage(seq.start, 0u);
+    __syncthreads();
+    for (unsigned int t = seq.start; t < seq.end; ++t) {
+        const unsigned int at = (t - seq.start) & 1u;
+        const aotx_u16x4 vh = *(const aotx_u16x4 *)(v + (unsigned long long)t * p.stride);
+        aotx_f4 sk = {0, 0, 0, 0}, sq = {0, 0, 0, 0};
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const float kr = lds.kq[at][0][n * RG + rg], qr = lds.kq[at][1][n * RG + rg];
+            sk += S[n] * kr;
+            sq += S[n] * qr;
+        }
+#pragma unroll
+        for (int off = 32; off >= LC; off >>= 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sk[e] += __shfl_xor(sk[e], off, 64);
+                sq[e] += __shfl_xor(sq[e], off, 64);
+            }
+        }
+        if (lane < LC) {
+            *(aotx_f4 *)&lds.part[at][wave][0][c4] = sk;
+            *(aotx_f4 *)&lds.part[at][wave][1][c4] = sq;
+        }
+        if (t + 1u < seq.end) stage(t + 1u, at ^ 1u);
+        __syncthreads();
+        sk = *(const aotx_f4 *)&lds.part[at][0][0][c4];
+        sq = *(const aotx_f4 *)&lds.part[at][0][1][c4];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) {
+            sk += *(const aotx_f4 *)&lds.part[at][w][0][c4];
+            sq += *(const aotx_f4 *)&lds.part[at][w][1][c4];
+        }
+        const float fade = lds.gate[at][0], beta = lds.gate[at][1], dot = lds.gate[at][2];
+        aotx_f4 u, o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            u[e] = beta * (aotx_h2f(vh[e]) - fade * sk[e]);
+            o[e] = fade * sq[e] + dot * u[e];
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n) S[n] = S[n] * fade + u * lds.kq[at][0][n * RG + rg];
+        if (rg == 0u) {
+            aotx_u16x4 oh;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) oh[e] = aotx_f2h(o[e]);
+            *(aotx_u16x4 *)(out + t * width) = oh;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NR; ++n) __builtin_nontemporal_store(S[n], (aotx_f4 *)(sp + (n * RG + rg) * D));
+}
+
 /* Rows r0 .. r0 + n - 1 of a call's qkv: what is read past them is zeros. */
 struct aotx_rows_view {
     __amdgpu_buffer_rsrc_t rs;
@@ -341,11 +474,20 @@ static __device__ __forceinline__ void aotx_delta_rates(const aotx_delta_args &p
     __syncthreads();
 }
 
-template <int D>
+/* FEW: the workgroups past those of the chunks take the sequences of few rows. */
+template <int D, bool FEW>
 __global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
 {
     constexpr int KS = D / 32;
-    __shared__ aotx_delta_within_lds<D> lds;
+    __shared__ union {
+        aotx_delta_within_lds<D> chunk;
+        aotx_delta_rows_lds<D, 64> rows;
+    } share;
+    aotx_delta_within_lds<D> &lds = share.chunk;
+    if (FEW && blockIdx.x >= p.chunks * p.heads) {      /* a sequence of few rows, the fifth wave idle */
+        aotx_delta_by_rows<D, 64>(p, share.rows, blockIdx.x - p.chunks * p.heads);
+        return;
+    }
     const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4;
     const unsigned int w = (unsigned int)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const unsigned int c = blockIdx.x / p.heads, h = aotx_delta_head(p, blockIdx.x % p.heads);
