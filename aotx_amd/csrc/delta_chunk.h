@@ -137,12 +137,13 @@ static __device__ __forceinline__ unsigned int aotx_delta_place(unsigned int j)
  * every RG-th row a thread; S^T k' and S^T q' come from one walk over them, since
  *   out = exp(g) S^T q' + (k' . q') u,
  * so a token costs one reduction over the rows: lanes of a wave first, then the four waves
- * through LDS with one barrier. The next token's rows are normed by wave 0 before it.
+ * through LDS with one barrier. The next token's rows are normed by wave 0 before it, into the
+ * third of three places: a slower wave may still be at the S of the token before.
  * ------------------------------------------------------------------------------------- */
 template <int D, int CS>
 struct aotx_delta_rows_lds {
-    __align__(16) float kq[2][2][D];
-    float gate[2][4];                            /* exp(g), beta, k' . q' */
+    __align__(16) float kq[3][2][D];
+    float gate[3][4];                            /* exp(g), beta, k' . q' */
     __align__(16) float part[2][4][2][CS];
 };
 
@@ -214,8 +215,9 @@ static __device__ __forceinline__ void aotx_delta_by_rows(const aotx_delta_args 
     };
     stage(seq.start, 0u);
     __syncthreads();
+    unsigned int at = 0u;
     for (unsigned int t = seq.start; t < seq.end; ++t) {
-        const unsigned int at = (t - seq.start) & 1u;
+        const unsigned int side = t & 1u, next = at < 2u ? at + 1u : 0u;
         const aotx_u16x4 vh = *(const aotx_u16x4 *)(v + (unsigned long long)t * p.stride);
         aotx_f4 sk = {0, 0, 0, 0}, sq = {0, 0, 0, 0};
 #pragma unroll
@@ -233,17 +235,17 @@ static __device__ __forceinline__ void aotx_delta_by_rows(const aotx_delta_args 
             }
         }
         if (lane < LC) {
-            *(aotx_f4 *)&lds.part[at][wave][0][c4] = sk;
-            *(aotx_f4 *)&lds.part[at][wave][1][c4] = sq;
+            *(aotx_f4 *)&lds.part[side][wave][0][c4] = sk;
+            *(aotx_f4 *)&lds.part[side][wave][1][c4] = sq;
         }
-        if (t + 1u < seq.end) stage(t + 1u, at ^ 1u);
+        if (t + 1u < seq.end) stage(t + 1u, next);
         __syncthreads();
-        sk = *(const aotx_f4 *)&lds.part[at][0][0][c4];
-        sq = *(const aotx_f4 *)&lds.part[at][0][1][c4];
+        sk = *(const aotx_f4 *)&lds.part[side][0][0][c4];
+        sq = *(const aotx_f4 *)&lds.part[side][0][1][c4];
 #pragma unroll
         for (int w = 1; w < 4; ++w) {
-            sk += *(const aotx_f4 *)&lds.part[at][w][0][c4];
-            sq += *(const aotx_f4 *)&lds.part[at][w][1][c4];
+            sk += *(const aotx_f4 *)&lds.part[side][w][0][c4];
+            sq += *(const aotx_f4 *)&lds.part[side][w][1][c4];
         }
         const float fade = lds.gate[at][0], beta = lds.gate[at][1], dot = lds.gate[at][2];
         aotx_f4 u, o;
@@ -260,6 +262,7 @@ static __device__ __forceinline__ void aotx_delta_by_rows(const aotx_delta_args 
             for (int e = 0; e < 4; ++e) oh[e] = aotx_f2h(o[e]);
             *(aotx_u16x4 *)(out + t * width) = oh;
         }
+        at = next;
     }
 #pragma unroll
     for (int n = 0; n < NR; ++n) __builtin_nontemporal_store(S[n], (aotx_f4 *)(sp + (n * RG + rg) * D));

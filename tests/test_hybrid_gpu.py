@@ -231,6 +231,27 @@ def test_chunk_equals_steps(torch, lib):
     assert (np.abs(out - whole) - (2 * c.round + far)).max() <= 0
 
 
+def test_chunk_of_few_rows_is_steps_bit_by_bit(torch, lib):
+    """Sequences of a few rows do what as many calls of aotx_delta_step do, in the same order: waves that
+    run ahead of others leave what those still read."""
+    n, rows = 64, 12
+    c = Delta(torch, 17, [rows] * n, 16, 16, 128, slots=n).up()
+    start = c.dev["state"].clone()
+    KEEP.append(start)
+    g = {k: p(v) for k, v in c.dev.items()}
+    stepped = torch.zeros((rows, n, 16, 128), dtype=torch.float16, device="cuda")
+    for t in range(rows):
+        assert lib.aotx_delta_step(p(c.dev["x"][t]), rows * c.stride, p(c.dev["a"][t]), p(c.dev["b"][t]),
+                                   rows * c.ab_stride, g["decay"], g["dt"], g["pos"], g["agent"], n, 16, 16, 128, EPS,
+                                   g["state"], n, p(stepped[t]), None) == 0
+    state = c.dev["state"].clone()
+    for _ in range(4):
+        c.dev["state"].copy_(start)
+        c.call(lib)
+        assert torch.equal(c.dev["out"].view(n, rows, 16, 128).transpose(0, 1), stepped)
+        assert torch.equal(c.dev["state"], state)
+
+
 def test_chunk_slots_missing_and_named_twice(torch, lib):
     c = Delta(torch, 13, [70, 5, 66, 0, 30, 9], agent=[3, 8, 3, 1, 1, 1], slots=8, fresh=(0,)).up().call(lib).check(lib)
     assert lib.aotx_model_faulted() == 3                 # 8 is no slot; 3 and 1 again (the empty one does not count)
