@@ -136,6 +136,7 @@ extern "C" int aotx_delta_conv(const float *x, unsigned int stride, const float 
     if (channels == 0u || channels % 4u != 0u || stride % 4u != 0u || stride < channels) return 1;
     if (width < 2u || width > 4u || channels > (1u << 20) || tokens > (1u << 20)) return 1;
     if (seqs > AOTX_SLOTS || slots == 0u || slots > AOTX_SLOTS) return 1;
+    if ((unsigned long long)tokens * channels > (1ull << 37)) return 1;     /* threads of a launch: below 2^32 */
     if (offset == nullptr && seqs != tokens) return 1;
     if (!aotx_aligned16(x) || !aotx_aligned16(w) || !aotx_aligned16(bias) || !aotx_aligned16(state)
         || !aotx_aligned16(out))

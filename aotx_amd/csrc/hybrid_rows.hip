@@ -35,11 +35,20 @@ static __device__ __forceinline__ void aotx_gate_store(const aotx_norm_gate_args
     *(aotx_u16x8 *)(p.out + row * p.width + i) = y;
 }
 
+/* A launch has less than 2^32 threads along x: the workgroups past AOTX_GATE_X of a row of the grid
+ * are in the next. */
+#define AOTX_GATE_X (1u << 20)
+
+static __device__ __forceinline__ unsigned long long aotx_gate_block()
+{
+    return (unsigned long long)blockIdx.y * AOTX_GATE_X + blockIdx.x;
+}
+
 /* L lanes a row (a power of two, L * 8 >= width). */
 template <int L>
 __global__ __launch_bounds__(256) void aotx_norm_gate_kernel(aotx_norm_gate_args p)
 {
-    const unsigned long long row = (unsigned long long)blockIdx.x * (256u / L) + threadIdx.x / L;
+    const unsigned long long row = aotx_gate_block() * (256u / L) + threadIdx.x / L;
     const unsigned int i = (threadIdx.x % L) * 8u;
     const bool live = row < p.rows && i < p.width;
     float x[8], sum = 0.0f;
@@ -60,7 +69,8 @@ __global__ __launch_bounds__(256) void aotx_norm_gate_kernel(aotx_norm_gate_args
 __global__ __launch_bounds__(256) void aotx_norm_gate_wide_kernel(aotx_norm_gate_args p)
 {
     __shared__ float share[4];
-    const unsigned long long row = blockIdx.x;
+    const unsigned long long row = aotx_gate_block();
+    if (row >= p.rows) return;
     float x[4][8], sum = 0.0f;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
@@ -86,6 +96,12 @@ __global__ __launch_bounds__(256) void aotx_norm_gate_wide_kernel(aotx_norm_gate
     }
 }
 
+static dim3 aotx_gate_grid(unsigned long long blocks)
+{
+    return blocks <= AOTX_GATE_X ? dim3((unsigned int)blocks)
+                                 : dim3(AOTX_GATE_X, (unsigned int)((blocks + AOTX_GATE_X - 1u) / AOTX_GATE_X));
+}
+
 extern "C" int aotx_norm_gate(const void *x, const float *z, unsigned int z_stride, const float *w,
                               unsigned int tokens, unsigned int heads, unsigned int width,
                               float eps, void *out, void *stream)
@@ -98,7 +114,6 @@ extern "C" int aotx_norm_gate(const void *x, const float *z, unsigned int z_stri
     aotx_norm_gate_args p;
     p.rows = (unsigned long long)tokens * heads;
     if (p.rows == 0ull) return 0;
-    if (p.rows > 0x7FFFFFFFull) return 1;        /* workgroups of one launch */
     p.x = (const unsigned short *)x;
     p.z = z;
     p.w = w;
@@ -108,14 +123,13 @@ extern "C" int aotx_norm_gate(const void *x, const float *z, unsigned int z_stri
     p.width = width;
     p.eps = eps;
     hipStream_t s = aotx_stream(stream);
-#define AOTX_GATE_GO(L)                                                                          \
-    hipLaunchKernelGGL(aotx_norm_gate_kernel<L>, dim3((unsigned int)((p.rows + 256 / L - 1) / (256 / L))), \
-                       dim3(256), 0, s, p)
+#define AOTX_GATE_GO(L) \
+    hipLaunchKernelGGL(aotx_norm_gate_kernel<L>, aotx_gate_grid((p.rows + 256 / L - 1) / (256 / L)), dim3(256), 0, s, p)
     if (width <= 64u) AOTX_GATE_GO(8);
     else if (width <= 128u) AOTX_GATE_GO(16);
     else if (width <= 256u) AOTX_GATE_GO(32);
     else if (width <= 512u) AOTX_GATE_GO(64);
-    else hipLaunchKernelGGL(aotx_norm_gate_wide_kernel, dim3((unsigned int)p.rows), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL(aotx_norm_gate_wide_kernel, aotx_gate_grid(p.rows), dim3(256), 0, s, p);
 #undef AOTX_GATE_GO
     AOTX_LAUNCH_CHECK();
     return 0;

@@ -21,9 +21,9 @@
  * position of its first row. A sequence at position 0 starts from zeros, whatever its slot
  * held. A sequence without rows leaves its slot as it was. Rows before offset[0] and from
  * offset[seqs] on are neither read nor written; an offset past `tokens` is taken as `tokens`, and
- * one below an earlier one as that one. A sequence that names no slot of the caller's (agent[i] >= slots), or a slot that an earlier
- * sequence with rows names too, gets rows of zeros, changes no state, and adds 1 to
- * aotx_model_faulted(). At most AOTX_SLOTS sequences and slots.
+ * one below an earlier one as that one. A sequence that names no slot of the caller's
+ * (agent[i] >= slots), or a slot that an earlier sequence with rows names too, gets rows of zeros,
+ * changes no state, and adds 1 to aotx_model_faulted(). At most AOTX_SLOTS sequences and slots.
  *
  * Two calls that use the same state, or the same workspace, have to follow one another (one
  * stream, or an event between streams). What a call writes overlaps nothing that it reads, but
@@ -45,8 +45,8 @@ extern "C" {
  * [tokens][channels]. Rows before a sequence's first are those that its slot keeps:
  * state fp32 [slots][width - 1][channels], oldest first, which the call leaves holding the
  * last width - 1 rows of x. offset null: sequence i is row i alone (seqs = tokens).
- * channels and stride multiples of 4, width 2 to 4, x, w and state 16-byte aligned, bias and
- * out as well. */
+ * channels (up to 2^20) and stride multiples of 4, tokens up to 2^20 and tokens times channels to
+ * 2^37, width 2 to 4, x, w and state 16-byte aligned, bias and out as well. */
 int aotx_delta_conv(const float *x, unsigned int stride, const float *w, const float *bias,
                     const unsigned int *offset, const unsigned int *pos,
                     const unsigned int *agent, unsigned int seqs, unsigned int tokens,
@@ -95,7 +95,8 @@ int aotx_delta_chunk(const void *qkv, unsigned int stride, const float *a, const
  *   out[t][h][i] = x[t][h][i] / sqrt(mean over i of x^2 + eps) * w[i] * silu(z[t][h][i])
  * x fp16 [tokens][heads][width]; z fp32, row t at z + t * z_stride (heads * width values); w
  * fp32 [width]; out fp16 [tokens][heads][width], which may be x itself. width a multiple of 8
- * up to 8192, z_stride a multiple of 4, all four 16-byte aligned, eps >= 0. */
+ * up to 8192, up to 2^20 tokens and 65536 heads, z_stride a multiple of 4, all four 16-byte
+ * aligned, eps >= 0 (with 0 a row of zeros has no norm: NaN). */
 int aotx_norm_gate(const void *x, const float *z, unsigned int z_stride, const float *w,
                    unsigned int tokens, unsigned int heads, unsigned int width, float eps,
                    void *out, void *stream);
@@ -123,8 +124,8 @@ typedef struct aotx_rope_how {
  * [kv_heads][head_dim]; q_norm, k_norm fp32 [head_dim], each null for no norm; how host;
  * factor fp32 [rope_dim / 2] or null; place unsigned [tokens][axes]; q, k, v fp16
  * [tokens][heads or kv_heads][head_dim] (v null: not written; k and v null with kv_heads = 0).
- * head_dim 64 or 128; rope_dim a multiple of 8, 8 to head_dim; stride a multiple of 4; qkv,
- * the norms, q, k and v 16-byte aligned. */
+ * head_dim 64 or 128, up to 1024 heads and kv_heads, tokens up to 2^20; rope_dim a multiple of 8,
+ * 8 to head_dim; stride a multiple of 4; qkv, the norms, q, k and v 16-byte aligned. */
 int aotx_rope_axes(const float *qkv, unsigned int stride, const float *q_norm,
                    const float *k_norm, const aotx_rope_how *how, const float *factor,
                    const unsigned int *place, unsigned int tokens, unsigned int heads,

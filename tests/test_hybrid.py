@@ -131,7 +131,8 @@ def test_delta_call_refusals(lib):
     dict(x=None), dict(w=None), dict(pos=None), dict(agent=None), dict(state=None), dict(out=None), dict(x=A4),
     dict(w=A4), dict(bias=A4), dict(state=A4), dict(out=A4), dict(channels=0), dict(channels=62), dict(stride=60),
     dict(stride=66), dict(width=1), dict(width=5), dict(seqs=65), dict(slots=0), dict(slots=65),
-    dict(tokens=(1 << 20) + 1), dict(offset=None), dict(channels=(1 << 20) + 4, stride=(1 << 20) + 4)])
+    dict(tokens=(1 << 20) + 1), dict(offset=None), dict(channels=(1 << 20) + 4, stride=(1 << 20) + 4),
+    dict(tokens=1 << 20, channels=(1 << 17) + 4, stride=(1 << 17) + 4)])
 def test_conv_refusals(lib, change):
     assert lib.aotx_delta_conv(*{**CONV, **change}.values()) == 1
     assert lib.aotx_delta_conv(*{**CONV, "tokens": 0}.values()) == 0
@@ -140,7 +141,8 @@ def test_conv_refusals(lib, change):
 @pytest.mark.parametrize("change", [
     dict(x=None), dict(z=None), dict(w=None), dict(out=None), dict(x=A4), dict(z=A4), dict(w=A4), dict(out=A4),
     dict(width=0), dict(width=124), dict(width=8200, z_stride=16400), dict(heads=0), dict(z_stride=252),
-    dict(z_stride=258), dict(eps=-1.0), dict(eps=float("nan")), dict(tokens=(1 << 20) + 1)])
+    dict(z_stride=258), dict(eps=-1.0), dict(eps=float("nan")), dict(tokens=(1 << 20) + 1),
+    dict(heads=65537, width=8, z_stride=1 << 20)])
 def test_norm_gate_refusals(lib, change):
     assert lib.aotx_norm_gate(*{**NORM, **change}.values()) == 1
     assert lib.aotx_norm_gate(*{**NORM, "tokens": 0}.values()) == 0

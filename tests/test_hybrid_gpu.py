@@ -403,6 +403,32 @@ def test_norm_gate(torch, lib, heads, width, tokens, inplace):
     assert (np.abs(got - want) - (2.0 ** -11 + 32 * 2.0 ** -24) * np.abs(want)).max() <= 2.0 ** -25
 
 
+@pytest.mark.parametrize("tokens,heads,width", [(1 << 20, 17, 520), (1 << 20, 1040, 8)])
+def test_norm_gate_more_rows_than_one_grid_row(torch, lib, tokens, heads, width):
+    """Rows past 2^32 threads and outputs past 2^32 bytes: the last rows as any others."""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GiB of device memory")
+    rng = np.random.default_rng(3)
+    x = torch.ones((tokens, heads, width), dtype=torch.float16, device="cuda")
+    z = torch.zeros((tokens, heads * width), dtype=torch.float32, device="cuda")     # a gate of 0
+    w = _up(torch, rng.normal(1, 0.3, width), np.float32)
+    some = [0, tokens // 2 + 1, tokens - 1]
+    xs, zs = rng.normal(0, 2, (3, heads, width)).astype(np.float16), rng.normal(0, 2, (3, heads * width)).astype(np.float32)
+    for i, t in enumerate(some):
+        x[t], z[t] = torch.from_numpy(xs[i]).cuda(), torch.from_numpy(zs[i]).cuda()
+    assert lib.aotx_norm_gate(p(x), p(z), heads * width, p(w), tokens, heads, width, EPS, p(x), None) == 0
+    torch.cuda.synchronize()
+    want = H.norm_gate(xs, zs.reshape(xs.shape), w.cpu().numpy(), EPS)
+    for i, t in enumerate(some):
+        got = x[t].cpu().numpy().astype(np.float64)
+        assert (np.abs(got - want[i]) - (2.0 ** -11 + 32 * 2.0 ** -24) * np.abs(want[i])).max() <= 2.0 ** -25
+        x[t] = 0
+    for part in x.split(1 << 16):
+        assert not part.any()
+    del x, z
+    torch.cuda.empty_cache()
+
+
 # ---- rotary turn -----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("d,rope_dim,spans,order,split,norm,factor", [
