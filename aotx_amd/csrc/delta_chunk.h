@@ -44,7 +44,7 @@ struct aotx_delta_chunk_work {
     float of_k[64];         /* exp(G) r_k 2^e; the rows of K are over 2^e */
     float of_q[64];         /* exp(G) r_q */
     float of_u[64];         /* exp(G_last - G) r_k 2^e */
-    unsigned char vmax[128];/* of every column of V the exponent field of its largest size */
+    unsigned char vmax[128];/* of every column of V: 0 for zeros alone, else its largest size is below 2^(vmax - 15) */
     float fade;             /* exp(G_last) */
     unsigned int odd;       /* first row that is taken out, 64 for none; + 256 if V has a value that is no number */
     unsigned int pad[30];
@@ -465,7 +465,10 @@ static __device__ __forceinline__ void aotx_delta_rates(const aotx_delta_args &p
         u2 v = __builtin_bit_cast(u2, lds.vm[0][lane]);
 #pragma unroll
         for (int x = 1; x < 4; ++x) v = __builtin_elementwise_max(v, __builtin_bit_cast(u2, lds.vm[x][lane]));
-        *(unsigned short *)&to->vmax[2u * lane] = (unsigned short)((v[0] >> 10) | ((v[1] >> 10) << 8));
+        /* exponent fields, one more; below the smallest normal number the one of that */
+        const unsigned int e0 = v[0] != 0u ? (v[0] >> 10 != 0u ? v[0] >> 10 : 1u) + 1u : 0u;
+        const unsigned int e1 = v[1] != 0u ? (v[1] >> 10 != 0u ? v[1] >> 10 : 1u) + 1u : 0u;
+        *(unsigned short *)&to->vmax[2u * lane] = (unsigned short)(e0 | (e1 << 8));
     }
     if (lane == 63u) {
         unsigned int first = badgates != 0ull ? (unsigned int)__builtin_ctzll(badgates) : 64u;
@@ -823,7 +826,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
     };
     auto scale = [&](unsigned int c) {
         /* in the period |S| and |U| of a column stay below sqrt(d) max|S| + 257 max|V|, which the
-         * exponents plus 5 and plus 10 are bounds of */
+         * exponents plus 5 and plus 10 are bounds of. Of zeros alone in V there is none. */
         float ms = 0.0f;
 #pragma unroll
         for (int t = 0; t < TW; ++t)
@@ -834,7 +837,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         int ex = aotx_exponent(ms) - shift + 5, ev = 0;
 #pragma unroll
         for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q) ev = top[q] > ev ? top[q] : ev;
-        ev += 10 - 15;
+        ev = ev != 0 ? ev - 1 + 10 - 15 : -127;
         ex = ex > ev ? ex : ev;
         if (g == 0u) lds.size[w][k.m] = ex;
         __syncthreads();
@@ -842,7 +845,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
 #pragma unroll
         for (int v = 1; v < 4; ++v) ex = lds.size[v][k.m] > ex ? lds.size[v][k.m] : ex;
         ex = 14 - ex;
-        ex = ex > 100 ? 100 : ex < -100 ? -100 : ex;
+        ex = ex > 100 ? 100 : ex < -120 ? -120 : ex;
 #pragma unroll
         for (int t = 0; t < TW; ++t)
 #pragma unroll

@@ -188,6 +188,28 @@ def test_chunk_small_and_large_values(torch, lib, scale):
     Delta(torch, 5, [200, 70], 1, 2, 128, scale=scale).up().call(lib).check(lib)
 
 
+@pytest.mark.parametrize("values", [0.0, 2.0 ** -24, 1.0])
+@pytest.mark.parametrize("state", [1e-20, 1e-9, 1e30])
+def test_chunk_states_far_from_one(torch, lib, state, values):
+    """The state's columns have a scale of their own: a state of any size is as exact, in parts of itself
+    and of the values that join it."""
+    c = Delta(torch, 18, [330], 1, 2, 128)
+    c.state[:] = c.state * np.float32(state / 0.3)
+    c.x[:, 2 * 128:] = np.sign(c.x[:, 2 * 128:].astype(np.float32)) * values
+    c.decay[:] = -0.05
+    c.up().call(lib)
+    want, S, _, _ = c.want()
+    out, got = c.got()
+    # what a column holds at most: its state's length in the unit directions that the keys take, or the
+    # sum of the values
+    top = np.sqrt(128) * np.abs(c.state).max() + 330 * values
+    far = 4 * np.sqrt(128 * 330) * 2.0 ** -24 * top
+    assert np.abs(got - S).max() <= far, (np.abs(got - S).max(), far)
+    big = np.abs(want) + c.round + far > 65504                      # no numbers of fp16
+    assert (np.abs(out - want) - (c.round + far))[~big].max(initial=0) <= 0
+    assert not np.isnan(out).any()
+
+
 @pytest.mark.parametrize("decay,dt,b", [(0.0, 0.0, 30.0), (-1.0, -100.0, 30.0), (-16.0, 30.0, 0.0), (-1e4, 30.0, 0.0),
                                         (-1.0, -3.0, -200.0), (3.0, 0.0, 0.0)])
 def test_chunk_gates_at_their_ends(torch, lib, decay, dt, b):
