@@ -50,6 +50,7 @@ class Delta:
     def __init__(self, torch, seed, lens, key_heads=2, heads=4, d=128, lead=0, tail=0, pad=0, slots=8, fresh=(),
                  agent=None, scale=1.0):
         rng = np.random.default_rng(seed)
+        self.eps = EPS
         self.torch, self.key_heads, self.heads, self.d, self.lens = torch, key_heads, heads, d, lens
         self.tokens = lead + sum(lens) + tail
         self.offset = lead + np.concatenate([[0], np.cumsum(lens)]).astype(np.uint32)
@@ -71,7 +72,7 @@ class Delta:
         out = np.full((self.tokens, self.heads, self.d), 7.0)
         faults, top, near = H.delta(self.x, self.a[:, :self.heads], self.b[:, :self.heads], self.decay.astype(np.float64),
                               self.dt.astype(np.float64), self.offset, self.pos, self.agent, self.key_heads, self.heads,
-                              self.d, EPS, state, out)
+                              self.d, self.eps, state, out)
         self.round = 2.0 ** -11 * (np.abs(out) + near) + 2.0 ** -25      # of out and of its factors
         return out, state, faults, top
 
@@ -87,7 +88,7 @@ class Delta:
         g = {k: p(v) for k, v in self.dev.items()}
         if step:
             rc = lib.aotx_delta_step(g["x"], self.stride, g["a"], g["b"], self.ab_stride, g["decay"], g["dt"], g["pos"],
-                                     g["agent"], self.tokens, self.key_heads, self.heads, self.d, EPS, g["state"],
+                                     g["agent"], self.tokens, self.key_heads, self.heads, self.d, self.eps, g["state"],
                                      len(self.state), g["out"], stream)
         else:
             need = lib.aotx_delta_work(self.tokens, len(self.lens), self.heads, self.d)
@@ -96,7 +97,7 @@ class Delta:
                 KEEP.append(work)
             rc = lib.aotx_delta_chunk(g["x"], self.stride, g["a"], g["b"], self.ab_stride, g["decay"], g["dt"],
                                       g["offset"], g["pos"], g["agent"], len(self.lens), self.tokens, self.key_heads,
-                                      self.heads, self.d, EPS, g["state"], len(self.state), p(work), need, g["out"], stream)
+                                      self.heads, self.d, self.eps, g["state"], len(self.state), p(work), need, g["out"], stream)
         assert rc == 0
         return self
 
@@ -186,6 +187,15 @@ def test_chunk_long(torch, lib):
 def test_chunk_small_and_large_values(torch, lib, scale):
     """Values from far below 1 to near the end of fp16: the state follows them."""
     Delta(torch, 5, [200, 70], 1, 2, 128, scale=scale).up().call(lib).check(lib)
+
+
+@pytest.mark.parametrize("step", [False, True])
+def test_rows_of_subnormal_values(torch, lib, step):
+    """q and k whose values are all below fp16's smallest normal number are brought to length all the same."""
+    c = Delta(torch, 19, [1] * 5 if step else [150, 3], 1, 2, 128)
+    c.x[:, :256] = (c.x[:, :256].astype(np.float32) * 2.0 ** -18).astype(np.float16)
+    c.eps = 1e-14
+    c.up().call(lib, step=step).check(lib)
 
 
 @pytest.mark.parametrize("values", [0.0, 2.0 ** -24, 1.0])
