@@ -139,6 +139,11 @@ static __device__ __forceinline__ unsigned int aotx_delta_place(unsigned int j)
  * so a token costs one reduction over the rows: lanes of a wave first, then the four waves
  * through LDS with one barrier. The next token's rows are normed by wave 0 before it, into the
  * third of three places: a slower wave may still be at the S of the token before.
+ *
+ * Bound by the state's bytes, read and written once whatever the number of rows: a token of 64
+ * slots, 32 heads of 128, moves 270 MB in 50.4 us, 5.3 TB/s, the rate of a large copy; of 1 slot 5
+ * us, what a launch and one trip to memory take. Each further row of a sequence adds 1.7 us, its
+ * reduction's latency. Four columns a thread: a wave's load is whole pieces of 256 bytes.
  * ------------------------------------------------------------------------------------- */
 template <int D, int CS>
 struct aotx_delta_rows_lds {
@@ -290,8 +295,15 @@ static __device__ __forceinline__ unsigned short aotx_rows_2(const aotx_rows_vie
 
 /* ---------------------------------------------------------------------------------------
  * T, P and the row factors of one chunk and head, and K and Q as operands; a workgroup of five
- * waves, wave w < 4 has rows 16 w .. 16 w + 15, wave 4 the gates of all. The products are taken transposed (K_j Q_i^T), so that a lane holds
- * one row i and four columns j along its registers, as the operands above need them.
+ * waves, wave w < 4 has rows 16 w .. 16 w + 15, wave 4 the gates of all. The products are taken
+ * transposed (K_j Q_i^T), so that a lane holds one row i and four columns j along its registers, as
+ * the operands above need them. (1 + M)^-1 goes by blocks of 16: substitution in the blocks on the
+ * diagonal, matrix products below them. The gates have a wave of their own because their
+ * exponentials and the sum over 64 rows are as long a chain as the loads that the others wait for.
+ *
+ * Large calls are bound by memory, the workspace above all (20 KB a chunk and head, 32 a key head):
+ * 8192 rows, 32 heads of 128, read 136 MB and write 146 in 65 us, 4.3 TB/s; 512 rows, a workgroup a
+ * CU, take 8.6 us of latency, 40 rows 7.2.
  * ------------------------------------------------------------------------------------- */
 template <int D>
 struct aotx_delta_within_lds {
@@ -632,6 +644,13 @@ __global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
  * next chunk's S is read.
  * Row x of tile t of S is key 32 (t / 2) + 8 (x / 4) + 4 (t % 2) + x % 4, so that two tiles'
  * accumulators hold keys 8 g .. 8 g + 7 of a step, as 16 bytes of a row of K do.
+ *
+ * Bound by the chain of chunks: 32 heads of 128 are 256 workgroups, one a CU, and each waits for
+ * itself; 8192 rows take 212 to 220 us, 1.7 us a chunk, of which the four passes through LDS and
+ * their products are 1.2 (with all loads in the caches, 512 rows, a chunk takes 1.6 to 2.0). Of that
+ * time LDS works a quarter and the matrix cores 12 %. Columns in slices of 16 make the workgroups
+ * that fill the chip: slices of 32 halve the traffic and took 369 to 400 us; eight waves, four of
+ * them for the output, took as long as four.
  * ------------------------------------------------------------------------------------- */
 #define AOTX_DELTA_PERIOD 4u        /* chunks for which a column's scale holds */
 
