@@ -103,6 +103,14 @@ extern "C" unsigned long long aotx_delta_work(unsigned int tokens, unsigned int 
 }
 
 template <int D>
+static void aotx_delta_one(const aotx_delta_args &p, hipStream_t s)
+{
+    const unsigned int units = (p.seqs.seqs * p.heads + 7u) / 8u * 8u;
+    hipLaunchKernelGGL((aotx_delta_short<D>), dim3(units * (D / 16)), dim3(320), 0, s, p);
+    AOTX_LAUNCH_CHECK();
+}
+
+template <int D>
 static void aotx_delta_chunked(const aotx_delta_args &p, hipStream_t s)
 {
     /* The sequences of few rows, if there can be any, are workgroups of this launch in small calls,
@@ -155,13 +163,19 @@ extern "C" int aotx_delta_chunk(const void *qkv, unsigned int stride, const floa
     p.work = (aotx_delta_chunk_work *)work;
     p.rows = (aotx_h8 *)(p.work + (unsigned long long)p.chunks * heads);
     /* Sequences of few rows go row by row: no matrices to make first, and a decode row beside a
-     * prompt costs what a step does. A row takes 1.7 us, a chunk 7 to 12 if the chip is idle beside
-     * (32 heads of 128: 4 rows 9.8 us and 11.4, 8 rows 16.9 and 11.4); a chip full of sequences is
-     * kept busy longer by chunks (64 sequences of 8 rows 136 us row by row and 202 in chunks, of 16
-     * rows 214 and 204). */
+     * prompt costs what a step does. A row takes 1.7 us, a chunk 11 if the chip is idle beside (32
+     * heads of 128: 4 rows 9.8 us and 11.4, 8 rows 16.9 and 11.4); a chip full of sequences is kept
+     * busy longer by chunks (64 sequences of 8 rows 136 us row by row and 202 in chunks, of 16 rows
+     * 214 and 204). */
     p.few = seqs * heads >= 1024u ? 12u : 4u;
+    /* Calls of at most a chunk a sequence go in one launch while each workgroup of it has a CU (32
+     * heads of 128: 40 rows 8.2 us, in two launches 12.0; 2 sequences of 32 rows 14.3 and 13.9, 4 of
+     * 16 rows 26.1 and 19.6), where 3 rows are as long as 3 by themselves (7.8 us and 8.1). */
+    const bool one = tokens <= AOTX_DELTA_CHUNK && seqs * heads * (head_dim / 16u) <= 256u;
     hipStream_t s = aotx_stream(stream);
-    if (tokens <= p.few) head_dim == 128u ? aotx_delta_rows<128>(p, s) : aotx_delta_rows<64>(p, s);
+    if (tokens <= (one && seqs == 1u ? 2u : p.few))
+        head_dim == 128u ? aotx_delta_rows<128>(p, s) : aotx_delta_rows<64>(p, s);
+    else if (one) head_dim == 128u ? aotx_delta_one<128>(p, s) : aotx_delta_one<64>(p, s);
     else head_dim == 128u ? aotx_delta_chunked<128>(p, s) : aotx_delta_chunked<64>(p, s);
     return 0;
 }

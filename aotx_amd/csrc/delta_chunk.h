@@ -1,4 +1,4 @@
-/* The chunked form of the gated delta rule (aotx_delta_chunk): device code of its two kernels.
+/* The chunked form of the gated delta rule (aotx_delta_chunk): device code of its kernels.
  *
  * Within a chunk of 64 rows of one head, with K, Q the raw rows, V the values, r_k and r_q the
  * rows' inverse lengths (r_q with 1 / sqrt(d)), G the running sum of g, the rule unrolls to
@@ -8,6 +8,7 @@
  *   S <- exp(G_last) S + K^T diag(r_k exp(G_last - G)) U
  * T and P need no state: aotx_delta_within makes them for every chunk at once. What is left,
  * aotx_delta_across, walks a sequence's chunks with a slice of columns of S in registers.
+ * aotx_delta_short does both where no sequence has more than one chunk.
  *
  * Numbers. K, Q and V are fp16 and enter the matrix cores as they are; S, U, X = V - K S and T
  * enter as two fp16 parts (high and rest, 21 bits), so that the state's products are nearly as
@@ -39,8 +40,7 @@ typedef _Float16 aotx_h8 __attribute__((ext_vector_type(8)));
  * loads them, 16 bytes a lane. Row tile w (16 rows), step s (32 columns): lane (m, g) holds row
  * 16 w + m, columns 32 s + 16 (e / 4) + 4 g + e % 4 for e < 8, which is the order in which a
  * wave's accumulators of two row tiles make the other operand. */
-struct aotx_delta_chunk_work {
-    aotx_h8 p[4][2][64], t_hi[4][2][64], t_lo[4][2][64];
+struct aotx_delta_factors {
     float of_k[64];         /* exp(G) r_k 2^e; the rows of K are over 2^e */
     float of_q[64];         /* exp(G) r_q */
     float of_u[64];         /* exp(G_last - G) r_k 2^e */
@@ -48,6 +48,11 @@ struct aotx_delta_chunk_work {
     float fade;             /* exp(G_last) */
     unsigned int odd;       /* first row that is taken out, 64 for none; + 256 if V has a value that is no number */
     unsigned int pad[30];
+};
+
+struct aotx_delta_chunk_work {
+    aotx_h8 p[4][2][64], t_hi[4][2][64], t_lo[4][2][64];
+    aotx_delta_factors of;
 };
 
 struct aotx_delta_args {
@@ -318,12 +323,20 @@ struct aotx_delta_within_lds {
     unsigned int badk[4], badv[4];
 };
 
+/* What a wave of one chunk has in registers: its rows of K, Q, P and T as operands and, of a chunk
+ * that stays in its workgroup, four rows of one column of V. */
+template <int D>
+struct aotx_delta_made {
+    aotx_h8 k[D / 32], q[D / 32], p[2], th[2], tl[2];
+    unsigned short v[4];
+    int top;                    /* of the wave's rows of the column, as vmax */
+};
+
 /* P and M of row 16 W + m. Between blocks, exp(G_i - G_j) is the product of two factors by way of
  * the last row of j's block: both are at most 1, and one exponential a row serves four columns. */
 template <int D, int W>
 static __device__ __forceinline__ void aotx_delta_pairs(aotx_delta_within_lds<D> &lds, aotx_delta_chunk_work *to,
-                                                        const aotx_h8 (&kf)[D / 32], const aotx_h8 (&qf)[D / 32], float inv,
-                                                        float qinv)
+                                                        aotx_delta_made<D> &made, float inv, float qinv)
 {
     constexpr int KS = D / 32;
     const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4, row = 16u * W + m;
@@ -337,8 +350,8 @@ static __device__ __forceinline__ void aotx_delta_pairs(aotx_delta_within_lds<D>
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const aotx_h8 kj = lds.kfrag[jt][s][lane];
-            kks = aotx_mma(kj, kf[s], kks);
-            qks = aotx_mma(kj, qf[s], qks);
+            kks = aotx_mma(kj, made.k[s], kks);
+            qks = aotx_mma(kj, made.q[s], qks);
         }
         const unsigned int j0 = 16u * jt + 4u * g;
         const aotx_f4 rkj = *(const aotx_f4 *)&lds.rk[j0];
@@ -373,7 +386,8 @@ static __device__ __forceinline__ void aotx_delta_pairs(aotx_delta_within_lds<D>
             o[r] = (_Float16)pt[2 * s][r];
             o[4 + r] = (_Float16)pt[2 * s + 1][r];
         }
-        *(aotx_h8 *)((char *)to->p[W][s] + lane * 16u) = o;
+        if (to != nullptr) *(aotx_h8 *)((char *)to->p[W][s] + lane * 16u) = o;
+        else made.p[s] = o;
     }
     /* inverse of 1 + the diagonal block by substitution, a column a lane; every value found is
      * taken from all rows below at once, which do not wait for one another */
@@ -447,11 +461,18 @@ static __device__ __forceinline__ void aotx_delta_column(aotx_delta_within_lds<D
         for (int r = 0; r < 4; ++r) lds.tp[0][16u * (W & 2) + 4u * g + r][at] = lds.tp[1][16u * (W & 2) + 4u * g + r][at] = 0;
 }
 
+/* Of the bits of a size in fp16: 0 of 0, else e with the size below 2^(e - 15), which is the exponent
+ * field and one, below the smallest normal number that number's. */
+static __device__ __forceinline__ unsigned int aotx_delta_top(unsigned int v)
+{
+    return v != 0u ? (v >> 10 != 0u ? v >> 10 : 1u) + 1u : 0u;
+}
+
 /* The fifth wave: gates, a row a lane, and what follows from them. Sums of g are in 64 bits,
  * kept as two floats, so that differences of far sums stay exact. */
-template <int D>
+template <int D, bool STAYS>
 static __device__ __forceinline__ void aotx_delta_rates(const aotx_delta_args &p, aotx_delta_within_lds<D> &lds,
-                                                        aotx_delta_chunk_work *to, unsigned int r0, unsigned int n,
+                                                        aotx_delta_factors *to, unsigned int r0, unsigned int n,
                                                         unsigned int h)
 {
     const unsigned int lane = threadIdx.x & 63u;
@@ -472,15 +493,12 @@ static __device__ __forceinline__ void aotx_delta_rates(const aotx_delta_args &p
     to->of_k[lane] = all * lds.ks[lane];
     to->of_q[lane] = all * lds.rq[lane];
     to->of_u[lane] = last * lds.ks[lane];
-    if (lane < D / 2) {                 /* two columns a lane */
+    if (!STAYS && lane < D / 2) {       /* two columns a lane */
         typedef unsigned short u2 __attribute__((ext_vector_type(2)));
         u2 v = __builtin_bit_cast(u2, lds.vm[0][lane]);
 #pragma unroll
         for (int x = 1; x < 4; ++x) v = __builtin_elementwise_max(v, __builtin_bit_cast(u2, lds.vm[x][lane]));
-        /* exponent fields, one more; below the smallest normal number the one of that */
-        const unsigned int e0 = v[0] != 0u ? (v[0] >> 10 != 0u ? v[0] >> 10 : 1u) + 1u : 0u;
-        const unsigned int e1 = v[1] != 0u ? (v[1] >> 10 != 0u ? v[1] >> 10 : 1u) + 1u : 0u;
-        *(unsigned short *)&to->vmax[2u * lane] = (unsigned short)(e0 | (e1 << 8));
+        *(unsigned short *)&to->vmax[2u * lane] = (unsigned short)(aotx_delta_top(v[0]) | (aotx_delta_top(v[1]) << 8));
     }
     if (lane == 63u) {
         unsigned int first = badgates != 0ull ? (unsigned int)__builtin_ctzll(badgates) : 64u;
@@ -492,57 +510,41 @@ static __device__ __forceinline__ void aotx_delta_rates(const aotx_delta_args &p
     __syncthreads();
 }
 
-/* FEW: the workgroups past those of the chunks take the sequences of few rows. */
-template <int D, bool FEW>
-__global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
+/* A wave's part of one chunk and head, of the first four waves. STAYS: its workgroup goes on with it,
+ * for the 16 columns from col; else it goes to the workspace. */
+template <int D, bool STAYS>
+static __device__ __forceinline__ void aotx_delta_make(const aotx_delta_args &p, aotx_delta_within_lds<D> &lds,
+                                                       aotx_delta_chunk_work *to, unsigned int c, unsigned int h,
+                                                       unsigned int w, unsigned int r0, unsigned int n,
+                                                       unsigned int col, aotx_delta_made<D> &made)
 {
     constexpr int KS = D / 32;
-    __shared__ union {
-        aotx_delta_within_lds<D> chunk;
-        aotx_delta_rows_lds<D, 64> rows;
-    } share;
-    aotx_delta_within_lds<D> &lds = share.chunk;
-    if (FEW && blockIdx.x >= p.chunks * p.heads) {      /* a sequence of few rows, the fifth wave idle */
-        aotx_delta_by_rows<D, 64>(p, share.rows, blockIdx.x - p.chunks * p.heads);
-        return;
-    }
-    const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4;
-    const unsigned int w = (unsigned int)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const unsigned int c = blockIdx.x / p.heads, h = aotx_delta_head(p, blockIdx.x % p.heads);
-
-    unsigned int mine, before;
-    const aotx_seq_lanes seqs = aotx_seqs_read(p.seqs);
-    aotx_delta_chunks(p, seqs, &mine, &before);
-    const unsigned int i = (unsigned int)__popcll(__ballot(lane < p.seqs.seqs && before + mine <= c));
-    if (i >= p.seqs.seqs) return;
-    const aotx_seq_view seq = aotx_seq_of(p.seqs, i, seqs);
-    if (seq.refused) return;
-    const unsigned int r0 = seq.start + (c - (unsigned int)__builtin_amdgcn_readlane((int)before, (int)i)) * 64u;
-    const unsigned int n = seq.end - r0 < 64u ? seq.end - r0 : 64u;
-    aotx_delta_chunk_work *to = p.work + (unsigned long long)c * p.heads + h;
-
-    if (w == 4u) {
-        aotx_delta_rates<D>(p, lds, to, r0, n, h);
-        return;
-    }
     /* rows of K and Q, columns 32 s + 8 g .. of row 16 w + m; rows past the chunk read as zeros */
+    const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4;
     const unsigned int kh = h / p.group;
     const unsigned int row = 16u * w + m;
     const aotx_rows_view rows = aotx_rows_of(p, r0, n);
     const unsigned int at_q = row * p.stride * 2u + (kh * D + 8u * g) * 2u, at_k = at_q + p.key_heads * D * 2u;
-    aotx_h8 kf[KS], qf[KS];
+    aotx_h8 (&kf)[KS] = made.k, (&qf)[KS] = made.q;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         kf[s] = aotx_rows_16(rows, at_k + 64u * s);
         qf[s] = aotx_rows_16(rows, at_q + 64u * s);
     }
-    /* V: eight columns of every 256 / (D / 8)-th row a thread */
+    /* V: eight columns of every 256 / (D / 8)-th row a thread, or rows 16 w + 4 g .. of one */
     constexpr unsigned int VR = 256 / (D / 8);
     aotx_u16x8 vv[64 / VR];
+    const unsigned int at_v = (2u * p.key_heads * D + h * D) * 2u;
+    if constexpr (STAYS) {
 #pragma unroll
-    for (unsigned int r = 0; r < 64u / VR; ++r)
-        vv[r] = __builtin_bit_cast(aotx_u16x8, aotx_rows_16(rows, (r * VR + threadIdx.x / (D / 8)) * p.stride * 2u
-                                   + (2u * p.key_heads * D + h * D + threadIdx.x % (D / 8) * 8u) * 2u));
+        for (int r = 0; r < 4; ++r)
+            made.v[r] = aotx_rows_2(rows, (16u * w + 4u * g + r) * p.stride * 2u + at_v + (col + m) * 2u);
+    } else {
+#pragma unroll
+        for (unsigned int r = 0; r < 64u / VR; ++r)
+            vv[r] = __builtin_bit_cast(aotx_u16x8, aotx_rows_16(rows, (r * VR + threadIdx.x / (D / 8)) * p.stride * 2u
+                                       + at_v + threadIdx.x % (D / 8) * 16u));
+    }
     float kk = 0.0f, qq = 0.0f;
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -574,11 +576,15 @@ __global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
         lds.ks[row] = ldexpf(inv, ex);
         lds.rq[row] = qinv;
     }
-    if (h % p.group == 0u) {
-        aotx_h8 *k = aotx_delta_rows_of(p, c, kh, D) + w * KS * 64u, *q = k + 8u * D;
-        /* over 2^ex in two steps, each a number of fp16; ex below -28 is of rows of zeros */
+    /* over 2^ex in two steps, each a number of fp16; ex below -28 is of rows of zeros */
+    _Float16 a, z;
+    {
         const int one = ex > 14 ? 14 : ex < -14 ? -14 : ex, two = ex - one < -14 ? -14 : ex - one;
-        const _Float16 a = (_Float16)ldexpf(1.0f, -one), z = (_Float16)ldexpf(1.0f, -two);
+        a = (_Float16)ldexpf(1.0f, -one);
+        z = (_Float16)ldexpf(1.0f, -two);
+    }
+    if (!STAYS && h % p.group == 0u) {
+        aotx_h8 *k = aotx_delta_rows_of(p, c, kh, D) + w * KS * 64u, *q = k + 8u * D;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             *(aotx_h8 *)((char *)(k + s * 64) + lane * 16u) = kf[s] * a * z;
@@ -587,7 +593,22 @@ __global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
     }
     /* the largest size of V's columns: sizes of fp16 are in the order of their bits. What is no
      * number is left out, and told of. */
-    {
+    if constexpr (STAYS) {
+        unsigned int top = 0u;
+        bool none = false;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const unsigned int v = made.v[r] & 0x7FFFu;
+            if (v >= 0x7C00u) none = true;
+            else if (v > top) top = v;
+        }
+        const unsigned long long told = __ballot(none);
+        if (lane == 0u) lds.badv[w] = told != 0ull ? 1u : 0u;
+        unsigned int o = (unsigned int)__shfl_xor((int)top, 16, 64);
+        top = o > top ? o : top;
+        o = (unsigned int)__shfl_xor((int)top, 32, 64);
+        made.top = (int)aotx_delta_top(o > top ? o : top);
+    } else {
         aotx_u16x8 top = vv[0] & (unsigned short)0x7FFF;
 #pragma unroll
         for (unsigned int r = 1; r < 64u / VR; ++r) top = __builtin_elementwise_max(top, vv[r] & (unsigned short)0x7FFF);
@@ -615,10 +636,10 @@ __global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
         if (lane < D / 8) *(aotx_u16x8 *)((unsigned short *)lds.vm[w] + lane * 8u) = top;
     }
     __syncthreads();
-    if (w == 0u) aotx_delta_pairs<D, 0>(lds, to, kf, qf, inv, qinv);
-    else if (w == 1u) aotx_delta_pairs<D, 1>(lds, to, kf, qf, inv, qinv);
-    else if (w == 2u) aotx_delta_pairs<D, 2>(lds, to, kf, qf, inv, qinv);
-    else aotx_delta_pairs<D, 3>(lds, to, kf, qf, inv, qinv);
+    if (w == 0u) aotx_delta_pairs<D, 0>(lds, to, made, inv, qinv);
+    else if (w == 1u) aotx_delta_pairs<D, 1>(lds, to, made, inv, qinv);
+    else if (w == 2u) aotx_delta_pairs<D, 2>(lds, to, made, inv, qinv);
+    else aotx_delta_pairs<D, 3>(lds, to, made, inv, qinv);
     __syncthreads();
 
     if (w == 0u) aotx_delta_column<D, 0>(lds);
@@ -629,9 +650,55 @@ __global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
 #pragma unroll
     for (unsigned int s = 0; s < 2u; ++s) {
         if (s > w / 2u) continue;
-        to->t_hi[w][s][lane] = *(const aotx_h8 *)&lds.tp[0][row][32u * s + 8u * g];
-        to->t_lo[w][s][lane] = *(const aotx_h8 *)&lds.tp[1][row][32u * s + 8u * g];
+        const aotx_h8 hi = *(const aotx_h8 *)&lds.tp[0][row][32u * s + 8u * g];
+        const aotx_h8 lo = *(const aotx_h8 *)&lds.tp[1][row][32u * s + 8u * g];
+        if constexpr (STAYS) {
+            made.th[s] = hi;
+            made.tl[s] = lo;
+        } else {
+            to->t_hi[w][s][lane] = hi;
+            to->t_lo[w][s][lane] = lo;
+        }
     }
+    if constexpr (STAYS)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kf[s] = kf[s] * a * z;
+}
+
+/* FEW: the workgroups past those of the chunks take the sequences of few rows. */
+template <int D, bool FEW>
+__global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
+{
+    __shared__ union {
+        aotx_delta_within_lds<D> chunk;
+        aotx_delta_rows_lds<D, 64> rows;
+    } share;
+    aotx_delta_within_lds<D> &lds = share.chunk;
+    if (FEW && blockIdx.x >= p.chunks * p.heads) {      /* a sequence of few rows, the fifth wave idle */
+        aotx_delta_by_rows<D, 64>(p, share.rows, blockIdx.x - p.chunks * p.heads);
+        return;
+    }
+    const unsigned int lane = threadIdx.x & 63u;
+    const unsigned int w = (unsigned int)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const unsigned int c = blockIdx.x / p.heads, h = aotx_delta_head(p, blockIdx.x % p.heads);
+
+    unsigned int mine, before;
+    const aotx_seq_lanes seqs = aotx_seqs_read(p.seqs);
+    aotx_delta_chunks(p, seqs, &mine, &before);
+    const unsigned int i = (unsigned int)__popcll(__ballot(lane < p.seqs.seqs && before + mine <= c));
+    if (i >= p.seqs.seqs) return;
+    const aotx_seq_view seq = aotx_seq_of(p.seqs, i, seqs);
+    if (seq.refused) return;
+    const unsigned int r0 = seq.start + (c - (unsigned int)__builtin_amdgcn_readlane((int)before, (int)i)) * 64u;
+    const unsigned int n = seq.end - r0 < 64u ? seq.end - r0 : 64u;
+    aotx_delta_chunk_work *to = p.work + (unsigned long long)c * p.heads + h;
+
+    if (w == 4u) {
+        aotx_delta_rates<D, false>(p, lds, &to->of, r0, n, h);
+        return;
+    }
+    aotx_delta_made<D> made;
+    aotx_delta_make<D, false>(p, lds, to, c, h, w, r0, n, 0u, made);
 }
 
 /* ---------------------------------------------------------------------------------------
@@ -704,10 +771,12 @@ struct aotx_delta_tile {
 
 /* NS: steps of 32 columns that the wave's rows of T and P have, 1 for waves 0 and 1, else 2.
  * AHEAD: how many chunks ahead the loads run, one or two; with 3, two, and their lines are asked
- * for before. */
+ * for before; with 0, there is one chunk, and it and the state are in registers (one, the top of V's
+ * column, one_state). */
 template <int D, int NS, int AHEAD>
 static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &p, const aotx_delta_walk k,
-                                                         aotx_delta_lds<D> &lds)
+                                                         aotx_delta_lds<D> &lds, const aotx_delta_tile<D, NS> *one,
+                                                         int one_top, const aotx_f4 (*one_state)[D / 64])
 {
     constexpr int KS = D / 32, TW = D / 64;
     typedef aotx_delta_tile<D, NS> tile_t;
@@ -717,7 +786,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
     /* a wave's places within a chunk's parts, in bytes */
     typedef aotx_delta_chunk_work work_t;
     const unsigned int at_k = w * KS * 1024u + l16, at_p = w * 2048u + l16;
-    const unsigned int at_of = (unsigned int)offsetof(work_t, of_k) + i0 * 4u;
+    const unsigned int at_of = (unsigned int)offsetof(work_t, of) + i0 * 4u;
     const unsigned int at_v = i0 * p.stride * 2u + (2u * p.key_heads * D + k.h * D + k.col) * 2u;
     /* the chunk that is loaded, and 1 while there is one: past the end the loads go through views
      * of no size, which read zeros and touch no memory, so that every pass has the same in flight */
@@ -793,8 +862,8 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         x.of_k = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 0u));
         x.of_q = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 256u));
         x.of_u = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 512u));
-        x.fade = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(f, 0, (int)offsetof(work_t, fade), 0));
-        x.odd = __builtin_amdgcn_raw_buffer_load_b32(f, 0, (int)offsetof(work_t, odd), 0);
+        x.fade = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(f, 0, (int)(offsetof(work_t, of) + offsetof(aotx_delta_factors, fade)), 0));
+        x.odd = __builtin_amdgcn_raw_buffer_load_b32(f, 0, (int)(offsetof(work_t, of) + offsetof(aotx_delta_factors, odd)), 0);
         if constexpr (NS == 1 && AHEAD == 3) x.touched = touch();
         advance();
     };
@@ -803,27 +872,36 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
 #pragma unroll
         for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q)
                 top[q] = p.work[(unsigned long long)(k.c0 + (c + q < k.chunks ? c + q : k.chunks - 1u)) * p.heads
-                                   + k.h].vmax[k.col];
+                                   + k.h].of.vmax[k.col];
     };
 
     aotx_f4 S[TW];                              /* times 2^shift */
     int shift = 0;
     float *sp = p.state + ((unsigned long long)k.seq.slot * p.heads + k.h) * D * D + k.col;
+    if constexpr (AHEAD > 0) {
 #pragma unroll
-    for (int t = 0; t < TW; ++t)
+        for (int t = 0; t < TW; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const unsigned int tile = w * TW + t;
-            const unsigned int key = 32u * (tile >> 1) + 8u * g + 4u * (tile & 1u) + r;
-            S[t][r] = k.seq.fresh ? 0.0f : sp[key * D];
-        }
+            for (int r = 0; r < 4; ++r) {
+                const unsigned int tile = w * TW + t;
+                const unsigned int key = 32u * (tile >> 1) + 8u * g + 4u * (tile & 1u) + r;
+                S[t][r] = k.seq.fresh ? 0.0f : sp[key * D];
+            }
+    } else {
+#pragma unroll
+        for (int t = 0; t < TW; ++t) S[t] = (*one_state)[t];
+    }
     /* in the order in which the passes load, so that the waits for them count alike */
     tile_t A, B;
-    load_top(0u);
-    load_k(A);
-    load_q(A);
-    load_t(A);
-    load_rest(A);
+    if constexpr (AHEAD == 0) {
+        A = *one;
+    } else {
+        load_top(0u);
+        load_k(A);
+        load_q(A);
+        load_t(A);
+        load_rest(A);
+    }
     if constexpr (AHEAD > 1) {
         load_k(B);
         load_q(B);
@@ -853,9 +931,10 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             for (int r = 0; r < 4; ++r) ms = fmaxf(ms, fabsf(S[t][r]));
         ms = fmaxf(ms, __shfl_xor(ms, 16, 64));
         ms = fmaxf(ms, __shfl_xor(ms, 32, 64));
-        int ex = aotx_exponent(ms) - shift + 5, ev = 0;
+        int ex = aotx_exponent(ms) - shift + 5, ev = one_top;
+        if constexpr (AHEAD > 0)
 #pragma unroll
-        for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q) ev = top[q] > ev ? top[q] : ev;
+            for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q) ev = top[q] > ev ? top[q] : ev;
         ev = ev != 0 ? ev - 1 + 10 - 15 : -127;
         ex = ex > ev ? ex : ev;
         if (g == 0u) lds.size[w][k.m] = ex;
@@ -870,7 +949,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
 #pragma unroll
             for (int r = 0; r < 4; ++r) S[t][r] = ldexpf(S[t][r], ex - shift);
         shift = ex;
-        load_top(c + AOTX_DELTA_PERIOD);
+        if constexpr (AHEAD > 0) load_top(c + AOTX_DELTA_PERIOD);
     };
     auto pass = [&](tile_t &x, unsigned int c) {
         /* rows that are taken out, or past the chunk, have zeros in K, Q and V: their X, U and T
@@ -930,7 +1009,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
 #pragma unroll
         for (int s = 0; s < KS; ++s) *(aotx_h8 *)&lds.k[16u * w + k.m][32 * s + 8u * g] = x.k[s];
         __syncthreads();
-        load_k(x);
+        if constexpr (AHEAD > 0) load_k(x);
         aotx_h8 xh[NS], xl[NS];
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -971,8 +1050,10 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
                 const s4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(at + 16 * (D + 8)));
                 kt[t][s] = __builtin_bit_cast(aotx_h8, __builtin_shufflevector(a, z, 0, 1, 2, 3, 4, 5, 6, 7));
             }
-        load_q(x);
-        load_t(x);
+        if constexpr (AHEAD > 0) {
+            load_q(x);
+            load_t(x);
+        }
         aotx_h8 vh[2], vl[2], uh[NS], ul[NS];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -1010,13 +1091,13 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             for (int r = 0; r < 4; ++r)
                 if (i0 + r >= lim) o[r] = nan;
         }
-        load_rest(x);
+        if constexpr (AHEAD > 0) load_rest(x);
     };
     /* a period a turn: no branch but the ways out, and the loads in flight are always the same */
     for (unsigned int c = 0;;) {
         scale(c);
         pass(A, c);
-        if (++c >= k.chunks) break;
+        if (AHEAD == 0 || ++c >= k.chunks) break;
         pass(AHEAD > 1 ? B : A, c);
         if (++c >= k.chunks) break;
         pass(A, c);
@@ -1066,8 +1147,95 @@ __global__ __launch_bounds__(256, AHEAD > 1 ? 2 : 3) void aotx_delta_across(aotx
         return;
     }
     /* (scalar: the barriers of both ways count together) */
-    if (k.w < 2u) aotx_delta_follow<D, 1, AHEAD>(p, k, lds);
-    else aotx_delta_follow<D, 2, AHEAD>(p, k, lds);
+    if (k.w < 2u) aotx_delta_follow<D, 1, AHEAD>(p, k, lds, nullptr, 0, nullptr);
+    else aotx_delta_follow<D, 2, AHEAD>(p, k, lds, nullptr, 0, nullptr);
+}
+
+/* ---------------------------------------------------------------------------------------
+ * A call of up to 64 rows: no sequence has more than one chunk, and a workgroup (five waves, as
+ * within) makes T and P for its 16 columns by itself. They stay in the registers of the waves that
+ * take them, and a second launch and the way through memory are saved; the slices of a head make
+ * the same T and P, which costs nothing while the chip has room. 40 rows of 32 heads of 128 take
+ * 8.2 us, the latency of a launch, the rows and one chunk's chain; in two launches 12.0.
+ * ------------------------------------------------------------------------------------- */
+template <int D, int NS>
+static __device__ __forceinline__ void aotx_delta_go_on(const aotx_delta_args &p, const aotx_delta_walk &k,
+                                                        aotx_delta_lds<D> &lds, const aotx_delta_factors &of,
+                                                        const aotx_f4 (&S)[D / 64], const aotx_delta_made<D> &made)
+{
+    aotx_delta_tile<D, NS> x;
+    const unsigned int i0 = 16u * k.w + 4u * k.g;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+        x.k[s] = made.k[s];
+        x.q[s] = made.q[s];
+    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        x.p[s] = made.p[s];
+        x.th[s] = made.th[s];
+        x.tl[s] = made.tl[s];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x.v[r] = made.v[r];
+    x.of_k = *(const aotx_f4 *)&of.of_k[i0];
+    x.of_q = *(const aotx_f4 *)&of.of_q[i0];
+    x.of_u = *(const aotx_f4 *)&of.of_u[i0];
+    x.fade = of.fade;
+    x.odd = of.odd;
+    aotx_delta_follow<D, NS, 0>(p, k, lds, &x, made.top, &S);
+}
+
+template <int D>
+__global__ __launch_bounds__(320) void aotx_delta_short(aotx_delta_args p)
+{
+    constexpr unsigned int SLICES = D / 16;
+    __shared__ aotx_delta_within_lds<D> made_lds;
+    __shared__ aotx_delta_lds<D> lds;
+    __shared__ __align__(16) aotx_delta_factors of;
+    aotx_delta_walk k;
+    k.lane = threadIdx.x & 63u;
+    k.m = k.lane & 15u;
+    k.g = k.lane >> 4;
+    k.w = (unsigned int)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const unsigned int unit = blockIdx.x / (8u * SLICES) * 8u + blockIdx.x % 8u;
+    const unsigned int slice = blockIdx.x / 8u % SLICES;
+    if (unit >= p.seqs.seqs * p.heads) return;
+    k.h = aotx_delta_head(p, unit % p.heads);
+    k.seq = aotx_seq_of(p.seqs, unit / p.heads, aotx_seqs_read(p.seqs));
+    const unsigned int n = k.seq.end - k.seq.start;
+    if (n == 0u) return;
+    k.c0 = 0u;
+    k.chunks = 1u;
+    k.col = slice * 16u + k.m;
+    if (k.seq.refused) {
+        if (threadIdx.x == 0u && slice == 0u && k.h == 0u) atomicAdd(p.seqs.faults, 1u);
+        if (k.w < 4u)
+            for (unsigned int t = k.seq.start + k.w * 4u + k.g; t < k.seq.end; t += 16u)
+                p.out[((unsigned long long)t * p.heads + k.h) * D + k.col] = 0;
+        return;
+    }
+    if (k.w == 4u) {
+        aotx_delta_rates<D, true>(p, made_lds, &of, k.seq.start, n, k.h);
+        /* the barriers of the others: one in scale, three in a pass, one more of an odd chunk */
+        const unsigned int more = __builtin_amdgcn_readfirstlane((int)of.odd) != 64 ? 5u : 4u;
+        for (unsigned int b = 0; b < more; ++b) __syncthreads();
+        return;
+    }
+    aotx_f4 S[D / 64];
+    const float *sp = p.state + ((unsigned long long)k.seq.slot * p.heads + k.h) * D * D + k.col;
+#pragma unroll
+    for (int t = 0; t < D / 64; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const unsigned int tile = k.w * (D / 64) + t;
+            const unsigned int key = 32u * (tile >> 1) + 8u * k.g + 4u * (tile & 1u) + r;
+            S[t][r] = k.seq.fresh ? 0.0f : sp[key * D];
+        }
+    aotx_delta_made<D> made;
+    aotx_delta_make<D, true>(p, made_lds, nullptr, 0u, k.h, k.w, k.seq.start, n, slice * 16u, made);
+    if (k.w < 2u) aotx_delta_go_on<D, 1>(p, k, lds, of, S, made);
+    else aotx_delta_go_on<D, 2>(p, k, lds, of, S, made);
 }
 
 #endif

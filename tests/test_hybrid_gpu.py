@@ -160,6 +160,26 @@ def test_chunk_few_rows_beside_many(torch, lib, key_heads, heads, d):
           agent=list(range(33)) + [5]).up().call(lib).check(lib)
 
 
+@pytest.mark.parametrize("key_heads,heads,d", [(2, 4, 128), (1, 1, 64), (4, 8, 64)])
+@pytest.mark.parametrize("lens,lead,tail", [([3], 0, 0), ([64], 0, 0), ([17, 0, 33, 1], 5, 8), ([1, 2, 3, 4, 5, 6], 1, 0),
+                                            ([0, 31], 0, 33), ([16, 48], 0, 0)])
+def test_chunk_short_calls(torch, lib, key_heads, heads, d, lens, lead, tail):
+    """Up to 64 rows: one launch, whatever the sequences."""
+    Delta(torch, len(lens) + heads, lens, key_heads, heads, d, lead=lead, tail=tail, pad=16, fresh=(1, 2)).up().call(
+        lib).check(lib)
+
+
+@pytest.mark.parametrize("heads", [32, 33])
+def test_chunk_short_calls_up_to_a_workgroup_a_cu(torch, lib, heads):
+    """The largest call of one launch, and one head more."""
+    Delta(torch, 23, [29], heads, heads, 128).up().call(lib).check(lib)
+
+
+def test_chunk_short_slots_missing_and_named_twice(torch, lib):
+    Delta(torch, 24, [7, 5, 6, 0, 30, 9], agent=[3, 8, 3, 1, 1, 1], slots=8, fresh=(0,)).up().call(lib).check(lib)
+    assert lib.aotx_model_faulted() == 3
+
+
 @pytest.mark.parametrize("lens", [[3], [70, 1, 130]])
 def test_chunk_keeps_to_its_workspace(torch, lib, lens):
     """What lies behind the workspace's stated size stays as it was, and what a workspace holds
@@ -303,20 +323,21 @@ def test_chunk_offsets_out_of_order_stay_in_bounds(torch, lib, offset):
     assert np.abs(S - state).max() <= far and (np.abs(out - want) <= far + c.round).all()
 
 
-@pytest.mark.parametrize("what,bad", [("v", np.inf), ("v", np.nan), ("k", np.nan), ("k", -np.inf), ("q", np.nan),
-                                      ("a", np.nan), ("b", np.nan), ("a", np.inf), ("a", -np.inf), ("b", np.inf)])
-@pytest.mark.parametrize("at", [0, 37, 63, 64, 100])
-def test_chunk_inf_and_nan_reach_no_earlier_row(torch, lib, what, bad, at):
+BAD = pytest.mark.parametrize("what,bad", [("v", np.inf), ("v", np.nan), ("k", np.nan), ("k", -np.inf), ("q", np.nan),
+                                         ("a", np.nan), ("b", np.nan), ("a", np.inf), ("a", -np.inf), ("b", np.inf)])
+
+
+def _bad_value(torch, lib, lens, what, bad, at):
     """Row `at` of the first sequence gets a value that is no number. Rows before it, the second
     sequence, heads of other keys (or, from v, a and b, all other heads), and columns beside a bad
     value are what they are without it, bit for bit; a bad q reaches its row alone. In the column of
     a bad v the rows before it are right, but not always to the bit: a column's numbers are split
     into two parts at a scale that goes by the sizes of its values in four chunks, the replaced one
     among them, so they may round elsewhere, by 2^-21 a product, which the sums' own bound holds."""
-    heads, d = 4, 128
-    clean = Delta(torch, 15, [130, 20], 2, heads, d).up().call(lib)
+    heads, d, n = 4, 128, lens[0]
+    clean = Delta(torch, 15, lens, 2, heads, d).up().call(lib)
     base, S0 = clean.got()
-    c = Delta(torch, 15, [130, 20], 2, heads, d)
+    c = Delta(torch, 15, lens, 2, heads, d)
     col = {"q": 5, "k": 2 * d + 5, "v": 4 * d + d + 9}      # head 0's query, head 0's key, head 1's value 9
     if what in col:
         c.x[at, col[what]] = bad
@@ -329,19 +350,19 @@ def test_chunk_inf_and_nan_reach_no_earlier_row(torch, lib, what, bad, at):
     if what == "q":
         hit[at, 0:2] = True
     elif what == "k":
-        hit[at:130, 0:2] = True
+        hit[at:n, 0:2] = True
         hit_state[slot, 0:2] = True
     elif what == "v":
-        hit[at:130, 1, 9] = True
+        hit[at:n, 1, 9] = True
         hit_state[slot, 1, :, 9] = True
     else:
-        hit[at:130, 1] = True
+        hit[at:n, 1] = True
         hit_state[slot, 1] = True
     near = np.zeros(out.shape, dtype=bool)
     if what == "v":
         near[:at, 1, 9] = True
         want, _, _, top = clean.want()
-        far = 4 * np.sqrt(d * 130) * 2.0 ** -24 * top
+        far = 4 * np.sqrt(d * n) * 2.0 ** -24 * top
         assert (np.abs(out[near] - want[near]) <= clean.round[near] + far).all()
     assert np.array_equal(out[~hit & ~near], base[~hit & ~near])
     assert np.array_equal(S[~hit_state], S0[~hit_state])
@@ -350,9 +371,21 @@ def test_chunk_inf_and_nan_reach_no_earlier_row(torch, lib, what, bad, at):
         assert not np.isfinite(S[hit_state]).any()
     else:                                                   # an infinite gate is a decay or rate at its end
         want, state, _, top = c.want()
-        far = 4 * np.sqrt(d * 130) * 2.0 ** -24 * top
+        far = 4 * np.sqrt(d * n) * 2.0 ** -24 * top
         assert np.abs(S - state).max() <= far
         assert (np.abs(out - want) - (c.round + far)).max() <= 0
+
+
+@BAD
+@pytest.mark.parametrize("at", [0, 37, 63, 64, 100])
+def test_chunk_inf_and_nan_reach_no_earlier_row(torch, lib, what, bad, at):
+    _bad_value(torch, lib, [130, 20], what, bad, at)
+
+
+@BAD
+@pytest.mark.parametrize("at", [0, 15, 16, 39])
+def test_short_call_inf_and_nan_reach_no_earlier_row(torch, lib, what, bad, at):
+    _bad_value(torch, lib, [40, 20], what, bad, at)
 
 
 # ---- convolution -----------------------------------------------------------------------------
