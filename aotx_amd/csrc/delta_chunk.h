@@ -1006,10 +1006,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         aotx_split4(y, &hi, &lo);
         *((aotx_h4 *)&lds.x[w >> 1][0][lane] + (w & 1u)) = hi;
         *((aotx_h4 *)&lds.x[w >> 1][1][lane] + (w & 1u)) = lo;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) *(aotx_h8 *)&lds.k[16u * w + k.m][32 * s + 8u * g] = x.k[s];
         __syncthreads();
-        if constexpr (AHEAD > 0) load_k(x);
         aotx_h8 xh[NS], xl[NS];
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -1022,6 +1019,10 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             qs = aotx_mma(x.q[s], sl[s], qs);
             qs = aotx_mma(x.q[s], sh[s], qs);
         }
+        /* K's rows go to LDS for the state's update where nothing waits for them yet */
+#pragma unroll
+        for (int s = 0; s < KS; ++s) *(aotx_h8 *)&lds.k[16u * w + k.m][32 * s + 8u * g] = x.k[s];
+        if constexpr (AHEAD > 0) load_k(x);
         a = aotx_f4{0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -1036,6 +1037,17 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         *((aotx_h4 *)&lds.u[w >> 1][0][lane] + (w & 1u)) = hi;
         *((aotx_h4 *)&lds.u[w >> 1][1][lane] + (w & 1u)) = lo;
         __syncthreads();
+        aotx_h8 vh[2], vl[2], uh[NS], ul[NS];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            vh[s] = lds.v[s][0][lane];
+            vl[s] = lds.v[s][1][lane];
+        }
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            uh[s] = lds.u[s][0][lane];
+            ul[s] = lds.u[s][1][lane];
+        }
         /* K by columns: lane (m, g) addresses row m / 4 of four, keys 8 (m % 4) .. + 3 of the
          * tile's 16, and gets key m of it for all four rows */
         aotx_h8 kt[TW][2];
@@ -1054,22 +1066,12 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             load_q(x);
             load_t(x);
         }
-        aotx_h8 vh[2], vl[2], uh[NS], ul[NS];
+#pragma unroll
+        for (int t = 0; t < TW; ++t) S[t] *= x.fade;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            vh[s] = lds.v[s][0][lane];
-            vl[s] = lds.v[s][1][lane];
-        }
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            uh[s] = lds.u[s][0][lane];
-            ul[s] = lds.u[s][1][lane];
-        }
-#pragma unroll
-        for (int t = 0; t < TW; ++t) {
-            S[t] *= x.fade;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
+            for (int t = 0; t < TW; ++t) {
                 S[t] = aotx_mma(kt[t][s], vl[s], S[t]);
                 S[t] = aotx_mma(kt[t][s], vh[s], S[t]);
             }
