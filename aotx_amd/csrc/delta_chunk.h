@@ -971,6 +971,10 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
 #pragma unroll
             for (int v = 0; v < 4; ++v) lim = lds.bad[v][k.m] < lim ? lds.bad[v][k.m] : lim;
         }
+        /* K's rows to LDS while the state's last products run, and back by columns while the chain waits
+         * for X */
+#pragma unroll
+        for (int s = 0; s < KS; ++s) *(aotx_h8 *)&lds.k[16u * w + k.m][32 * s + 8u * g] = x.k[s];
         aotx_h4 hi, lo;
 #pragma unroll
         for (int t = 0; t < TW; ++t) {
@@ -1019,9 +1023,20 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             qs = aotx_mma(x.q[s], sl[s], qs);
             qs = aotx_mma(x.q[s], sh[s], qs);
         }
-        /* K's rows go to LDS for the state's update where nothing waits for them yet */
+        /* K by columns: lane (m, g) addresses row m / 4 of four, keys 8 (m % 4) .. + 3 of the
+         * tile's 16, and gets key m of it for all four rows */
+        aotx_h8 kt[TW][2];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) *(aotx_h8 *)&lds.k[16u * w + k.m][32 * s + 8u * g] = x.k[s];
+        for (int t = 0; t < TW; ++t)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                typedef short s4 __attribute__((ext_vector_type(4)));
+                const unsigned int tile = w * TW + t;
+                unsigned short *at = &lds.k[32 * s + 4u * g + (k.m >> 2)][32u * (tile >> 1) + 4u * (tile & 1u) + 8u * (k.m & 3u)];
+                const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at);
+                const s4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(at + 16 * (D + 8)));
+                kt[t][s] = __builtin_bit_cast(aotx_h8, __builtin_shufflevector(a, z, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
         if constexpr (AHEAD > 0) load_k(x);
         a = aotx_f4{0, 0, 0, 0};
 #pragma unroll
@@ -1048,20 +1063,6 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             uh[s] = lds.u[s][0][lane];
             ul[s] = lds.u[s][1][lane];
         }
-        /* K by columns: lane (m, g) addresses row m / 4 of four, keys 8 (m % 4) .. + 3 of the
-         * tile's 16, and gets key m of it for all four rows */
-        aotx_h8 kt[TW][2];
-#pragma unroll
-        for (int t = 0; t < TW; ++t)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                typedef short s4 __attribute__((ext_vector_type(4)));
-                const unsigned int tile = w * TW + t;
-                unsigned short *at = &lds.k[32 * s + 4u * g + (k.m >> 2)][32u * (tile >> 1) + 4u * (tile & 1u) + 8u * (k.m & 3u)];
-                const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at);
-                const s4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(at + 16 * (D + 8)));
-                kt[t][s] = __builtin_bit_cast(aotx_h8, __builtin_shufflevector(a, z, 0, 1, 2, 3, 4, 5, 6, 7));
-            }
         if constexpr (AHEAD > 0) {
             load_q(x);
             load_t(x);
