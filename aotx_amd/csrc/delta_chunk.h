@@ -906,7 +906,6 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         load_k(B);
         load_q(B);
         load_t(B);
-        load_rest(B);
     }
 
     /* the chunk before: its output, still to be stored */
@@ -951,7 +950,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         shift = ex;
         if constexpr (AHEAD > 0) load_top(c + AOTX_DELTA_PERIOD);
     };
-    auto pass = [&](tile_t &x, unsigned int c) {
+    auto pass = [&](tile_t &x, tile_t &other, unsigned int c) {
         /* rows that are taken out, or past the chunk, have zeros in K, Q and V: their X, U and T
          * are zeros by themselves. Only a chunk with values that are no numbers asks more. */
         const unsigned int odd = (unsigned int)__builtin_amdgcn_readfirstlane((int)x.odd);
@@ -990,13 +989,13 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             sh[s] = lds.s[s][0][lane];
             sl[s] = lds.s[s][1][lane];
         }
-        if (c != 0u) store(c - 1u);
         aotx_f4 a = {0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             a = aotx_mma(x.k[s], sl[s], a);
             a = aotx_mma(x.k[s], sh[s], a);
         }
+        if constexpr (AHEAD > 1) load_rest(other);
         const float up = ldexpf(1.0f, shift);
         aotx_f4 y;
 #pragma unroll
@@ -1017,6 +1016,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             xh[s] = lds.x[s][0][lane];
             xl[s] = lds.x[s][1][lane];
         }
+        if (c != 0u) store(c - 1u);
         aotx_f4 qs = {0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -1094,18 +1094,18 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             for (int r = 0; r < 4; ++r)
                 if (i0 + r >= lim) o[r] = nan;
         }
-        if constexpr (AHEAD > 0) load_rest(x);
+        if constexpr (AHEAD == 1) load_rest(x);
     };
     /* a period a turn: no branch but the ways out, and the loads in flight are always the same */
     for (unsigned int c = 0;;) {
         scale(c);
-        pass(A, c);
+        pass(A, B, c);
         if (AHEAD == 0 || ++c >= k.chunks) break;
-        pass(AHEAD > 1 ? B : A, c);
+        pass(AHEAD > 1 ? B : A, A, c);
         if (++c >= k.chunks) break;
-        pass(A, c);
+        pass(A, B, c);
         if (++c >= k.chunks) break;
-        pass(AHEAD > 1 ? B : A, c);
+        pass(AHEAD > 1 ? B : A, A, c);
         if (++c >= k.chunks) break;
     }
     store(k.chunks - 1u);
