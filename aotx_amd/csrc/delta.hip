@@ -127,10 +127,11 @@ static void aotx_delta_chunked(const aotx_delta_args &p, hipStream_t s)
     AOTX_LAUNCH_CHECK();
     const unsigned int units = (p.seqs.seqs * p.heads + 7u) / 8u * 8u;
     /* Two chunks' loads in flight where few workgroups share a CU or sequences are long; else one,
-     * in so few registers that three workgroups do (32 heads of 128: 4 sequences of 2048 rows 231
-     * us with two and 251 with one, 64 of 16 rows 245 and 204, 8 of 512 rows 124 and 121). Lines
+     * in so few registers that three workgroups do (32 heads of 128: 4 sequences of 2048 rows 211
+     * us with two and 229 with one, 64 of 16 rows 240 and 185, 8 of 512 rows 113 and 111). Lines
      * are asked for early where the caches of the XCDs do not hold the workspace any more (8192
-     * rows 265 us with and 280 without, 2048 rows 74 and 68). */
+     * rows 226 us with and 230 without, 4 sequences of 2048 rows 206 and 211, 4096 rows 118 and
+     * 116). */
     const dim3 grid(units * (D / 16));
     if (grid.x > 512u && p.seqs.tokens < 1024u * p.seqs.seqs)
         hipLaunchKernelGGL((aotx_delta_across<D, 1>), grid, dim3(256), 0, s, p);
@@ -165,12 +166,12 @@ extern "C" int aotx_delta_chunk(const void *qkv, unsigned int stride, const floa
     /* Sequences of few rows go row by row: no matrices to make first, and a decode row beside a
      * prompt costs what a step does. A row takes 1.7 us, a chunk 11 if the chip is idle beside (32
      * heads of 128: 4 rows 9.8 us and 11.4, 8 rows 16.9 and 11.4); a chip full of sequences is kept
-     * busy longer by chunks (64 sequences of 8 rows 136 us row by row and 202 in chunks, of 16 rows
-     * 214 and 204). */
+     * busy longer by chunks (64 sequences of 8 rows 136 us row by row and 183 in chunks, of 12 rows
+     * 174 and 184). */
     p.few = seqs * heads >= 1024u ? 12u : 4u;
     /* Calls of at most a chunk a sequence go in one launch while each workgroup of it has a CU (32
-     * heads of 128: 40 rows 8.2 us, in two launches 12.0; 2 sequences of 32 rows 14.3 and 13.9, 4 of
-     * 16 rows 26.1 and 19.6), where 3 rows are as long as 3 by themselves (7.8 us and 8.1). */
+     * heads of 128: 40 rows 8.2 us, in two launches 12.0; 2 sequences of 32 rows 14.1 and 13.6, 4 of
+     * 16 rows 26.0 and 18.6), where 3 rows take no longer than row by row (7.6 us and 8.1). */
     const bool one = tokens <= AOTX_DELTA_CHUNK && seqs * heads * (head_dim / 16u) <= 256u;
     hipStream_t s = aotx_stream(stream);
     if (tokens <= (one && seqs == 1u ? 2u : p.few))

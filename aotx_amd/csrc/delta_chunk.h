@@ -705,17 +705,18 @@ __global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
  * The walk over a sequence's chunks. Four waves have 16 columns of one head's S: wave w the rows
  * of S that one step of K S takes (D / 4 of them, in accumulators), and rows 16 w .. 16 w + 15 of
  * the chunk. S, X and U pass between the waves through LDS as operands, a
- * barrier each; everything else a chunk needs is loaded into registers two chunks ahead, each
- * register as soon as it has been used. A chunk's output is made where the state's chain waits:
- * Q S while X is on its way, P U behind the state's update, its rounding and stores while the
- * next chunk's S is read.
+ * barrier each; everything else a chunk needs is loaded into registers a chunk or two ahead. All
+ * that the state's chain does not need is where the chain waits: loads beside products that are
+ * under way, K's way through LDS and Q S while S and X are on theirs, P U behind the state's update,
+ * its rounding and stores while the next chunk's X is read. (At other places in the chain the same
+ * loads, stores and LDS writes made 8192 rows 3 to 40 us longer.)
  * Row x of tile t of S is key 32 (t / 2) + 8 (x / 4) + 4 (t % 2) + x % 4, so that two tiles'
  * accumulators hold keys 8 g .. 8 g + 7 of a step, as 16 bytes of a row of K do.
  *
  * Bound by the chain of chunks: 32 heads of 128 are 256 workgroups, one a CU, and each waits for
- * itself; 8192 rows take 212 to 220 us, 1.7 us a chunk, of which the four passes through LDS and
- * their products are 1.2 (with all loads in the caches, 512 rows, a chunk takes 1.6 to 2.0). Of that
- * time LDS works a quarter and the matrix cores 12 %. Columns in slices of 16 make the workgroups
+ * itself; 8192 rows take 177 to 187 us, 1.4 us a chunk, the latencies of its three passes through LDS
+ * and of the products between them. Of that time LDS works 30 % and the matrix cores 15 %; the
+ * vector caches wait for the L2 in 41 % of theirs. Columns in slices of 16 make the workgroups
  * that fill the chip: slices of 32 halve the traffic and took 369 to 400 us; eight waves, four of
  * them for the output, took as long as four.
  * ------------------------------------------------------------------------------------- */
