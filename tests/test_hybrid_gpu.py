@@ -742,6 +742,39 @@ def test_linear_layer_in_a_graph(torch, lib):
         assert torch.equal(now()[0][:2], want["token"][0][:2])
 
 
+@pytest.mark.parametrize("lens", [[40], [5, 3, 11], [2, 1], [200, 1, 70], [700, 65]])
+def test_chunk_forms_in_a_graph(torch, lib, lens):
+    """Each form that a call takes (one launch, row by row, both), captured and replayed with other
+    values, offsets and positions than it was captured with: as an eager call of those."""
+    c, other = (Delta(torch, seed, lens, 2, 4, 128, fresh=(0,)).up() for seed in (30, 31))
+    other.offset[:] = other.offset[::-1].max() - other.offset[::-1]         # the lengths in another order
+    other.pos[:] = other.pos[::-1]
+    other.up()
+    need = lib.aotx_delta_work(c.tokens, len(lens), 4, 128)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    KEEP.append(work)
+    want = []
+    for d in (c, other):
+        eager = {k: v.clone() for k, v in d.dev.items()}
+        d.call(lib, work=work)
+        torch.cuda.synchronize()
+        want.append((eager, d.dev["out"].clone(), d.dev["state"].clone()))
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=side):
+        c.call(lib, stream=ctypes.c_void_p(side.cuda_stream), work=work)
+    for turn in range(4):
+        inputs, out, state = want[turn % 2]
+        for k, v in inputs.items():
+            c.dev[k].copy_(v)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(c.dev["out"], out) and torch.equal(c.dev["state"], state), turn
+    assert lib.aotx_model_faulted() == 0
+
+
 def test_rope_axes_in_a_graph(torch, lib):
     """A captured turn, replayed with other places and rows in the same buffers: the frequencies
     are the call's, everything else is read at the replay."""
