@@ -113,11 +113,11 @@ static void aotx_delta_one(const aotx_delta_args &p, hipStream_t s)
 template <int D>
 static void aotx_delta_chunked(const aotx_delta_args &p, hipStream_t s)
 {
-    /* The sequences of few rows, if there can be any, are workgroups of this launch in small calls,
+    /* The sequences of few rows, if any go row by row, are workgroups of this launch in small calls,
      * where one launch less counts, and a launch of their own where the registers that they add
      * would cost the chunks more (32 heads of 128: 2 sequences of 512 rows 33.5 us in one and 35.7
      * in two, 8 of 512 rows 124 and 118). */
-    const unsigned int few = p.seqs.seqs > 1u ? p.seqs.seqs * p.heads * (D / 64) : 0u, blocks = p.chunks * p.heads;
+    const unsigned int few = p.few != 0u ? p.seqs.seqs * p.heads * (D / 64) : 0u, blocks = p.chunks * p.heads;
     if (few != 0u && blocks <= 1536u) {
         hipLaunchKernelGGL((aotx_delta_within<D, true>), dim3(blocks + few), dim3(320), 0, s, p);
     } else {
@@ -177,6 +177,11 @@ extern "C" int aotx_delta_chunk(const void *qkv, unsigned int stride, const floa
     if (tokens <= (one && seqs == 1u ? 2u : p.few))
         head_dim == 128u ? aotx_delta_rows<128>(p, s) : aotx_delta_rows<64>(p, s);
     else if (one) head_dim == 128u ? aotx_delta_one<128>(p, s) : aotx_delta_one<64>(p, s);
-    else head_dim == 128u ? aotx_delta_chunked<128>(p, s) : aotx_delta_chunked<64>(p, s);
+    else {
+        /* The lengths are the device's: of a call's one sequence, whatever the rows that there is room
+         * for. It goes in chunks at any length, so that no workgroups wait beside for few rows. */
+        if (seqs == 1u) p.few = 0u;
+        head_dim == 128u ? aotx_delta_chunked<128>(p, s) : aotx_delta_chunked<64>(p, s);
+    }
     return 0;
 }

@@ -199,6 +199,40 @@ def test_chunk_keeps_to_its_workspace(torch, lib, lens):
     assert np.array_equal(outs[0][0], outs[1][0]) and np.array_equal(outs[0][1], outs[1][1])
 
 
+@pytest.mark.parametrize("heads,d,tail", [(33, 128, 37), (4, 128, 97), (2, 64, 200), (65, 64, 17)])
+@pytest.mark.parametrize("rows", [0, 1, 3, 4, 5])
+@pytest.mark.parametrize("agent", [2, 8])
+def test_chunk_one_sequence_shorter_than_its_call(torch, lib, heads, d, tail, rows, agent):
+    """A call's one sequence may have fewer rows than the call has room for: any number of them is
+    taken, a fresh slot is cleared, and one that is none is told of."""
+    Delta(torch, heads + rows, [rows], 1, heads, d, lead=2, tail=tail, fresh=(0,) if rows == 3 else (), agent=[agent]).up().call(
+        lib).check(lib)
+    assert lib.aotx_model_faulted() == (agent == 8 and rows > 0)
+
+
+@pytest.mark.parametrize("heads,tokens", [(4, 200), (33, 40)])
+def test_chunk_one_sequence_shrinks_in_a_graph(torch, lib, heads, tokens):
+    """A call captured for a full bucket and replayed with pieces of any length, as a server does."""
+    c = Delta(torch, 25, [tokens], 1, heads, 128).up()
+    work = torch.empty(lib.aotx_delta_work(tokens, 1, heads, 128), dtype=torch.uint8, device="cuda")
+    KEEP.append(work)
+    first = {k: v.clone() for k, v in c.dev.items()}
+    c.call(lib, work=work)
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=side):
+        c.call(lib, stream=ctypes.c_void_p(side.cuda_stream), work=work)
+    for rows in (3, tokens, 1, 4, 0, 30, 3):
+        for k, v in first.items():
+            c.dev[k].copy_(v)
+        c.dev["offset"].copy_(torch.tensor([0, rows], dtype=torch.int32))
+        c.offset, c.lens = np.array([0, rows], dtype=np.uint32), [rows]
+        torch.cuda.synchronize()
+        g.replay()
+        c.check(lib)
+
+
 def test_chunk_long(torch, lib):
     Delta(torch, 21, [6000], 1, 2, 64, slots=1, fresh=(0,)).up().call(lib).check(lib)
 
