@@ -2,24 +2,26 @@
  *
  * Within a chunk of 64 rows of one head, with K, Q the raw rows, V the values, r_k and r_q the
  * rows' inverse lengths (r_q with 1 / sqrt(d)), G the running sum of g, the rule unrolls to
- *   M_ij = beta_i r_k,i r_k,j (K_i . K_j) exp(G_i - G_j) for i > j,   T = (1 + M)^-1 diag(beta)
- *   U = T (V - diag(exp(G) r_k) K S)
+ *   M_ij = beta_i r_k,i r_k,j (K_i . K_j) exp(G_i - G_j) for i > j,   T = (1 + M)^-1
+ *   X = diag(beta) (V - diag(exp(G) r_k) K S),   U = T X
  *   out = diag(exp(G) r_q) Q S + P U,   P_ij = r_q,i r_k,j (Q_i . K_j) exp(G_i - G_j) for i >= j
  *   S <- exp(G_last) S + K^T diag(r_k exp(G_last - G)) U
  * T and P need no state: aotx_delta_within makes them for every chunk at once. What is left,
  * aotx_delta_across, walks a sequence's chunks with a slice of columns of S in registers.
  * aotx_delta_short does both where no sequence has more than one chunk.
  *
- * Numbers. K, Q and V are fp16 and enter the matrix cores as they are; S, U, X = V - K S and T
- * enter as two fp16 parts (high and rest, 21 bits), so that the state's products are nearly as
+ * Numbers. K and Q are fp16 and enter the matrix cores as they are; S, U, X and T enter as two
+ * fp16 parts (high and rest, 21 bits), so that the state's products are nearly as
  * good as fp32 ones at two or three times the work of plain fp16 instead of sixteen times for
  * fp32 matrix instructions. P, which only the output sees, is rounded to fp16 once, by 2^-11 as
- * the output itself is. The parts have fp16's range: T and P are at most 1 (the rule only ever
- * takes away from what a unit key finds), rows of K are brought to lengths of 1/2 to 1 by a power
- * of two 2^e (entries below 2^-14 lose bits, 2^-24 of the length at most), whose scale goes
- * into the factors of X and U, and S, X and U carry a power of two for every column, set anew
- * every four chunks from the column's largest entries: a state's column grows by at most the
- * sum of the 256 values' sizes in that time.
+ * the output itself is. The parts have fp16's range, below which their step is 2^-24. M and T are at
+ * most 1 (the rule only ever takes away from what a unit key finds) and go times 2^14, where the step
+ * is 2^-38; beta is in X, not in T, whose entries would go with its square. Rows of K are brought to
+ * lengths of 1/2 to 1 by a power of two 2^e (entries below 2^-14 lose bits, 2^-24 of the length at
+ * most), whose scale goes into the factors of X and U. S, X and U carry a power of two for every
+ * column, set anew every four chunks from the column's largest state entry and beta |v|: a state's
+ * column grows by at most the sum of the 256 rows' in that time. So their step is 2^-33 of that entry
+ * or 2^-28 of that beta |v|, whichever is larger, or 2^-21 of the number itself.
  *
  * A row whose K, a or b is no number is taken out (its K, g and beta are zeros) and remembered:
  * from that row on, out and the state are NaN; the same for one column from a bad value in V on.
@@ -41,11 +43,12 @@ typedef _Float16 aotx_h8 __attribute__((ext_vector_type(8)));
  * 16 w + m, columns 32 s + 16 (e / 4) + 4 g + e % 4 for e < 8, which is the order in which a
  * wave's accumulators of two row tiles make the other operand. */
 struct aotx_delta_factors {
-    float of_k[64];         /* exp(G) r_k 2^e; the rows of K are over 2^e */
+    float of_k[64];         /* beta exp(G) r_k 2^e; the rows of K are over 2^e */
     float of_q[64];         /* exp(G) r_q */
-    float of_u[64];         /* exp(G_last - G) r_k 2^e */
-    unsigned char vmax[128];/* of every column of V: 0 for zeros alone, else its largest size is below 2^(vmax - 15) */
-    float fade;             /* exp(G_last) */
+    float of_u[64];         /* exp(G_last - G) r_k 2^e / AOTX_DELTA_UP */
+    float of_b[64];         /* beta */
+    unsigned char vmax[128];/* of every column: its largest beta |v| is below 2^(vmax - 126), or 0 */
+    float fade;             /* exp(G_last), with the sign bit set where odd is not 64 */
     unsigned int odd;       /* first row that is taken out, 64 for none; + 256 if V has a value that is no number */
     unsigned int pad[30];
 };
@@ -81,6 +84,8 @@ static __device__ __forceinline__ aotx_h8 *aotx_delta_rows_of(const aotx_delta_a
 }
 
 static __device__ __forceinline__ aotx_h8 aotx_h8_of(aotx_u16x8 v) { return __builtin_bit_cast(aotx_h8, v); }
+
+#define AOTX_DELTA_UP 16384.0f      /* of M and T as operands */
 
 /* x = hi + lo to 22 bits. x has to be one rounded number: where the compiler fuses the product
  * that makes x into one of its two uses, the parts belong to different roundings. */
@@ -372,7 +377,7 @@ static __device__ __forceinline__ void aotx_delta_pairs(aotx_delta_within_lds<D>
             const float from = expf((gi - lds.ghi[16 * jt + 15]) + (gil - lds.glo[16 * jt + 15]));
             const aotx_f4 fade = *(const aotx_f4 *)&lds.near_end[j0] * rkj * from;
             aotx_h4 hi, lo;
-            aotx_split4(kks * fade * bi, &hi, &lo);
+            aotx_split4(kks * fade * (bi * AOTX_DELTA_UP), &hi, &lo);
             *(aotx_h4 *)&lds.below[0][row - 16u][j0] = hi;
             *(aotx_h4 *)&lds.below[1][row - 16u][j0] = lo;
             pt[jt] = qks * fade * qinv;
@@ -418,18 +423,18 @@ static __device__ __forceinline__ aotx_f4 aotx_mma_parts(aotx_h4 ahi, aotx_h4 al
     return __builtin_amdgcn_mfma_f32_16x16x16f16(ahi, bhi, c, 0, 0, 0);
 }
 
-/* Column W of blocks of T, downwards: T_b = -D_b (sum of M_bq T_q), then times beta. A block in
- * accumulator order is the right operand of the next product as it stands. */
+/* Column W of blocks of T, downwards: T_b = -D_b (sum of M_bq T_q). A block in accumulator order is the
+ * right operand of the next product as it stands. All operands are times AOTX_DELTA_UP, and their
+ * products brought back to one of it. */
 template <int D, int W>
 static __device__ __forceinline__ void aotx_delta_column(aotx_delta_within_lds<D> &lds)
 {
     const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4;
-    const unsigned int row = 16u * W + m, at = aotx_delta_place(row);
-    const float bj = lds.beta[row];
+    const unsigned int at = aotx_delta_place(16u * W + m);
     aotx_f4 tc[4];
     aotx_h4 hi[4], lo[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) tc[0][r] = lds.diag[W][4u * g + r][m];
+    for (int r = 0; r < 4; ++r) tc[0][r] = lds.diag[W][4u * g + r][m] * AOTX_DELTA_UP;
     aotx_split4(tc[0], &hi[0], &lo[0]);
 #pragma unroll
     for (int off = 1; off < 4 - W; ++off) {
@@ -440,15 +445,15 @@ static __device__ __forceinline__ void aotx_delta_column(aotx_delta_within_lds<D
             acc = aotx_mma_parts(*(const aotx_h4 *)&lds.below[0][16 * (bt - 1) + m][16 * (W + q) + 4u * g],
                                  *(const aotx_h4 *)&lds.below[1][16 * (bt - 1) + m][16 * (W + q) + 4u * g], hi[q], lo[q], acc);
         aotx_h4 dhi, dlo, yhi, ylo;
-        aotx_split4(*(const aotx_f4 *)&lds.diag[bt][m][4u * g], &dhi, &dlo);
-        aotx_split4(-acc, &yhi, &ylo);
-        tc[off] = aotx_mma_parts(dhi, dlo, yhi, ylo, aotx_f4{0, 0, 0, 0});
+        aotx_split4(*(const aotx_f4 *)&lds.diag[bt][m][4u * g] * AOTX_DELTA_UP, &dhi, &dlo);
+        aotx_split4(acc * (-1.0f / AOTX_DELTA_UP), &yhi, &ylo);
+        tc[off] = aotx_mma_parts(dhi, dlo, yhi, ylo, aotx_f4{0, 0, 0, 0}) * (1.0f / AOTX_DELTA_UP);
         aotx_split4(tc[off], &hi[off], &lo[off]);
     }
 #pragma unroll
     for (int off = 0; off < 4 - W; ++off) {
         aotx_h4 th, tl;
-        aotx_split4(tc[off] * bj, &th, &tl);
+        aotx_split4(tc[off], &th, &tl);
         const aotx_u16x4 hb = __builtin_bit_cast(aotx_u16x4, th), lb = __builtin_bit_cast(aotx_u16x4, tl);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -459,13 +464,6 @@ static __device__ __forceinline__ void aotx_delta_column(aotx_delta_within_lds<D
     if (W & 1)
 #pragma unroll
         for (int r = 0; r < 4; ++r) lds.tp[0][16u * (W & 2) + 4u * g + r][at] = lds.tp[1][16u * (W & 2) + 4u * g + r][at] = 0;
-}
-
-/* Of the bits of a size in fp16: 0 of 0, else e with the size below 2^(e - 15), which is the exponent
- * field and one, below the smallest normal number that number's. */
-static __device__ __forceinline__ unsigned int aotx_delta_top(unsigned int v)
-{
-    return v != 0u ? (v >> 10 != 0u ? v >> 10 : 1u) + 1u : 0u;
 }
 
 /* The fifth wave: gates, a row a lane, and what follows from them. Sums of g are in 64 bits,
@@ -490,23 +488,25 @@ static __device__ __forceinline__ void aotx_delta_rates(const aotx_delta_args &p
     lds.near_end[lane] = expf((float)(__shfl(sum, (int)(lane | 15u), 64) - sum));
     lds.beta[lane] = rate;
     __syncthreads();
-    to->of_k[lane] = all * lds.ks[lane];
+    to->of_k[lane] = rate * all * lds.ks[lane];
     to->of_q[lane] = all * lds.rq[lane];
-    to->of_u[lane] = last * lds.ks[lane];
+    to->of_u[lane] = last * lds.ks[lane] * (1.0f / AOTX_DELTA_UP);
+    to->of_b[lane] = rate;
+    if (lane == 63u) {
+        unsigned int first = badgates != 0ull ? (unsigned int)__builtin_ctzll(badgates) : 64u;
+        for (int v = 0; v < 4; ++v) first = lds.badk[v] < first ? lds.badk[v] : first;
+        const unsigned int odd = first | (lds.badv[0] | lds.badv[1] | lds.badv[2] | lds.badv[3]) << 8;
+        to->fade = odd != 64u ? -all : all;
+        to->odd = odd;
+    }
+    __syncthreads();
     if (!STAYS && lane < D / 2) {       /* two columns a lane */
         typedef unsigned short u2 __attribute__((ext_vector_type(2)));
         u2 v = __builtin_bit_cast(u2, lds.vm[0][lane]);
 #pragma unroll
         for (int x = 1; x < 4; ++x) v = __builtin_elementwise_max(v, __builtin_bit_cast(u2, lds.vm[x][lane]));
-        *(unsigned short *)&to->vmax[2u * lane] = (unsigned short)(aotx_delta_top(v[0]) | (aotx_delta_top(v[1]) << 8));
+        *(unsigned short *)&to->vmax[2u * lane] = (unsigned short)(v[0] | (v[1] << 8));
     }
-    if (lane == 63u) {
-        unsigned int first = badgates != 0ull ? (unsigned int)__builtin_ctzll(badgates) : 64u;
-        for (int v = 0; v < 4; ++v) first = lds.badk[v] < first ? lds.badk[v] : first;
-        to->fade = all;
-        to->odd = first | (lds.badv[0] | lds.badv[1] | lds.badv[2] | lds.badv[3]) << 8;
-    }
-    __syncthreads();
     __syncthreads();
 }
 
@@ -591,40 +591,46 @@ static __device__ __forceinline__ void aotx_delta_make(const aotx_delta_args &p,
             *(aotx_h8 *)((char *)(q + s * 64) + lane * 16u) = qf[s];
         }
     }
-    /* the largest size of V's columns: sizes of fp16 are in the order of their bits. What is no
-     * number is left out, and told of. */
+    /* V's values that are no numbers are told of, and left out of what follows */
+    bool none = false;
     if constexpr (STAYS) {
-        unsigned int top = 0u;
-        bool none = false;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const unsigned int v = made.v[r] & 0x7FFFu;
-            if (v >= 0x7C00u) none = true;
-            else if (v > top) top = v;
-        }
-        const unsigned long long told = __ballot(none);
-        if (lane == 0u) lds.badv[w] = told != 0ull ? 1u : 0u;
-        unsigned int o = (unsigned int)__shfl_xor((int)top, 16, 64);
-        top = o > top ? o : top;
-        o = (unsigned int)__shfl_xor((int)top, 32, 64);
-        made.top = (int)aotx_delta_top(o > top ? o : top);
+        for (int r = 0; r < 4; ++r) none |= (made.v[r] & 0x7FFFu) >= 0x7C00u;
     } else {
         aotx_u16x8 top = vv[0] & (unsigned short)0x7FFF;
 #pragma unroll
         for (unsigned int r = 1; r < 64u / VR; ++r) top = __builtin_elementwise_max(top, vv[r] & (unsigned short)0x7FFF);
-        const bool none = __builtin_reduce_max(top) >= 0x7C00;
-        if (none) {
-            top = aotx_u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        none = __builtin_reduce_max(top) >= 0x7C00;
+        if (none)
 #pragma unroll
             for (unsigned int r = 0; r < 64u / VR; ++r)
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const unsigned short v = vv[r][x] & 0x7FFF;
-                    if (v < 0x7C00 && v > top[x]) top[x] = v;
-                }
+                for (int x = 0; x < 8; ++x)
+                    if ((vv[r][x] & 0x7FFF) >= 0x7C00) vv[r][x] = 0;
+    }
+    const unsigned long long told = __ballot(none);
+    if (lane == 0u) lds.badv[w] = told != 0ull ? 1u : 0u;
+    __syncthreads();
+    /* the largest beta |v| of V's columns, then its exponent */
+    if constexpr (STAYS) {
+        float top = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if ((made.v[r] & 0x7FFFu) < 0x7C00u) top = fmaxf(top, fabsf(aotx_h2f(made.v[r])) * lds.beta[16u * w + 4u * g + r]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        made.top = (int)(__float_as_uint(top) >> 23);
+    } else {
+        float most[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (unsigned int r = 0; r < 64u / VR; ++r) {
+            const float beta = lds.beta[r * VR + threadIdx.x / (D / 8)];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) most[x] = fmaxf(most[x], fabsf(fmaf(aotx_h2f(vv[r][x]), beta, 0.0f)));
         }
-        const unsigned long long told = __ballot(none);
-        if (lane == 0u) lds.badv[w] = told != 0ull ? 1u : 0u;
+        aotx_u16x8 top;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) top[x] = (unsigned short)(__float_as_uint(most[x]) >> 23);
         typedef unsigned int u4 __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (unsigned int off = D / 8; off < 64u; off <<= 1) {
@@ -635,7 +641,6 @@ static __device__ __forceinline__ void aotx_delta_make(const aotx_delta_args &p,
         }
         if (lane < D / 8) *(aotx_u16x8 *)((unsigned short *)lds.vm[w] + lane * 8u) = top;
     }
-    __syncthreads();
     if (w == 0u) aotx_delta_pairs<D, 0>(lds, to, made, inv, qinv);
     else if (w == 1u) aotx_delta_pairs<D, 1>(lds, to, made, inv, qinv);
     else if (w == 2u) aotx_delta_pairs<D, 2>(lds, to, made, inv, qinv);
@@ -764,20 +769,20 @@ template <int D, int NS>
 struct aotx_delta_tile {
     aotx_h8 k[D / 32], q[D / 32], th[NS], tl[NS], p[NS];
     unsigned short v[4];
-    aotx_f4 of_k, of_u, of_q;
+    aotx_f4 of_k, of_u, of_q, of_b;
     float fade;
-    unsigned int odd;
     unsigned int touched;
 };
 
 /* NS: steps of 32 columns that the wave's rows of T and P have, 1 for waves 0 and 1, else 2.
  * AHEAD: how many chunks ahead the loads run, one or two; with 3, two, and their lines are asked
- * for before; with 0, there is one chunk, and it and the state are in registers (one, the top of V's
- * column, one_state). */
+ * for before; with 0, there is one chunk, and it and the state are in registers (one, the column's
+ * vmax, odd, one_state). */
 template <int D, int NS, int AHEAD>
 static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &p, const aotx_delta_walk k,
                                                          aotx_delta_lds<D> &lds, const aotx_delta_tile<D, NS> *one,
-                                                         int one_top, const aotx_f4 (*one_state)[D / 64])
+                                                         int one_top, unsigned int one_odd,
+                                                         const aotx_f4 (*one_state)[D / 64])
 {
     constexpr int KS = D / 32, TW = D / 64;
     typedef aotx_delta_tile<D, NS> tile_t;
@@ -810,7 +815,8 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
     unsigned long long line_step = rows_step;
     unsigned int line_c = 2u;
     if constexpr (NS == 1 && AHEAD == 3) {
-        constexpr unsigned int SLICES = D / 16, OF_WORK = 152u / SLICES;
+        constexpr unsigned int LINES = sizeof(aotx_delta_factors) / 128u;
+        constexpr unsigned int SLICES = D / 16, OF_WORK = (144u + LINES + SLICES - 1u) / SLICES;
         bool some = lane < 32u;
         if (w == 0u && lane >= 32u) {
             const unsigned int l = (k.col >> 4) * 16u + (lane & 15u);
@@ -820,9 +826,10 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             some = lane < 48u;
         } else if (w == 1u) {
             const unsigned int l = (k.col >> 4) * OF_WORK + lane, part = l / 48u, block = l % 48u / 8u;
-            line = work + (part < 3u ? part * 8192u + (block < 2u ? 2u * block : block + 2u) * 1024u : 24576u) + l % 8u * 128u;
+            line = work + (part < 3u ? part * 8192u + (block < 2u ? 2u * block : block + 2u) * 1024u + l % 8u * 128u
+                                     : (unsigned int)offsetof(work_t, of) + (l - 144u) * 128u);
             line_step = work_step;
-            some = lane < OF_WORK;
+            some = lane < OF_WORK && l < 144u + LINES;
         }
         some = some && k.chunks > 3u;
         if (!some) line_step = 0ull;            /* the lane asks for a chunk's first line again */
@@ -863,8 +870,8 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         x.of_k = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 0u));
         x.of_q = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 256u));
         x.of_u = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 512u));
+        x.of_b = __builtin_bit_cast(aotx_f4, aotx_lane_16(f, at_of, 768u));
         x.fade = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(f, 0, (int)(offsetof(work_t, of) + offsetof(aotx_delta_factors, fade)), 0));
-        x.odd = __builtin_amdgcn_raw_buffer_load_b32(f, 0, (int)(offsetof(work_t, of) + offsetof(aotx_delta_factors, odd)), 0);
         if constexpr (NS == 1 && AHEAD == 3) x.touched = touch();
         advance();
     };
@@ -922,8 +929,8 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             __builtin_amdgcn_raw_buffer_store_b16(aotx_f2h(ldexpf(o[r], -o_shift)), to, (int)(at_out + r * width), 0, 0);
     };
     auto scale = [&](unsigned int c) {
-        /* in the period |S| and |U| of a column stay below sqrt(d) max|S| + 257 max|V|, which the
-         * exponents plus 5 and plus 10 are bounds of. Of zeros alone in V there is none. */
+        /* in the period |S|, |X| and |U| of a column stay below sqrt(d) max|S| + 257 max(beta |v|), which
+         * the exponents plus 5 and plus 10 are bounds of. Of zeros alone in V there is none. */
         float ms = 0.0f;
 #pragma unroll
         for (int t = 0; t < TW; ++t)
@@ -935,7 +942,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         if constexpr (AHEAD > 0)
 #pragma unroll
             for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q) ev = top[q] > ev ? top[q] : ev;
-        ev = ev != 0 ? ev - 1 + 10 - 15 : -127;
+        ev = ev != 0 ? ev - 1 + 10 - 126 : -512;
         ex = ex > ev ? ex : ev;
         if (g == 0u) lds.size[w][k.m] = ex;
         __syncthreads();
@@ -943,7 +950,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
 #pragma unroll
         for (int v = 1; v < 4; ++v) ex = lds.size[v][k.m] > ex ? lds.size[v][k.m] : ex;
         ex = 14 - ex;
-        ex = ex > 100 ? 100 : ex < -120 ? -120 : ex;
+        ex = ex > 126 ? 126 : ex < -120 ? -120 : ex;
 #pragma unroll
         for (int t = 0; t < TW; ++t)
 #pragma unroll
@@ -952,12 +959,13 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         if constexpr (AHEAD > 0) load_top(c + AOTX_DELTA_PERIOD);
     };
     auto pass = [&](tile_t &x, tile_t &other, unsigned int c) {
-        /* rows that are taken out, or past the chunk, have zeros in K, Q and V: their X, U and T
-         * are zeros by themselves. Only a chunk with values that are no numbers asks more. */
-        const unsigned int odd = (unsigned int)__builtin_amdgcn_readfirstlane((int)x.odd);
+        /* rows that are taken out, or past the chunk, have a beta or zeros in K, Q and V of 0: their X, U
+         * and T are zeros by themselves. Only a chunk with values that are no numbers asks more. */
+        const int fade = __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x.fade));
         if constexpr (NS == 1 && AHEAD == 3) asm volatile("" ::"v"(x.touched));
-        unsigned int lim = odd & 0xFFu;
-        if (odd != 64u) {
+        unsigned int lim = 64u;
+        if (fade < 0) {
+            lim = (AHEAD > 0 ? p.work[(unsigned long long)(k.c0 + c) * p.heads + k.h].of.odd : one_odd) & 0xFFu;
             unsigned int first = 64u;
 #pragma unroll
             for (int r = 3; r >= 0; --r)
@@ -997,11 +1005,10 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             a = aotx_mma(x.k[s], sh[s], a);
         }
         if constexpr (AHEAD > 1) load_rest(other);
-        const float up = ldexpf(1.0f, shift);
         aotx_f4 y;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = fmaf(aotx_h2f(x.v[r]), up, -(x.of_k[r] * a[r]));
-        if (odd != 64u) {
+        for (int r = 0; r < 4; ++r) y[r] = fmaf(aotx_h2f(x.v[r]), ldexpf(x.of_b[r], shift), -(x.of_k[r] * a[r]));
+        if (fade < 0) {
             asm volatile("");               /* a branch that is not taken, no selects */
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -1049,7 +1056,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         aotx_split4(a * x.of_u, &hi, &lo);
         *((aotx_h4 *)&lds.v[w >> 1][0][lane] + (w & 1u)) = hi;
         *((aotx_h4 *)&lds.v[w >> 1][1][lane] + (w & 1u)) = lo;
-        aotx_split4(a, &hi, &lo);
+        aotx_split4(a * (1.0f / AOTX_DELTA_UP), &hi, &lo);
         *((aotx_h4 *)&lds.u[w >> 1][0][lane] + (w & 1u)) = hi;
         *((aotx_h4 *)&lds.u[w >> 1][1][lane] + (w & 1u)) = lo;
         __syncthreads();
@@ -1069,7 +1076,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             load_t(x);
         }
 #pragma unroll
-        for (int t = 0; t < TW; ++t) S[t] *= x.fade;
+        for (int t = 0; t < TW; ++t) S[t] *= fabsf(__builtin_bit_cast(float, fade));
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
 #pragma unroll
@@ -1085,7 +1092,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             o = aotx_mma(x.p[s], uh[s], o);
         }
         o_shift = shift;
-        if (odd != 64u) {
+        if (fade < 0) {
             asm volatile("");
             const float nan = __builtin_nanf("");
 #pragma unroll
@@ -1151,8 +1158,8 @@ __global__ __launch_bounds__(256, AHEAD > 1 ? 2 : 3) void aotx_delta_across(aotx
         return;
     }
     /* (scalar: the barriers of both ways count together) */
-    if (k.w < 2u) aotx_delta_follow<D, 1, AHEAD>(p, k, lds, nullptr, 0, nullptr);
-    else aotx_delta_follow<D, 2, AHEAD>(p, k, lds, nullptr, 0, nullptr);
+    if (k.w < 2u) aotx_delta_follow<D, 1, AHEAD>(p, k, lds, nullptr, 0, 0u, nullptr);
+    else aotx_delta_follow<D, 2, AHEAD>(p, k, lds, nullptr, 0, 0u, nullptr);
 }
 
 /* ---------------------------------------------------------------------------------------
@@ -1185,9 +1192,9 @@ static __device__ __forceinline__ void aotx_delta_go_on(const aotx_delta_args &p
     x.of_k = *(const aotx_f4 *)&of.of_k[i0];
     x.of_q = *(const aotx_f4 *)&of.of_q[i0];
     x.of_u = *(const aotx_f4 *)&of.of_u[i0];
+    x.of_b = *(const aotx_f4 *)&of.of_b[i0];
     x.fade = of.fade;
-    x.odd = of.odd;
-    aotx_delta_follow<D, NS, 0>(p, k, lds, &x, made.top, &S);
+    aotx_delta_follow<D, NS, 0>(p, k, lds, &x, made.top, of.odd, &S);
 }
 
 template <int D>

@@ -243,6 +243,48 @@ def test_chunk_small_and_large_values(torch, lib, scale):
     Delta(torch, 5, [200, 70], 1, 2, 128, scale=scale).up().call(lib).check(lib)
 
 
+@pytest.mark.parametrize("b,spread", [(-4, 1), (-6, 1), (-8, 1), (-10, 0), (-14, 0), (-18, 0), (-40, 0), (-80, 0)])
+@pytest.mark.parametrize("lens,heads,d", [([64], 2, 128), ([40, 20], 4, 64), ([200, 70], 2, 128), ([330], 4, 64)])
+def test_chunk_small_rates(torch, lib, b, spread, lens, heads, d):
+    """Heads that write little, from a state of zeros: the state is then far below the values, and as exact
+    in parts of itself. The bound is the sums' own error in parts of a head's largest entry at the end,
+    which is the largest on the way but for a small factor, since what is written is alike in all rows."""
+    c = Delta(torch, 33 + d, lens, 2, heads, d, fresh=range(len(lens)))
+    c.b[:] = b + spread * c.b
+    c.up().call(lib)
+    want, state, faults, _ = c.want()
+    out, S = c.got()
+    for slot in c.agent:
+        size = np.abs(state[slot]).max(axis=(1, 2))
+        far = 4 * np.sqrt(d * max(lens)) * 2.0 ** -24 * size
+        off = np.abs(S[slot] - state[slot]).max(axis=(1, 2))
+        assert (off <= far).all(), (off / size, far / size)
+    for i, slot in enumerate(c.agent):
+        rows = slice(c.offset[i], c.offset[i + 1])
+        far = 4 * np.sqrt(d * max(lens)) * 2.0 ** -24 * np.abs(state[slot]).max(axis=(1, 2))[None, :, None]
+        assert (np.abs(out[rows] - want[rows]) - (c.round[rows] + far)).max() <= 0
+
+
+@pytest.mark.parametrize("lens,heads", [([64], 2), ([200, 70], 2)])
+def test_chunk_rates_and_values_of_many_sizes(torch, lib, lens, heads):
+    """Large values at rates near zero beside small values at rates of 1/2: what a row writes is its rate
+    times its value, and the column's numbers are as exact in parts of that."""
+    c = Delta(torch, 34, lens, 2, heads, 128, fresh=range(len(lens)))
+    small = np.random.default_rng(35).integers(0, 2, c.tokens).astype(bool)
+    c.b[:] = 0
+    c.b[small] = -30
+    c.x[small, 4 * 128:] *= np.float16(1000)
+    c.x[~small, 4 * 128:] *= np.float16(0.01)
+    c.up().call(lib)
+    want, state, _, _ = c.want()
+    out, S = c.got()
+    for i, slot in enumerate(c.agent):
+        far = 4 * np.sqrt(128 * max(lens)) * 2.0 ** -24 * np.abs(state[slot]).max(axis=(1, 2))
+        assert (np.abs(S[slot] - state[slot]).max(axis=(1, 2)) <= far).all()
+        rows = slice(c.offset[i], c.offset[i + 1])
+        assert (np.abs(out[rows] - want[rows]) - (c.round[rows] + far[None, :, None])).max() <= 0
+
+
 @pytest.mark.parametrize("step", [False, True])
 def test_rows_of_subnormal_values(torch, lib, step):
     """q and k whose values are all below fp16's smallest normal number are brought to length all the same."""
