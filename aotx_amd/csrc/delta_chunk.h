@@ -14,7 +14,8 @@
  * fp16 parts (high and rest, 21 bits), so that the state's products are nearly as
  * good as fp32 ones at two or three times the work of plain fp16 instead of sixteen times for
  * fp32 matrix instructions. P, which only the output sees, is rounded to fp16 once, by 2^-11 as
- * the output itself is. The parts have fp16's range, below which their step is 2^-24. M and T are at
+ * the output itself is; it is at most 1 / sqrt(d) and goes times 2^18, so that a weight that has faded
+ * to 2^-32 still has its 11 bits, and none is off by more than 2^-43. The parts have fp16's range, below which their step is 2^-24. M and T are at
  * most 1 (the rule only ever takes away from what a unit key finds) and go times 2^14, where the step
  * is 2^-38; beta is in X, not in T, whose entries would go with its square. Rows of K are brought to
  * lengths of 1/2 to 1 by a power of two 2^e (entries below 2^-14 lose bits, 2^-24 of the length at
@@ -44,7 +45,7 @@ typedef _Float16 aotx_h8 __attribute__((ext_vector_type(8)));
  * wave's accumulators of two row tiles make the other operand. */
 struct aotx_delta_factors {
     float of_k[64];         /* beta exp(G) r_k 2^e; the rows of K are over 2^e */
-    float of_q[64];         /* exp(G) r_q */
+    float of_q[64];         /* exp(G) r_q 2^AOTX_DELTA_OUT_UP */
     float of_u[64];         /* exp(G_last - G) r_k 2^e / AOTX_DELTA_UP */
     float of_b[64];         /* beta */
     unsigned char vmax[128];/* of every column: its largest beta |v| is below 2^(vmax - 126), or 0 */
@@ -86,6 +87,7 @@ static __device__ __forceinline__ aotx_h8 *aotx_delta_rows_of(const aotx_delta_a
 static __device__ __forceinline__ aotx_h8 aotx_h8_of(aotx_u16x8 v) { return __builtin_bit_cast(aotx_h8, v); }
 
 #define AOTX_DELTA_UP 16384.0f      /* of M and T as operands */
+#define AOTX_DELTA_OUT_UP 18        /* P, and with it the sums of outputs, go times 2^18 */
 
 /* x = hi + lo to 22 bits. x has to be one rounded number: where the compiler fuses the product
  * that makes x into one of its two uses, the parts belong to different roundings. */
@@ -568,7 +570,8 @@ static __device__ __forceinline__ void aotx_delta_make(const aotx_delta_args &p,
     const unsigned long long badrows = __ballot(bad) & 0xFFFFull;
     if (lane == 0u) lds.badk[w] = badrows != 0ull ? 16u * w + (unsigned int)__builtin_ctzll(badrows) : 64u;
     const float inv = __builtin_amdgcn_rsqf(kk + p.eps);
-    const float qinv = __builtin_amdgcn_rsqf(qq + p.eps) * (D == 128 ? 0.08838834764831845f : 0.125f);
+    const float qinv = __builtin_amdgcn_rsqf(qq + p.eps) * (D == 128 ? 0.08838834764831845f : 0.125f)
+        * ldexpf(1.0f, AOTX_DELTA_OUT_UP);
     /* 2^ex: the row's length over it is 1/2 to 1 */
     const int ex = __builtin_amdgcn_frexp_expf(__builtin_amdgcn_sqrtf(kk + p.eps));
     if (g == 0u) {
@@ -1091,7 +1094,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             o = aotx_mma(x.p[s], ul[s], o);
             o = aotx_mma(x.p[s], uh[s], o);
         }
-        o_shift = shift;
+        o_shift = shift + AOTX_DELTA_OUT_UP;
         if (fade < 0) {
             asm volatile("");
             const float nan = __builtin_nanf("");

@@ -68,7 +68,7 @@ int aotx_delta_conv(const float *x, unsigned int stride, const float *w, const f
  * state is fp32, and its arithmetic is that or as near: the products of aotx_delta_chunk take
  * their operands as two fp16 parts, 2^-21 each, or 2^-33 of the largest state entry and 2^-28 of the
  * largest beta |v| that their column has in 256 rows, where that is more; the weights with which an
- * output takes the rows of its own 64 are rounded to fp16 once, as the output is. A value of Inf or NaN reaches the rows
+ * output takes the rows of its own 64 are rounded once, by 2^-11 of themselves or 2^-43. A value of Inf or NaN reaches the rows
  * from its own on and no earlier ones.
  *
  * aotx_delta_step: one token of each of `tokens` slots (row i is sequence i). */

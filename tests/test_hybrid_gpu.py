@@ -285,6 +285,30 @@ def test_chunk_rates_and_values_of_many_sizes(torch, lib, lens, heads):
         assert (np.abs(out[rows] - want[rows]) - (c.round[rows] + far[None, :, None])).max() <= 0
 
 
+@pytest.mark.parametrize("lens,heads,d", [([64], 2, 128), ([40, 20], 4, 64), ([200, 70], 2, 128)])
+@pytest.mark.parametrize("fade", [-7.0, -14.0, -20.0])
+def test_chunk_heads_that_forget_fast(torch, lib, lens, heads, d, fade):
+    """Every row fades what came before by exp(fade), and every other row's values are 10^5 times the
+    others': the weights of the rows before are far below 1, and as exact in parts of themselves.
+    Beside its roundings (of 2^-11 of the terms' sizes) an output has the parts' errors: X, U, T and S
+    2^-21 each, in parts of the same sizes, and of X and U 2^-28 of the largest rate times value, by way
+    of weights whose sum is at most 2 / sqrt(d)."""
+    c = Delta(torch, 37, lens, 2, heads, d)
+    c.decay[:], c.dt[:], c.a[:] = fade, 0, np.log(np.e - 1)
+    v = c.x[:, 4 * d:4 * d + heads * d]
+    v[::2] *= np.float16(1000)
+    v[1::2] *= np.float16(0.01)
+    rate = 1 / (1 + np.exp(-c.b[:, :heads, None].astype(np.float64)))
+    most = np.abs(rate * v.reshape(c.tokens, heads, d)).max()
+    c.state[:] = 0
+    c.up().call(lib)
+    want, state, _, _ = c.want()
+    out, S = c.got()
+    far = 4 / np.sqrt(d) * 2.0 ** -28 * most
+    off = np.abs(out - want) - (c.round * (1 + 2.0 ** -8) + far)
+    assert off.max() <= 0, (off.max(), far)
+
+
 @pytest.mark.parametrize("step", [False, True])
 def test_rows_of_subnormal_values(torch, lib, step):
     """q and k whose values are all below fp16's smallest normal number are brought to length all the same."""
