@@ -233,6 +233,52 @@ def test_chunk_one_sequence_shrinks_in_a_graph(torch, lib, heads, tokens):
         c.check(lib)
 
 
+def _check_heads(c, lib, picks):
+    """Delta.check of some heads alone, which share nothing but keys, for calls whose 64-bit walk of all
+    would take too long."""
+    d, kh, n = c.d, c.key_heads, len(picks)
+    keys = [h // (c.heads // kh) for h in picks]
+    cut = [c.x[:, j * d:(j + 1) * d] for j in keys + [kh + j for j in keys] + [2 * kh + h for h in picks]]
+    some = Delta(c.torch, 0, c.lens, n, n, d, slots=1, agent=c.agent)
+    some.x, some.a, some.b = np.concatenate(cut, 1), c.a[:, picks], c.b[:, picks]
+    some.decay, some.dt, some.state, some.pos, some.offset, some.tokens = (c.decay[picks], c.dt[picks], c.state[:, picks], c.pos,
+                                                                           c.offset, c.tokens)
+    out, S = c.got()
+    some.got = lambda: (out[:, picks], S[:, picks])
+    some.check(lib)
+
+
+@pytest.mark.parametrize("key_heads,heads,d,lens", [(2, 32, 128, [6540]), (2, 32, 128, [6500]), (4, 128, 64, [1700]),
+                                                    (1, 32, 128, [4000, 2700])])
+def test_chunk_workspace_past_the_caches(torch, lib, key_heads, heads, d, lens):
+    """Calls whose lines are asked for two chunks before they are loaded, the last chunk whole or a part."""
+    tokens, n = sum(lens), len(lens)
+    assert lib.aotx_delta_work(tokens, n, heads, d) > 100 << 20
+    c = Delta(torch, 38, lens, key_heads, heads, d, slots=n, fresh=(0,)).up().call(lib)
+    _check_heads(c, lib, [1, heads - 1])
+    for at in (64 * 3, tokens - 1):                         # and a row that is no number, early and last
+        c = Delta(torch, 38, lens, key_heads, heads, d, slots=n, fresh=(0,))
+        c.x[at, (2 * key_heads + 1) * d + 5] = np.inf
+        base, S0 = Delta(torch, 38, lens, key_heads, heads, d, slots=n, fresh=(0,)).up().call(lib).got()
+        out, S = c.up().call(lib).got()
+        end = int(c.offset[np.searchsorted(c.offset, at, side="right")])
+        assert not np.isfinite(out[at:end, 1, 5]).any() and np.isfinite(out[:at, 1, 5]).all()
+        out[:end, 1, 5] = base[:end, 1, 5] = 0
+        S[:, 1, :, 5] = S0[:, 1, :, 5] = 0
+        assert np.array_equal(out, base) and np.array_equal(S, S0)
+
+
+@pytest.mark.parametrize("key_heads,heads,d", [(2, 32, 64), (4, 32, 128)])
+def test_chunk_few_rows_beside_a_large_call(torch, lib, key_heads, heads, d):
+    """Sequences of few rows in a launch of their own: beside more than 1536 chunks and heads, and beside
+    so many sequences that 12 rows are few, at lengths on both sides."""
+    for lens in ([2900, 3, 1, 0, 4, 5, 300, 2], [700] * 3 + [12, 1, 13, 0, 5] * 6):
+        n = len(lens)
+        c = Delta(torch, n, lens, key_heads, heads, d, lead=1, tail=3, slots=40, fresh=(1, 4),
+                  agent=list(range(n - 1)) + [3]).up().call(lib)
+        _check_heads(c, lib, [0, 17, heads - 1])
+
+
 def test_chunk_long(torch, lib):
     Delta(torch, 21, [6000], 1, 2, 64, slots=1, fresh=(0,)).up().call(lib).check(lib)
 
@@ -530,6 +576,80 @@ def test_conv_lengths(torch, lib, width, channels):
 @pytest.mark.parametrize("lens", [[1] * 64, [14, 1, 1, 1, 30], [15, 40], [13, 2, 2, 2, 2, 2, 2, 2]])
 def test_conv_sequences_around_a_run(torch, lib, lens):
     _conv(torch, lib, 5, lens, 128, 4, slots=64, fresh=(1,))
+
+
+@pytest.mark.parametrize("width", [2, 3, 4])
+@pytest.mark.parametrize("tokens,run", [(600, 2), (900, 3), (1300, 5), (2100, 8), (4099, 16)])
+def test_conv_runs_of_rows(torch, lib, tokens, run, width):
+    """A thread's run of 2 to 16 rows, sequences that begin, end and lie within one, and the last run short."""
+    channels = 4096                                         # 4 workgroups a row: runs of tokens / 256 rows
+    assert min(16, tokens * 4 // 1024) == run
+    rng = np.random.default_rng(tokens + width)
+    lens = [0, 1, run - 1, run, run + 1, 2, 3, 0, 1, 1, 4, 17, 2 * run, 1] + [int(n) for n in rng.integers(0, 2 * run, 30)]
+    while sum(lens) > tokens - 40:
+        lens.pop()
+    lens.append(tokens - 9 - sum(lens))
+    _conv(torch, lib, tokens, lens, channels, width, bias=width == 2, lead=4, tail=5, slots=60, fresh=range(0, 60, 3))
+
+
+@pytest.mark.parametrize("lens,channels,width,pad", [([500, 1, 0, 3, 200, 16], 8192, 4, 0), ([700], 8200, 3, 4),
+                                                     ([5400, 2, 60, 1, 17], 8192, 4, 0), ([3, 11000], 4104, 2, 4)])
+def test_conv_past_the_caches(torch, lib, lens, channels, width, pad):
+    """Calls whose rows go past the caches: out alone, and x too."""
+    assert sum(lens) * channels * 6 > (256 << 20 if sum(lens) > 5000 else 32 << 20)
+    _conv(torch, lib, 6, lens, channels, width, bias=True, lead=1, tail=2, pad=pad, slots=8, fresh=(0,))
+
+
+def test_conv_refused_sequences_in_runs(torch, lib):
+    """Slots that are missing or named twice where a run holds several sequences."""
+    lens = [400, 3, 2, 1, 0, 250, 7, 1300, 5, 2]
+    assert _conv(torch, lib, 9, lens, 4096, 4, lead=3, tail=30, agent=[2, 9, 2, 5, 5, 5, 1, 0, 0, 3], slots=8) == 4
+
+
+@pytest.mark.parametrize("width", [2, 4])
+def test_conv_in_a_graph(torch, lib, width):
+    """A captured call of many rows, replayed with other rows, lengths and positions."""
+    rng = np.random.default_rng(95)
+    tokens, channels, slots = 2100, 4096, 4
+    x = torch.zeros(tokens, channels, device="cuda")
+    w = _up(torch, rng.normal(0, 0.5, (channels, width)), np.float32)
+    offset, pos = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    agent = _up(torch, [2, 0, 3], np.int32)
+    state = torch.zeros(slots, width - 1, channels, device="cuda")
+    out = torch.zeros(tokens, channels, dtype=torch.float16, device="cuda")
+
+    def call(s):
+        assert lib.aotx_delta_conv(p(x), channels, p(w), None, p(offset), p(pos), p(agent), 3, tokens, channels, width,
+                                   p(state), slots, p(out), s) == 0
+
+    call(None)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        call(ctypes.c_void_p(side.cuda_stream))
+    for at, begin in (([0, 5, 6, 2100], [0, 3, 9]), ([0, 1, 1, 3], [4, 0, 0]), ([20, 700, 1500, 1502], [1, 1, 0])):
+        rows = rng.normal(0, 1, (tokens, channels)).astype(np.float32)
+        kept = rng.normal(0, 1, (slots, width - 1, channels)).astype(np.float32)
+        for t, v in ((x, rows), (state, kept)):
+            t.copy_(torch.from_numpy(v))
+        offset.copy_(torch.tensor(at, dtype=torch.int32))
+        pos.copy_(torch.tensor(begin, dtype=torch.int32))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        got, S = out.clone(), state.clone()
+        state.copy_(torch.from_numpy(kept))
+        out.fill_(7.0)
+        call(None)
+        torch.cuda.synchronize()
+        assert torch.equal(out, got) and torch.equal(state, S)
+        want, S64 = np.full((tokens, channels), 7.0), kept.astype(np.float64)
+        H.conv(rows, w.cpu().numpy().astype(np.float64), None, np.array(at), begin, [2, 0, 3], S64, want)
+        far = 2.0 ** -11 * np.abs(want) + 2.0 ** -25 + 16 * 2.0 ** -24 * 8
+        assert (np.abs(got.cpu().numpy().astype(np.float64) - want) - far).max() <= 0
+        assert np.array_equal(S.cpu().numpy().astype(np.float64), S64)
 
 
 @pytest.mark.parametrize("tokens", [1, 64])
