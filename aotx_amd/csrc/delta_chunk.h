@@ -84,22 +84,11 @@ static __device__ __forceinline__ aotx_h8 *aotx_delta_rows_of(const aotx_delta_a
     return p.rows + ((unsigned long long)c * p.key_heads + kh) * (16u * d);
 }
 
-static __device__ __forceinline__ aotx_h8 aotx_h8_of(aotx_u16x8 v) { return __builtin_bit_cast(aotx_h8, v); }
-
 #define AOTX_DELTA_UP 16384.0f      /* of M and T as operands */
 #define AOTX_DELTA_OUT_UP 18        /* P, and with it the sums of outputs, go times 2^18 */
 
-/* x = hi + lo to 22 bits. x has to be one rounded number: where the compiler fuses the product
- * that makes x into one of its two uses, the parts belong to different roundings. */
-static __device__ __forceinline__ void aotx_split(float x, _Float16 *hi, _Float16 *lo)
-{
-    asm("" : "+v"(x));
-    *hi = (_Float16)x;
-    *lo = (_Float16)(x - (float)*hi);
-}
-
-/* Four of them, rounded toward zero: the rest makes up for the high part's rounding, and ends
- * 2^-21 below x at most. */
+/* x = hi + lo, four of them, rounded toward zero: the rest makes up for the high part's rounding, and
+ * ends 2^-21 below x at most. */
 typedef _Float16 aotx_h2 __attribute__((ext_vector_type(2)));
 static __device__ __forceinline__ void aotx_split4(aotx_f4 x, aotx_h4 *hi, aotx_h4 *lo)
 {
