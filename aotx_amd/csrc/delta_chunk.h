@@ -4,7 +4,7 @@
  * rows' inverse lengths (r_q with 1 / sqrt(d)), G the running sum of g, the rule unrolls to
  *   M_ij = beta_i r_k,i r_k,j (K_i . K_j) exp(G_i - G_j) for i > j,   T = (1 + M)^-1
  *   X = diag(beta) (V - diag(exp(G) r_k) K S),   U = T X
- *   out = diag(exp(G) r_q) Q S + P U,   P_ij = r_q,i r_k,j (Q_i . K_j) exp(G_i - G_j) for i >= j
+ *   out = diag(exp(G) r_q) Q S + P X,   P = N T,   N_ij = r_q,i r_k,j (Q_i . K_j) exp(G_i - G_j) for i >= j
  *   S <- exp(G_last) S + K^T diag(r_k exp(G_last - G)) U
  * T and P need no state: aotx_delta_within makes them for every chunk at once. What is left,
  * aotx_delta_across, walks a sequence's chunks with a slice of columns of S in registers.
@@ -15,7 +15,10 @@
  * good as fp32 ones at two or three times the work of plain fp16 instead of sixteen times for
  * fp32 matrix instructions. P, which only the output sees, is rounded to fp16 once, by 2^-11 as
  * the output itself is; it is at most 1 / sqrt(d) and goes times 2^18, so that a weight that has faded
- * to 2^-32 still has its 11 bits, and none is off by more than 2^-43. The parts have fp16's range, below which their step is 2^-24. M and T are at
+ * to 2^-32 still has its 11 bits, and none is off by more than 2^-43. (In two parts 8192 rows took 278
+ * us and not 229. P X and not N U, because where keys are alike U are differences far above their sum,
+ * in parts of which the weights' rounding counts: rates near 1 and keys at 0.95 of one another gave
+ * outputs off by 1.2e-3.) The parts have fp16's range, below which their step is 2^-24. M and T are at
  * most 1 (the rule only ever takes away from what a unit key finds) and go times 2^14, where the step
  * is 2^-38; beta is in X, not in T, whose entries would go with its square. Rows of K are brought to
  * lengths of 1/2 to 1 by a power of two 2^e (entries below 2^-14 lose bits, 2^-24 of the length at
@@ -324,22 +327,21 @@ struct aotx_delta_within_lds {
 template <int D>
 struct aotx_delta_made {
     aotx_h8 k[D / 32], q[D / 32], p[2], th[2], tl[2];
+    aotx_f4 qk[4];              /* N, the wave's rows by tiles of columns */
     unsigned short v[4];
     int top;                    /* of the wave's rows of the column, as vmax */
 };
 
-/* P and M of row 16 W + m. Between blocks, exp(G_i - G_j) is the product of two factors by way of
+/* N and M of row 16 W + m. Between blocks, exp(G_i - G_j) is the product of two factors by way of
  * the last row of j's block: both are at most 1, and one exponential a row serves four columns. */
 template <int D, int W>
-static __device__ __forceinline__ void aotx_delta_pairs(aotx_delta_within_lds<D> &lds, aotx_delta_chunk_work *to,
-                                                        aotx_delta_made<D> &made, float inv, float qinv)
+static __device__ __forceinline__ void aotx_delta_pairs(aotx_delta_within_lds<D> &lds, aotx_delta_made<D> &made, float inv,
+                                                        float qinv)
 {
     constexpr int KS = D / 32;
     const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4, row = 16u * W + m;
     const float gi = lds.ghi[row], gil = lds.glo[row], bi = lds.beta[row] * inv;
-    aotx_f4 pt[4], block;
-#pragma unroll
-    for (int jt = 0; jt < 4; ++jt) pt[jt] = aotx_f4{0, 0, 0, 0};
+    aotx_f4 block;
 #pragma unroll
     for (int jt = 0; jt <= W; ++jt) {
         aotx_f4 kks = {0, 0, 0, 0}, qks = {0, 0, 0, 0};
@@ -363,7 +365,7 @@ static __device__ __forceinline__ void aotx_delta_pairs(aotx_delta_within_lds<D>
                 qks[r] = row >= j0 + r ? qks[r] : 0.0f;
             }
             block = kks * fade * bi;
-            pt[jt] = qks * fade * qinv;
+            made.qk[jt] = qks * fade * qinv;
         } else {
             const float from = expf((gi - lds.ghi[16 * jt + 15]) + (gil - lds.glo[16 * jt + 15]));
             const aotx_f4 fade = *(const aotx_f4 *)&lds.near_end[j0] * rkj * from;
@@ -371,19 +373,8 @@ static __device__ __forceinline__ void aotx_delta_pairs(aotx_delta_within_lds<D>
             aotx_split4(kks * fade * (bi * AOTX_DELTA_UP), &hi, &lo);
             *(aotx_h4 *)&lds.below[0][row - 16u][j0] = hi;
             *(aotx_h4 *)&lds.below[1][row - 16u][j0] = lo;
-            pt[jt] = qks * fade * qinv;
+            made.qk[jt] = qks * fade * qinv;
         }
-    }
-#pragma unroll
-    for (int s = 0; s <= W / 2; ++s) {
-        aotx_h8 o;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            o[r] = (_Float16)pt[2 * s][r];
-            o[4 + r] = (_Float16)pt[2 * s + 1][r];
-        }
-        if (to != nullptr) *(aotx_h8 *)((char *)to->p[W][s] + lane * 16u) = o;
-        else made.p[s] = o;
     }
     /* inverse of 1 + the diagonal block by substitution, a column a lane; every value found is
      * taken from all rows below at once, which do not wait for one another */
@@ -455,6 +446,41 @@ static __device__ __forceinline__ void aotx_delta_column(aotx_delta_within_lds<D
     if (W & 1)
 #pragma unroll
         for (int r = 0; r < 4; ++r) lds.tp[0][16u * (W & 2) + 4u * g + r][at] = lds.tp[1][16u * (W & 2) + 4u * g + r][at] = 0;
+}
+
+/* Rows 16 W + m of P = N T, from two parts of both: taken transposed, T's columns by transposing reads
+ * (as K's in the walk), so that a row stays in its lane. */
+template <int D, int W>
+static __device__ __forceinline__ void aotx_delta_weights(aotx_delta_within_lds<D> &lds, aotx_delta_made<D> &made)
+{
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    const unsigned int lane = threadIdx.x & 63u, m = lane & 15u, g = lane >> 4;
+    aotx_h4 hi[4], lo[4];
+#pragma unroll
+    for (int q = 0; q <= W; ++q) aotx_split4(made.qk[q], &hi[q], &lo[q]);
+    aotx_f4 pt[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        pt[c] = aotx_f4{0, 0, 0, 0};
+#pragma unroll
+        for (int q = c; q <= W; ++q) {
+            aotx_h4 t[2];
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                unsigned short *at = &lds.tp[part][16u * q + 4u * g + (m >> 2)][32 * (c >> 1) + 4 * (c & 1) + 8u * (m & 3u)];
+                t[part] = __builtin_bit_cast(aotx_h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)at));
+            }
+            pt[c] = aotx_mma_parts(t[0], t[1], hi[q], lo[q], pt[c]);
+        }
+        pt[c] *= 1.0f / AOTX_DELTA_UP;
+    }
+#pragma unroll
+    for (int s = 0; s <= W / 2; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            made.p[s][r] = (_Float16)pt[2 * s][r];
+            made.p[s][4 + r] = (_Float16)pt[2 * s + 1][r];
+        }
 }
 
 /* The fifth wave: gates, a row a lane, and what follows from them. Sums of g are in 64 bits,
@@ -633,10 +659,10 @@ static __device__ __forceinline__ void aotx_delta_make(const aotx_delta_args &p,
         }
         if (lane < D / 8) *(aotx_u16x8 *)((unsigned short *)lds.vm[w] + lane * 8u) = top;
     }
-    if (w == 0u) aotx_delta_pairs<D, 0>(lds, to, made, inv, qinv);
-    else if (w == 1u) aotx_delta_pairs<D, 1>(lds, to, made, inv, qinv);
-    else if (w == 2u) aotx_delta_pairs<D, 2>(lds, to, made, inv, qinv);
-    else aotx_delta_pairs<D, 3>(lds, to, made, inv, qinv);
+    if (w == 0u) aotx_delta_pairs<D, 0>(lds, made, inv, qinv);
+    else if (w == 1u) aotx_delta_pairs<D, 1>(lds, made, inv, qinv);
+    else if (w == 2u) aotx_delta_pairs<D, 2>(lds, made, inv, qinv);
+    else aotx_delta_pairs<D, 3>(lds, made, inv, qinv);
     __syncthreads();
 
     if (w == 0u) aotx_delta_column<D, 0>(lds);
@@ -644,6 +670,10 @@ static __device__ __forceinline__ void aotx_delta_make(const aotx_delta_args &p,
     else if (w == 2u) aotx_delta_column<D, 2>(lds);
     else aotx_delta_column<D, 3>(lds);
     __syncthreads();
+    if (w == 0u) aotx_delta_weights<D, 0>(lds, made);
+    else if (w == 1u) aotx_delta_weights<D, 1>(lds, made);
+    else if (w == 2u) aotx_delta_weights<D, 2>(lds, made);
+    else aotx_delta_weights<D, 3>(lds, made);
 #pragma unroll
     for (unsigned int s = 0; s < 2u; ++s) {
         if (s > w / 2u) continue;
@@ -655,6 +685,7 @@ static __device__ __forceinline__ void aotx_delta_make(const aotx_delta_args &p,
         } else {
             to->t_hi[w][s][lane] = hi;
             to->t_lo[w][s][lane] = lo;
+            to->p[w][s][lane] = made.p[s];
         }
     }
     if constexpr (STAYS)
@@ -662,9 +693,11 @@ static __device__ __forceinline__ void aotx_delta_make(const aotx_delta_args &p,
         for (int s = 0; s < KS; ++s) kf[s] = kf[s] * a * z;
 }
 
-/* FEW: the workgroups past those of the chunks take the sequences of few rows. */
+/* FEW: the workgroups past those of the chunks take the sequences of few rows. Five waves a SIMD are the
+ * four workgroups that LDS has room for: with 99 registers, for four waves, 2048 rows of 32 heads of 128
+ * took 66.7 us, with 96 61.1. */
 template <int D, bool FEW>
-__global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
+__global__ __launch_bounds__(320, FEW ? 1 : 5) void aotx_delta_within(aotx_delta_args p)
 {
     __shared__ union {
         aotx_delta_within_lds<D> chunk;
@@ -704,8 +737,8 @@ __global__ __launch_bounds__(320) void aotx_delta_within(aotx_delta_args p)
  * the chunk. S, X and U pass between the waves through LDS as operands, a
  * barrier each; everything else a chunk needs is loaded into registers a chunk or two ahead. All
  * that the state's chain does not need is where the chain waits: loads beside products that are
- * under way, K's way through LDS and Q S while S and X are on theirs, P U behind the state's update,
- * its rounding and stores while the next chunk's X is read. (At other places in the chain the same
+ * under way, K's way through LDS and Q S while S and X are on theirs, P X behind the products of U, its
+ * rounding and stores while the next chunk's X is read. (At other places in the chain the same
  * loads, stores and LDS writes made 8192 rows 3 to 40 us longer.)
  * Row x of tile t of S is key 32 (t / 2) + 8 (x / 4) + 4 (t % 2) + x % 4, so that two tiles'
  * accumulators hold keys 8 g .. 8 g + 7 of a step, as 16 bytes of a row of K do.
@@ -723,7 +756,7 @@ template <int D>
 struct aotx_delta_lds {
     aotx_h8 s[D / 32][2][64];               /* S by steps of keys, two parts */
     aotx_h8 x[2][2][64];                    /* X by steps of rows */
-    aotx_h8 u[2][2][64], v[2][2][64];       /* U, and U with the state update's factors */
+    aotx_h8 v[2][2][64];                    /* U with the state update's factors */
     __align__(16) unsigned short k[64][D + 8];  /* the chunk's rows of K, to be read by columns */
     int size[4][16];                        /* exponents of the state's columns, by wave */
     unsigned int bad[4][16];                /* first bad rows of V's columns, by wave */
@@ -1045,23 +1078,22 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             a = aotx_mma(x.tl[s], xh[s], a);
             a = aotx_mma(x.th[s], xh[s], a);
         }
+        o = x.of_q * qs;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            o = aotx_mma(x.p[s], xl[s], o);
+            o = aotx_mma(x.p[s], xh[s], o);
+        }
+        o_shift = shift + AOTX_DELTA_OUT_UP;
         aotx_split4(a * x.of_u, &hi, &lo);
         *((aotx_h4 *)&lds.v[w >> 1][0][lane] + (w & 1u)) = hi;
         *((aotx_h4 *)&lds.v[w >> 1][1][lane] + (w & 1u)) = lo;
-        aotx_split4(a * (1.0f / AOTX_DELTA_UP), &hi, &lo);
-        *((aotx_h4 *)&lds.u[w >> 1][0][lane] + (w & 1u)) = hi;
-        *((aotx_h4 *)&lds.u[w >> 1][1][lane] + (w & 1u)) = lo;
         __syncthreads();
-        aotx_h8 vh[2], vl[2], uh[NS], ul[NS];
+        aotx_h8 vh[2], vl[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             vh[s] = lds.v[s][0][lane];
             vl[s] = lds.v[s][1][lane];
-        }
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            uh[s] = lds.u[s][0][lane];
-            ul[s] = lds.u[s][1][lane];
         }
         if constexpr (AHEAD > 0) {
             load_q(x);
@@ -1077,13 +1109,6 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
                 S[t] = aotx_mma(kt[t][s], vh[s], S[t]);
             }
         }
-        o = x.of_q * qs;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            o = aotx_mma(x.p[s], ul[s], o);
-            o = aotx_mma(x.p[s], uh[s], o);
-        }
-        o_shift = shift + AOTX_DELTA_OUT_UP;
         if (fade < 0) {
             asm volatile("");
             const float nan = __builtin_nanf("");

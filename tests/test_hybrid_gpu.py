@@ -355,6 +355,42 @@ def test_chunk_heads_that_forget_fast(torch, lib, lens, heads, d, fade):
     assert off.max() <= 0, (off.max(), far)
 
 
+@pytest.mark.parametrize("lens,heads,d", [([64], 2, 128), ([40, 20], 4, 64), ([200, 70], 2, 128)])
+def test_chunk_keys_alike(torch, lib, lens, heads, d):
+    """Keys that lean the same way, at rates near 1: each row takes most of the last one's value back. An
+    output is the state's before its chunk and weights times the rows' beta (v - S^T k) of that state; the
+    weights are rounded by 2^-11, and so is the output. What else there is are parts of 2^-21 of the factors
+    of its products, some in a row, and the state's own roundings: 2^-18 of all terms' sizes."""
+    rng = np.random.default_rng(39)
+    c = Delta(torch, 39 + d, lens, 2, heads, d)
+    lean = rng.normal(0, 1, 4 * d)
+    c.x[:, :4 * d] = (3 * lean + rng.normal(0, 1, (c.tokens, 4 * d))).astype(np.float16)
+    c.b[:] = 5 + 0.5 * c.b
+    c.decay[:] = -0.05
+    c.up().call(lib)
+    want, state, _, top = c.want()
+    out, S = c.got()
+    assert np.abs(S - state).max() <= 4 * np.sqrt(d * max(lens)) * 2.0 ** -24 * top
+    q, k, v = H.rows(c.x[:, :c.width], 2, heads, d, c.eps)
+    g, beta = H.gates(c.a[:, :heads], c.b[:, :heads], c.decay.astype(np.float64), c.dt.astype(np.float64))
+    size, far = np.zeros(out.shape), np.zeros(out.shape)
+    for i in range(len(lens)):
+        for h in range(heads):
+            s = c.state[c.agent[i], h].astype(np.float64)
+            for lo in range(c.offset[i], c.offset[i + 1], 64):
+                at = slice(lo, min(lo + 64, c.offset[i + 1]))
+                K, Q, B, G = k[at, h], q[at, h], beta[at, h], np.cumsum(g[at, h])
+                fade = np.tril(np.exp(np.minimum(G[:, None] - G[None], 0)))
+                T = np.linalg.inv(np.eye(len(G)) + np.tril(B[:, None] * (K @ K.T) * fade, -1))
+                X = B[:, None] * (v[at, h] - np.exp(G)[:, None] * (K @ s))
+                N, all_x = (Q @ K.T) * fade, B[:, None] * (np.abs(v[at, h]) + np.exp(G)[:, None] * (np.abs(K) @ np.abs(s)))
+                size[at, h] = np.abs(N @ T) @ np.abs(X)
+                far[at, h] = np.abs(N) @ np.abs(T) @ all_x + np.exp(G)[:, None] * (np.abs(Q) @ np.abs(s))
+                s = np.exp(G[-1]) * s + (K * np.exp(G[-1] - G)[:, None]).T @ (T @ X)
+    off = np.abs(out - want) - (2.0 ** -11 * (np.abs(out) + size) + 2.0 ** -25 + 2.0 ** -18 * far)
+    assert off.max() <= 0, (off.max(), np.sqrt(((out - want) ** 2).mean() / (want ** 2).mean()))
+
+
 @pytest.mark.parametrize("step", [False, True])
 def test_rows_of_subnormal_values(torch, lib, step):
     """q and k whose values are all below fp16's smallest normal number are brought to length all the same."""
