@@ -115,8 +115,8 @@ static void aotx_delta_chunked(const aotx_delta_args &p, hipStream_t s)
 {
     /* The sequences of few rows, if any go row by row, are workgroups of this launch in small calls,
      * where one launch less counts, and a launch of their own where the registers that they add
-     * would cost the chunks more (32 heads of 128: 2 sequences of 512 rows 33.5 us in one and 35.7
-     * in two, 8 of 512 rows 124 and 118). */
+     * would cost the chunks more (32 heads of 128: 2 sequences of 512 rows 34.0 us in one and 36.0
+     * in two, 4 of 512 rows 65.4 and 61.6, 8 of 512 rows 117 and 113). */
     const unsigned int few = p.few != 0u ? p.seqs.seqs * p.heads * (D / 64) : 0u, blocks = p.chunks * p.heads;
     if (few != 0u && blocks <= 1536u) {
         hipLaunchKernelGGL((aotx_delta_within<D, true>), dim3(blocks + few), dim3(320), 0, s, p);
@@ -127,11 +127,11 @@ static void aotx_delta_chunked(const aotx_delta_args &p, hipStream_t s)
     AOTX_LAUNCH_CHECK();
     const unsigned int units = (p.seqs.seqs * p.heads + 7u) / 8u * 8u;
     /* Two chunks' loads in flight where few workgroups share a CU or sequences are long; else one,
-     * in so few registers that three workgroups do (32 heads of 128: 4 sequences of 2048 rows 211
-     * us with two and 229 with one, 64 of 16 rows 240 and 185, 8 of 512 rows 113 and 111). Lines
+     * in so few registers that three workgroups do (32 heads of 128: 4 sequences of 2048 rows 214
+     * us with two and 233 with one, 64 of 16 rows 244 and 195, 16 of 512 rows 235 and 234). Lines
      * are asked for early where the caches of the XCDs do not hold the workspace any more (8192
-     * rows 226 us with and 230 without, 4 sequences of 2048 rows 206 and 211, 4096 rows 118 and
-     * 116). */
+     * rows 226 us with and 231 without, 4 sequences of 2048 rows 208 and 214, 4096 rows 117 and
+     * 114). */
     const dim3 grid(units * (D / 16));
     if (grid.x > 512u && p.seqs.tokens < 1024u * p.seqs.seqs)
         hipLaunchKernelGGL((aotx_delta_across<D, 1>), grid, dim3(256), 0, s, p);
@@ -164,14 +164,14 @@ extern "C" int aotx_delta_chunk(const void *qkv, unsigned int stride, const floa
     p.work = (aotx_delta_chunk_work *)work;
     p.rows = (aotx_h8 *)(p.work + (unsigned long long)p.chunks * heads);
     /* Sequences of few rows go row by row: no matrices to make first, and a decode row beside a
-     * prompt costs what a step does. A row takes 1.7 us, a chunk 11 if the chip is idle beside (32
-     * heads of 128: 4 rows 9.8 us and 11.4, 8 rows 16.9 and 11.4); a chip full of sequences is kept
-     * busy longer by chunks (64 sequences of 8 rows 136 us row by row and 183 in chunks, of 12 rows
-     * 174 and 184). */
+     * prompt costs what a step does. A row takes 1.7 us, a chunk 12 if the chip is idle beside (32
+     * heads of 128: 4 rows 9.9 us and 12.0, 8 rows 17.0 and 12.0); a chip full of sequences is kept
+     * busy longer by chunks (64 sequences of 8 rows 136 us row by row and 189 in chunks, of 12 rows
+     * 175 and 190). */
     p.few = seqs * heads >= 1024u ? 12u : 4u;
-    /* Calls of at most a chunk a sequence go in one launch while each workgroup of it has a CU (32
-     * heads of 128: 40 rows 8.2 us, in two launches 12.0; 2 sequences of 32 rows 14.1 and 13.6, 4 of
-     * 16 rows 26.0 and 18.6), where 3 rows take no longer than row by row (7.6 us and 8.1). */
+    /* Calls of up to 64 rows in all go in one launch while each workgroup of it has a CU (32 heads of
+     * 128: 40 rows 8.6 us, in two launches 12.5; 2 sequences of 32 rows 15.5 and 14.4, 4 of 16 rows
+     * 27.7 and 19.8), where 3 rows take no longer than row by row (8.1 us and 8.2). */
     const bool one = tokens <= AOTX_DELTA_CHUNK && seqs * heads * (head_dim / 16u) <= 256u;
     hipStream_t s = aotx_stream(stream);
     if (tokens <= (one && seqs == 1u ? 2u : p.few))

@@ -8,7 +8,7 @@
  *   S <- exp(G_last) S + K^T diag(r_k exp(G_last - G)) U
  * T and P need no state: aotx_delta_within makes them for every chunk at once. What is left,
  * aotx_delta_across, walks a sequence's chunks with a slice of columns of S in registers.
- * aotx_delta_short does both where no sequence has more than one chunk.
+ * aotx_delta_short does both in calls of up to 64 rows, while each of its workgroups has a CU.
  *
  * Numbers. K and Q are fp16 and enter the matrix cores as they are; S, U, X and T enter as two
  * fp16 parts (high and rest, 21 bits), so that the state's products are nearly as
@@ -306,8 +306,8 @@ static __device__ __forceinline__ unsigned short aotx_rows_2(const aotx_rows_vie
  * exponentials and the sum over 64 rows are as long a chain as the loads that the others wait for.
  *
  * Large calls are bound by memory, the workspace above all (20 KB a chunk and head, 32 a key head):
- * 8192 rows, 32 heads of 128, read 136 MB and write 146 in 65 us, 4.3 TB/s; 512 rows, a workgroup a
- * CU, take 8.6 us of latency, 40 rows 7.2.
+ * 8192 rows, 32 heads of 128, read 136 MB and write 148 in 66 us, 4.3 TB/s; 512 rows, a workgroup a
+ * CU, take 8.8 us of latency.
  * ------------------------------------------------------------------------------------- */
 template <int D>
 struct aotx_delta_within_lds {
@@ -744,9 +744,9 @@ __global__ __launch_bounds__(320, FEW ? 1 : 5) void aotx_delta_within(aotx_delta
  * accumulators hold keys 8 g .. 8 g + 7 of a step, as 16 bytes of a row of K do.
  *
  * Bound by the chain of chunks: 32 heads of 128 are 256 workgroups, one a CU, and each waits for
- * itself; 8192 rows take 177 to 187 us, 1.4 us a chunk, the latencies of its three passes through LDS
- * and of the products between them. Of that time LDS works 30 % and the matrix cores 15 %; the
- * vector caches wait for the L2 in 41 % of theirs. Columns in slices of 16 make the workgroups
+ * itself; 8192 rows take 178 to 194 us in a trace, 1.4 us a chunk, the latencies of its three passes
+ * through LDS and of the products between them. Of that time LDS works 27 % and the matrix cores 16 %;
+ * the vector caches wait for the L2 in 40 % of theirs. Columns in slices of 16 make the workgroups
  * that fill the chip: slices of 32 halve the traffic and took 369 to 400 us; eight waves, four of
  * them for the output, took as long as four.
  * ------------------------------------------------------------------------------------- */
@@ -1184,7 +1184,7 @@ __global__ __launch_bounds__(256, AHEAD > 1 ? 2 : 3) void aotx_delta_across(aotx
  * within) makes T and P for its 16 columns by itself. They stay in the registers of the waves that
  * take them, and a second launch and the way through memory are saved; the slices of a head make
  * the same T and P, which costs nothing while the chip has room. 40 rows of 32 heads of 128 take
- * 8.2 us, the latency of a launch, the rows and one chunk's chain; in two launches 12.0.
+ * 8.6 us, the latency of a launch, the rows and one chunk's chain; in two launches 12.5.
  * ------------------------------------------------------------------------------------- */
 template <int D, int NS>
 static __device__ __forceinline__ void aotx_delta_go_on(const aotx_delta_args &p, const aotx_delta_walk &k,

@@ -68,8 +68,9 @@ int aotx_delta_conv(const float *x, unsigned int stride, const float *w, const f
  * state is fp32, and its arithmetic is that or as near: the products of aotx_delta_chunk take
  * their operands as two fp16 parts, 2^-21 each, or 2^-33 of the largest state entry and 2^-28 of the
  * largest beta |v| that their column has in 256 rows, where that is more; the weights with which an
- * output takes the rows of its own 64 are rounded once, by 2^-11 of themselves or 2^-43. A value of Inf or NaN reaches the rows
- * from its own on and no earlier ones.
+ * output takes the rows of its own 64 are rounded once, by 2^-11 of themselves or 2^-43. (Keys are taken
+ * as they are while eps is at most 1/4; above that those much shorter than sqrt(eps) lose bits.) A value
+ * of Inf or NaN reaches the rows from its own on and no earlier ones.
  *
  * aotx_delta_step: one token of each of `tokens` slots (row i is sequence i). */
 int aotx_delta_step(const void *qkv, unsigned int stride, const float *a, const float *b,
@@ -80,7 +81,9 @@ int aotx_delta_step(const void *qkv, unsigned int stride, const float *a, const 
 
 /* aotx_delta_chunk: sequences of any lengths, up to 2^20 rows a call. work is a workspace of
  * work_bytes bytes, at least aotx_delta_work of the same tokens, seqs, heads and head_dim,
- * 256-byte aligned; it holds nothing between calls. */
+ * 256-byte aligned; it holds nothing between calls. Those are 58 KB for every 64 rows and head of 128
+ * (42 KB of 64): a prompt may be cut into calls of some thousand rows, each of which goes on where
+ * the last one left the slot. */
 unsigned long long aotx_delta_work(unsigned int tokens, unsigned int seqs, unsigned int heads,
                                    unsigned int head_dim);
 int aotx_delta_chunk(const void *qkv, unsigned int stride, const float *a, const float *b,
