@@ -128,7 +128,7 @@ static void aotx_delta_chunked(const aotx_delta_args &p, hipStream_t s)
     const unsigned int units = (p.seqs.seqs * p.heads + 7u) / 8u * 8u;
     /* Two chunks' loads in flight where few workgroups share a CU or sequences are long; else one,
      * in so few registers that three workgroups do (32 heads of 128: 4 sequences of 2048 rows 214
-     * us with two and 233 with one, 64 of 16 rows 244 and 195, 16 of 512 rows 235 and 234). Lines
+     * us with two and 233 with one, 64 of 16 rows 244 and 185, 16 of 512 rows 235 and 232). Lines
      * are asked for early where the caches of the XCDs do not hold the workspace any more (8192
      * rows 226 us with and 231 without, 4 sequences of 2048 rows 208 and 214, 4096 rows 117 and
      * 114). */

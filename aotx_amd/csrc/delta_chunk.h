@@ -900,7 +900,10 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
         if constexpr (NS == 1 && AHEAD == 3) x.touched = touch();
         advance();
     };
-    unsigned char top[AOTX_DELTA_PERIOD];       /* V's exponents in the coming period */
+    /* The columns' vmax in the coming period, or, one chunk ahead, in the one that begins: there four
+     * registers are worth more than the wait (64 sequences of 16 rows of 32 heads of 128 185 us, with
+     * them held for a period and others spilled 195). */
+    unsigned char top[AOTX_DELTA_PERIOD];
     auto load_top = [&](unsigned int c) {
 #pragma unroll
         for (unsigned int q = 0; q < AOTX_DELTA_PERIOD; ++q)
@@ -929,7 +932,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
     if constexpr (AHEAD == 0) {
         A = *one;
     } else {
-        load_top(0u);
+        if constexpr (AHEAD > 1) load_top(0u);
         load_k(A);
         load_q(A);
         load_t(A);
@@ -963,6 +966,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
             for (int r = 0; r < 4; ++r) ms = fmaxf(ms, fabsf(S[t][r]));
         ms = fmaxf(ms, __shfl_xor(ms, 16, 64));
         ms = fmaxf(ms, __shfl_xor(ms, 32, 64));
+        if constexpr (AHEAD == 1) load_top(c);
         int ex = aotx_exponent(ms) - shift + 5, ev = one_top;
         if constexpr (AHEAD > 0)
 #pragma unroll
@@ -981,7 +985,7 @@ static __device__ __forceinline__ void aotx_delta_follow(const aotx_delta_args &
 #pragma unroll
             for (int r = 0; r < 4; ++r) S[t][r] = ldexpf(S[t][r], ex - shift);
         shift = ex;
-        if constexpr (AHEAD > 0) load_top(c + AOTX_DELTA_PERIOD);
+        if constexpr (AHEAD > 1) load_top(c + AOTX_DELTA_PERIOD);
     };
     auto pass = [&](tile_t &x, tile_t &other, unsigned int c) {
         /* rows that are taken out, or past the chunk, have a beta or zeros in K, Q and V of 0: their X, U
