@@ -37,6 +37,15 @@ AOTX_ROPE_PAIRS_ADJACENT = 1
 AOTX_ROPE_AXES_MAX = 4
 AOTX_ROPE_AXES_RUNS = 0
 AOTX_ROPE_AXES_TURN = 1
+AOTX_ACT_NONE = 0
+AOTX_ACT_SILU = 1
+AOTX_ACT_GELU = 2
+AOTX_ACT_GELU_TANH = 3
+AOTX_ACT_RELU = 4
+AOTX_LINEAR_F32 = 0
+AOTX_LINEAR_F16 = 1
+AOTX_LINEAR_ZERO = 65536
+AOTX_LINEAR_ROWS_MAX = 1 << 18
 AOTX_MODEL_ABSENT = (1 << 64) - 1
 AOTX_MODEL_ROWS_ALL = 0
 AOTX_MODEL_ROWS_LAST = 1
@@ -198,6 +207,20 @@ class RopeHow(ctypes.Structure):
                 ("order", u32), ("span", u32 * AOTX_ROPE_AXES_MAX)]
 
 
+class LinearHow(ctypes.Structure):
+    """include/aotx_layer.h aotx_linear_how."""
+    _fields_ = [("w", vp), ("up", vp), ("bias", vp), ("up_bias", vp), ("resid", vp), ("n", u32),
+                ("k", u32), ("ldx", u32), ("ldy", u32), ("ldr", u32), ("act", u32), ("out", u32),
+                ("packed", u32)]
+
+
+class AdjustHow(ctypes.Structure):
+    """include/aotx_layer.h aotx_adjust_how."""
+    _fields_ = [("sample", vp), ("agent", vp), ("list", vp), ("length", vp), ("lists", u32),
+                ("list_stride", u32), ("bias_at", vp), ("bias_token", vp), ("bias", vp),
+                ("biases", u32), ("mask", vp), ("mask_of", vp), ("masks", u32), ("mask_stride", u32)]
+
+
 PROTOTYPES = {
     "aotx_mem_weights_set": (i32, [u64, u64]),
     "aotx_mem_weights_base": (u64, []),
@@ -269,6 +292,13 @@ PROTOTYPES = {
     "aotx_norm_gate": (i32, [vp, vp, u32, vp, u32, u32, u32, f32, vp, vp]),
     "aotx_rope_axes": (i32, [vp, u32, vp, vp, ctypes.POINTER(RopeHow), vp, vp, u32, u32, u32,
                              u32, vp, vp, vp, vp]),
+    # the operators of a full layer and of a step's answer (include/aotx_layer.h)
+    "aotx_q8_linear_work": (u64, [u32, u32, u32, u32]),
+    "aotx_q8_linear": (i32, [ctypes.POINTER(LinearHow), vp, u32, vp, vp, u64, vp]),
+    "aotx_norm_rows": (i32, [vp, u32, vp, u32, u32, f32, vp, vp]),
+    "aotx_kv_append": (i32, [vp, u32, vp, vp, ctypes.POINTER(RopeHow), vp, f32, vp, vp, vp, vp,
+                             u32, u32, u32, u32, u32, u32, u32, vp, vp, vp, vp, vp]),
+    "aotx_logits_adjust": (i32, [ctypes.POINTER(AdjustHow), vp, u32, u32, u32, vp, u32, vp]),
     # GGUF model files (include/aotx_modelfile.h)
     "aotx_modelfile_open": (i32, [ctypes.c_char_p, ctypes.POINTER(vp)]),
     "aotx_modelfile_close": (None, [vp]),

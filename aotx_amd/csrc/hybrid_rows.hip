@@ -2,10 +2,7 @@
  * (aotx_norm_gate) and the turn of q and k by several axes (aotx_rope_axes). Both are bound by
  * memory: every value is read once in 16-byte loads and written once.
  */
-#include "delta_dev.h"
-#include "../../include/aotx_hybrid.h"
-
-#include <math.h>
+#include "rope_dev.h"
 
 /* ---------------------------------------------------------------------------------------
  * out = half(x * rsqrt(mean(x^2) + eps) * w * silu(z)). A lane takes 8 values of a row, whose sum
@@ -152,8 +149,7 @@ struct aotx_rope_axes_args {
     unsigned short *q, *k, *v;
     unsigned int stride, tokens, heads, kv_heads, pairs, rope_dim, axes;
     float eps;
-    double turns[64];           /* of pair i at place 1: theta^(-2i/r) / (2 pi) */
-    unsigned char axis[64];
+    aotx_rope_turns rope;
 };
 
 template <int D>
@@ -165,9 +161,8 @@ __global__ __launch_bounds__(256) void aotx_rope_axes_kernel(aotx_rope_axes_args
     const unsigned int half = p.rope_dim / 2u;
     if (threadIdx.x < half) {
         const unsigned int i = threadIdx.x;
-        double a = (double)p.place[(unsigned long long)t * p.axes + p.axis[i]] * p.turns[i];
-        if (p.factor != nullptr) a /= (double)p.factor[i];
-        const float f = (float)(a - floor(a));          /* [0, 1] turns */
+        const float f = aotx_rope_angle((double)p.place[(unsigned long long)t * p.axes + p.rope.axis[i]],
+                                        p.rope.turns[i], p.factor, i);
         cs[i] = cospif(2.0f * f);
         sn[i] = sinpif(2.0f * f);
     }
@@ -211,20 +206,8 @@ __global__ __launch_bounds__(256) void aotx_rope_axes_kernel(aotx_rope_axes_args
                 y0[e] = aotx_f2h(x0[e]);
                 y1[e] = aotx_f2h(x1[e]);
             }
-        } else if (p.pairs == AOTX_ROPE_PAIRS_SPLIT) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                y0[e] = aotx_f2h(x0[e] * c[e] - x1[e] * s[e]);
-                y1[e] = aotx_f2h(x0[e] * s[e] + x1[e] * c[e]);
-            }
         } else {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                y0[2 * e] = aotx_f2h(x0[2 * e] * c[e] - x0[2 * e + 1] * s[e]);
-                y0[2 * e + 1] = aotx_f2h(x0[2 * e] * s[e] + x0[2 * e + 1] * c[e]);
-                y1[2 * e] = aotx_f2h(x1[2 * e] * c[2 + e] - x1[2 * e + 1] * s[2 + e]);
-                y1[2 * e + 1] = aotx_f2h(x1[2 * e] * s[2 + e] + x1[2 * e + 1] * c[2 + e]);
-            }
+            aotx_rope_pairs(p.pairs, x0, x1, c, s, y0, y1);
         }
         unsigned short *to = is_q ? p.q + ((unsigned long long)t * p.heads + h) * D
             : is_v ? p.v + ((unsigned long long)t * p.kv_heads + (h - p.heads - p.kv_heads)) * D
@@ -245,15 +228,7 @@ extern "C" int aotx_rope_axes(const float *qkv, unsigned int stride, const float
     if (heads == 0u || heads > 1024u || kv_heads > 1024u || tokens > (1u << 20)) return 1;
     if (kv_heads == 0u ? (k != nullptr || v != nullptr) : k == nullptr) return 1;
     if (stride % 4u != 0u || stride < (heads + 2u * kv_heads) * head_dim) return 1;
-    const unsigned int r = how->rope_dim;
-    if (r == 0u || r % 8u != 0u || r > head_dim) return 1;
-    if (how->pairs != AOTX_ROPE_PAIRS_SPLIT && how->pairs != AOTX_ROPE_PAIRS_ADJACENT) return 1;
-    if (how->axes == 0u || how->axes > AOTX_ROPE_AXES_MAX) return 1;
-    if (how->order != AOTX_ROPE_AXES_RUNS && how->order != AOTX_ROPE_AXES_TURN) return 1;
-    if (!(how->theta > 0.0f) || !isfinite(how->theta) || !(how->eps >= 0.0f)) return 1;
-    unsigned long long sum = 0u;
-    for (unsigned int i = 0; i < how->axes; ++i) sum += how->span[i];
-    if (sum != r / 2u) return 1;
+    if (!aotx_rope_ok(how, head_dim)) return 1;
     if (!aotx_aligned16(qkv) || !aotx_aligned16(q_norm) || !aotx_aligned16(k_norm) || !aotx_aligned16(q)
         || !aotx_aligned16(k) || !aotx_aligned16(v))
         return 1;
@@ -272,26 +247,10 @@ extern "C" int aotx_rope_axes(const float *qkv, unsigned int stride, const float
     p.heads = heads;
     p.kv_heads = kv_heads;
     p.pairs = how->pairs;
-    p.rope_dim = r;
+    p.rope_dim = how->rope_dim;
     p.axes = how->axes;
     p.eps = how->eps;
-    /* powers of one step: 64 products round by less than 2^-46 of a frequency */
-    const double step = pow((double)how->theta, -2.0 / (double)r);
-    double turn = 0.15915494309189533577;       /* 1 / (2 pi) */
-    unsigned int axis = 0u, left = how->span[0];
-    for (unsigned int i = 0; i < 64u; ++i, turn *= step) {
-        p.turns[i] = turn;
-        p.axis[i] = 0u;
-        if (i >= r / 2u) continue;
-        if (how->order == AOTX_ROPE_AXES_TURN) {
-            const unsigned int a = i % how->axes;
-            p.axis[i] = (unsigned char)(i < how->axes * how->span[a] ? a : 0u);
-        } else {
-            while (left == 0u) left = how->span[++axis];
-            --left;
-            p.axis[i] = (unsigned char)axis;
-        }
-    }
+    aotx_rope_fill(how, &p.rope);
     hipStream_t s = aotx_stream(stream);
     if (head_dim == 128u) hipLaunchKernelGGL(aotx_rope_axes_kernel<128>, dim3(tokens), dim3(256), 0, s, p);
     else hipLaunchKernelGGL(aotx_rope_axes_kernel<64>, dim3(tokens), dim3(256), 0, s, p);

@@ -71,12 +71,12 @@ void aotx_q8r_repack(const void *src, unsigned int n, unsigned int k, void *dst,
 
 /* ---- narrow batches ------------------------------------------------------------- */
 
-template <int MT, int RT, int PD, int NW, bool NORM, bool DIRECT, bool FILE>
-__global__ __launch_bounds__(64 * NW) void aotx_rgemv(aotx_rgemv_args a)
+template <int MT, int RT, int PD, int NW, bool NORM, bool DIRECT, bool FILE, class E>
+__global__ __launch_bounds__(64 * NW) void aotx_rgemv(aotx_rgemv_args a, E e)
 {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     aotx_args_touch(a);
-    rg_narrow<MT, RT, PD, NW, NORM, DIRECT, FILE>(a, blockIdx.x, blockIdx.y, lds);
+    rg_narrow<MT, RT, PD, NW, NORM, DIRECT, FILE>(a, e, blockIdx.x, blockIdx.y, lds);
 }
 
 /* Wide batches (MT rows of fp16 x at most, 32 or 64): a workgroup owns T 16-row tiles; its W = T * P
@@ -88,8 +88,8 @@ __global__ __launch_bounds__(64 * NW) void aotx_rgemv(aotx_rgemv_args a)
  * phase order through LDS and the workgroup applies the epilogue (with k split over
  * workgroups, the last split to finish adds the splits first). More phases put more waves
  * on the same tiles (more loads in flight per CU) at the price of more x staging. */
-template <int T, int P, int KC, int PDQ, bool FILE, int MT>
-__global__ __launch_bounds__(64 * T * P, MT == 64 ? 2 : 4) void aotx_rgemv_wide(aotx_rgemv_args a0)
+template <int T, int P, int KC, int PDQ, bool FILE, int MT, class E>
+__global__ __launch_bounds__(64 * T * P, MT == 64 ? 2 : 4) void aotx_rgemv_wide(aotx_rgemv_args a0, E e)
 {
     /* direct rows: grid.y is the pass of MT rows (routed experts: the expert) */
     aotx_rgemv_args a = a0;
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(64 * T * P, MT == 64 ? 2 : 4) void aotx_rgemv_wide(
     do {                                                                                 \
         _Pragma("unroll") for (int qi = 0; qi < PDQ; ++qi) {                             \
             const unsigned int qq = RGW_QUAD((N) + (unsigned int)qi);                    \
-            const unsigned int qx = FILE || T == 2 || MT == 64 || qq < q1 ? qq : q1 - 1u; \
+            const unsigned int qx = FILE || E::LINEAR || T == 2 || MT == 64 || qq < q1 ? qq : q1 - 1u; \
             const unsigned short *xq = (XB) + ((qx - q0) % KC) * 128u + 32u * g;         \
             rg_h8 B[CB][4];                                                              \
             if (MT == 32)                                                                \
@@ -234,12 +234,12 @@ __global__ __launch_bounds__(64 * T * P, MT == 64 ? 2 : 4) void aotx_rgemv_wide(
      * requested before chunk c's later weight loads, so storing it waits for nothing
      * issued after it. */
     rg_ss_pre<MT, NT> ssp;
-    const bool ss_pre = list == nullptr && rg_row_ss_load<MT, NT>(a, cap, ssp);
+    const bool ss_pre = !E::LINEAR && list == nullptr && rg_row_ss_load<MT, NT>(a, cap, ssp);
     RGW_XLOAD(0u);
     /* the residual epilogue's residual values and next norm weights of few-tile products
      * (down), for direct rows: read with the first loads, unconditionally (from clamped
      * addresses; masked where used), instead of in dependent rounds after the split merge */
-    constexpr bool RP = T <= 2;
+    constexpr bool RP = !E::LINEAR && T <= 2;
     constexpr unsigned int RPT = (T * 16u * MT + NT - 1u) / NT;
     __shared__ float rres[RP ? T * 16 * rg_os<MT>() : 1];
     __shared__ float rgw[RP ? T * 16 : 1];
@@ -336,11 +336,12 @@ __global__ __launch_bounds__(64 * T * P, MT == 64 ? 2 : 4) void aotx_rgemv_wide(
         /* rs was written before the loop; the barriers since have published it */
         for (unsigned int idx = tid; idx < gr * MT; idx += NT) out[rg_of<MT>(idx)] *= rs[idx % MT];
         __syncthreads();
-    } else if (a.row_ss != nullptr) {
+    } else if (!E::LINEAR && a.row_ss != nullptr) {
         rg_row_scale<MT, NT>(a, out, gr, mrows, rs);
     }
-    rg_epilogue<MT, NT>(a, out, group, T, mrows, list, resid_pre ? rres : nullptr, nullptr,
-                        resid_pre ? rgw : nullptr);
+    if constexpr (E::LINEAR) rg_linear<MT, NT>(a, e, out, group, T, mrows);
+    else rg_epilogue<MT, NT>(a, out, group, T, mrows, list, resid_pre ? rres : nullptr, nullptr,
+                             resid_pre ? rgw : nullptr);
 }
 
 /* Wide batches (5..32 rows) of a dense model with x in the fragment layout (aotx_xfrag_at):
@@ -571,8 +572,8 @@ __global__ __launch_bounds__(64 * NW) void aotx_rgemv_frag(aotx_rgemv_args a)
  * of at most one workgroup per CU; larger grids run two per CU at 128 registers, where
  * the second workgroup hides the first one's waits (gate/up at 512 rows: 163 against
  * 181 us), and the MFMA loop reads one x fragment at a time. */
-template <int MB, bool WIDE_REGS, bool FILE, bool TAIL>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(WIDE_REGS ? 2 : 4))) void aotx_rgemm(aotx_rgemv_args a0, unsigned int ny)
+template <int MB, bool WIDE_REGS, bool FILE, bool TAIL, class E>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(WIDE_REGS ? 2 : 4))) void aotx_rgemm(aotx_rgemv_args a0, unsigned int ny, E e)
 {
     aotx_args_touch(a0);
     constexpr int RT = RGM_RT;                    /* weight tiles per workgroup */
@@ -742,7 +743,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(WIDE_REGS ?
      * round trip overlaps the split merge), then the tile results into LDS as
      * out[rg_o(tile * 16 + row, batch row)] (the x buffers are free after the last
      * barrier), the split merge and the epilogue */
-    const bool gresid = a.epi == AOTX_EPI_RESID && a.sumsq_out != nullptr;
+    const bool gresid = !E::LINEAR && a.epi == AOTX_EPI_RESID && a.sumsq_out != nullptr;
     /* one register block holds either (the residual products have no row scale) */
     rg_ss_pre<MB, NT> sspre;
     static_assert(sizeof(sspre.v) == rg_gres<MB, NT, RT>::ITER * sizeof(float), "one block");
@@ -750,7 +751,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(WIDE_REGS ?
     float gw = 0.0f;
     bool ss_early = false;
     if (gresid) rg_gres_load<MB, NT, RT>(a, group, mrows, gres, gw);
-    else ss_early = rg_row_ss_load<MB, NT>(a, mrows, sspre);
+    else if (!E::LINEAR) ss_early = rg_row_ss_load<MB, NT>(a, mrows, sspre);
     float *out = (float *)lds;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -773,10 +774,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(WIDE_REGS ?
         for (unsigned int idx = tid; idx < RT * 16u * MB; idx += NT)
             out[rg_of<MB>(idx)] *= rs[idx % MB];
         __syncthreads();
-    } else if (a.row_ss != nullptr) {
+    } else if (!E::LINEAR && a.row_ss != nullptr) {
         rg_row_scale<MB, NT>(a, out, RT * 16u, mrows, rs);
     }
-    if (gresid) rg_gres_store<MB, NT, RT>(a, out, group, mrows, gres, gw);
+    if constexpr (E::LINEAR) rg_linear<MB, NT>(a, e, out, group, RT, mrows);
+    else if (gresid) rg_gres_store<MB, NT, RT>(a, out, group, mrows, gres, gw);
     else rg_epilogue<MB, NT, RT>(a, out, group, RT, mrows, nullptr);
 }
 
@@ -808,7 +810,7 @@ static int aotx_rgemv_plan_n(aotx_rgemv_args *a, const void *const *w, const uns
         a->w[s] = (const unsigned char *)w[s];
         total += rows[s];
         a->seg_end[s] = total;
-        if (s + 1u < nseg && rows[s] % 16u != 0u) return 1;
+        if (s + 1u < nseg && rows[s] % 16u != 0u && epi != AOTX_EPI_SWIGLU) return 1;
     }
     unsigned int tiles;
     if (epi == AOTX_EPI_SWIGLU) {
@@ -1026,7 +1028,7 @@ unsigned int aotx_rgemv_count_words(const aotx_rgemv_args &a)
 }
 
 template <int MT, int RT, int PD>
-static void aotx_rgemv_go(const aotx_rgemv_args &a, hipStream_t s)
+static void aotx_rgemv_go(const aotx_rgemv_args &a, const rg_step_epi &e, hipStream_t s)
 {
     unsigned int ey = a.expert_stride != 0ull ? a.experts : 1u;
     size_t lds = aotx_rgemv_lds(a, MT);
@@ -1035,13 +1037,13 @@ static void aotx_rgemv_go(const aotx_rgemv_args &a, hipStream_t s)
     const bool direct = a.expert_stride == 0ull && a.list == nullptr && a.xrow == nullptr;
 #define RGN_GO(NW, NORM)                                                                   \
     do {                                                                                   \
-        if (direct) hipLaunchKernelGGL((aotx_rgemv<MT, RT, PD, NW, NORM, true, false>), grid, dim3(64 * NW), lds, s, a); \
-        else hipLaunchKernelGGL((aotx_rgemv<MT, RT, PD, NW, NORM, false, false>), grid, dim3(64 * NW), lds, s, a); \
+        if (direct) hipLaunchKernelGGL((aotx_rgemv<MT, RT, PD, NW, NORM, true, false, rg_step_epi>), grid, dim3(64 * NW), lds, s, a, e); \
+        else hipLaunchKernelGGL((aotx_rgemv<MT, RT, PD, NW, NORM, false, false, rg_step_epi>), grid, dim3(64 * NW), lds, s, a, e); \
     } while (0)
 #define RGN_FILE(NW)                                                                       \
     do {                                                                                   \
-        if (direct) hipLaunchKernelGGL((aotx_rgemv<MT, RT, PD, NW, false, true, true>), grid, dim3(64 * NW), lds, s, a); \
-        else hipLaunchKernelGGL((aotx_rgemv<MT, RT, PD, NW, false, false, true>), grid, dim3(64 * NW), lds, s, a); \
+        if (direct) hipLaunchKernelGGL((aotx_rgemv<MT, RT, PD, NW, false, true, true, rg_step_epi>), grid, dim3(64 * NW), lds, s, a, e); \
+        else hipLaunchKernelGGL((aotx_rgemv<MT, RT, PD, NW, false, false, true, rg_step_epi>), grid, dim3(64 * NW), lds, s, a, e); \
     } while (0)
     if (a.file) {
         if (a.nw == 8u) RGN_FILE(8); else RGN_FILE(4);
@@ -1052,6 +1054,46 @@ static void aotx_rgemv_go(const aotx_rgemv_args &a, hipStream_t s)
     }
 #undef RGN_GO
 #undef RGN_FILE
+    AOTX_LAUNCH_CHECK();
+}
+
+template <class E>
+static void aotx_rgemv_wide_go(const aotx_rgemv_args &a, const E &e, hipStream_t s)
+{
+    const dim3 grid(a.groups * a.splits, aotx_rgemv_rows_y(a));
+#define RGW_GO(T, P, KC, PDQ, MT)                                                            \
+    do {                                                                                     \
+        const size_t xb = 2u * MT * (KC * 128u + 8u) * 2u;                                   \
+        if (a.file) hipLaunchKernelGGL((aotx_rgemv_wide<T, P, KC, PDQ, true, MT, E>), grid, dim3(512), xb, s, a, e); \
+        else hipLaunchKernelGGL((aotx_rgemv_wide<T, P, KC, PDQ, false, MT, E>), grid, dim3(512), xb, s, a, e); \
+    } while (0)
+    if (a.wide == 2u) RGW_GO(4, 2, 4, 1, 64);
+    else if (a.rt == 2u) RGW_GO(2, 4, 8, 1, 32);
+    else if (a.rt == 4u) RGW_GO(4, 2, 4, 1, 32);
+    else RGW_GO(8, 1, 4, 2, 32);
+#undef RGW_GO
+    AOTX_LAUNCH_CHECK();
+}
+
+template <class E>
+static void aotx_rgemm_go(const aotx_rgemv_args &a, const E &e, hipStream_t s)
+{
+    const unsigned int ny = (a.m + RGM_MB - 1u) / RGM_MB;
+    const dim3 g1(((a.groups + 7u) / 8u) * 8u * ny * a.splits);
+    const size_t x2 = 2u * RGM_MB * (256u + 8u) * 2u, res = RGM_RT * 16u * RGM_MB * 4u;
+#define RGM_GO(WIDE, FILE, TAIL)                                                             \
+    hipLaunchKernelGGL((aotx_rgemm<RGM_MB, WIDE, FILE, TAIL, E>), g1, dim3(512), x2 > res ? x2 : res, s, a, ny, e)
+    const bool tail = a.k % 128u != 0u;
+    if (g1.x <= 256u) {
+        if (a.file) RGM_GO(true, true, true);
+        else if (tail) RGM_GO(true, false, true);
+        else RGM_GO(true, false, false);
+    } else {
+        if (a.file) RGM_GO(false, true, true);
+        else if (tail) RGM_GO(false, false, true);
+        else RGM_GO(false, false, false);
+    }
+#undef RGM_GO
     AOTX_LAUNCH_CHECK();
 }
 
@@ -1076,23 +1118,7 @@ int aotx_rgemv_launch(const aotx_rgemv_args &a0, hipStream_t s)
             fprintf(stderr, "aotx: the GEMM takes fp16 x of direct rows only\n");
             return 1;
         }
-        const unsigned int ny = (a.m + RGM_MB - 1u) / RGM_MB;
-        const dim3 g1(((a.groups + 7u) / 8u) * 8u * ny * a.splits);
-        const size_t x2 = 2u * RGM_MB * (256u + 8u) * 2u, res = RGM_RT * 16u * RGM_MB * 4u;
-#define RGM_GO(WIDE, FILE, TAIL)                                                           \
-    hipLaunchKernelGGL((aotx_rgemm<RGM_MB, WIDE, FILE, TAIL>), g1, dim3(512), x2 > res ? x2 : res, s, a, ny)
-        const bool tail = a.k % 128u != 0u;
-        if (g1.x <= 256u) {
-            if (a.file) RGM_GO(true, true, true);
-            else if (tail) RGM_GO(true, false, true);
-            else RGM_GO(true, false, false);
-        } else {
-            if (a.file) RGM_GO(false, true, true);
-            else if (tail) RGM_GO(false, false, true);
-            else RGM_GO(false, false, false);
-        }
-#undef RGM_GO
-        AOTX_LAUNCH_CHECK();
+        aotx_rgemm_go(a, rg_step_epi(), s);
         return 0;
     }
     if (a.frag) {
@@ -1129,28 +1155,15 @@ int aotx_rgemv_launch(const aotx_rgemv_args &a0, hipStream_t s)
         return 1;
     }
     if (a.wide) {
-        const unsigned int ey = aotx_rgemv_rows_y(a);
-        const dim3 grid(a.groups * a.splits, ey);
         if (a.xmode != AOTX_X_F16) {
             fprintf(stderr, "aotx: the wide-batch product takes fp16 x only\n");
             return 1;
         }
-#define RGW_GO(T, P, KC, PDQ, MT)                                                            \
-        do {                                                                               \
-            const size_t xb = 2u * MT * (KC * 128u + 8u) * 2u;                             \
-            if (a.file) hipLaunchKernelGGL((aotx_rgemv_wide<T, P, KC, PDQ, true, MT>), grid, dim3(512), xb, s, a); \
-            else hipLaunchKernelGGL((aotx_rgemv_wide<T, P, KC, PDQ, false, MT>), grid, dim3(512), xb, s, a); \
-        } while (0)
-        if (a.wide == 2u) RGW_GO(4, 2, 4, 1, 64);
-        else if (a.rt == 2u) RGW_GO(2, 4, 8, 1, 32);
-        else if (a.rt == 4u) RGW_GO(4, 2, 4, 1, 32);
-        else RGW_GO(8, 1, 4, 2, 32);
-#undef RGW_GO
-        AOTX_LAUNCH_CHECK();
+        aotx_rgemv_wide_go(a, rg_step_epi(), s);
         return 0;
     }
-    if (a.rt == 1u) aotx_rgemv_go<16, 1, 4>(a, s);
-    else aotx_rgemv_go<16, 4, 1>(a, s);
+    if (a.rt == 1u) aotx_rgemv_go<16, 1, 4>(a, rg_step_epi(), s);
+    else aotx_rgemv_go<16, 4, 1>(a, rg_step_epi(), s);
     return 0;
 }
 
@@ -1222,4 +1235,109 @@ extern "C" int aotx_q8_gemv_f16(const void *w, unsigned int n, unsigned int k,
                                 const void *x, unsigned int m, void *y, void *stream)
 {
     return aotx_q8r_gemv_any(w, n, k, x, m, y, AOTX_EPI_F16, true, stream);
+}
+
+/* ---- products with an epilogue of their own (aotx_layer.h) --------------------------------
+ * The plans, kernels and order of sums of the products above, with rg_linear in place of the step's
+ * epilogues. Partials and arrival counters are the caller's, so that calls on several streams or
+ * in several graphs share nothing; the counters have a place of fixed size before the partials
+ * (a word a tile group at most), because a call of other sizes finds them there. */
+
+static_assert(AOTX_LINEAR_ROWS_MAX / 16u * sizeof(unsigned int) <= AOTX_LINEAR_ZERO, "a counter per tile");
+
+static int aotx_linear_plan(aotx_rgemv_args *a, const void *w, const void *up, unsigned int n, unsigned int k,
+                            unsigned int m)
+{
+    const void *ws[2] = {w, up};
+    const unsigned int rows[2] = {n, n};
+    const bool gated = up != nullptr;
+    /* (the streaming kernel's rows: as aotx_q8r_gemv_any) */
+    const unsigned int narrow_max = !gated && (n + 15u) / 16u <= 256u && k <= 4096u ? 8u : AOTX_NARROW_ROWS;
+    return aotx_rgemv_plan_n(a, ws, rows, gated ? 2u : 1u, k, gated ? AOTX_EPI_SWIGLU : AOTX_EPI_F32,
+                             m < AOTX_RGEMM_ROWS ? m : AOTX_RGEMM_ROWS, narrow_max);
+}
+
+static bool aotx_linear_sizes(unsigned int n, unsigned int k, unsigned int m)
+{
+    return n != 0u && n <= AOTX_LINEAR_ROWS_MAX && k != 0u && k % 32u == 0u && k <= (1u << 18) && m <= (1u << 20);
+}
+
+extern "C" unsigned long long aotx_q8_linear_work(unsigned int n, unsigned int k, unsigned int m, unsigned int gated)
+{
+    if (!aotx_linear_sizes(n, k, m)) return 0ull;
+    size_t most = 0u;
+    /* the full passes and the last one */
+    for (unsigned int left : {m < AOTX_RGEMM_ROWS ? m : AOTX_RGEMM_ROWS, m % AOTX_RGEMM_ROWS}) {
+        aotx_rgemv_args a;
+        if (left == 0u) continue;
+        if (aotx_linear_plan(&a, &a, gated != 0u ? &a : nullptr, n, k, left) != 0) return 0ull;
+        const size_t bytes = aotx_rgemv_partial_bytes(a);
+        most = bytes > most ? bytes : most;
+    }
+    return AOTX_LINEAR_ZERO + most;
+}
+
+static void aotx_linear_launch(const aotx_rgemv_args &a, const aotx_linear_epi &e, hipStream_t s)
+{
+    if (a.gemm) return aotx_rgemm_go(a, e, s);
+    if (a.wide) return aotx_rgemv_wide_go(a, e, s);
+    const dim3 grid(a.groups * a.splits);
+    const size_t lds = aotx_rgemv_lds(a, 16u);
+#define RGL_GO(RT, PD, NW)                                                                   \
+    do {                                                                                     \
+        if (a.file) hipLaunchKernelGGL((aotx_rgemv<16, RT, PD, NW, false, true, true, aotx_linear_epi>), grid, dim3(64 * NW), lds, s, a, e); \
+        else hipLaunchKernelGGL((aotx_rgemv<16, RT, PD, NW, false, true, false, aotx_linear_epi>), grid, dim3(64 * NW), lds, s, a, e); \
+    } while (0)
+    if (a.rt == 1u) {
+        if (a.nw == 8u) RGL_GO(1, 4, 8); else RGL_GO(1, 4, 4);
+    } else {
+        if (a.nw == 8u) RGL_GO(4, 1, 8); else RGL_GO(4, 1, 4);
+    }
+#undef RGL_GO
+    AOTX_LAUNCH_CHECK();
+}
+
+static bool aotx_is_aligned(const void *p, uintptr_t to) { return ((uintptr_t)p & (to - 1u)) == 0u; }
+
+extern "C" int aotx_q8_linear(const aotx_linear_how *how, const void *x, unsigned int m, void *y, void *work,
+                              unsigned long long work_bytes, void *stream)
+{
+    if (how == nullptr || how->w == nullptr || x == nullptr || y == nullptr || work == nullptr) return 1;
+    const unsigned int n = how->n, k = how->k;
+    if (!aotx_linear_sizes(n, k, m)) return 1;
+    if (how->ldx % 8u != 0u || how->ldx < k || how->ldx > (1u << 22)) return 1;
+    if (how->ldy < n || how->ldy > (1u << 22)) return 1;
+    if (how->resid != nullptr && (how->ldr < n || how->ldr > (1u << 22))) return 1;
+    if (how->act > AOTX_ACT_RELU || how->out > AOTX_LINEAR_F16 || how->packed > 1u) return 1;
+    if (how->up_bias != nullptr && how->up == nullptr) return 1;
+    if ((const void *)how->resid == y && (how->out != AOTX_LINEAR_F32 || how->ldr != how->ldy)) return 1;
+    const uintptr_t matrix = how->packed ? 16u : 2u;
+    if (!aotx_is_aligned(how->w, matrix) || !aotx_is_aligned(how->up, matrix) || !aotx_is_aligned(x, 16u)) return 1;
+    if (!aotx_is_aligned(y, how->out == AOTX_LINEAR_F16 ? 2u : 4u) || !aotx_is_aligned(how->resid, 4u)
+        || !aotx_is_aligned(how->bias, 4u) || !aotx_is_aligned(how->up_bias, 4u) || !aotx_is_aligned(work, 256u))
+        return 1;
+    if (work_bytes < aotx_q8_linear_work(n, k, m, how->up != nullptr)) return 1;
+    aotx_linear_epi e;
+    e.bias = how->bias;
+    e.up_bias = how->up_bias;
+    e.resid = how->resid;
+    e.ldr = how->ldr;
+    e.act = how->act;
+    e.half = how->out == AOTX_LINEAR_F16;
+    for (unsigned int m0 = 0u, rows = 0u; m0 < m; m0 += rows) {
+        rows = m - m0 < AOTX_RGEMM_ROWS ? m - m0 : AOTX_RGEMM_ROWS;
+        aotx_rgemv_args a;
+        if (aotx_linear_plan(&a, how->w, how->up, n, k, rows) != 0) return 1;
+        if (!how->packed) aotx_rgemv_file(&a);
+        a.xmode = AOTX_X_F16;
+        a.x = (const unsigned short *)x;
+        a.ldx = how->ldx;
+        a.m0 = m0;
+        a.y = y;
+        a.ldy = how->ldy;
+        a.count = (unsigned int *)work;
+        a.partial = (float *)((unsigned char *)work + AOTX_LINEAR_ZERO);
+        aotx_linear_launch(a, e, aotx_stream(stream));
+    }
+    return 0;
 }

@@ -6,12 +6,24 @@
 
 #include "coherent.h"
 #include "rgemv.h"
+#include "../../include/aotx_layer.h"
 
 typedef _Float16 rg_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 rg_h2 __attribute__((ext_vector_type(2)));
 typedef float rg_f4 __attribute__((ext_vector_type(4)));
 typedef unsigned int rg_u4 __attribute__((ext_vector_type(4)));
 
+
+/* What a product does with its sums, as a type of its kernels: the step's epilogues
+ * (aotx_rgemv_args.epi), or that of aotx_q8_linear, whose code the step's kernels do not carry. */
+struct rg_step_epi {
+    static constexpr bool LINEAR = false;
+};
+struct aotx_linear_epi {
+    static constexpr bool LINEAR = true;
+    const float *bias, *up_bias, *resid;
+    unsigned int ldr, act, half;
+};
 
 /* A kernel-constant word read through the scalar cache (counted by lgkmcnt, so waiting for
  * it does not wait for the vector loads issued before it). Only for memory no kernel of
@@ -649,6 +661,43 @@ static __device__ __forceinline__ void rg_epilogue(const aotx_rgemv_args &a, con
 #undef RG_YROW
 }
 
+/* ---- the epilogue of aotx_q8_linear ----
+ * y = act(sum + bias) [* (up sum + up_bias)] + resid, everything in fp32 and rounded once where y
+ * is fp16. a.epi says how tiles pair: AOTX_EPI_SWIGLU for two matrices, else AOTX_EPI_F32. */
+static __device__ __forceinline__ float rg_act(float v, unsigned int act)
+{
+    if (act == AOTX_ACT_SILU) return v / (1.0f + expf(-v));
+    if (act == AOTX_ACT_GELU) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+    if (act == AOTX_ACT_GELU_TANH) return 0.5f * v * (1.0f + tanhf(0.79788456080286536f * (v + 0.044715f * v * v * v)));
+    if (act == AOTX_ACT_RELU) return v < 0.0f ? 0.0f : v;      /* a NaN stays one */
+    return v;
+}
+
+template <int MT, int NT>
+static __device__ __forceinline__ void rg_linear(const aotx_rgemv_args &a, const aotx_linear_epi &e, const float *out,
+                                                 unsigned int group, unsigned int rt, unsigned int mrows)
+{
+    const bool gated = a.epi == AOTX_EPI_SWIGLU;
+    const unsigned int gr = gated ? rt * 8u : rt * 16u;
+    for (unsigned int idx = threadIdx.x; idx < gr * MT; idx += NT) {
+        const unsigned int row = idx % gr, mm = idx / gr;
+        const unsigned int v = rg_vrow(a, group, row / 16u, row % 16u, rt);
+        if (mm >= mrows || v >= a.n) continue;
+        float val = out[rg_o<MT>(row, mm)];
+        if (e.bias != nullptr) val += e.bias[v];
+        val = rg_act(val, e.act);
+        if (gated) {
+            float up = out[rg_o<MT>(row + gr, mm)];
+            if (e.up_bias != nullptr) up += e.up_bias[v];
+            val *= up;
+        }
+        const unsigned long long i = a.m0 + mm;
+        if (e.resid != nullptr) val += e.resid[i * e.ldr + v];
+        if (e.half) ((unsigned short *)a.y)[i * a.ldy + v] = aotx_f2h(val);
+        else ((float *)a.y)[i * a.ldy + v] = val;
+    }
+}
+
 /* The RMSNorm scale of batch rows given as unscaled x (a.row_ss): out[row][mm] *= rsqrt(
  * sum_i row_ss[m0 + mm][i] / k + eps), 16 threads per batch row adding its k/16 partial
  * sums in a fixed order. rs is MT floats of LDS; ends with a barrier. */
@@ -874,9 +923,9 @@ static __device__ __forceinline__ bool rg_split_merge(const aotx_rgemv_args &a, 
 
 /* MT: batch columns of the MFMA (16 or 32); RT: 16-row tiles per workgroup; PD: quads
  * loaded ahead per wave; NW: waves per workgroup, splitting the k range (8 for products of
- * few tiles, so that each wave's share of the dequantisation is short). */
-template <int MT, int RT, int PD, int NW, bool NORM, bool DIRECT, bool FILE>
-static __device__ __forceinline__ void rg_narrow(const aotx_rgemv_args &a, unsigned int bx,
+ * few tiles, so that each wave's share of the dequantisation is short). E: the epilogue. */
+template <int MT, int RT, int PD, int NW, bool NORM, bool DIRECT, bool FILE, class E>
+static __device__ __forceinline__ void rg_narrow(const aotx_rgemv_args &a, const E &e, unsigned int bx,
                                                  unsigned int expert_in, unsigned char *lds)
 {
     /* DIRECT: batch row i is row m0 + i (no expert list, no row map), known when compiled */
@@ -945,7 +994,7 @@ static __device__ __forceinline__ void rg_narrow(const aotx_rgemv_args &a, unsig
     } while (0)
 
     /* Branch-free: a quad past the wave's range reads the last quad's x and has its scale
-     * forced to zero (it adds nothing; FILE: its x too, as 0 times an infinity would be NaN); a
+     * forced to zero (it adds nothing; FILE and LINEAR: its x too, as 0 times an infinity would be NaN); a
      * batch column past mrows reads row 0 of x (its results are never written). */
 #define RG_COMPUTE(BUF, QS)                                                              \
     do {                                                                                 \
@@ -959,7 +1008,7 @@ static __device__ __forceinline__ void rg_narrow(const aotx_rgemv_args &a, unsig
                 const unsigned int mr = mm < mrows ? mm : 0u;                            \
                 _Pragma("unroll") for (int s = 0; s < 4; ++s) {                          \
                     B[t][s] = *(const rg_h8 *)(xq + mr * xs + 8u * s);                   \
-                    if (FILE && qq >= wq1) B[t][s] = (rg_h8)(_Float16)0.0f;              \
+                    if ((FILE || E::LINEAR) && qq >= wq1) B[t][s] = (rg_h8)(_Float16)0.0f;   \
                 }                                                                        \
             }                                                                            \
             _Pragma("unroll") for (int j = 0; j < RT; ++j) {                             \
@@ -987,7 +1036,7 @@ static __device__ __forceinline__ void rg_narrow(const aotx_rgemv_args &a, unsig
     const bool direct = DIRECT || (list == nullptr && a.xrow == nullptr);
     const bool early = direct;
     const bool norm = NORM;
-    const bool resid_pre = early && a.epi == AOTX_EPI_RESID && a.sumsq_out != nullptr;
+    const bool resid_pre = !E::LINEAR && early && a.epi == AOTX_EPI_RESID && a.sumsq_out != nullptr;
     const unsigned int cap = a.m < (unsigned int)MT ? a.m : (unsigned int)MT;
     const unsigned int kbeg = q0 * 128u;
     const unsigned int pieces = (q1 - q0) * 16u;       /* 16-byte pieces (8 values) per row */
@@ -1032,7 +1081,7 @@ static __device__ __forceinline__ void rg_narrow(const aotx_rgemv_args &a, unsig
     /* the QKV epilogue's batch words (position, slot) and rope factor go out with them: its
      * destinations and rotations are resolved while the weights stream */
     constexpr unsigned int QU = RT * 8u * MT;          /* output pairs of the workgroup */
-    const bool qkv_pre = a.epi == AOTX_EPI_QKV && QU <= NT;
+    const bool qkv_pre = !E::LINEAR && a.epi == AOTX_EPI_QKV && QU <= NT;
     unsigned int q_pos = 0u, q_agent = 0u;
     float q_fac = 1.0f;
     if (qkv_pre && tid < QU) {
@@ -1189,8 +1238,9 @@ static __device__ __forceinline__ void rg_narrow(const aotx_rgemv_args &a, unsig
         __shared__ unsigned int last;
         if (!rg_split_merge<NT>(a, out, gr * rg_os<MT>(), expert, group, split, &last)) return;
     }
-    rg_epilogue<MT, NT>(a, out, group, RT, mrows, list, resid_pre ? rres : nullptr,
-                        qkv_pre ? &qpre : nullptr, resid_pre ? rgw : nullptr);
+    if constexpr (E::LINEAR) rg_linear<MT, NT>(a, e, out, group, RT, mrows);
+    else rg_epilogue<MT, NT>(a, out, group, RT, mrows, list, resid_pre ? rres : nullptr,
+                             qkv_pre ? &qpre : nullptr, resid_pre ? rgw : nullptr);
 }
 
 

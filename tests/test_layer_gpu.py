@@ -1,0 +1,895 @@
+"""The operators of a full layer and of a step's answer on the GPU against the 64-bit oracle
+(oracle/layer.py): every form that sizes choose, odd sizes and padded rows, what lies outside the rows, slots
+and pages that are missing, values of Inf and NaN, capture, other streams, and a layer and an answer of them.
+
+Tolerances are oracle/layer.py's: counted roundings of fp32, and half a step of the type that is
+written."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import aotx_amd as A
+from aotx_amd.model import layout_pages, normal, quantize_q8
+from oracle import hybrid as H
+from oracle import layer as O
+from tests.gpu_util import KEEP, p
+
+pytestmark = pytest.mark.gpu
+
+EPS = 1e-6
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    return torch
+
+
+@pytest.fixture(autouse=True)
+def _no_faults(lib):
+    lib.aotx_model_forget()
+
+
+def _up(torch, a, dtype):
+    """A device tensor of `a` with its own shape."""
+    t = torch.from_numpy(np.ascontiguousarray(a, dtype=dtype)).cuda()
+    KEEP.append(t)
+    return t
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _graph(torch, call):
+    """The call (of a stream) captured."""
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        call(ctypes.c_void_p(side.cuda_stream))
+    return g
+
+
+# ---- the product -----------------------------------------------------------------------------
+
+class Linear:
+    """One product's operands, on the host and the device."""
+
+    def __init__(self, torch, lib, seed, m, n, k, gated=False, act=0, bias=False, resid=None, half=False, packed=True,
+                 pad=(0, 0, 0), scale=1.0):
+        rng = np.random.default_rng(seed)
+        self.torch, self.lib, self.m, self.n, self.k = torch, lib, m, n, k
+        self.gated, self.act, self.half, self.packed = gated, act, half, packed
+        self.ldx, self.ldy, self.ldr = k + pad[0], n + pad[1], n + pad[2]
+        self.raw = [quantize_q8((scale * k ** -0.5 * normal(seed + i, 0, n * k)).astype(np.float32).reshape(n, k))
+                    for i in range(1 + gated)]
+        self.w = [O.q8_values(r, n, k) for r in self.raw]
+        self.x = rng.normal(0, 1, (m, self.ldx)).astype(np.float16)
+        self.bias = [rng.normal(0, 1, n).astype(np.float32) if bias else None for _ in range(1 + gated)]
+        self.resid = rng.normal(0, 2, (m, self.ldr)).astype(np.float32) if resid else None
+        self.inplace = resid == "inplace"
+
+    def up(self):
+        t, lib = self.torch, self.lib
+        self.dx = _up(t, self.x, np.float16)
+        self.dw = []
+        for r in self.raw:
+            w = _up(t, r.reshape(-1), np.uint8)
+            if self.packed:
+                q = t.zeros(lib.aotx_q8r_size(self.n, self.k), dtype=t.uint8, device="cuda")
+                assert lib.aotx_q8_repack(p(w), self.n, self.k, p(q), None) == 0
+                w = q
+            self.dw.append(w)
+        self.db = [None if b is None else _up(t, b, np.float32) for b in self.bias]
+        self.y = t.full((self.m + 2, self.ldy), 7.0, dtype=t.float16 if self.half else t.float32, device="cuda")
+        self.dr = None
+        if self.inplace:
+            self.y[:self.m] = t.from_numpy(self.resid).cuda()
+            self.dr = self.y
+        elif self.resid is not None:
+            self.dr = _up(t, self.resid, np.float32)
+        self.how = A.LinearHow(w=_at(self.dw[0]), up=_at(self.dw[1]) if self.gated else None, bias=_at(self.db[0]),
+                               up_bias=_at(self.db[1]) if self.gated else None, resid=_at(self.dr), n=self.n, k=self.k,
+                               ldx=self.ldx, ldy=self.ldy, ldr=self.ldr, act=self.act, out=int(self.half),
+                               packed=int(self.packed))
+        need = lib.aotx_q8_linear_work(self.n, self.k, self.m, int(self.gated))
+        self.need = need
+        self.work = t.full((need + 256,), 0xAB, dtype=t.uint8, device="cuda")
+        self.work[:A.AOTX_LINEAR_ZERO] = 0
+        return self
+
+    def call(self, stream=None, work=None, m=None):
+        work = self.work if work is None else work
+        assert self.lib.aotx_q8_linear(ctypes.byref(self.how), p(self.dx), self.m if m is None else m, p(self.y), p(work),
+                                       self.need, stream) == 0
+        return self
+
+    def want(self):
+        x = self.x[:, :self.k].astype(np.float64)
+        b = [None if v is None else v.astype(np.float64) for v in self.bias] + [None]
+        r = None if self.resid is None else self.resid[:, :self.n].astype(np.float64)
+        with np.errstate(invalid="ignore", over="ignore"):
+            return O.linear(x, self.w[0], self.w[1] if self.gated else None, b[0], b[1], r, self.act)
+
+    def check(self, untouched=True):
+        self.torch.cuda.synchronize()
+        y = self.y.cpu().numpy().astype(np.float64)
+        want, far = self.want()
+        got = y[:self.m, :self.n]
+        off = np.abs(got - want) - O.rounded(far, want, self.half)
+        assert off.max() <= 0, (off.max(), np.unravel_index(off.argmax(), off.shape))
+        if untouched:
+            before = self.resid[:, self.n:] if self.inplace else 7.0
+            assert (y[:self.m, self.n:] == before).all() and (y[self.m:] == 7.0).all()
+            assert not self.work[:A.AOTX_LINEAR_ZERO].any() and (self.work[self.need:] == 0xAB).all()
+        return self
+
+
+SIZES = [(1, 1, 32), (1, 17, 64), (2, 100, 352), (4, 4096, 256), (5, 130, 1024), (8, 64, 4096), (9, 1001, 544),
+         (16, 33, 2080), (31, 250, 128), (32, 512, 4096), (33, 1001, 160), (48, 16, 14336), (63, 700, 1024), (64, 2048, 1024),
+         (65, 48, 96), (100, 1000, 2080), (128, 512, 1056), (129, 257, 512), (257, 300, 768), (511, 640, 256), (512, 96, 4096),
+         (513, 200, 128), (1030, 70, 288)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("gated", [True, False])
+def test_linear_sizes(torch, lib, m, n, k, packed, gated):
+    i = m + n + k
+    Linear(torch, lib, i, m, n, k, gated, 1 if gated else i % 5, i % 2 == 0, "apart" if i % 3 == 0 else None, i % 4 < 2,
+           packed, (8 * (i % 3), i % 5, i % 7)).up().call().check()
+
+
+@pytest.mark.parametrize("act", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("m", [3, 20, 40, 300])
+def test_linear_activations(torch, lib, act, gated, m):
+    """Arguments to 40 and more, where exponentials leave fp32."""
+    c = Linear(torch, lib, act + 10 * m, m, 75, 256, gated, act, True, scale=12.0)
+    c.x[0] = 0
+    c.bias[0][:8] = (0, -200, 200, -90, 90, 1e-30, -5, 5)
+    c.up().call().check()
+
+
+@pytest.mark.parametrize("m", [1, 7, 30, 64, 90, 400])
+@pytest.mark.parametrize("gated", [True, False])
+def test_linear_residual_in_place(torch, lib, m, gated):
+    Linear(torch, lib, m, m, 333, 512, gated, 0, False, "inplace", pad=(0, 3, 3)).up().call().check()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1 << 18, 32), (3, 1 << 18, 64), (2, 3, 1 << 18), (20, 5, 65536), (600, 20000, 64)])
+def test_linear_ends_of_the_range(torch, lib, m, n, k):
+    Linear(torch, lib, 5, m, n, k, half=True).up().call().check()
+
+
+def test_linear_all_blocks_one_side(torch, lib):
+    """Quants at both ends and scales of zero, of the smallest and the largest."""
+    c = Linear(torch, lib, 6, 12, 64, 256)
+    raw = c.raw[0].reshape(64, 8, 34)
+    raw[:, 0, 2:] = 127
+    raw[:, 1, 2:] = 0x80                                                 # -128
+    for i, s in ((2, 0.0), (3, 6e-8), (4, 60000.0 / 128)):
+        raw[:, i, :2] = np.full((64, 1), s, dtype=np.float16).view(np.uint8)
+    c.w[0] = O.q8_values(c.raw[0], 64, 256)
+    c.up().call().check()
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 1024), (6, 4100, 512), (20, 40, 4128), (40, 3000, 256), (64, 40, 1024),
+                                   (200, 400, 1024), (300, 4000, 160), (600, 520, 416)])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_linear_inf_and_nan_stay_in_their_row(torch, lib, packed, m, n, k, bad):
+    """In x: its row alone (an infinity gives infinities by the weights' signs); in a scale: its column."""
+    c = Linear(torch, lib, 8, m, n, k, packed=packed)
+    rows = [0, m - 1, m // 2]
+    for i, r in enumerate(rows):
+        c.x[r, (0, k - 1, k // 2)[i]] = bad
+    c.up().call()
+    torch.cuda.synchronize()
+    y = c.y[:m, :n].cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        want, _ = c.want()
+    assert np.array_equal(np.isnan(y), np.isnan(want)) and np.array_equal(y[np.isinf(want)], want[np.isinf(want)])
+    fine = np.ones(m, dtype=bool)
+    fine[rows] = False
+    assert np.isfinite(y[fine]).all()
+    # one bad scale
+    d = Linear(torch, lib, 9, m, n, k, packed=packed)
+    d.raw[0].reshape(n, k // 32, 34)[n - 1, k // 64, :2] = np.array([bad], dtype=np.float16).view(np.uint8)
+    d.up().call()
+    torch.cuda.synchronize()
+    y = d.y[:m, :n].cpu().numpy()
+    assert np.isfinite(y[:, :n - 1]).all() and not np.isfinite(y[:, n - 1]).any()
+
+
+def test_linear_is_the_product_with_nothing_beside(torch, lib):
+    """Bit for bit aotx_q8r_gemv where the same form runs, and the same on every run."""
+    for m in (1, 8, 32):
+        c = Linear(torch, lib, 3, m, 500, 1024).up().call()
+        y = torch.zeros(m, 500, device="cuda")
+        assert lib.aotx_q8r_gemv(p(c.dw[0]), 500, 1024, p(c.dx), m, p(y), None) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(y, c.y[:m])
+    for m in (40, 300):
+        c = Linear(torch, lib, 3, m, 500, 4096).up().call()
+        torch.cuda.synchronize()
+        first = c.y.clone()
+        for _ in range(3):
+            c.y.fill_(7.0)
+            c.call()
+            torch.cuda.synchronize()
+            assert torch.equal(first, c.y)
+
+
+def test_linear_one_workspace_for_all_sizes(torch, lib):
+    """Calls of any sizes one after another on one workspace."""
+    calls = [Linear(torch, lib, i, m, n, k, g, g, half=h).up() for i, (m, n, k, g, h) in enumerate(
+        [(1, 4096, 4096, 0, 0), (32, 300, 14336, 1, 1), (512, 96, 4096, 0, 0), (2, 70000, 12800, 0, 1), (64, 2048, 1024, 1, 0),
+         (8, 64, 4096, 0, 0), (700, 130, 2048, 0, 1)])]
+    work = torch.full((max(c.need for c in calls),), 0xFF, dtype=torch.uint8, device="cuda")
+    work[:A.AOTX_LINEAR_ZERO] = 0
+    for turn in range(2):
+        for c in calls:
+            c.y.fill_(7.0)
+            c.call(work=work)
+    for c in calls:
+        c.check()
+    assert not work[:A.AOTX_LINEAR_ZERO].any()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 500, 4096), (20, 200, 4096), (64, 256, 2048), (300, 256, 4096), (600, 128, 1024)])
+def test_linear_in_graphs(torch, lib, m, n, k):
+    """Two captured calls that share a workspace, replayed in turn with other rows, with eager calls between."""
+    a, b = (Linear(torch, lib, 20 + i, m, n, k, i == 1, i, True, half=i == 1).up() for i in range(2))
+    work = torch.zeros(max(a.need, b.need), dtype=torch.uint8, device="cuda")
+    a.call(work=work), b.call(work=work)
+    graphs = [_graph(torch, lambda s, c=c: c.call(s, work)) for c in (a, b)]
+    rng = np.random.default_rng(21)
+    for turn in range(4):
+        for c, g in zip((a, b), graphs):
+            c.x = rng.normal(0, 1, c.x.shape).astype(np.float16)
+            c.dx.copy_(torch.from_numpy(c.x))
+            c.y.fill_(7.0)
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            got = c.y.clone()
+            c.check()
+            c.y.fill_(7.0)
+            c.call(work=work)
+            torch.cuda.synchronize()
+            assert torch.equal(got, c.y), turn
+
+
+@pytest.mark.parametrize("m", [1, 24, 64, 300])
+def test_linear_on_two_streams(torch, lib, m):
+    """At once, each with its own workspace."""
+    calls = [Linear(torch, lib, 30 + i, m, 512, 8192, half=True).up() for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, s in zip(calls, streams):
+            c.call(ctypes.c_void_p(s.cuda_stream))
+    for c in calls:
+        c.check()
+
+
+# ---- the norm --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("width", [8, 64, 72, 504, 512, 520, 1024, 2048, 2056, 4096, 5000, 8192, 8200, 16384, 32768])
+@pytest.mark.parametrize("tokens,pad", [(1, 0), (7, 12), (130, 4)])
+def test_norm_rows(torch, lib, width, tokens, pad):
+    rng = np.random.default_rng(width + tokens)
+    x = (rng.normal(0, 1, (tokens, width + pad)) * 10.0 ** rng.uniform(-6, 6, (tokens, 1))).astype(np.float32)
+    x[0, :width] = 0
+    w = rng.normal(1, 0.3, width).astype(np.float32)
+    out = torch.full((tokens + 1, width), 7.0, dtype=torch.float16, device="cuda")
+    assert lib.aotx_norm_rows(p(_up(torch, x, np.float32)), width + pad, p(_up(torch, w, np.float32)), tokens, width, EPS,
+                              p(out), None) == 0
+    torch.cuda.synchronize()
+    got = out.cpu().numpy().astype(np.float64)
+    want = O.norm_rows(x[:, :width], w, EPS)
+    # squares and their sum (up to 128 a lane one after another, then ten levels: half of it through the
+    # root), the root, the quotient and two products: 80 roundings; and the last
+    assert (np.abs(got[:-1] - want) - (2.0 ** -11 + 80 * O.E32) * np.abs(want)).max() <= 2.0 ** -25
+    assert (got[-1] == 7.0).all()
+
+
+@pytest.mark.parametrize("width", [64, 1000, 4096, 9000])
+def test_norm_rows_inf_and_nan_stay_in_their_row(torch, lib, width):
+    x = np.ones((5, width), dtype=np.float32)
+    x[1, 3], x[3, width - 1] = np.inf, np.nan
+    out = torch.zeros((5, width), dtype=torch.float16, device="cuda")
+    assert lib.aotx_norm_rows(p(_up(torch, x, np.float32)), width, p(_up(torch, np.ones(width), np.float32)), 5, width, 0.0,
+                              p(out), None) == 0
+    got = out.cpu().numpy()
+    assert (got[[0, 2, 4]] == 1).all() and np.isnan(got[3]).all() and np.isnan(got[1, 3]) and (np.delete(got[1], 3) == 0).all()
+
+
+def test_norm_rows_in_a_graph(torch, lib):
+    x, w = torch.zeros(30, 1000, device="cuda"), torch.ones(1000, device="cuda")
+    out = torch.zeros(30, 1000, dtype=torch.float16, device="cuda")
+
+    def call(s):
+        assert lib.aotx_norm_rows(p(x), 1000, p(w), 30, 1000, EPS, p(out), s) == 0
+    call(None)
+    g = _graph(torch, call)
+    for turn in range(3):
+        x.normal_(generator=torch.Generator("cuda").manual_seed(turn))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        call(None)
+        torch.cuda.synchronize()
+        assert torch.equal(got, out)
+
+
+# ---- rows into the pages -----------------------------------------------------------------------
+
+class Append:
+    def __init__(self, torch, seed, lens, first, agent=None, heads=4, kv=2, d=64, rope_dim=None, split=True, spans=None,
+                 norm=False, factor=False, gain=1.0, layers=2, layer=1, lead=0, tail=0, pad=0, missing=(), theta=1e4):
+        rng = np.random.default_rng(seed)
+        self.torch, self.heads, self.kv, self.d, self.layers, self.layer, self.gain = torch, heads, kv, d, layers, layer, gain
+        self.split, self.rope_dim, self.theta = split, rope_dim or d, theta
+        self.spans = spans or [self.rope_dim // 2]
+        self.tokens = lead + sum(lens) + tail
+        self.offset = (lead + np.concatenate([[0], np.cumsum(lens)])).astype(np.uint32)
+        self.pos = np.array(first, dtype=np.uint32)
+        self.agent = np.array(rng.permutation(64)[:len(lens)] if agent is None else agent, dtype=np.uint32)
+        self.width = (heads + 2 * kv) * d
+        self.x = rng.normal(0, 1, (self.tokens, self.width + pad)).astype(np.float32)
+        self.place = rng.integers(0, 1 << 20, (self.tokens, len(self.spans))).astype(np.uint32) if spans else None
+        self.norms = {n: rng.normal(1, 0.2, d).astype(np.float32) if norm else None for n in "qk"}
+        self.factor = rng.uniform(1, 8, self.rope_dim // 2).astype(np.float32) if factor else None
+        # the pages that the rows stand in, in mixed order
+        per = (A.AOTX_KV_PAGE_BYTES - 256) // (64 * kv * d)
+        need = sorted({(int(s), (int(f) + t) // 16 * layers + layer) for s, f, n in zip(self.agent, first, lens)
+                       for t in range(n) if s < 64})
+        need = [u for u in sorted({(s, b // per) for s, b in need}) if u[1] < 640 and u not in missing]
+        self.table = np.full((64, 640), -1, dtype=np.int64)
+        for i, at in zip(rng.permutation(len(need)), need):
+            self.table[at] = int(i) << 21
+        self.pool = rng.integers(0, 15000, max(1, len(need)) << 20, dtype=np.uint16).view(np.float16)
+
+    def up(self):
+        t = self.torch
+        self.dpool = _up(t, self.pool, np.float16)
+        self.dtable = _up(t, np.where(self.table < 0, 0, self.table + self.dpool.data_ptr()), np.int64)
+        i32 = lambda a: None if a is None else _up(t, a.view(np.int32), np.int32)  # noqa: E731
+        f32 = lambda a: None if a is None else _up(t, a, np.float32)  # noqa: E731
+        self.dx, self.doff, self.dpos, self.dagent, self.dplace = (f32(self.x), i32(self.offset), i32(self.pos), i32(self.agent),
+                                                                   i32(self.place))
+        self.dn, self.dfac = {n: f32(v) for n, v in self.norms.items()}, f32(self.factor)
+        self.q = t.full((self.tokens, self.heads, self.d), 7.0, dtype=t.float16, device="cuda")
+        self.rpos, self.ragent = (t.full((self.tokens,), 99, dtype=t.int32, device="cuda") for _ in range(2))
+        self.how = A.RopeHow(theta=self.theta, eps=EPS, rope_dim=self.rope_dim, pairs=0 if self.split else 1, axes=len(self.spans),
+                             order=0, span=(ctypes.c_uint32 * 4)(*self.spans))
+        return self
+
+    def call(self, lib, stream=None, rows=True, offset=True):
+        opt = lambda t: None if t is None else p(t)  # noqa: E731
+        assert lib.aotx_kv_append(p(self.dx), self.x.shape[1], opt(self.dn["q"]), opt(self.dn["k"]), ctypes.byref(self.how),
+                                  opt(self.dfac), self.gain, opt(self.dplace), p(self.doff) if offset else None, p(self.dpos),
+                                  p(self.dagent), len(self.agent), self.tokens, self.heads, self.kv, self.d, self.layer,
+                                  self.layers, p(self.dtable), p(self.q), p(self.rpos) if rows else None,
+                                  p(self.ragent) if rows else None, stream) == 0
+        return self
+
+    def want(self):
+        fac = None if self.factor is None else self.factor.astype(np.float64)
+
+        def rope(x, name, where):
+            nw = self.norms[name]
+            y = H.rope_axes(x, nw, EPS, where, np.float32(self.theta), self.rope_dim, self.split, self.spans, 0, fac)
+            y[..., :self.rope_dim] *= np.float32(self.gain)
+            return y
+        pool, q = self.pool.astype(np.float64), np.full((self.tokens, self.heads, self.d), 7.0)
+        rpos, ragent = np.full(self.tokens, 99, dtype=np.int64), np.full(self.tokens, 99, dtype=np.int64)
+        faults = O.kv_append(self.x[:, :self.width], self.heads, self.kv, self.d, rope, self.place, self.offset, self.pos,
+                             self.agent, self.layer, self.layers, self.table, pool, q, rpos, ragent)
+        return faults, pool, q, rpos, ragent
+
+    def check(self, lib, rows=True):
+        self.torch.cuda.synchronize()
+        faults, pool, q, rpos, ragent = self.want()
+        gq, gp = self.q.cpu().numpy().astype(np.float64), self.dpool.cpu().numpy().astype(np.float64)
+        # as aotx_rope_axes: sines to 2^-22, a norm's 20 steps
+        far = lambda w: 2.0 ** -11 * np.abs(w) + 2.0 ** -25 + 32 * O.E32 * max(1.0, np.abs(q).max())  # noqa: E731
+        assert (np.abs(gq - q) - far(q)).max() <= 0
+        changed = pool != self.pool.astype(np.float64)
+        assert np.array_equal(gp[~changed], pool[~changed])
+        assert (np.abs(gp - pool) - far(pool))[changed].max(initial=0) <= 0
+        if rows:
+            assert np.array_equal(self.rpos.cpu().numpy().view(np.uint32), rpos & 0xFFFFFFFF)
+            assert np.array_equal(self.ragent.cpu().numpy(), ragent)
+        assert lib.aotx_model_faulted() == faults
+        return faults
+
+
+@pytest.mark.parametrize("kw", [
+    dict(), dict(d=128, heads=32, kv=8, norm=True), dict(split=False, factor=True), dict(d=128, rope_dim=64, gain=1.25, norm=True),
+    dict(d=128, rope_dim=40, split=False, spans=[7, 0, 13]), dict(rope_dim=8, heads=3, kv=1), dict(kv=5, heads=5, pad=12),
+    dict(spans=[12, 10, 10], norm=True, factor=True), dict(heads=64, kv=2, d=128, theta=1e6), dict(heads=1, kv=17, gain=0.5),
+    dict(d=128, heads=24, kv=24, norm=True)])
+@pytest.mark.parametrize("lens,first", [([1], [0]), ([1], [8000]), ([37], [5]), ([1, 0, 16, 3], [15, 9, 16, 100]), ([1] * 64, range(64))])
+def test_append(torch, lib, kw, lens, first):
+    assert Append(torch, len(lens) + sum(lens), lens, list(first), lead=2, tail=3, **kw).up().call(lib).check(lib) == 0
+
+
+def test_append_rows_alone(torch, lib):
+    """No offsets: row i is sequence i; no row arrays."""
+    for n in (1, 5, 64):
+        c = Append(torch, n, [1] * n, [7 * i for i in range(n)]).up().call(lib, rows=False, offset=False)
+        c.check(lib, rows=False)
+        assert (c.rpos == 99).all() and (c.ragent == 99).all()
+
+
+def test_append_slots_missing_and_named_twice(torch, lib):
+    c = Append(torch, 3, [3, 2, 4, 0, 5, 1], [0, 9, 20, 3, 3, 1], agent=[2, 64, 2, 5, 5, 0xFFFFFFFF], lead=1, tail=2)
+    assert c.up().call(lib).check(lib) == 3
+
+
+def test_append_pages_missing(torch, lib):
+    """A row whose position has no page, behind the last page or past the table."""
+    per = (A.AOTX_KV_PAGE_BYTES - 256) // (64 * 2 * 64)          # layout blocks of a page
+    far = per * 640 // 2 * 16                                     # the table's end with two layers
+    c = Append(torch, 4, [3, 2, 20, 2, 2], [0, far - 2, far - 5, 0xFFFFFFF0, 0xFFFFFFFF], agent=[4, 5, 6, 7, 8], missing={(4, 0)})
+    assert c.table[5, 639] >= 0
+    assert c.up().call(lib).check(lib) == 3 + 15 + 2 + 2
+
+
+@pytest.mark.parametrize("offset", [[0, 9, 12, 20], [5, 2, 9, 9], [0xFFFFFFFF, 3, 0xFFFFFFF0, 1], [4, 4, 4, 30]])
+def test_append_offsets_out_of_order_stay_in_bounds(torch, lib, offset):
+    c = Append(torch, 5, [12, 12, 12], [0, 40, 80])
+    c.offset = np.array(offset, dtype=np.uint32)
+    c.up().call(lib).check(lib)
+
+
+def test_append_far_positions_keep_their_angles(torch, lib):
+    """Places near 2^32 turn as exactly as near ones."""
+    c = Append(torch, 6, [9], [3], d=128, spans=[64], theta=1e6)
+    c.place[:, 0] = 0xFFFFFFFF - np.arange(9)
+    c.up().call(lib).check(lib)
+
+
+def test_append_inf_and_nan_stay_in_their_pair(torch, lib):
+    c = Append(torch, 7, [4], [0], heads=2, kv=1)
+    c.x[1, 5], c.x[2, 2 * 64 + 9], c.x[3, 3 * 64 + 1] = np.inf, np.nan, -np.inf
+    c.up().call(lib)
+    torch.cuda.synchronize()
+    q, pool = c.q.cpu().numpy(), c.dpool.cpu().numpy().astype(np.float64)
+    assert not np.isfinite(q[1, 0, [5, 37]]).any()
+    q[1, 0, [5, 37]] = 0
+    assert np.isfinite(q).all()
+    at = [O.places(int(c.agent[0]), t, c.table, 1, 2, 1, 64) for t in range(4)]
+    assert np.isnan(pool[at[2] + 9]) and np.isnan(pool[at[2] + 41]) and pool[at[3] + 16 * 64 + 1] == -np.inf
+    assert np.isfinite(pool).sum() == pool.size - 3
+
+
+def test_append_in_a_graph(torch, lib):
+    """Captured, and replayed with other rows, offsets, positions and slots."""
+    c = Append(torch, 8, [20, 10], [0, 100], agent=[3, 9], norm=True).up()
+    pool0 = c.dpool.clone()
+    c.call(lib)
+    g = _graph(torch, lambda s: c.call(lib, s))
+    rng = np.random.default_rng(9)
+    for off, pos, agent in (([0, 20, 30], [0, 100], [3, 9]), ([0, 1, 2], [40, 7], [9, 3]), ([3, 3, 30], [1, 0], [9, 3]),
+                            ([0, 15, 30], [0, 0], [3, 3])):
+        c.offset, c.pos, c.agent = (np.array(v, dtype=np.uint32) for v in (off, pos, agent))
+        c.x = rng.normal(0, 1, c.x.shape).astype(np.float32)
+        for t, v in ((c.doff, c.offset), (c.dpos, c.pos), (c.dagent, c.agent)):
+            t.copy_(torch.from_numpy(v.view(np.int32)))
+        c.dx.copy_(torch.from_numpy(c.x))
+        got = []
+        for eager in (False, True):
+            c.dpool.copy_(pool0)
+            c.q.fill_(7.0), c.rpos.fill_(99), c.ragent.fill_(99)
+            lib.aotx_model_forget()
+            torch.cuda.synchronize()
+            c.call(lib) if eager else g.replay()
+            c.check(lib)
+            got.append([t.clone() for t in (c.q, c.dpool, c.rpos, c.ragent)])
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_append_is_rope_axes_and_kv_write(torch, lib):
+    """Bit for bit, in the library's own pages; the rows' places are what attention takes."""
+    n, heads, kv, d, layers, layer = 45, 8, 2, 128, 3, 2
+    m = A.KvMap()
+    m.limit = 16
+    assert lib.aotx_kv_open(ctypes.byref(m)) == 0
+    try:
+        for slot in (3, 11):
+            assert lib.aotx_kv_request(slot, layout_pages(80, layers, kv, d)) == 1
+        assert lib.aotx_kv_serve(ctypes.byref(m), None) == 2
+        rng = np.random.default_rng(10)
+        width = (heads + 2 * kv) * d
+        x = _up(torch, rng.normal(0, 1, (n, width)), np.float32)
+        offset, pos, agent = (_up(torch, v, np.int32) for v in ([0, 30, 45], [20, 3], [11, 3]))
+        nq, nk = (_up(torch, rng.normal(1, 0.2, d), np.float32) for _ in range(2))
+        how = A.RopeHow(theta=5e5, eps=EPS, rope_dim=96, pairs=1, axes=1, order=0, span=(ctypes.c_uint32 * 4)(48))
+        f16 = dict(dtype=torch.float16, device="cuda")
+        q, q2, k, v = (torch.zeros(n, h, d, **f16) for h in (heads, heads, kv, kv))
+        rpos, ragent = (torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(2))
+        size = m.limit << 20
+        pool = torch.empty(size, **f16)
+        hip = A.lib()
+        hip.hipMemcpy.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int]
+
+        def pages():
+            torch.cuda.synchronize()
+            assert hip.hipMemcpy(pool.data_ptr(), m.range, 2 * size, 3) == 0
+            return pool.view(torch.int16).clone()
+        assert lib.aotx_kv_append(p(x), width, p(nq), p(nk), ctypes.byref(how), None, 1.0, None, p(offset), p(pos), p(agent), 2, n,
+                                  heads, kv, d, layer, layers, lib.aotx_kv_table_device(), p(q), p(rpos), p(ragent), None) == 0
+        one = pages()
+        assert rpos.tolist() == list(range(20, 50)) + list(range(3, 18)) and ragent.tolist() == [11] * 30 + [3] * 15
+        assert lib.aotx_rope_axes(p(x), width, p(nq), p(nk), ctypes.byref(how), None, p(rpos), n, heads, kv, d, p(q2), p(k), p(v), None) == 0
+        assert lib.aotx_kv_write(p(torch.zeros_like(k)), p(torch.zeros_like(v)), p(rpos), p(ragent), n, kv, d, layer, layers, None) == 0
+        blank = pages()
+        assert lib.aotx_kv_write(p(k), p(v), p(rpos), p(ragent), n, kv, d, layer, layers, None) == 0
+        two = pages()
+        assert torch.equal(q, q2) and torch.equal(one, two) and not torch.equal(one, blank)
+        assert lib.aotx_model_faulted() == 0
+        # a refused sequence's rows go through attention as rows of zeros
+        bad = _up(torch, [64, 3], np.int32)
+        assert lib.aotx_kv_append(p(x), width, p(nq), p(nk), ctypes.byref(how), None, 1.0, None, p(offset), p(pos), p(bad), 2, n,
+                                  heads, kv, d, layer, layers, lib.aotx_kv_table_device(), p(q), p(rpos), p(ragent), None) == 0
+        out = torch.full((n, heads, d), 7.0, **f16)
+        assert lib.aotx_attend_paged(p(q), p(rpos), p(ragent), n, heads, kv, d, layer, layers, p(out), None) == 0
+        torch.cuda.synchronize()
+        assert (out[:30] == 0).all() and torch.isfinite(out[30:]).all()
+    finally:
+        lib.aotx_kv_close(ctypes.byref(m))
+
+
+# ---- logits ------------------------------------------------------------------------------------
+
+class Adjust:
+    def __init__(self, torch, seed, rows, vocab, length=0, biases=0, masks=0, allow=0.5, pad=(0, 0), inplace=False, by_agent=True):
+        rng = np.random.default_rng(seed)
+        self.torch, self.rows, self.vocab, self.inplace = torch, rows, vocab, inplace
+        self.ld = vocab + pad[0]
+        self.ld_out = self.ld if inplace else vocab + pad[1]
+        self.x = rng.normal(0, 3, (rows, self.ld)).astype(np.float32)
+        self.lists = 8 if by_agent else rows
+        self.agent = rng.integers(0, self.lists, rows).astype(np.uint32) if by_agent else None
+        self.stride = length + 3
+        self.list = (vocab * rng.uniform(0, 1, (self.lists, self.stride)) ** 4).astype(np.int32)
+        self.length = rng.integers(length // 2, length + 1, self.lists).astype(np.uint32)
+        self.sample = None
+        if length:
+            self.sample = (A.ModelHow * rows)(*[A.neutral_how(
+                presence_penalty=float(rng.choice([0, 0.5, -0.3])), frequency_penalty=float(rng.choice([0, 0.1, 0.02])),
+                repeat_penalty=float(rng.choice([1, 1.3, 0.8])), repeat_window=int(rng.choice([0, 7, length, 10 * length])))
+                for _ in range(rows)])
+        self.biases = [[(int(t), float(np.float32(v))) for t, v in zip(rng.integers(0, vocab, biases), rng.normal(0, 5, biases))]
+                       for _ in range(rows)]
+        self.bias_at = np.concatenate([[0], np.cumsum([len(b) for b in self.biases])]).astype(np.uint32) if biases else None
+        self.words = (vocab + 31) // 32 + masks % 2
+        self.masks = masks
+        bits = rng.uniform(0, 1, (masks, self.words * 32)) < allow
+        self.mask = np.packbits(bits, axis=1, bitorder="little").view(np.uint32) if masks else None
+        self.mask_of = rng.integers(0, masks + 2, rows).astype(np.uint32) if masks else None
+
+    def up(self):
+        t = self.torch
+        i32 = lambda a: None if a is None else _up(t, a.view(np.int32), np.int32)  # noqa: E731
+        flat = [b for r in self.biases for b in r]
+        self.dx = _up(t, self.x, np.float32)
+        self.out = self.dx if self.inplace else t.full((self.rows + 1, self.ld_out), 7.0, device="cuda")
+        self.d = dict(sample=None if self.sample is None else _up(t, np.frombuffer(bytes(self.sample), dtype=np.uint8), np.uint8),
+                      agent=i32(self.agent), list=i32(self.list), length=i32(self.length), bias_at=i32(self.bias_at),
+                      bias_token=_up(t, [b[0] for b in flat], np.int32) if flat else None,
+                      bias=_up(t, [b[1] for b in flat], np.float32) if flat else None, mask=i32(self.mask), mask_of=i32(self.mask_of))
+        self.how = A.AdjustHow(lists=self.lists, list_stride=self.stride, biases=len(flat), masks=self.masks, mask_stride=self.words,
+                               **{k: _at(v) for k, v in self.d.items()})
+        return self
+
+    def call(self, lib, stream=None):
+        assert lib.aotx_logits_adjust(ctypes.byref(self.how), p(self.dx), self.ld, self.rows, self.vocab, p(self.out), self.ld_out,
+                                      stream) == 0
+        return self
+
+    def want(self, r):
+        s, tokens = None, ()
+        if self.sample is not None:
+            a = r if self.agent is None else int(self.agent[r])
+            h = self.sample[r]
+            s = (h.presence_penalty, h.frequency_penalty, h.repeat_penalty, h.repeat_window)
+            if a < self.lists:
+                tokens = self.list[a, :min(int(self.length[a]), self.stride)].tolist()
+        b, e = (0, 0) if self.bias_at is None else (min(int(v), int(self.how.biases)) for v in self.bias_at[r:r + 2])
+        flat = [v for row in self.biases for v in row]
+        mask = None
+        if self.mask is not None:
+            of = r if self.mask_of is None else int(self.mask_of[r])
+            if of < self.masks:
+                mask = np.unpackbits(self.mask[of].view(np.uint8), bitorder="little")[:self.vocab].astype(bool)
+        z, far = O.adjust(self.x[r, :self.vocab], s, tokens, flat[b:e], mask)
+        return z, far, mask is not None and not mask.any()
+
+    def check(self, lib):
+        self.torch.cuda.synchronize()
+        got, faults = self.out.cpu().numpy(), 0
+        for r in range(self.rows):
+            z, far, none = self.want(r)
+            g = got[r, :self.vocab].astype(np.float64)
+            faults += none
+            same = (g == z) | (np.isnan(g) & np.isnan(z))
+            with np.errstate(invalid="ignore"):
+                assert (same | (np.abs(g - z) <= far)).all(), (r, np.flatnonzero(~(same | (np.abs(g - z) <= far)))[:5])
+            rest = self.x[r, self.vocab:] if self.inplace else 7.0
+            assert (got[r, self.vocab:] == rest).all()
+        assert self.inplace or (got[self.rows:] == 7.0).all()
+        assert lib.aotx_model_faulted() == faults
+        return faults
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 31), (3, 33), (2, 4095), (2, 4096), (1, 4097), (5, 32000), (64, 5003), (1, 128256),
+                                        (70, 1000)])
+@pytest.mark.parametrize("length,biases,masks", [(0, 0, 0), (1, 0, 0), (50, 0, 0), (3000, 0, 0), (0, 40, 0), (0, 0, 3), (700, 300, 2),
+                                                 (20, 1, 1)])
+@pytest.mark.parametrize("inplace", [True, False])
+def test_adjust(torch, lib, rows, vocab, length, biases, masks, inplace):
+    i = rows + vocab + length
+    c = Adjust(torch, i, rows, vocab, length, biases, masks, pad=((i % 3), i % 5) if i % 2 else (4 * (i % 3), 8), inplace=inplace,
+               by_agent=i % 4 != 0)
+    c.up().call(lib).check(lib)
+
+
+def test_adjust_long_lists(torch, lib):
+    Adjust(torch, 1, 3, 20000, 100000, 5000, 1).up().call(lib).check(lib)
+
+
+def test_adjust_masks_that_allow_nothing(torch, lib):
+    """All -inf, counted; bits past the vocabulary allow nothing; a mask of everything changes nothing."""
+    c = Adjust(torch, 2, 6, 4100, 30, 4, 4)
+    c.mask[0] = 0
+    c.mask[1] = 0
+    c.mask[1, 128] = 0xFFFFFFF0                         # tokens 4100 and on
+    c.mask[2] = 0xFFFFFFFF
+    c.mask[3] = 0
+    c.mask[3, 128] = 8                                  # the last token alone
+    c.mask_of = np.array([0, 1, 2, 3, 4, 0xFFFFFFFF], dtype=np.uint32)
+    assert c.up().call(lib).check(lib) == 2
+    assert np.isneginf(c.out[:2, :4100].cpu().numpy()).all() and not torch.isinf(c.out[2, :4100]).any()
+
+
+def test_adjust_tokens_and_slots_that_are_not_there(torch, lib):
+    c = Adjust(torch, 3, 5, 600, 80, 20)
+    c.list[:, ::3] = -1
+    c.list[:, 1::5] = 600
+    c.list[:, 2::7] = -2 ** 31
+    c.agent[0], c.agent[1] = 8, 0xFFFFFFFF
+    c.length[:] = (0, 1, 83, 84, 0xFFFFFFFF, 7, 80, 79)
+    c.agent[2:] = (0, 4, 3)
+    for i, r in enumerate(c.biases):
+        r[3], r[5] = (-1, 9.0), (600 + i, 9.0)
+    c.up().call(lib).check(lib)
+
+
+def test_adjust_the_last_bias_of_a_token_counts(torch, lib):
+    c = Adjust(torch, 4, 2, 300, 0, 1000)
+    c.up().call(lib).check(lib)
+    assert len({t for t, _ in c.biases[0]}) < 300
+
+
+@pytest.mark.parametrize("at", [[0, 5, 3, 20], [0xFFFFFFFF, 3, 7, 0xFFFFFFF0], [15, 15, 15, 15], [4, 2, 1, 0]])
+def test_adjust_bias_offsets_out_of_order_stay_in_bounds(torch, lib, at):
+    c = Adjust(torch, 5, 3, 300, 0, 5)
+    c.bias_at = np.array(at, dtype=np.uint32)
+    c.up().call(lib).check(lib)
+
+
+def test_adjust_inf_and_nan(torch, lib):
+    """They go their way through every step and reach no other token; masks take them out."""
+    c = Adjust(torch, 6, 3, 200, 60, 0, 1)
+    c.x[:, ::7], c.x[:, 3::11], c.x[:, 5::13] = np.inf, -np.inf, np.nan
+    c.x[:, 1] = -3.4e38
+    c.mask_of[:] = (0, 1, 1)
+    c.biases = [[(0, np.inf), (3, -np.inf), (8, np.nan), (9, np.inf), (10, -np.inf), (1, -3.4e38)]] * 3
+    c.bias_at = np.array([0, 6, 12, 18], dtype=np.uint32)
+    with np.errstate(over="ignore"):
+        c.up().call(lib)
+        torch.cuda.synchronize()
+        got = c.out.cpu().numpy()[:3, :200]
+        for r in range(3):
+            z, far, _ = c.want(r)
+            z = z.astype(np.float32).astype(np.float64)     # past fp32's end: infinite
+            assert np.array_equal(np.isnan(got[r]), np.isnan(z))
+            fine = np.isfinite(z)
+            assert np.array_equal(got[r][~fine & ~np.isnan(z)], z[~fine & ~np.isnan(z)].astype(np.float32))
+            assert (np.abs(got[r] - z)[fine] <= far[fine] + 2.0 ** -24 * np.abs(z[fine])).all()
+
+
+def test_adjust_in_a_graph(torch, lib):
+    """Captured, and replayed with other logits, lists and masks."""
+    c = Adjust(torch, 7, 6, 9000, 300, 12, 3).up().call(lib)
+    g = _graph(torch, lambda s: c.call(lib, s))
+    rng = np.random.default_rng(8)
+    for turn in range(3):
+        c.x = rng.normal(0, 3, c.x.shape).astype(np.float32)
+        c.list = rng.integers(0, 9000, c.list.shape).astype(np.int32)
+        c.length = rng.integers(0, 300, 8).astype(np.uint32)
+        c.mask_of = rng.integers(0, 5, 6).astype(np.uint32)
+        c.dx.copy_(torch.from_numpy(c.x))
+        for name in ("list", "length", "mask_of"):
+            c.d[name].copy_(torch.from_numpy(getattr(c, name).view(np.int32)))
+        c.out.fill_(7.0)
+        lib.aotx_model_forget()
+        torch.cuda.synchronize()
+        g.replay()
+        c.check(lib)
+        got = c.out.clone()
+        lib.aotx_model_forget()
+        c.out.fill_(7.0)
+        c.call(lib).check(lib)
+        assert torch.equal(got, c.out)
+
+
+def test_adjust_then_pick(torch, lib):
+    """Greedy and sampled tokens of adjusted rows are among those that the mask allows."""
+    c = Adjust(torch, 9, 32, 5000, 200, 20, 2, allow=0.01)
+    c.mask_of = (np.arange(32) % 2).astype(np.uint32)
+    c.ld_out = 5000
+    c.up().call(lib)
+    agent = _up(torch, np.arange(32), np.int32)
+    token = torch.zeros(32, dtype=torch.int32, device="cuda")
+    for temperature in (0.0, 1.5):
+        assert lib.aotx_pick(p(c.out), 32, 5000, p(agent), None, 0, 1.0, temperature, 11, p(token), None, None) == 0
+        got = token.cpu().numpy()
+        allowed = np.unpackbits(c.mask.view(np.uint8), axis=1, bitorder="little")
+        assert all(allowed[r % 2, t] for r, t in enumerate(got))
+        if temperature == 0:
+            assert np.array_equal(got, c.out[:32].argmax(1).cpu().numpy())
+
+
+# ---- a layer and an answer of them ---------------------------------------------------------------
+
+def test_layer_and_answer(torch, lib):
+    """A prompt of 37 and one of 5 rows through a whole layer to the picked token, then two single tokens
+    each, eager and as one captured graph, against the sequences in 64 bits."""
+    hidden, heads, kv, d, ffn, vocab, more = 256, 4, 2, 64, 416, 1003, 2
+    lens, slots = [37, 5], [6, 1]
+    rng = np.random.default_rng(90)
+    att = (heads + 2 * kv) * d
+    sizes = {"qkv": (att, hidden), "o": (hidden, heads * d), "gate": (ffn, hidden), "up": (ffn, hidden), "down": (hidden, ffn),
+             "head": (vocab, hidden)}
+    w, w64 = {}, {}
+    for i, (name, (n, k)) in enumerate(sizes.items()):
+        raw = quantize_q8((k ** -0.5 * normal(70 + i, 0, n * k)).astype(np.float32).reshape(n, k))
+        w64[name] = O.q8_values(raw, n, k)
+        packed = torch.zeros(lib.aotx_q8r_size(n, k), dtype=torch.uint8, device="cuda")
+        assert lib.aotx_q8_repack(p(_up(torch, raw.reshape(-1), np.uint8)), n, k, p(packed), None) == 0
+        w[name] = packed
+    bias = rng.normal(0, 0.5, att).astype(np.float32)
+    norms = {n: rng.normal(1, 0.1, hidden if n in "abc" else d).astype(np.float32) for n in "abcqk"}
+    dbias, dn = _up(torch, bias, np.float32), {n: _up(torch, v, np.float32) for n, v in norms.items()}
+    rope = A.RopeHow(theta=1e4, eps=EPS, rope_dim=32, pairs=0, axes=1, order=0, span=(ctypes.c_uint32 * 4)(16))
+    rows = sum(lens)
+    z = dict(device="cuda")
+    b = {n: torch.zeros(rows, s, **z) for n, s in (("resid", hidden), ("qkv", att), ("logits", vocab), ("out", vocab))}
+    b |= {n: torch.zeros(rows, s, dtype=torch.float16, **z) for n, s in (("x", hidden), ("q", heads * d), ("a", heads * d), ("f", ffn))}
+    rpos, ragent = (torch.zeros(rows, dtype=torch.int32, **z) for _ in range(2))
+    work = torch.zeros(max(lib.aotx_q8_linear_work(n, k, m, g) for n, k in sizes.values() for m in (2, rows) for g in (0, 1)),
+                       dtype=torch.uint8, **z)
+    mask = rng.uniform(0, 1, 1024) < 0.7
+    sample = (A.ModelHow * 2)(*[A.neutral_how(presence_penalty=0.4, frequency_penalty=0.1, repeat_penalty=1.2, repeat_window=16)] * 2)
+    tokens = rng.integers(0, vocab, (64, 40)).astype(np.int32)
+    length = np.zeros(64, dtype=np.uint32)
+    for s, n in zip(slots, lens):
+        length[s] = n
+    dsample, dtokens, dlength = (_up(torch, np.frombuffer(bytes(sample), dtype=np.uint8), np.uint8), _up(torch, tokens, np.int32),
+                                 _up(torch, length.view(np.int32), np.int32))
+    dmask = _up(torch, np.packbits(mask, bitorder="little").view(np.int32), np.int32)
+    dzero = _up(torch, [0, 0], np.int32)
+    agent = _up(torch, slots, np.int32)
+    adjust = A.AdjustHow(sample=_at(dsample), agent=_at(agent), list=_at(dtokens), length=_at(dlength), lists=64, list_stride=40,
+                         mask=_at(dmask), mask_of=_at(dzero), masks=1, mask_stride=32)
+    token = torch.zeros(2, dtype=torch.int32, **z)
+
+    def linear(name, x, m, y, s, up=None, bias=None, resid=None, act=0, half=0):
+        n, k = sizes[name]
+        how = A.LinearHow(w=_at(w[name]), up=_at(w[up]) if up else None, bias=_at(bias), resid=_at(resid), n=n, k=k, ldx=k, ldy=n,
+                          ldr=n, act=act, out=half, packed=1)
+        assert lib.aotx_q8_linear(ctypes.byref(how), p(x), m, p(y), p(work), work.numel(), s) == 0
+
+    def norm(n, m, s):
+        assert lib.aotx_norm_rows(p(b["resid"]), hidden, p(dn[n]), m, hidden, EPS, p(b["x"]), s) == 0
+
+    def step(m, offset, pos, s=None):
+        norm("a", m, s)
+        linear("qkv", b["x"], m, b["qkv"], s, bias=dbias)
+        assert lib.aotx_kv_append(p(b["qkv"]), att, p(dn["q"]), p(dn["k"]), ctypes.byref(rope), None, 1.0, None, offset, p(pos),
+                                  p(agent), 2, m, heads, kv, d, 0, 1, lib.aotx_kv_table_device(), p(b["q"]), p(rpos), p(ragent), s) == 0
+        assert lib.aotx_attend_paged(p(b["q"]), p(rpos), p(ragent), m, heads, kv, d, 0, 1, p(b["a"]), s) == 0
+        linear("o", b["a"], m, b["resid"], s, resid=b["resid"])
+        norm("b", m, s)
+        linear("gate", b["x"], m, b["f"], s, up="up", act=1, half=1)
+        linear("down", b["f"], m, b["resid"], s, resid=b["resid"])
+        norm("c", m, s)
+        linear("head", b["x"], m, b["logits"], s)
+
+    def answer(s=None):
+        """Of two single rows."""
+        assert lib.aotx_logits_adjust(ctypes.byref(adjust), p(b["logits"]), vocab, 2, vocab, p(b["out"]), vocab, s) == 0
+        assert lib.aotx_pick(p(b["out"]), 2, vocab, p(agent), None, 0, 1.0, 0.0, 0, p(token), None, s) == 0
+
+    def whole(h):
+        """A sequence's rows in 64 bits: (residual, logits)."""
+        n = len(h)
+        x = O.norm_rows(h, norms["a"], EPS) @ w64["qkv"].T + bias
+        x = x.reshape(n, -1, d)
+        where = np.arange(n)[:, None]
+        q, k = (H.rope_axes(part, norms[c], EPS, where, 1e4, 32, True, [16], 0)
+                for c, part in (("q", x[:, :heads]), ("k", x[:, heads:heads + kv])))
+        v = x[:, heads + kv:]
+        out = np.zeros((n, heads, d))
+        for t in range(n):
+            for i in range(heads):
+                s = k[:t + 1, i // 2] @ q[t, i] / np.sqrt(d)
+                e = np.exp(s - s.max())
+                out[t, i] = (e / e.sum()) @ v[:t + 1, i // 2]
+        h = h + out.reshape(n, -1) @ w64["o"].T
+        x = O.norm_rows(h, norms["b"], EPS)
+        h = h + (O.act(x @ w64["gate"].T, 1)[0] * (x @ w64["up"].T)) @ w64["down"].T
+        return h, O.norm_rows(h, norms["c"], EPS) @ w64["head"].T
+
+    m = A.KvMap()
+    m.limit = 8
+    assert lib.aotx_kv_open(ctypes.byref(m)) == 0
+    try:
+        for s in slots:
+            assert lib.aotx_kv_request(s, layout_pages(40, 1, kv, d)) == 1
+        assert lib.aotx_kv_serve(ctypes.byref(m), None) == 2
+        hs = [rng.normal(0, 1, (n + more, hidden)).astype(np.float32) for n in lens]
+        want = [whole(h.astype(np.float64)) for h in hs]
+        offset = _up(torch, [0, 37, 42], np.int32)
+        pos = _up(torch, [0, 0], np.int32)
+        b["resid"].copy_(torch.from_numpy(np.concatenate([h[:n] for h, n in zip(hs, lens)])))
+        step(rows, p(offset), pos)
+        torch.cuda.synchronize()
+
+        def near(got, want):
+            rms = np.sqrt((want ** 2).mean())
+            err = np.abs(got - want) / np.maximum(np.abs(want), rms)
+            assert err.max() < 1e-2, err.max()             # fp16 between the operators: the framework's 1e-2
+        for i, (lo, hi) in enumerate(((0, 37), (37, 42))):
+            near(b["resid"][lo:hi].cpu().numpy(), want[i][0][:lens[i]])
+            near(b["logits"][lo:hi].cpu().numpy(), want[i][1][:lens[i]])
+        graph = None
+        for t in range(more):
+            pos.copy_(torch.tensor([lens[0] + t, lens[1] + t], dtype=torch.int32))
+            first = torch.from_numpy(np.stack([hs[0][37 + t], hs[1][5 + t]])).cuda()
+            got = []
+            for eager in (True, False):
+                if not eager and graph is None:
+                    graph = _graph(torch, lambda s: (step(2, None, pos, s), answer(s)))
+                b["resid"][:2] = first
+                b["out"].zero_(), token.zero_()
+                torch.cuda.synchronize()
+                if eager:
+                    step(2, None, pos)
+                    answer()
+                else:
+                    graph.replay()
+                torch.cuda.synchronize()
+                got.append([v.clone() for v in (b["resid"][:2], b["logits"][:2], b["out"][:2], token)])
+            assert all(torch.equal(x, y) for x, y in zip(*got))
+            for i in range(2):
+                near(got[0][0][i].cpu().numpy(), want[i][0][lens[i] + t])
+                near(got[0][1][i].cpu().numpy(), want[i][1][lens[i] + t])
+                logits = got[0][1][i].cpu().numpy()
+                zz, far = O.adjust(logits, (np.float32(0.4), np.float32(0.1), np.float32(1.2), 16),
+                                   tokens[slots[i], :lens[i]].tolist(), mask=mask[:vocab])
+                out = got[0][2][i].cpu().numpy().astype(np.float64)
+                assert ((out == zz) | (np.abs(out - zz) <= far)).all()
+                assert int(got[0][3][i]) == int(out.argmax())
+        assert lib.aotx_model_faulted() == 0
+    finally:
+        lib.aotx_kv_close(ctypes.byref(m))
