@@ -1262,17 +1262,52 @@ static bool aotx_linear_sizes(unsigned int n, unsigned int k, unsigned int m)
     return n != 0u && n <= AOTX_LINEAR_ROWS_MAX && k != 0u && k % 32u == 0u && k <= (1u << 18) && m <= (1u << 20);
 }
 
+/* The rows of a call's next pass where linear.hip does not take them. */
+static unsigned int aotx_linear_rows(unsigned int left) { return left < AOTX_RGEMM_ROWS ? left : AOTX_RGEMM_ROWS; }
+
+/* Whether linear.hip takes the call: where its time is below that of passes of up to 512 rows, which is taken as what
+ * those measured, in ns: a quad of the GEMM 1450 with a workgroup on each CU and 1150 for each of several (over
+ * the file's layout 1950, 1900), of the others 200 and 250, and 8000 for sums of splits. (2048 rows of the gated 14336 x 4096: 443
+ * us there, 579 in passes; 512 rows 115 and 145; 512 of 4096 square 43 and 36; 1024 of 1024 x 4096 43 and 42.) */
+static bool aotx_linear_many(aotx_lgemm_plan *p, unsigned int n, unsigned int k, unsigned int m, bool gated, bool file)
+{
+    if (m <= 64u) return false;
+    unsigned long long passes = 0ull;
+    const unsigned int full = m / AOTX_RGEMM_ROWS;
+    for (unsigned int rows : {full != 0u ? AOTX_RGEMM_ROWS : 0u, m % AOTX_RGEMM_ROWS}) {
+        if (rows == 0u) continue;
+        aotx_rgemv_args a;
+        if (aotx_linear_plan(&a, &a, gated ? &a : nullptr, n, k, rows) != 0) return false;
+        const unsigned int wgs = a.groups * a.splits * (a.gemm ? (rows + RGM_MB - 1u) / RGM_MB : a.passes > 1u ? a.passes : 1u);
+        const unsigned int each = (wgs + 255u) / 256u;
+        const unsigned int one = file ? 1950u : 1450u, more = file ? 1900u : 1150u;
+        passes += (rows == AOTX_RGEMM_ROWS ? full : 1u)
+                * ((a.gemm ? 4000ull : 6000ull)
+                   + (unsigned long long)a.qps * (a.gemm ? (each <= 1u ? one : more * each) : (each <= 1u ? 200u : 250u * each))
+                   + (a.splits > 1u ? 8000u : 0u));
+    }
+    return aotx_lgemm_choose(p, n, k, m, gated, file) < passes;
+}
+
 extern "C" unsigned long long aotx_q8_linear_work(unsigned int n, unsigned int k, unsigned int m, unsigned int gated)
 {
     if (!aotx_linear_sizes(n, k, m)) return 0ull;
     size_t most = 0u;
-    /* the full passes and the last one */
-    for (unsigned int left : {m < AOTX_RGEMM_ROWS ? m : AOTX_RGEMM_ROWS, m % AOTX_RGEMM_ROWS}) {
-        aotx_rgemv_args a;
-        if (left == 0u) continue;
-        if (aotx_linear_plan(&a, &a, gated != 0u ? &a : nullptr, n, k, left) != 0) return 0ull;
-        const size_t bytes = aotx_rgemv_partial_bytes(a);
-        most = bytes > most ? bytes : most;
+    /* over either layout: all rows at once, or the full passes and the last one */
+    for (const bool file : {false, true}) {
+        aotx_lgemm_plan g;
+        if (aotx_linear_many(&g, n, k, m, gated != 0u, file)) {
+            const size_t bytes = aotx_lgemm_partial_bytes(g);
+            most = bytes > most ? bytes : most;
+            continue;
+        }
+        for (unsigned int rows : {aotx_linear_rows(m), m % AOTX_RGEMM_ROWS}) {
+            aotx_rgemv_args a;
+            if (rows == 0u) continue;
+            if (aotx_linear_plan(&a, &a, gated != 0u ? &a : nullptr, n, k, rows) != 0) return 0ull;
+            const size_t bytes = aotx_rgemv_partial_bytes(a);
+            most = bytes > most ? bytes : most;
+        }
     }
     return AOTX_LINEAR_ZERO + most;
 }
@@ -1324,8 +1359,10 @@ extern "C" int aotx_q8_linear(const aotx_linear_how *how, const void *x, unsigne
     e.ldr = how->ldr;
     e.act = how->act;
     e.half = how->out == AOTX_LINEAR_F16;
+    aotx_lgemm_plan g;
+    const bool many = aotx_linear_many(&g, n, k, m, how->up != nullptr, !how->packed);
     for (unsigned int m0 = 0u, rows = 0u; m0 < m; m0 += rows) {
-        rows = m - m0 < AOTX_RGEMM_ROWS ? m - m0 : AOTX_RGEMM_ROWS;
+        rows = many ? m : aotx_linear_rows(m - m0);
         aotx_rgemv_args a;
         if (aotx_linear_plan(&a, how->w, how->up, n, k, rows) != 0) return 1;
         if (!how->packed) aotx_rgemv_file(&a);
@@ -1333,11 +1370,13 @@ extern "C" int aotx_q8_linear(const aotx_linear_how *how, const void *x, unsigne
         a.x = (const unsigned short *)x;
         a.ldx = how->ldx;
         a.m0 = m0;
+        a.m = rows;
         a.y = y;
         a.ldy = how->ldy;
         a.count = (unsigned int *)work;
         a.partial = (float *)((unsigned char *)work + AOTX_LINEAR_ZERO);
-        aotx_linear_launch(a, e, aotx_stream(stream));
+        if (many) aotx_lgemm_launch(g, a, e, aotx_stream(stream));
+        else aotx_linear_launch(a, e, aotx_stream(stream));
     }
     return 0;
 }

@@ -62,7 +62,7 @@ def test_linear_no_rows_is_nothing(lib):
 
 
 def test_linear_workspace(lib):
-    """As much for m rows as for any call of them; 0 for refused sizes; a call with a byte less is refused."""
+    """0 for refused sizes, bounded for the others; a call with a byte less is refused."""
     work = lib.aotx_q8_linear_work
     for bad in ((0, 64, 1, 0), (100, 48, 1, 0), (100, 0, 1, 0), ((1 << 18) + 1, 64, 1, 0), (100, (1 << 18) + 32, 1, 0),
                 (100, 64, (1 << 20) + 1, 0)):
@@ -77,8 +77,6 @@ def test_linear_workspace(lib):
                 how = A.LinearHow(**{**LINEAR, "n": n, "k": k, "ldx": k, "ldy": n, "ldr": n, "up": A256 if gated else None,
                                      "up_bias": None})
                 assert lib.aotx_q8_linear(ctypes.byref(how), *{**LCALL, "m": m, "work_bytes": need - 1}.values()) == 1
-            # whole passes of 512 rows, and the last one's
-            assert work(n, k, 1024 + 100, gated) == max(work(n, k, 512, gated), work(n, k, 100, gated))
 
 
 NORM = dict(x=A256, stride=64, w=A256, tokens=3, width=64, eps=1e-6, out=A256, stream=None)
