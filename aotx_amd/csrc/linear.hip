@@ -286,9 +286,11 @@ __global__ __launch_bounds__(512, 2) void aotx_linear_gemm(aotx_rgemv_args a, ao
     /* The sums go through LDS, half of the batch rows at a time: a loop of little code then writes whole lines of y
      * (from the registers, where every sum has code of its own, the activations alone would be 20000
      * instructions). Quad u of row m is in place u ^ (m % 16) of the row's kilobyte. */
-    const unsigned int units = gated ? 32u : 64u;            /* four outputs each */
-    const bool v4 = (a.ldy & 3u) == 0u && ((uintptr_t)a.y & (e.half ? 7u : 15u)) == 0u;
-    const bool r4 = (e.ldr & 3u) == 0u && ((uintptr_t)e.resid & 15u) == 0u;
+    const unsigned int shift_u = gated ? 5u : 6u, units = 1u << shift_u;        /* four outputs each */
+    /* Fours of y and resid at any alignment, as the memory takes such accesses whole (the outputs one at a time take
+     * 1511 rows of 14029 x 256 with a residual from 88 to 109 us, 700 of 9001 x 1024 in halves from 37 to 43). */
+    typedef float quad_f __attribute__((ext_vector_type(4), aligned(4)));
+    typedef unsigned short quad_h __attribute__((ext_vector_type(4), aligned(2)));
     const auto sums = [&](unsigned int row, unsigned int unit) {
         return (rg_f4 *)((row < BM / 4u ? x0 : x1) + (row % (BM / 4u)) * 1024u + ((unit ^ (row & 15u)) * 16u));
     };
@@ -302,22 +304,19 @@ __global__ __launch_bounds__(512, 2) void aotx_linear_gemm(aotx_rgemv_args a, ao
                 for (int c = 0; c < CB; ++c) *sums(16u * (unsigned int)c + r, tile[j] * 4u + g) = acc[j][c];
         }
         __syncthreads();
+        const unsigned int mb = m0 + h * (BM / 2u), nb = group * units * 4u;
+        const unsigned int left = a.m > mb ? a.m - mb : 0u, mend = left < BM / 2u ? left : BM / 2u;
         constexpr unsigned int U = 4u;
 #pragma unroll 1
-        for (unsigned int i0 = tid; i0 < units * (BM / 2u); i0 += 512u * U) {
-            rg_f4 v[U], up[U], res[U];
+        for (unsigned int i0 = tid; i0 < units * mend; i0 += 512u * U) {
+            rg_f4 res[U];
 #pragma unroll
             for (unsigned int u = 0u; u < U; ++u) {
-                const unsigned int i = i0 + 512u * u, unit = i % units, row = i / units;
-                const unsigned int n0 = group * units * 4u + unit * 4u;
-                const unsigned long long m = m0 + h * (BM / 2u) + row;
+                const unsigned int i = i0 + 512u * u, unit = i & (units - 1u), row = i >> shift_u, n0 = nb + unit * 4u;
                 res[u] = (rg_f4){0.0f, 0.0f, 0.0f, 0.0f};
-                if (row >= BM / 2u) continue;
-                v[u] = *sums(row, unit);
-                if (gated) up[u] = *sums(row, unit + 32u);
-                if (e.resid == nullptr || m >= a.m) continue;
-                const float *from = e.resid + m * e.ldr + n0;
-                if (r4 && n0 + 4u <= a.n) res[u] = *(const rg_f4 *)from;
+                if (e.resid == nullptr || row >= mend || n0 >= a.n) continue;
+                const float *from = e.resid + (unsigned long long)(mb + row) * e.ldr + n0;
+                if (n0 + 4u <= a.n) res[u] = *(const quad_f *)from;
                 else
 #pragma unroll
                     for (unsigned int k = 0u; k < 4u; ++k)
@@ -325,37 +324,33 @@ __global__ __launch_bounds__(512, 2) void aotx_linear_gemm(aotx_rgemv_args a, ao
             }
 #pragma unroll
             for (unsigned int u = 0u; u < U; ++u) {
-                const unsigned int i = i0 + 512u * u, unit = i % units, row = i / units;
-                const unsigned int n0 = group * units * 4u + unit * 4u;
-                const unsigned long long m = m0 + h * (BM / 2u) + row;
-                if (row >= BM / 2u || m >= a.m || n0 >= a.n) continue;
+                const unsigned int i = i0 + 512u * u, unit = i & (units - 1u), row = i >> shift_u, n0 = nb + unit * 4u;
+                if (row >= mend || n0 >= a.n) continue;
+                rg_f4 v = *sums(row, unit), up = gated ? *sums(row, unit + 32u) : v;
 #pragma unroll
                 for (unsigned int k = 0u; k < 4u; ++k) {
                     const bool in = n0 + k < a.n;
-                    float one = v[u][k];
+                    float one = v[k];
                     if (e.bias != nullptr && in) one += e.bias[n0 + k];
                     one = rg_act(one, e.act);
-                    if (gated) one *= up[u][k] + (e.up_bias != nullptr && in ? e.up_bias[n0 + k] : 0.0f);
-                    v[u][k] = one + res[u][k];
+                    if (gated) one *= up[k] + (e.up_bias != nullptr && in ? e.up_bias[n0 + k] : 0.0f);
+                    v[k] = one + res[u][k];
                 }
-                if (e.half) {
-                    unsigned short *to = (unsigned short *)a.y + m * a.ldy + n0;
-                    typedef unsigned int u2 __attribute__((ext_vector_type(2)));
-                    unsigned int half[4];
+                const unsigned long long to = (unsigned long long)(mb + row) * a.ldy + n0;
+                quad_h half = {0, 0, 0, 0};
+                if (e.half)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) half[k] = aotx_f2h(v[u][k]);
-                    if (v4 && n0 + 4u <= a.n) *(u2 *)to = (u2){half[0] | (half[1] << 16), half[2] | (half[3] << 16)};
-                    else
-#pragma unroll
-                        for (unsigned int k = 0u; k < 4u; ++k)
-                            if (n0 + k < a.n) to[k] = (unsigned short)half[k];
+                    for (int k = 0; k < 4; ++k) half[k] = aotx_f2h(v[k]);
+                if (n0 + 4u <= a.n) {
+                    if (e.half) *(quad_h *)((unsigned short *)a.y + to) = half;
+                    else *(quad_f *)((float *)a.y + to) = v;
                 } else {
-                    float *to = (float *)a.y + m * a.ldy + n0;
-                    if (v4 && n0 + 4u <= a.n) *(rg_f4 *)to = v[u];
-                    else
 #pragma unroll
-                        for (unsigned int k = 0u; k < 4u; ++k)
-                            if (n0 + k < a.n) to[k] = v[u][k];
+                    for (unsigned int k = 0u; k < 4u; ++k) {
+                        if (n0 + k >= a.n) continue;
+                        if (e.half) ((unsigned short *)a.y)[to + k] = half[k];
+                        else ((float *)a.y)[to + k] = v[k];
+                    }
                 }
             }
         }

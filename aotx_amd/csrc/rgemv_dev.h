@@ -674,28 +674,42 @@ static __device__ __forceinline__ float rg_act(float v, unsigned int act)
     return v;
 }
 
+/* Eight outputs of a thread at a time, neighbours of the next thread's: their residuals are under way together. */
 template <int MT, int NT>
 static __device__ __forceinline__ void rg_linear(const aotx_rgemv_args &a, const aotx_linear_epi &e, const float *out,
                                                  unsigned int group, unsigned int rt, unsigned int mrows)
 {
+    constexpr unsigned int U = 8u;
     const bool gated = a.epi == AOTX_EPI_SWIGLU;
-    const unsigned int gr = gated ? rt * 8u : rt * 16u;
-    for (unsigned int idx = threadIdx.x; idx < gr * MT; idx += NT) {
-        const unsigned int row = idx % gr, mm = idx / gr;
-        const unsigned int v = rg_vrow(a, group, row / 16u, row % 16u, rt);
-        if (mm >= mrows || v >= a.n) continue;
-        float val = out[rg_o<MT>(row, mm)];
-        if (e.bias != nullptr) val += e.bias[v];
-        val = rg_act(val, e.act);
-        if (gated) {
-            float up = out[rg_o<MT>(row + gr, mm)];
-            if (e.up_bias != nullptr) up += e.up_bias[v];
-            val *= up;
+    const unsigned int shift = (unsigned int)__builtin_ctz(rt) + (gated ? 3u : 4u), gr = 1u << shift;      /* rt is a power of two */
+    const unsigned int total = gr * (mrows < (unsigned int)MT ? mrows : (unsigned int)MT);
+    for (unsigned int base = threadIdx.x; base < total; base += NT * U) {
+        float res[U];
+        if (e.resid != nullptr)
+#pragma unroll
+            for (unsigned int u = 0u; u < U; ++u) {
+                const unsigned int idx = base + u * NT < total ? base + u * NT : base, row = idx & (gr - 1u);
+                const unsigned int v = rg_vrow(a, group, row / 16u, row % 16u, rt);
+                res[u] = e.resid[(unsigned long long)(a.m0 + (idx >> shift)) * e.ldr + (v < a.n ? v : 0u)];
+            }
+#pragma unroll
+        for (unsigned int u = 0u; u < U; ++u) {
+            const unsigned int idx = base + u * NT, row = idx & (gr - 1u), mm = idx >> shift;
+            const unsigned int v = rg_vrow(a, group, row / 16u, row % 16u, rt);
+            if (idx >= total || v >= a.n) continue;
+            float val = out[rg_o<MT>(row, mm)];
+            if (e.bias != nullptr) val += e.bias[v];
+            val = rg_act(val, e.act);
+            if (gated) {
+                float up = out[rg_o<MT>(row + gr, mm)];
+                if (e.up_bias != nullptr) up += e.up_bias[v];
+                val *= up;
+            }
+            if (e.resid != nullptr) val += res[u];
+            const unsigned long long i = a.m0 + mm;
+            if (e.half) ((unsigned short *)a.y)[i * a.ldy + v] = aotx_f2h(val);
+            else ((float *)a.y)[i * a.ldy + v] = val;
         }
-        const unsigned long long i = a.m0 + mm;
-        if (e.resid != nullptr) val += e.resid[i * e.ldr + v];
-        if (e.half) ((unsigned short *)a.y)[i * a.ldy + v] = aotx_f2h(val);
-        else ((float *)a.y)[i * a.ldy + v] = val;
     }
 }
 

@@ -106,18 +106,18 @@ class Linear:
                                        self.need, stream) == 0
         return self
 
-    def want(self):
+    def want(self, cols=slice(None)):
         x = self.x[:, :self.k].astype(np.float64)
-        b = [None if v is None else v.astype(np.float64) for v in self.bias] + [None]
-        r = None if self.resid is None else self.resid[:, :self.n].astype(np.float64)
+        b = [None if v is None else v[cols].astype(np.float64) for v in self.bias] + [None]
+        r = None if self.resid is None else self.resid[:, :self.n][:, cols].astype(np.float64)
         with np.errstate(invalid="ignore", over="ignore"):
-            return O.linear(x, self.w[0], self.w[1] if self.gated else None, b[0], b[1], r, self.act)
+            return O.linear(x, self.w[0][cols], self.w[1][cols] if self.gated else None, b[0], b[1], r, self.act)
 
-    def check(self, untouched=True):
+    def check(self, untouched=True, cols=slice(None)):
         self.torch.cuda.synchronize()
         y = self.y.cpu().numpy().astype(np.float64)
-        want, far = self.want()
-        got = y[:self.m, :self.n]
+        want, far = self.want(cols)
+        got = y[:self.m, :self.n][:, cols]
         off = np.abs(got - want) - O.rounded(far, want, self.half)
         assert off.max() <= 0, (off.max(), np.unravel_index(off.argmax(), off.shape))
         if untouched:
@@ -140,6 +140,29 @@ def test_linear_sizes(torch, lib, m, n, k, packed, gated):
     i = m + n + k
     Linear(torch, lib, i, m, n, k, gated, 1 if gated else i % 5, i % 2 == 0, "apart" if i % 3 == 0 else None, i % 4 < 2,
            packed, (8 * (i % 3), i % 5, i % 7)).up().call().check()
+
+
+# rows enough for tiles of all of them: tiles of 256, 192 and 128 batch rows, one round of them and more, with
+# the last ones whole, in two and in three; less than one quad of columns, whole quads and a rest
+MANY = [(677, 1350, 1184), (630, 1044, 1440), (2023, 2056, 32), (2294, 2096, 160), (2220, 241, 4032), (2063, 3109, 2336),
+        (2275, 2326, 96), (1996, 3178, 512), (2168, 3133, 2592), (768, 4096, 4096), (4097, 513, 1056), (20000, 300, 64)]
+
+
+@pytest.mark.parametrize("m,n,k", MANY)
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("gated", [True, False])
+def test_linear_many_rows(torch, lib, m, n, k, packed, gated):
+    i = m + n + k
+    c = Linear(torch, lib, i, m, n, k, gated, 1 if gated else i % 5, i % 3 == 0,
+               ("inplace", "apart", None)[(i + packed) % 3], (i + packed) % 3 != 0 and i % 2 == 0, packed,
+               (8 * (i % 3), i % 5, i % 7 if (i + packed) % 3 else i % 5)).up().call()
+    c.check(cols=np.r_[0:n - 20:5, n - 20:n])
+    first = c.y.clone()
+    if not c.inplace:
+        c.y.fill_(7.0)
+        c.call()
+        torch.cuda.synchronize()
+        assert torch.equal(first, c.y)
 
 
 @pytest.mark.parametrize("act", [0, 1, 2, 3, 4])
@@ -178,7 +201,7 @@ def test_linear_all_blocks_one_side(torch, lib):
 
 @pytest.mark.parametrize("packed", [True, False])
 @pytest.mark.parametrize("m,n,k", [(3, 40, 1024), (6, 4100, 512), (20, 40, 4128), (40, 3000, 256), (64, 40, 1024),
-                                   (200, 400, 1024), (300, 4000, 160), (600, 520, 416)])
+                                   (200, 400, 1024), (300, 4000, 160), (600, 520, 416), (677, 1350, 1184)])
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
 def test_linear_inf_and_nan_stay_in_their_row(torch, lib, packed, m, n, k, bad):
     """In x: its row alone (an infinity gives infinities by the weights' signs); in a scale: its column."""
@@ -227,7 +250,7 @@ def test_linear_one_workspace_for_all_sizes(torch, lib):
     """Calls of any sizes one after another on one workspace."""
     calls = [Linear(torch, lib, i, m, n, k, g, g, half=h).up() for i, (m, n, k, g, h) in enumerate(
         [(1, 4096, 4096, 0, 0), (32, 300, 14336, 1, 1), (512, 96, 4096, 0, 0), (2, 70000, 12800, 0, 1), (64, 2048, 1024, 1, 0),
-         (8, 64, 4096, 0, 0), (700, 130, 2048, 0, 1)])]
+         (8, 64, 4096, 0, 0), (700, 130, 2048, 0, 1), (677, 1350, 1184, 0, 1), (630, 1044, 1440, 0, 0)])]
     work = torch.full((max(c.need for c in calls),), 0xFF, dtype=torch.uint8, device="cuda")
     work[:A.AOTX_LINEAR_ZERO] = 0
     for turn in range(2):
@@ -239,7 +262,8 @@ def test_linear_one_workspace_for_all_sizes(torch, lib):
     assert not work[:A.AOTX_LINEAR_ZERO].any()
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 500, 4096), (20, 200, 4096), (64, 256, 2048), (300, 256, 4096), (600, 128, 1024)])
+@pytest.mark.parametrize("m,n,k", [(1, 500, 4096), (20, 200, 4096), (64, 256, 2048), (300, 256, 4096), (600, 128, 1024),
+                                   (630, 1044, 1440)])
 def test_linear_in_graphs(torch, lib, m, n, k):
     """Two captured calls that share a workspace, replayed in turn with other rows, with eager calls between."""
     a, b = (Linear(torch, lib, 20 + i, m, n, k, i == 1, i, True, half=i == 1).up() for i in range(2))
@@ -263,10 +287,10 @@ def test_linear_in_graphs(torch, lib, m, n, k):
             assert torch.equal(got, c.y), turn
 
 
-@pytest.mark.parametrize("m", [1, 24, 64, 300])
-def test_linear_on_two_streams(torch, lib, m):
+@pytest.mark.parametrize("m,n,k", [(1, 512, 8192), (24, 512, 8192), (64, 512, 8192), (300, 512, 8192), (677, 1350, 1184)])
+def test_linear_on_two_streams(torch, lib, m, n, k):
     """At once, each with its own workspace."""
-    calls = [Linear(torch, lib, 30 + i, m, 512, 8192, half=True).up() for i in range(2)]
+    calls = [Linear(torch, lib, 30 + i, m, n, k, half=True).up() for i in range(2)]
     streams = [torch.cuda.Stream() for _ in calls]
     torch.cuda.synchronize()
     for _ in range(5):
