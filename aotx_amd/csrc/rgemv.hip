@@ -843,9 +843,9 @@ static int aotx_rgemv_plan_n(aotx_rgemv_args *a, const void *const *w, const uns
          * a short k against the GEMM). The larger forms fill the chip with such a matrix only by
          * cutting k into many short splits: 128 rows of 2048 square take 7.0 us against 19.0 by
          * the GEMM, 512 of 512 x 1024 6.9 against 16.1, 400 of 100 x 14336 13.5 against 42.5 (28.9
-         * unsplit), 128 of 4096 x 3072 in two rounds 15.8 against 23.4; 64 rows of 4096 x 2048 7.7
+         * unsplit), 128 of 4096 x 3584 in two rounds 18.6 against 25.4; 64 rows of 4096 x 2048 7.7
          * against 11.3 by the 64-row form, of 1024 x 8064 10.7 against 16.2, but in two rounds
-         * (6144 x 3072) 15.7 against 13.8. */
+         * (6144 x 2560) 15.1 against 13.4. */
         const unsigned int passes = (mt + 31u) / 32u;
         const unsigned int pairs = epi == AOTX_EPI_SWIGLU ? (unsigned int)aotx_q8r_tiles(rows[0])
                                                           : (tiles + 1u) / 2u;
