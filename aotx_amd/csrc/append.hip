@@ -30,7 +30,9 @@ static __device__ __forceinline__ void aotx_norm_put(const aotx_norm_rows_args &
     *(aotx_u16x8 *)(p.out + (unsigned long long)t * p.width + i) = y;
 }
 
-/* A workgroup a row, N times 2048 values. */
+/* A workgroup a row, N times 2048 values: all loads are under way before the first square, and a row is read
+ * once. The memory bounds it: 8192 rows of 4096 take 37 us (201 MB at 5.4 TB/s, a part of x comes from the last
+ * level's cache), 64 rows 2.6, of 16384 4.5. */
 template <int N>
 __global__ __launch_bounds__(256) void aotx_norm_rows_kernel(aotx_norm_rows_args p)
 {
@@ -87,7 +89,11 @@ extern "C" int aotx_norm_rows(const float *x, unsigned int stride, const float *
 /* ---------------------------------------------------------------------------------------
  * Rows into the pages. A workgroup takes one token: its sequence, the place of its row in the
  * pages and its pairs' sines once, then all heads, a lane 8 values of one, which are 4 whole pairs (or
- * 8 values past rope_dim); the angle as in aotx_rope_axes.
+ * 8 values past rope_dim); the angle as in aotx_rope_axes. Where there are fewer tokens than CUs, a token has
+ * a workgroup for every 2048 of its values, which takes them in one pass and makes the sines again: 32 and 8 heads of
+ * 128, 64 sequences of one row with head norms, take 3.7 us so and 5.1 by a workgroup each, one row 2.9 and 3.4. Past that
+ * the memory bounds it: 512 rows 7.4 us, 8192 rows 59.4 (302 MB: 5.1 TB/s, as a copy). Loads for four
+ * heads ahead take 512 rows down by 0.2 and 640 up by 0.5: left out.
  * ------------------------------------------------------------------------------------- */
 struct aotx_append_args {
     const float *qkv, *q_norm, *k_norm, *factor;
@@ -132,23 +138,23 @@ __global__ __launch_bounds__(256) void aotx_append_kernel(aotx_append_args p)
                                  + (t - seq.start);
     const unsigned int total = p.heads + 2u * p.kv_heads;
     if (seq.refused) {
-        if (threadIdx.x == 0u) {
+        if (threadIdx.x == 0u && blockIdx.y == 0u) {
             if (t == seq.start) atomicAdd(p.seqs.faults, 1u);
             if (p.row_pos != nullptr) {
                 p.row_pos[t] = 0u;
                 p.row_agent[t] = AOTX_SLOTS;
             }
         }
-        for (unsigned int j = threadIdx.x; j < p.heads * L; j += 256u)
+        for (unsigned int j = blockIdx.y * 256u + threadIdx.x; j < p.heads * L; j += gridDim.y * 256u)
             *(aotx_u16x8 *)(p.q + ((unsigned long long)t * p.heads * L + j) * 8u) = (aotx_u16x8)(0);
         return;
     }
     unsigned short *at = aotx_append_at(p, seq.slot, pos);
-    if (threadIdx.x == 0u) {
+    if (threadIdx.x == 0u && blockIdx.y == 0u) {
         if (at == nullptr) atomicAdd(p.seqs.faults, 1u);
         if (p.row_pos != nullptr) {
             p.row_pos[t] = (unsigned int)pos;
-            p.row_agent[t] = seq.slot;
+            p.row_agent[t] = pos >> 32 == 0ull ? seq.slot : AOTX_SLOTS;   /* 32 bits hold the place, or it is none */
         }
     }
     if (threadIdx.x < half) {
@@ -175,7 +181,7 @@ __global__ __launch_bounds__(256) void aotx_append_kernel(aotx_append_args p)
         s[e] = turns ? sn[4u * j + e] : 0.0f;
     }
     const float *row = p.qkv + (unsigned long long)t * p.stride;
-    for (unsigned int h = threadIdx.x / L; h < total; h += HEADS) {
+    for (unsigned int h = blockIdx.y * HEADS + threadIdx.x / L; h < total; h += gridDim.y * HEADS) {
         const bool is_q = h < p.heads, is_v = h >= p.heads + p.kv_heads;
         if (!is_q && at == nullptr) break;
         aotx_f4 x0 = *(const aotx_f4 *)(row + h * D + lo);
@@ -253,8 +259,10 @@ extern "C" int aotx_kv_append(const float *qkv, unsigned int stride, const float
     p.gain = gain;
     aotx_rope_fill(how, &p.rope);
     hipStream_t s = aotx_stream(stream);
-    if (head_dim == 128u) hipLaunchKernelGGL(aotx_append_kernel<128>, dim3(tokens), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL(aotx_append_kernel<64>, dim3(tokens), dim3(256), 0, s, p);
+    const unsigned int each = ((heads + 2u * kv_heads) * head_dim + 2047u) / 2048u;
+    const dim3 grid(tokens, tokens <= 256u ? each : 1u);
+    if (head_dim == 128u) hipLaunchKernelGGL(aotx_append_kernel<128>, grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL(aotx_append_kernel<64>, grid, dim3(256), 0, s, p);
     AOTX_LAUNCH_CHECK();
     return 0;
 }

@@ -99,8 +99,8 @@ int aotx_norm_rows(const float *x, unsigned int stride, const float *w, unsigned
  * page is the table [AOTX_SLOTS][AOTX_KV_PAGES_EACH] of the pages' addresses (0: none), as
  * aotx_kv_table_device() gives it; layer of layers as in aotx_kv_write. q fp16
  * [tokens][heads][head_dim], 16-byte aligned. row_pos and row_agent unsigned [tokens], both given or both null:
- * every row's position and slot, as aotx_attend_paged takes them (a refused sequence's rows:
- * AOTX_SLOTS as their slot). */
+ * every row's position and slot, as aotx_attend_paged takes them (a refused sequence's rows, and those
+ * whose position 32 bits do not hold: AOTX_SLOTS as their slot, where attention gives zeros). */
 int aotx_kv_append(const float *qkv, unsigned int stride, const float *q_norm, const float *k_norm,
                    const aotx_rope_how *how, const float *factor, float gain,
                    const unsigned int *place, const unsigned int *offset, const unsigned int *pos,
@@ -138,7 +138,8 @@ typedef struct aotx_adjust_how {
  * (ld_out = ld). Tokens of lists and biases that the vocabulary does not have count
  * nowhere; a row whose agent is no list has no penalties; an offset past `biases` is taken as `biases`,
  * and a row whose end is below its begin has no biases. A row with a mask that allows none of the
- * vocabulary is -inf everywhere and adds 1 to aotx_model_faulted(). rows up to 4096, vocab up to 2^20,
+ * vocabulary is -inf everywhere and adds 1 to aotx_model_faulted(); aotx_pick, which has no
+ * token to give, then gives 0 at temperature 0 and -1 above. rows up to 4096, vocab up to 2^20,
  * ld and ld_out from vocab to 2^22. */
 int aotx_logits_adjust(const aotx_adjust_how *how, const float *logits, unsigned int ld,
                        unsigned int rows, unsigned int vocab, float *out, unsigned int ld_out,

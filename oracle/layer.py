@@ -91,7 +91,7 @@ def kv_append(qkv, heads, kv, d, rope, place, offset, pos, agent, layer, layers,
             faults += 1
             continue
         at = int(pos[i]) + np.arange(e - b)
-        row_pos[b:e], row_agent[b:e] = at & 0xFFFFFFFF, slot
+        row_pos[b:e], row_agent[b:e] = at & 0xFFFFFFFF, np.where(at >> 32, slots, slot)
         x = qkv[b:e].reshape(e - b, -1, d)
         where = at[:, None] if place is None else place[b:e]
         q[b:e] = rope(x[:, :heads], "q", where)

@@ -452,8 +452,11 @@ def test_append_rows_alone(torch, lib):
         assert (c.rpos == 99).all() and (c.ragent == 99).all()
 
 
-def test_append_slots_missing_and_named_twice(torch, lib):
-    c = Append(torch, 3, [3, 2, 4, 0, 5, 1], [0, 9, 20, 3, 3, 1], agent=[2, 64, 2, 5, 5, 0xFFFFFFFF], lead=1, tail=2)
+@pytest.mark.parametrize("kw", [dict(), dict(heads=32, kv=8, d=128, norm=True), dict(heads=40, kv=3)])
+@pytest.mark.parametrize("tail", [2, 300])
+def test_append_slots_missing_and_named_twice(torch, lib, kw, tail):
+    """Few rows, a workgroup for some heads of each, and many."""
+    c = Append(torch, 3, [3, 2, 4, 0, 5, 1], [0, 9, 20, 3, 3, 1], agent=[2, 64, 2, 5, 5, 0xFFFFFFFF], lead=1, tail=tail, **kw)
     assert c.up().call(lib).check(lib) == 3
 
 
@@ -771,6 +774,22 @@ def test_adjust_then_pick(torch, lib):
         assert all(allowed[r % 2, t] for r, t in enumerate(got))
         if temperature == 0:
             assert np.array_equal(got, c.out[:32].argmax(1).cpu().numpy())
+
+
+def test_adjust_then_pick_of_rows_with_no_token(torch, lib):
+    """A mask that allows nothing: the first token by the largest logit, none (-1) by a draw; others are not touched."""
+    c = Adjust(torch, 10, 6, 3000, 0, 0, 2, allow=0.1)
+    c.mask[0], c.mask_of = 0, np.array([0, 1, 0, 1, 9, 0], dtype=np.uint32)
+    c.ld_out = 3000
+    c.up().call(lib)
+    agent = _up(torch, np.arange(6), np.int32)
+    token = torch.zeros(6, dtype=torch.int32, device="cuda")
+    for temperature, none in ((0.0, 0), (1.0, -1)):
+        assert lib.aotx_pick(p(c.out), 6, 3000, p(agent), None, 0, 1.0, temperature, 5, p(token), None, None) == 0
+        got = token.cpu().numpy()
+        allowed = np.unpackbits(c.mask.view(np.uint8), axis=1, bitorder="little")
+        assert (got[[0, 2, 5]] == none).all() and allowed[1, got[1]] and allowed[1, got[3]] and 0 <= got[4] < 3000
+    assert lib.aotx_model_faulted() == 3
 
 
 # ---- a layer and an answer of them ---------------------------------------------------------------
