@@ -791,13 +791,15 @@ static size_t aotx_rgemv_lds(const aotx_rgemv_args &a, unsigned int mt)
     return x > red ? x : red;
 }
 
-/* narrow_max: the most batch rows that take the streaming (narrow) kernel. */
+/* narrow_max: the most batch rows that take the streaming (narrow) kernel; wide_max: the most workgroups of the
+ * wide kernel that passes of more than 64 rows over a short k may be; rows_max: the most batch rows. */
 static int aotx_rgemv_plan_n(aotx_rgemv_args *a, const void *const *w, const unsigned int *rows,
                              unsigned int nseg, unsigned int k, int epi, unsigned int mt,
-                             unsigned int narrow_max, bool routed = false)
+                             unsigned int narrow_max, bool routed = false, unsigned int wide_max = 512u,
+                             unsigned int rows_max = AOTX_RGEMM_ROWS)
 {
     memset(a, 0, sizeof *a);
-    if (k == 0u || k % 32u != 0u || nseg == 0u || nseg > 3u || mt == 0u || mt > AOTX_RGEMM_ROWS)
+    if (k == 0u || k % 32u != 0u || nseg == 0u || nseg > 3u || mt == 0u || mt > rows_max)
         return 1;
     a->m = mt;
     a->k = k;
@@ -858,7 +860,7 @@ static int aotx_rgemv_plan_n(aotx_rgemv_args *a, const void *const *w, const uns
                 s += 1u;
             const unsigned int qps = (a->qn + s - 1u) / s;
             if (wgs <= 256u ? qps <= (mt <= 64u ? 48u : 128u)
-                            : mt > 64u && wgs <= 512u && a->qn <= 32u) {
+                            : mt > 64u && wgs <= wide_max && a->qn <= 32u) {
                 a->gemm = 0u;
                 a->wide = 1u;
                 a->rt = 2u;
@@ -1245,16 +1247,20 @@ extern "C" int aotx_q8_gemv_f16(const void *w, unsigned int n, unsigned int k,
 
 static_assert(AOTX_LINEAR_ROWS_MAX / 16u * sizeof(unsigned int) <= AOTX_LINEAR_ZERO, "a counter per tile");
 
+#define AOTX_LINEAR_WIDE 768u
+
 static int aotx_linear_plan(aotx_rgemv_args *a, const void *w, const void *up, unsigned int n, unsigned int k,
                             unsigned int m)
 {
     const void *ws[2] = {w, up};
     const unsigned int rows[2] = {n, n};
     const bool gated = up != nullptr;
-    /* (the streaming kernel's rows: as aotx_q8r_gemv_any) */
+    /* (The streaming kernel's rows: as aotx_q8r_gemv_any. Of the wide kernel three rounds of workgroups, which are a
+     * whole chip of them: 73 rows of 6000 x 1024 14.2 us against 20.6 by the GEMM, 96 of 8000 x 2048 22.9 and 25.2, over
+     * the file's layout 23.1 and 30.3; in a fourth round 26.0 and 24.8.) */
     const unsigned int narrow_max = !gated && (n + 15u) / 16u <= 256u && k <= 4096u ? 8u : AOTX_NARROW_ROWS;
     return aotx_rgemv_plan_n(a, ws, rows, gated ? 2u : 1u, k, gated ? AOTX_EPI_SWIGLU : AOTX_EPI_F32,
-                             m < AOTX_RGEMM_ROWS ? m : AOTX_RGEMM_ROWS, narrow_max);
+                             m, narrow_max, false, AOTX_LINEAR_WIDE, AOTX_LINEAR_WIDE * 32u);
 }
 
 static bool aotx_linear_sizes(unsigned int n, unsigned int k, unsigned int m)
@@ -1262,8 +1268,20 @@ static bool aotx_linear_sizes(unsigned int n, unsigned int k, unsigned int m)
     return n != 0u && n <= AOTX_LINEAR_ROWS_MAX && k != 0u && k % 32u == 0u && k <= (1u << 18) && m <= (1u << 20);
 }
 
-/* The rows of a call's next pass where linear.hip does not take them. */
-static unsigned int aotx_linear_rows(unsigned int left) { return left < AOTX_RGEMM_ROWS ? left : AOTX_RGEMM_ROWS; }
+/* The passes of a call that linear.hip does not take: of AOTX_RGEMM_ROWS rows each, and then the last one, which takes
+ * all rows that the wide kernel's rounds hold (670 rows of 541 x 800 in one launch 12.1 us, in 512 and 158 17.6;
+ * 2040 of 100 x 1024 7.2 and 30.2). Returns the last one's. */
+static unsigned int aotx_linear_last(unsigned int n, unsigned int k, unsigned int m, bool gated)
+{
+    const unsigned int pairs = gated ? (n + 15u) / 16u : (n + 31u) / 32u, qn = (unsigned int)aotx_q8r_quads(k);
+    unsigned int last = m % AOTX_RGEMM_ROWS;
+    while (last + AOTX_RGEMM_ROWS <= m) {
+        const unsigned long long wgs = (unsigned long long)pairs * ((last + AOTX_RGEMM_ROWS + 31u) / 32u);
+        if (wgs > 256u ? wgs > AOTX_LINEAR_WIDE || qn > 32u : qn > 128u) break;
+        last += AOTX_RGEMM_ROWS;
+    }
+    return last;
+}
 
 /* Whether linear.hip takes the call: where its time is below that of passes of up to 512 rows, which is taken as what
  * those measured, in ns: a quad of the GEMM 1450 with a workgroup on each CU and 1150 for each of several (over
@@ -1273,15 +1291,16 @@ static bool aotx_linear_many(aotx_lgemm_plan *p, unsigned int n, unsigned int k,
 {
     if (m <= 64u) return false;
     unsigned long long passes = 0ull;
-    const unsigned int full = m / AOTX_RGEMM_ROWS;
-    for (unsigned int rows : {full != 0u ? AOTX_RGEMM_ROWS : 0u, m % AOTX_RGEMM_ROWS}) {
-        if (rows == 0u) continue;
+    const unsigned int last = aotx_linear_last(n, k, m, gated), full = (m - last) / AOTX_RGEMM_ROWS;
+    for (const bool tail : {false, true}) {
+        const unsigned int rows = tail ? last : AOTX_RGEMM_ROWS, times = tail ? 1u : full;
+        if (rows == 0u || times == 0u) continue;
         aotx_rgemv_args a;
         if (aotx_linear_plan(&a, &a, gated ? &a : nullptr, n, k, rows) != 0) return false;
         const unsigned int wgs = a.groups * a.splits * (a.gemm ? (rows + RGM_MB - 1u) / RGM_MB : a.passes > 1u ? a.passes : 1u);
         const unsigned int each = (wgs + 255u) / 256u;
         const unsigned int one = file ? 1950u : 1450u, more = file ? 1900u : 1150u;
-        passes += (rows == AOTX_RGEMM_ROWS ? full : 1u)
+        passes += times
                 * ((a.gemm ? 4000ull : 6000ull)
                    + (unsigned long long)a.qps * (a.gemm ? (each <= 1u ? one : more * each) : (each <= 1u ? 200u : 250u * each))
                    + (a.splits > 1u ? 8000u : 0u));
@@ -1301,7 +1320,8 @@ extern "C" unsigned long long aotx_q8_linear_work(unsigned int n, unsigned int k
             most = bytes > most ? bytes : most;
             continue;
         }
-        for (unsigned int rows : {aotx_linear_rows(m), m % AOTX_RGEMM_ROWS}) {
+        const unsigned int last = aotx_linear_last(n, k, m, gated != 0u);
+        for (unsigned int rows : {m > last ? AOTX_RGEMM_ROWS : 0u, last}) {
             aotx_rgemv_args a;
             if (rows == 0u) continue;
             if (aotx_linear_plan(&a, &a, gated != 0u ? &a : nullptr, n, k, rows) != 0) return 0ull;
@@ -1361,10 +1381,11 @@ extern "C" int aotx_q8_linear(const aotx_linear_how *how, const void *x, unsigne
     e.half = how->out == AOTX_LINEAR_F16;
     aotx_lgemm_plan g;
     const bool many = aotx_linear_many(&g, n, k, m, how->up != nullptr, !how->packed);
+    const unsigned int last = many ? m : aotx_linear_last(n, k, m, how->up != nullptr);
     for (unsigned int m0 = 0u, rows = 0u; m0 < m; m0 += rows) {
-        rows = many ? m : aotx_linear_rows(m - m0);
+        rows = m - m0 > last ? AOTX_RGEMM_ROWS : last;
         aotx_rgemv_args a;
-        if (aotx_linear_plan(&a, how->w, how->up, n, k, rows) != 0) return 1;
+        if (aotx_linear_plan(&a, how->w, how->up, n, k, many && rows > AOTX_RGEMM_ROWS ? AOTX_RGEMM_ROWS : rows) != 0) return 1;
         if (!how->packed) aotx_rgemv_file(&a);
         a.xmode = AOTX_X_F16;
         a.x = (const unsigned short *)x;
