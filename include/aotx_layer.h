@@ -66,7 +66,7 @@ typedef struct aotx_linear_how {
  * Inf and NaN reach the values whose sum holds them and no others.
  *
  * work is a workspace of work_bytes bytes, at least aotx_q8_linear_work of the same n, k, m and
- * up, 256-byte aligned. The caller sets its first AOTX_LINEAR_ZERO bytes to zero once, before the first
+ * up (fewer rows may ask for more than many do), 256-byte aligned. The caller sets its first AOTX_LINEAR_ZERO bytes to zero once, before the first
  * call that uses it; every call leaves them zero, so that calls of any shapes may use it one
  * after another. aotx_q8_linear_work returns 0 for sizes that are refused. */
 #define AOTX_LINEAR_ZERO 65536ull
