@@ -791,15 +791,16 @@ static size_t aotx_rgemv_lds(const aotx_rgemv_args &a, unsigned int mt)
     return x > red ? x : red;
 }
 
-/* narrow_max: the most batch rows that take the streaming (narrow) kernel; wide_max: the most workgroups of the
- * wide kernel that passes of more than 64 rows over a short k may be; rows_max: the most batch rows. */
+#define AOTX_LINEAR_WIDE 768u
+/* narrow_max: the most batch rows that take the streaming (narrow) kernel. linear: of aotx_q8_linear, whose products
+ * may take more workgroups and rows of the wide kernel, and its 16-row form. */
 static int aotx_rgemv_plan_n(aotx_rgemv_args *a, const void *const *w, const unsigned int *rows,
                              unsigned int nseg, unsigned int k, int epi, unsigned int mt,
-                             unsigned int narrow_max, bool routed = false, unsigned int wide_max = 512u,
-                             unsigned int rows_max = AOTX_RGEMM_ROWS)
+                             unsigned int narrow_max, bool routed = false, bool linear = false)
 {
     memset(a, 0, sizeof *a);
-    if (k == 0u || k % 32u != 0u || nseg == 0u || nseg > 3u || mt == 0u || mt > rows_max)
+    if (k == 0u || k % 32u != 0u || nseg == 0u || nseg > 3u || mt == 0u
+        || mt > (linear ? AOTX_LINEAR_WIDE * 32u : AOTX_RGEMM_ROWS))
         return 1;
     a->m = mt;
     a->k = k;
@@ -860,7 +861,7 @@ static int aotx_rgemv_plan_n(aotx_rgemv_args *a, const void *const *w, const uns
                 s += 1u;
             const unsigned int qps = (a->qn + s - 1u) / s;
             if (wgs <= 256u ? qps <= (mt <= 64u ? 48u : 128u)
-                            : mt > 64u && wgs <= wide_max && a->qn <= 32u) {
+                            : mt > 64u && wgs <= (linear ? AOTX_LINEAR_WIDE : 512u) && a->qn <= 32u) {
                 a->gemm = 0u;
                 a->wide = 1u;
                 a->rt = 2u;
@@ -913,6 +914,9 @@ static int aotx_rgemv_plan_n(aotx_rgemv_args *a, const void *const *w, const uns
          * chunk, and the last split of a group to finish adds the partials. */
         a->wide = 1u;
         a->rt = tiles >= 1536u ? 8u : (tiles >= 768u ? 4u : 2u);
+        /* (up to 16 rows the form of 2 tiles has a 16-row kernel, two workgroups of it to a CU: 14336 x 4096 at 8 rows 16.0
+         * us against 17.2 by 4 tiles) */
+        if (linear && mt <= 16u && a->rt == 4u) a->rt = 2u;
         /* routed experts' single products (down): the launch has a workgroup row per
          * expert, so fewer, larger tile groups fill the chip and each reads the expert's x
          * half as often (Mixtral shape, 64 tokens: 73.7 -> 58.3 us per pass with 4 tiles,
@@ -1069,6 +1073,14 @@ static void aotx_rgemv_wide_go(const aotx_rgemv_args &a, const E &e, hipStream_t
         if (a.file) hipLaunchKernelGGL((aotx_rgemv_wide<T, P, KC, PDQ, true, MT, E>), grid, dim3(512), xb, s, a, e); \
         else hipLaunchKernelGGL((aotx_rgemv_wide<T, P, KC, PDQ, false, MT, E>), grid, dim3(512), xb, s, a, e); \
     } while (0)
+    if constexpr (E::LINEAR)
+        if (a.wide == 1u && a.rt == 2u && a.m <= 16u) {
+            /* half the x to load and hold and half the matrix instructions: 6144 x 4096 at 8 rows 9.3 us against 11.1, over
+             * the file's layout 11.3 against 12.1 */
+            RGW_GO(2, 4, 8, 1, 16);
+            AOTX_LAUNCH_CHECK();
+            return;
+        }
     if (a.wide == 2u) RGW_GO(4, 2, 4, 1, 64);
     else if (a.rt == 2u) RGW_GO(2, 4, 8, 1, 32);
     else if (a.rt == 4u) RGW_GO(4, 2, 4, 1, 32);
@@ -1247,8 +1259,6 @@ extern "C" int aotx_q8_gemv_f16(const void *w, unsigned int n, unsigned int k,
 
 static_assert(AOTX_LINEAR_ROWS_MAX / 16u * sizeof(unsigned int) <= AOTX_LINEAR_ZERO, "a counter per tile");
 
-#define AOTX_LINEAR_WIDE 768u
-
 static int aotx_linear_plan(aotx_rgemv_args *a, const void *w, const void *up, unsigned int n, unsigned int k,
                             unsigned int m)
 {
@@ -1260,7 +1270,7 @@ static int aotx_linear_plan(aotx_rgemv_args *a, const void *w, const void *up, u
      * the file's layout 23.1 and 30.3; in a fourth round 26.0 and 24.8.) */
     const unsigned int narrow_max = !gated && (n + 15u) / 16u <= 256u && k <= 4096u ? 8u : AOTX_NARROW_ROWS;
     return aotx_rgemv_plan_n(a, ws, rows, gated ? 2u : 1u, k, gated ? AOTX_EPI_SWIGLU : AOTX_EPI_F32,
-                             m, narrow_max, false, AOTX_LINEAR_WIDE, AOTX_LINEAR_WIDE * 32u);
+                             m, narrow_max, false, true);
 }
 
 static bool aotx_linear_sizes(unsigned int n, unsigned int k, unsigned int m)
