@@ -1252,8 +1252,8 @@ extern "C" int aotx_q8_gemv_f16(const void *w, unsigned int n, unsigned int k,
 }
 
 /* ---- products with an epilogue of their own (aotx_layer.h) --------------------------------
- * The plans, kernels and order of sums of the products above, with rg_linear in place of the step's
- * epilogues. Partials and arrival counters are the caller's, so that calls on several streams or
+ * The kernels and order of sums of the products above, with rg_linear in place of the step's
+ * epilogues, and plans that know one form more. Partials and arrival counters are the caller's, so that calls on several streams or
  * in several graphs share nothing; the counters have a place of fixed size before the partials
  * (a word a tile group at most), because a call of other sizes finds them there. */
 
@@ -1265,10 +1265,17 @@ static int aotx_linear_plan(aotx_rgemv_args *a, const void *w, const void *up, u
     const void *ws[2] = {w, up};
     const unsigned int rows[2] = {n, n};
     const bool gated = up != nullptr;
-    /* (The streaming kernel's rows: as aotx_q8r_gemv_any. Of the wide kernel three rounds of workgroups, which are a
-     * whole chip of them: 73 rows of 6000 x 1024 14.2 us against 20.6 by the GEMM, 96 of 8000 x 2048 22.9 and 25.2, over
-     * the file's layout 23.1 and 30.3; in a fourth round 26.0 and 24.8.) */
-    const unsigned int narrow_max = !gated && (n + 15u) / 16u <= 256u && k <= 4096u ? 8u : AOTX_NARROW_ROWS;
+    const unsigned int tiles = (n + 15u) / 16u;
+    /* The streaming kernel takes up to 4 rows where its workgroups of one tile need few splits, and of pairs where the
+     * wide kernel has 8 tiles to a workgroup: one row of 4096 square 6.5 us against 8.0 by the wide one, two of 2048 x 4096 6.8
+     * and 7.5, of 8192 x 2048 5.9 and 6.5, of the gated 14336 x 4096 25.8 and 28.2. Else the 16-row form of the wide one is the faster:
+     * two rows of 1000 x 4096 6.9 against 7.9, of 14336 x 1024 6.5 and 7.0, of the gated 2048 x 4096 7.7 and 10.0, of 7168 x
+     * 4096 14.7 and 17.5; but of 512 x 12288 8.9 and 7.5. */
+    const bool streams = gated ? 2u * tiles >= 1536u : k >= 1536u && (tiles >= 128u || k > 8192u);
+    const unsigned int narrow_max = streams ? AOTX_NARROW_ROWS : 0u;
+    /* (Of the wide kernel three rounds of workgroups, which are a whole chip of them: 73 rows of 6000 x 1024 14.2 us
+     * against 20.6 by the GEMM, 96 of 8000 x 2048 22.9 and 25.2, over the file's layout 23.1 and 30.3; in a fourth
+     * round 26.0 and 24.8.) */
     return aotx_rgemv_plan_n(a, ws, rows, gated ? 2u : 1u, k, gated ? AOTX_EPI_SWIGLU : AOTX_EPI_F32,
                              m, narrow_max, false, true);
 }

@@ -231,10 +231,10 @@ def test_linear_inf_and_nan_stay_in_their_row(torch, lib, packed, m, n, k, bad):
 
 def test_linear_is_the_product_with_nothing_beside(torch, lib):
     """Bit for bit aotx_q8r_gemv where the same form runs, and the same on every run."""
-    for m in (1, 8, 32):
-        c = Linear(torch, lib, 3, m, 500, 1024).up().call()
-        y = torch.zeros(m, 500, device="cuda")
-        assert lib.aotx_q8r_gemv(p(c.dw[0]), 500, 1024, p(c.dx), m, p(y), None) == 0
+    for m, n in ((1, 4200), (20, 500), (32, 500)):
+        c = Linear(torch, lib, 3, m, n, 2048).up().call()
+        y = torch.zeros(m, n, device="cuda")
+        assert lib.aotx_q8r_gemv(p(c.dw[0]), n, 2048, p(c.dx), m, p(y), None) == 0
         torch.cuda.synchronize()
         assert torch.equal(y, c.y[:m])
     for m in (40, 300):
