@@ -1253,9 +1253,9 @@ extern "C" int aotx_q8_gemv_f16(const void *w, unsigned int n, unsigned int k,
 
 /* ---- products with an epilogue of their own (aotx_layer.h) --------------------------------
  * The kernels and order of sums of the products above, with rg_linear in place of the step's
- * epilogues, and plans that know one form more. Partials and arrival counters are the caller's, so that calls on several streams or
- * in several graphs share nothing; the counters have a place of fixed size before the partials
- * (a word a tile group at most), because a call of other sizes finds them there. */
+ * epilogues, and plans that know one form more. Partials and arrival counters are the caller's, so that
+ * calls on several streams or in several graphs share nothing; the counters have a place of fixed size
+ * before the partials (a word a tile group at most), because a call of other sizes finds them there. */
 
 static_assert(AOTX_LINEAR_ROWS_MAX / 16u * sizeof(unsigned int) <= AOTX_LINEAR_ZERO, "a counter per tile");
 
@@ -1268,9 +1268,9 @@ static int aotx_linear_plan(aotx_rgemv_args *a, const void *w, const void *up, u
     const unsigned int tiles = (n + 15u) / 16u;
     /* The streaming kernel takes up to 4 rows where its workgroups of one tile need few splits, and of pairs where the
      * wide kernel has 8 tiles to a workgroup: one row of 4096 square 6.5 us against 8.0 by the wide one, two of 2048 x 4096 6.8
-     * and 7.5, of 8192 x 2048 5.9 and 6.5, of the gated 14336 x 4096 25.8 and 28.2. Else the 16-row form of the wide one is the faster:
-     * two rows of 1000 x 4096 6.9 against 7.9, of 14336 x 1024 6.5 and 7.0, of the gated 2048 x 4096 7.7 and 10.0, of 7168 x
-     * 4096 14.7 and 17.5; but of 512 x 12288 8.9 and 7.5. */
+     * and 7.5, of 8192 x 2048 5.9 and 6.5, of 512 x 12288 7.5 and 8.9, of the gated 14336 x 4096 25.8 and 28.2. Else the
+     * 16-row form of the wide one is the faster: two rows of 1000 x 4096 6.9 against 7.9, of 14336 x 1024 6.5 and 7.0, of the
+     * gated 2048 x 4096 7.7 and 10.0, of 7168 x 4096 14.7 and 17.5. */
     const bool streams = gated ? 2u * tiles >= 1536u : k >= 1536u && (tiles >= 128u || k > 8192u);
     const unsigned int narrow_max = streams ? AOTX_NARROW_ROWS : 0u;
     /* (Of the wide kernel three rounds of workgroups, which are a whole chip of them: 73 rows of 6000 x 1024 14.2 us
