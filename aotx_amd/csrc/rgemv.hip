@@ -791,7 +791,16 @@ static size_t aotx_rgemv_lds(const aotx_rgemv_args &a, unsigned int mt)
     return x > red ? x : red;
 }
 
-#define AOTX_LINEAR_WIDE 768u
+/* Whether aotx_q8_linear's passes of more than 64 rows take the wide kernel in more workgroups than CUs, two to a CU
+ * (its 4-wave form): 96 rows of 5440 x 4096 21.9 us against 34 by the GEMM, of 9600 x 2048 23.1 and 25.8, of 13536 x 1024
+ * 20.7 and 21.4, over the file's layout 22.9 and 41, 24.7 and 30.6, 18.6 and 24.6; but of 9600 x 4096 38.3 and 33.8, of 13536 x
+ * 2048 31.2 and 27.2, of 21312 x 1024 29.0 and 22.5. */
+#define AOTX_LINEAR_WIDE 1536u
+static bool aotx_linear_wide(unsigned long long wgs, unsigned int qn)
+{
+    return qn <= (wgs <= 768ull ? 32u : wgs <= 1024ull ? 16u : wgs <= AOTX_LINEAR_WIDE ? 8u : 0u);
+}
+
 /* narrow_max: the most batch rows that take the streaming (narrow) kernel. linear: of aotx_q8_linear, whose products
  * may take more workgroups and rows of the wide kernel, and its 16-row form. */
 static int aotx_rgemv_plan_n(aotx_rgemv_args *a, const void *const *w, const unsigned int *rows,
@@ -861,7 +870,7 @@ static int aotx_rgemv_plan_n(aotx_rgemv_args *a, const void *const *w, const uns
                 s += 1u;
             const unsigned int qps = (a->qn + s - 1u) / s;
             if (wgs <= 256u ? qps <= (mt <= 64u ? 48u : 128u)
-                            : mt > 64u && wgs <= (linear ? AOTX_LINEAR_WIDE : 512u) && a->qn <= 32u) {
+                            : mt > 64u && (linear ? aotx_linear_wide(wgs, a->qn) : wgs <= 512u && a->qn <= 32u)) {
                 a->gemm = 0u;
                 a->wide = 1u;
                 a->rt = 2u;
@@ -1070,14 +1079,17 @@ static void aotx_rgemv_wide_go(const aotx_rgemv_args &a, const E &e, hipStream_t
 #define RGW_GO(T, P, KC, PDQ, MT)                                                            \
     do {                                                                                     \
         const size_t xb = 2u * MT * (KC * 128u + 8u) * 2u;                                   \
-        if (a.file) hipLaunchKernelGGL((aotx_rgemv_wide<T, P, KC, PDQ, true, MT, E>), grid, dim3(512), xb, s, a, e); \
-        else hipLaunchKernelGGL((aotx_rgemv_wide<T, P, KC, PDQ, false, MT, E>), grid, dim3(512), xb, s, a, e); \
+        if (a.file) hipLaunchKernelGGL((aotx_rgemv_wide<T, P, KC, PDQ, true, MT, E>), grid, dim3(64 * T * P), xb, s, a, e); \
+        else hipLaunchKernelGGL((aotx_rgemv_wide<T, P, KC, PDQ, false, MT, E>), grid, dim3(64 * T * P), xb, s, a, e); \
     } while (0)
     if constexpr (E::LINEAR)
-        if (a.wide == 1u && a.rt == 2u && a.m <= 16u) {
-            /* half the x to load and hold and half the matrix instructions: 6144 x 4096 at 8 rows 9.3 us against 11.1, over
-             * the file's layout 11.3 against 12.1 */
-            RGW_GO(2, 4, 8, 1, 16);
+        if (a.wide == 1u && a.rt == 2u && (a.m <= 16u || grid.x * grid.y > 256u)) {
+            /* Up to 16 rows half the x to load and hold and half the matrix instructions: 6144 x 4096 at 8 rows 9.3 us against
+             * 11.1, over the file's layout 11.3 against 12.1. More workgroups than CUs: 4 waves and half the
+             * chunk of x, so that a CU has two: 96 rows of 4480 x 1024 8.8 against 10.6, of 5440 x 4096 21.9 against 24.0; but
+             * one to a CU 32 rows of 6144 x 4096 14.2 against 12.0. */
+            if (a.m <= 16u) RGW_GO(2, 4, 8, 1, 16);
+            else RGW_GO(2, 2, 4, 1, 32);
             AOTX_LAUNCH_CHECK();
             return;
         }
@@ -1273,9 +1285,6 @@ static int aotx_linear_plan(aotx_rgemv_args *a, const void *w, const void *up, u
      * gated 2048 x 4096 7.7 and 10.0, of 7168 x 4096 14.7 and 17.5. */
     const bool streams = gated ? 2u * tiles >= 1536u : k >= 1536u && (tiles >= 128u || k > 8192u);
     const unsigned int narrow_max = streams ? AOTX_NARROW_ROWS : 0u;
-    /* (Of the wide kernel three rounds of workgroups, which are a whole chip of them: 73 rows of 6000 x 1024 14.2 us
-     * against 20.6 by the GEMM, 96 of 8000 x 2048 22.9 and 25.2, over the file's layout 23.1 and 30.3; in a fourth
-     * round 26.0 and 24.8.) */
     return aotx_rgemv_plan_n(a, ws, rows, gated ? 2u : 1u, k, gated ? AOTX_EPI_SWIGLU : AOTX_EPI_F32,
                              m, narrow_max, false, true);
 }
@@ -1286,7 +1295,7 @@ static bool aotx_linear_sizes(unsigned int n, unsigned int k, unsigned int m)
 }
 
 /* The passes of a call that linear.hip does not take: of AOTX_RGEMM_ROWS rows each, and then the last one, which takes
- * all rows that the wide kernel's rounds hold (670 rows of 541 x 800 in one launch 12.1 us, in 512 and 158 17.6;
+ * all rows that the wide kernel's rounds hold (670 rows of 541 x 800 in one launch 10.0 us, in 512 and 158 17.6;
  * 2040 of 100 x 1024 7.2 and 30.2). Returns the last one's. */
 static unsigned int aotx_linear_last(unsigned int n, unsigned int k, unsigned int m, bool gated)
 {
@@ -1294,7 +1303,7 @@ static unsigned int aotx_linear_last(unsigned int n, unsigned int k, unsigned in
     unsigned int last = m % AOTX_RGEMM_ROWS;
     while (last + AOTX_RGEMM_ROWS <= m) {
         const unsigned long long wgs = (unsigned long long)pairs * ((last + AOTX_RGEMM_ROWS + 31u) / 32u);
-        if (wgs > 256u ? wgs > AOTX_LINEAR_WIDE || qn > 32u : qn > 128u) break;
+        if (wgs > 256u ? !aotx_linear_wide(wgs, qn) : qn > 128u) break;
         last += AOTX_RGEMM_ROWS;
     }
     return last;
@@ -1302,7 +1311,7 @@ static unsigned int aotx_linear_last(unsigned int n, unsigned int k, unsigned in
 
 /* Whether linear.hip takes the call: where its time is below that of passes of up to 512 rows, which is taken as what
  * those measured, in ns: a quad of the GEMM 1450 with a workgroup on each CU and 1150 for each of several (over
- * the file's layout 1950, 1900), of the others 200 and 250, and 8000 for sums of splits. (2048 rows of the gated 14336 x 4096: 443
+ * the file's layout 1950, 1900), of the wide kernel 200 and 250, beside them 4000 to 6500, and 8000 for sums of splits. (2048 rows of the gated 14336 x 4096: 443
  * us there, 579 in passes; 512 rows 115 and 145; 512 of 4096 square 43 and 36; 1024 of 1024 x 4096 43 and 42.) */
 static bool aotx_linear_many(aotx_lgemm_plan *p, unsigned int n, unsigned int k, unsigned int m, bool gated, bool file)
 {
@@ -1318,7 +1327,7 @@ static bool aotx_linear_many(aotx_lgemm_plan *p, unsigned int n, unsigned int k,
         const unsigned int each = (wgs + 255u) / 256u;
         const unsigned int one = file ? 1950u : 1450u, more = file ? 1900u : 1150u;
         passes += times
-                * ((a.gemm ? 4000ull : 6000ull)
+                * ((a.gemm ? 4000ull : each <= 1u ? 5000ull : 2500ull + 1000ull * each)
                    + (unsigned long long)a.qps * (a.gemm ? (each <= 1u ? one : more * each) : (each <= 1u ? 200u : 250u * each))
                    + (a.splits > 1u ? 8000u : 0u));
     }

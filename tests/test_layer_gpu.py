@@ -147,7 +147,8 @@ def test_linear_sizes(torch, lib, m, n, k, packed, gated):
 MANY = [(677, 1350, 1184), (630, 1044, 1440), (2023, 2056, 32), (2294, 2096, 160), (2220, 241, 4032), (2063, 3109, 2336),
         (2275, 2326, 96), (1996, 3178, 512), (2168, 3133, 2592), (768, 4096, 4096), (4097, 513, 1056), (20000, 300, 64),
         # and where passes take them, the last of more rows than the others
-        (1500, 100, 1024), (1300, 300, 7200), (1900, 541, 800), (2560, 90, 4096), (73, 7836, 1184)]
+        (1500, 100, 1024), (1300, 300, 7200), (1900, 541, 800), (2560, 90, 4096), (73, 7836, 1184),
+        (1292, 828, 384), (96, 9601, 1056), (130, 9001, 288), (32, 8500, 1024), (17, 12000, 160)]
 
 
 @pytest.mark.parametrize("m,n,k", MANY)
