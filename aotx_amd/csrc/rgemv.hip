@@ -1309,10 +1309,11 @@ static unsigned int aotx_linear_last(unsigned int n, unsigned int k, unsigned in
     return last;
 }
 
-/* Whether linear.hip takes the call: where its time is below that of passes of up to 512 rows, which is taken as what
- * those measured, in ns: a quad of the GEMM 1450 with a workgroup on each CU and 1150 for each of several (over
- * the file's layout 1950, 1900), of the wide kernel 200 and 250, beside them 4000 to 6500, and 8000 for sums of splits. (2048 rows of the gated 14336 x 4096: 443
- * us there, 579 in passes; 512 rows 115 and 145; 512 of 4096 square 43 and 36; 1024 of 1024 x 4096 43 and 42.) */
+/* Whether linear.hip takes the call: where its time is below that of passes, which is taken as what those measured, in
+ * ns: a quad of the GEMM 1450 with a workgroup on each CU and 1150 for each of several (over the file's layout 1950,
+ * 1900), of the wide kernel 200 and 250; 4000 to 6500 beside them, and 8000 for sums of splits. (2048 rows of the gated
+ * 14336 x 4096: 455 us there, 579 in passes of 512; 512 rows 115 and 145; 512 of 4096 square 43 there, 36 in passes;
+ * 1024 of 1024 x 4096 43 there, 37.5 in passes.) */
 static bool aotx_linear_many(aotx_lgemm_plan *p, unsigned int n, unsigned int k, unsigned int m, bool gated, bool file)
 {
     if (m <= 64u) return false;
