@@ -645,9 +645,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(WIDE_REGS ?
             rg_wload<FILE, false>(a, wsrc[t], qq_, lane, wr[BUF][t]);                    \
         }                                                                                \
     } while (0)
-    /* x pieces of quad Q (a quad past the split repeats its last). TAIL: k ends inside the
-     * last quad; a piece past it reads the row's first, and that and a quad past the split are
-     * stored as zeros */
+    /* x pieces of quad Q (a quad past the split repeats its last, and is stored as zeros for
+     * aotx_q8_linear, as 0 times an infinity would be NaN: a split of an odd number of quads
+     * multiplies one past its end). TAIL: k ends inside the last quad; a piece past it reads the
+     * row's first, and that and a quad past the split are stored as zeros */
     rg_u4 xr[2][PPT];                             /* register buffer XB = Q & 1 holds quad Q */
 #define RGM_XLOAD(XB, Q)                                                                 \
     do {                                                                                 \
@@ -666,7 +667,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(WIDE_REGS ?
         _Pragma("unroll") for (int i = 0; i < PPT; ++i)                                  \
             *(rg_u4 *)(xb_ + (unsigned int)i * RSTEP * XS) =                             \
                 xrow0 + (unsigned int)i * RSTEP < mrows                                  \
-                && (!TAIL || ((Q) < qn && (Q) * 128u + xpc * 8u < a.k)) ? xr[XB][i] : (rg_u4){0u, 0u, 0u, 0u}; \
+                && (!(TAIL || E::LINEAR) || (Q) < qn) && (!TAIL || (Q) * 128u + xpc * 8u < a.k)  \
+                ? xr[XB][i] : (rg_u4){0u, 0u, 0u, 0u};                                   \
     } while (0)
 
     /* Quad q is computed from LDS x buffer q & 1 and weight buffer q & 1. Its step first

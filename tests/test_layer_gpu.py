@@ -230,6 +230,30 @@ def test_linear_inf_and_nan_stay_in_their_row(torch, lib, packed, m, n, k, bad):
     assert np.isfinite(y[:, :n - 1]).all() and not np.isfinite(y[:, n - 1]).any()
 
 
+# packed products that the GEMM takes: 9 quads of k, 5, two splits of 16 and 15, pairs of 31, pairs whose k ends inside a quad; and
+# tiles of many rows, whole and in splits
+@pytest.mark.parametrize("m,n,k,gated", [(300, 9000, 1152, False), (100, 20480, 640, False), (300, 4096, 3968, False),
+                                         (512, 4096, 3968, False), (300, 2048, 3968, True), (300, 4000, 160, True),
+                                         (677, 4096, 1184, False), (2048, 1024, 4096, False)])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_linear_inf_and_nan_in_the_gemm_and_tiles(torch, lib, m, n, k, gated, bad):
+    """In the first, a middle and the last quad of k, which are not read again where quads go in pairs."""
+    c = Linear(torch, lib, 11, m, n, k, gated)
+    rows = [0, m - 1, m // 2, m // 3, 63]
+    for r, at in zip(rows, (0, k - 1, k // 2, (k - 1) // 128 * 128, k // 256 * 128 + 5)):
+        c.x[r, at] = bad if r else -bad
+    c.up().call()
+    torch.cuda.synchronize()
+    cols = np.r_[0:n - 20:7, n - 20:n]
+    y = c.y[:m, :n].cpu().numpy()[:, cols]
+    with np.errstate(invalid="ignore"):
+        want, far = c.want(cols)
+    assert np.array_equal(np.isnan(y), np.isnan(want)) and np.array_equal(y[np.isinf(want)], want[np.isinf(want)])
+    fine = np.ones(m, dtype=bool)
+    fine[rows] = False
+    assert (np.abs(y[fine] - want[fine]) <= far[fine]).all()
+
+
 def test_linear_is_the_product_with_nothing_beside(torch, lib):
     """Bit for bit aotx_q8r_gemv where the same form runs, and the same on every run."""
     for m, n in ((1, 4200), (20, 500), (32, 500)):
