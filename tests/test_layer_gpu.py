@@ -5,6 +5,7 @@ and pages that are missing, values of Inf and NaN, capture, other streams, and a
 Tolerances are oracle/layer.py's: counted roundings of fp32, and half a step of the type that is
 written."""
 import ctypes
+import math
 
 import numpy as np
 import pytest
@@ -177,6 +178,30 @@ def test_linear_activations(torch, lib, act, gated, m):
     c.x[0] = 0
     c.bias[0][:8] = (0, -200, 200, -90, 90, 1e-30, -5, 5)
     c.up().call().check()
+
+
+@pytest.mark.parametrize("act", [1, 2, 3])
+@pytest.mark.parametrize("m,n,k", [(1, 2048, 1536), (20, 1500, 32), (300, 9000, 32), (2023, 2056, 32)])
+def test_linear_activation_tails(torch, lib, act, m, n, k):
+    """Values that are small beside their argument keep their bits: relative to the value, arguments from -12 to 12.
+
+    In steps of 2^-24. Their argument's steps count by how much the result moves with it: SiLU's exponent has 2 of |v| (the
+    factor and the product), tanh-GELU's 5 of |u| (two factors, two products and a sum of one sign, the last product), GELU's 3
+    of v^2 / 2, or by erfc 2 of |z| = |v| / sqrt 2, where |z erfc'(z) / erfc(z)| <= 2 z^2 + 1 = v^2 + 1. An exponential and a
+    reciprocal are 2 each, erfc 32 (16 ulp), sums and products one. An exponential or reciprocal below 2^-126, fp32's least normal
+    value, may be 0: off by less than |v| 2^-126."""
+    c = Linear(torch, lib, 12, m, n, k, False, act, True)
+    v = np.linspace(-12, 12, n).astype(np.float32)
+    c.bias[0][:] = v
+    c.x[:] = 0
+    c.up().call()
+    torch.cuda.synchronize()
+    v = v.astype(np.float64)
+    u = np.abs(v) * (2 * np.sqrt(2 / np.pi) * (1 + 0.044715 * v * v))
+    want = {1: v / (1 + np.exp(-v)), 2: 0.5 * v * np.vectorize(math.erfc)(-v / math.sqrt(2)), 3: v / (1 + np.exp(-np.sign(v) * u))}[act]
+    steps = {1: 2 * np.abs(v) + 6, 2: 2 * (v * v + 1) + 34, 3: 5 * u + 6}[act]
+    off = np.abs(c.y[:m, :n].cpu().numpy() - want) - steps * O.E32 * np.abs(want) - np.abs(v) * 2.0 ** -126
+    assert off.max() <= 0, v[np.unravel_index(off.argmax(), off.shape)[1]]
 
 
 @pytest.mark.parametrize("m", [1, 7, 30, 64, 90, 400])
