@@ -43,7 +43,7 @@ enum {
 struct aotx_rgemv_args {
     const unsigned char *w[3];    /* Q8R tensors stacked along n (file: Q8_0 rows as the model
                                      file has them, [rows][k/32 blocks of 34 B]) */
-    unsigned int seg_end[3];      /* cumulative row ends (multiples of 16 except the last) */
+    unsigned int seg_end[3];      /* cumulative row ends (multiples of 16 except the last and aotx_q8_linear's pairs) */
     unsigned int nseg;
     unsigned int n;               /* rows (SWIGLU: rows of one of the pair) */
     unsigned int k;

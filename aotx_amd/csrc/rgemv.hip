@@ -804,7 +804,7 @@ static bool aotx_linear_wide(unsigned long long wgs, unsigned int qn)
 }
 
 /* narrow_max: the most batch rows that take the streaming (narrow) kernel. linear: of aotx_q8_linear, whose products
- * may take more workgroups and rows of the wide kernel, and its 16-row form. */
+ * may take more workgroups and rows of the wide kernel, its 16-row form, and pairs of any number of rows. */
 static int aotx_rgemv_plan_n(aotx_rgemv_args *a, const void *const *w, const unsigned int *rows,
                              unsigned int nseg, unsigned int k, int epi, unsigned int mt,
                              unsigned int narrow_max, bool routed = false, bool linear = false)
@@ -824,7 +824,7 @@ static int aotx_rgemv_plan_n(aotx_rgemv_args *a, const void *const *w, const uns
         a->w[s] = (const unsigned char *)w[s];
         total += rows[s];
         a->seg_end[s] = total;
-        if (s + 1u < nseg && rows[s] % 16u != 0u && epi != AOTX_EPI_SWIGLU) return 1;
+        if (s + 1u < nseg && rows[s] % 16u != 0u && !linear) return 1;
     }
     unsigned int tiles;
     if (epi == AOTX_EPI_SWIGLU) {

@@ -79,6 +79,18 @@ def test_linear_workspace(lib):
                 assert lib.aotx_q8_linear(ctypes.byref(how), *{**LCALL, "m": m, "work_bytes": need - 1}.values()) == 1
 
 
+def test_pairs_of_any_number_of_rows_are_for_the_product_with_an_epilogue_alone(lib):
+    """The plans of the step and of routed experts refuse a pair whose matrices are not whole tiles of 16 rows."""
+    two = (ctypes.c_void_p * 2)(A256, A256)
+    args, swiglu = ctypes.create_string_buffer(4096), 3
+    for name in ("_Z15aotx_rgemv_planP15aotx_rgemv_argsPKPKvPKjjjij", "_Z22aotx_rgemv_plan_routedP15aotx_rgemv_argsPKPKvPKjjjij"):
+        for n, want in ((96, 0), (100, 1), (8, 1), (112, 0)):
+            for m in (1, 8, 32, 64, 300):
+                assert getattr(lib, name)(args, two, (ctypes.c_uint * 2)(n, n), 2, 256, swiglu, m) == want, (name, n, m)
+    for n in (96, 100, 8, 112):
+        assert lib.aotx_q8_linear_work(n, 256, 8, 1) >= A.AOTX_LINEAR_ZERO
+
+
 NORM = dict(x=A256, stride=64, w=A256, tokens=3, width=64, eps=1e-6, out=A256, stream=None)
 
 
