@@ -64,6 +64,22 @@ __global__ __launch_bounds__(256) void aotx_norm_rows_kernel(aotx_norm_rows_args
         const unsigned int i = n * 2048u + threadIdx.x * 8u;
         if (i < p.width) aotx_norm_put(p, x[n][0], x[n][1], scale, t, i);
     }
+    if ((threadIdx.x & ~63u) * 8u >= p.width || !aotx_squares_lost(sum, p.eps)) return;
+    /* Every wave that has values reads the row again, for itself, and writes its values again: with the values kept for
+     * this, the case looked at before the stores, or the whole workgroup in it, every row would pay (8192 of 8192 75 us
+     * against 72.9, of 64 5.6 against 5.3). */
+    const float by = aotx_squares_by(sum), eps = p.eps * by * by;
+    sum = 0.0f;
+#pragma unroll 1
+    for (unsigned int i = (threadIdx.x & 63u) * 4u; i < p.width; i += 256u) {
+        const aotx_f4 v = *(const aotx_f4 *)(row + i) * by;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += v[e] * v[e];
+    }
+    const float again = 1.0f / sqrtf(aotx_wave_sum(sum) / (float)p.width + eps);
+#pragma unroll 1
+    for (unsigned int i = threadIdx.x * 8u; i < p.width; i += 2048u)
+        aotx_norm_put(p, *(const aotx_f4 *)(row + i) * by, *(const aotx_f4 *)(row + i + 4u) * by, again, t, i);
 }
 
 extern "C" int aotx_norm_rows(const float *x, unsigned int stride, const float *w, unsigned int tokens,

@@ -78,7 +78,8 @@ int aotx_q8_linear(const aotx_linear_how *how, const void *x, unsigned int m, vo
  *   out[t][i] = x[t][i] / sqrt(mean over i of x^2 + eps) * w[i]
  * x fp32, row t at x + t * stride; w fp32 [width]; out fp16 [tokens][width]. width a multiple of 8
  * up to 32768, up to 2^20 tokens, stride a multiple of 4, at least width; x, w and out 16-byte
- * aligned, eps >= 0 (with 0 a row of zeros has no norm: NaN). */
+ * aligned, eps >= 0 (with 0 a row of zeros has no norm: NaN). Rows whose squares fp32 does not hold have
+ * their norm too. */
 int aotx_norm_rows(const float *x, unsigned int stride, const float *w, unsigned int tokens,
                    unsigned int width, float eps, void *out, void *stream);
 

@@ -373,6 +373,24 @@ def test_norm_rows(torch, lib, width, tokens, pad):
     assert (got[-1] == 7.0).all()
 
 
+@pytest.mark.parametrize("width", [8, 200, 2056, 6000, 20000])
+@pytest.mark.parametrize("eps", [0.0, EPS, 1e-30, 1e-42])
+def test_norm_rows_of_any_size(torch, lib, width, eps):
+    """Rows whose squares fp32 does not hold: up to its end, down to its subnormal values, and one value alone."""
+    rng = np.random.default_rng(width)
+    x = (rng.normal(0, 1, (9, width)) * np.array([[1e20], [1e18], [1.0], [1e-15], [1e-20], [1e-23], [1e-38], [0], [0]])).astype(np.float32)
+    x[7, width // 2], x[8] = -1e-45, np.finfo(np.float32).max
+    x[8, ::2] *= -1
+    w = rng.normal(1, 0.3, width).astype(np.float32)
+    out = torch.zeros((9, width), dtype=torch.float16, device="cuda")
+    assert lib.aotx_norm_rows(p(_up(torch, x, np.float32)), width, p(_up(torch, w, np.float32)), 9, width, eps, p(out), None) == 0
+    torch.cuda.synchronize()
+    want = O.norm_rows(x, w, float(np.float32(eps)))
+    # as in test_norm_rows
+    off = np.abs(out.cpu().numpy().astype(np.float64) - want) - (2.0 ** -11 + 80 * O.E32) * np.abs(want)
+    assert off.max() <= 2.0 ** -25, np.unravel_index(off.argmax(), off.shape)
+
+
 @pytest.mark.parametrize("width", [64, 1000, 4096, 9000])
 def test_norm_rows_inf_and_nan_stay_in_their_row(torch, lib, width):
     x = np.ones((5, width), dtype=np.float32)
