@@ -30,6 +30,15 @@ static __device__ __forceinline__ void aotx_norm_put(const aotx_norm_rows_args &
     *(aotx_u16x8 *)(p.out + (unsigned long long)t * p.width + i) = y;
 }
 
+/* Whether fp32 lost a row's sum of squares: past its end (or NaN), or so small that squares went under and eps does
+ * not outweigh them. The row times aotx_squares_by, a power of two, and eps times that twice give the same norm
+ * with squares between 2^-118 and 2^111 (a row has at most 2^15 values). */
+static __device__ __forceinline__ bool aotx_squares_lost(float sum, float eps)
+{
+    return !(sum <= 3.4028234663852886e38f) || (sum < 0x1p-80f && eps < 0x1p-80f);
+}
+static __device__ __forceinline__ float aotx_squares_by(float sum) { return sum < 1.0f ? 0x1p90f : 0x1p-80f; }
+
 /* A workgroup a row, N times 2048 values: all loads are under way before the first square, and a row is read
  * once. The memory bounds it: 8192 rows of 4096 take 37 us (201 MB at 5.4 TB/s, a part of x comes from the last
  * level's cache), 64 rows 2.6, of 16384 4.5. */

@@ -78,15 +78,6 @@ static __device__ __forceinline__ float aotx_wave_sum(float v)
     return v;
 }
 
-/* Whether fp32 lost a row's sum of squares: past its end (or NaN), or so small that squares went under and eps does
- * not outweigh them. The row times aotx_squares_by, a power of two, and eps times that twice give the same norm
- * with squares between 2^-118 and 2^111 (a row has at most 2^15 values). */
-static __device__ __forceinline__ bool aotx_squares_lost(float sum, float eps)
-{
-    return !(sum <= 3.4028234663852886e38f) || (sum < 0x1p-80f && eps < 0x1p-80f);
-}
-static __device__ __forceinline__ float aotx_squares_by(float sum) { return sum < 1.0f ? 0x1p90f : 0x1p-80f; }
-
 /* Running sum of 64 lanes' values, in 64 bits. */
 template <int CTRL, int ROWS>
 static __device__ __forceinline__ double aotx_dpp_add(double v)

@@ -129,7 +129,9 @@ typedef struct aotx_rope_how {
  * factor fp32 [rope_dim / 2] or null; place unsigned [tokens][axes]; q, k, v fp16
  * [tokens][heads or kv_heads][head_dim] (v null: not written; k and v null with kv_heads = 0).
  * head_dim 64 or 128, up to 1024 heads and kv_heads, tokens up to 2^20; rope_dim a multiple of 8,
- * 8 to head_dim; stride a multiple of 4; qkv, the norms, q, k and v 16-byte aligned. */
+ * 8 to head_dim; stride a multiple of 4; qkv, the norms, q, k and v 16-byte aligned. A head's norm takes
+ * its squares as fp32 has them: values are below 2^60 in size, and where eps is below 2^-100 the largest of a
+ * head is above 2^-50. */
 int aotx_rope_axes(const float *qkv, unsigned int stride, const float *q_norm,
                    const float *k_norm, const aotx_rope_how *how, const float *factor,
                    const unsigned int *place, unsigned int tokens, unsigned int heads,
