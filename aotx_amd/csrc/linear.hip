@@ -77,8 +77,8 @@ static __device__ __forceinline__ rg_h8 lg_values(const rg_wreg &o, unsigned int
  * A weight value is half(quant * scale), made in registers by the two waves that multiply it, so that LDS holds x
  * alone, two quads of 128 columns of it, which the loads write without passing through registers; a quad's weights
  * are loaded one quad ahead. Every weight is read m / BM times and x n / 256 times, from L2 and the last level's cache.
- * The matrix cores bound it, and the clock that they pull down: 2048 rows of the gated 14336 x 4096 take 455 us, 1.06
- * PFLOP/s, where a library's fp16 product of 8192 cubed reaches 1.14 on the same card; the same rows through x and
+ * The matrix cores bound it, and the clock that they pull down: 2048 rows of the gated 14336 x 4096 take 455 us (445 to
+ * 480 by the card), 1.06 PFLOP/s, where a library's fp16 product of 8192 cubed reaches 1.14 on the same card; the same rows through x and
  * weights staged in LDS in passes of 512 take 579. Instructions of 32 x 32 x 16, weights without the second buffer, a
  * fixed order of instructions and loads of weights into L2 ahead took 487 to 526. */
 template <int BM, bool FILE>
@@ -368,8 +368,9 @@ __global__ __launch_bounds__(512, 2) void aotx_linear_gemm(aotx_rgemv_args a, ao
 
 /* The plan and its time, in ns: a round of tiles on all CUs takes so long a quad of k and so long beside them, and the
  * sums of a split tile go to memory and back at 4.5 TB/s, and to the workgroup that adds them at 0.13. Measured over
- * 1000 to 14336 weight rows, 512 to 14336 columns and 64 to 2048 batch rows; 2048 rows of the gated 14336 x 4096 take 443 us in tiles of 256 rows, 476 of 192 and 526 of
- * 128, of 4096 square 95, 91 and 82. Over the file's layout, where addresses are what a quad costs, 192 rows
+ * 1000 to 14336 weight rows, 512 to 14336 columns and 64 to 2048 batch rows; on one card 2048 rows of the gated 14336 x 4096
+ * take 477 us in tiles of 256 rows, 511 of 192 and 557 of 128, of 4096 square 109, 102 and 90, 1024 of 4096 square 80, 78
+ * and 63. Over the file's layout, where addresses are what a quad costs, 192 rows
  * are the most whose sums stay in registers. */
 unsigned long long aotx_lgemm_choose(aotx_lgemm_plan *p, unsigned int n, unsigned int k, unsigned int m, bool gated, bool file)
 {

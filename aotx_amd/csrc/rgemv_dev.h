@@ -406,9 +406,9 @@ static __device__ __forceinline__ rg_qkv_pre rg_qkv_prep_flat(const aotx_rgemv_a
 /* The place of output row `row`, batch row mm in a workgroup's result block out[]. The
  * epilogues read one batch row of consecutive output rows with consecutive lanes; with a
  * plain row stride of 32 or 64 floats those fall in one or two LDS banks. Blocks of 64
- * batch rows (the GEMM's) XOR mm with the row's low bits; blocks of 32 pad each row to 33
- * floats (a constant offset per row, so the accumulators' stores keep immediate offsets);
- * blocks of 16 keep the plain layout. rg_os is the row stride, the block is rows * rg_os. */
+ * batch rows (the GEMM's) XOR mm with the row's low bits; blocks of 32 and 16 pad each row by a
+ * float (a constant offset per row, so the accumulators' stores keep immediate offsets).
+ * rg_os is the row stride, the block is rows * rg_os. */
 template <int MT>
 static __device__ __forceinline__ constexpr unsigned int rg_os()
 {
