@@ -665,7 +665,7 @@ static __device__ __forceinline__ float rg_gelu(float v)
 {
     /* x Phi(x), where Phi(-a) = erfc(a / sqrt 2) / 2 = exp(-a^2 / 2) s P(s), s = 1 / (1 + 0.35 a), so that small values
      * keep their bits (of 1 + erf(x / sqrt 2), 5 % would be lost at -5 and everything from -5.6 on). P was fitted to
-     * least relative error in 64 bits over a from 0 to 14.5, where fp32 ends: 2^-24.9. Half of erfc's own instructions:
+     * least relative error in 64 bits over a from 0 to 14.5, where fp32 ends: 2^-24.9. Cheaper than either function:
      * 2048 rows of 14336 x 4096 take 284 us, 301 by erfc, 298 by erf */
     const float a = __builtin_fabsf(v), s = __builtin_amdgcn_rcpf(1.0f + 0.35f * a);
     float p = -0.029158009216189384f;
