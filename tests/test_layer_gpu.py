@@ -279,6 +279,28 @@ def test_linear_inf_and_nan_in_the_gemm_and_tiles(torch, lib, m, n, k, gated, ba
     assert (np.abs(y[fine] - want[fine]) <= far[fine]).all()
 
 
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("m,n,k", [(1, 2048, 1568), (3, 200, 352), (12, 200, 352), (20, 40, 4128), (40, 3000, 160), (64, 2048, 1056),
+                                   (300, 9000, 1184), (300, 4096, 3968), (677, 4096, 1184), (1100, 1024, 4128)])
+def test_linear_reads_nothing_past_k(torch, lib, packed, m, n, k):
+    """Rows of a wider buffer whose other columns hold NaN, and an infinite scale in the last block of one weight row."""
+    c = Linear(torch, lib, 13, m, n, k, packed=packed, pad=(136, 1, 0))
+    c.x[:, k:] = np.nan
+    c.x[0, k - 32:k] = 1
+    raw = c.raw[0].reshape(n, k // 32, 34)
+    raw[n - 1, -1, :2] = np.array([np.inf], dtype=np.float16).view(np.uint8)
+    raw[n - 1, -1, 2:] = 1
+    c.w[0] = O.q8_values(c.raw[0], n, k)
+    c.up().call()
+    torch.cuda.synchronize()
+    cols = np.r_[0:n - 20:9, n - 20:n - 1]
+    y = c.y[:m, :n].cpu().numpy()
+    want, far = c.want(cols)
+    assert (np.abs(y[:, cols] - want) <= far).all()
+    assert not np.isfinite(y[:, n - 1]).any() and y[0, n - 1] == np.inf
+    assert (c.y[:m, n:] == 7.0).all()
+
+
 def test_linear_is_the_product_with_nothing_beside(torch, lib):
     """Bit for bit aotx_q8r_gemv where the same form runs, and the same on every run."""
     for m, n in ((1, 4200), (20, 500), (32, 500)):
